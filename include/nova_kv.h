@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define NKV_ABI_VERSION 12
+#define NKV_ABI_VERSION 13
 
 #define NKV_OK 0
 #define NKV_ERR_INVALID 1     /* argument outside what the reference accepts */
@@ -584,6 +584,65 @@ int nkv_paged_decode_step_tok(const uint16_t* q, const uint16_t* k_new, const ui
                               const int32_t* wg_map, const int32_t* seq_parts, int64_t total_parts,
                               uint16_t* out, float* lse_out, void* workspace, int64_t workspace_bytes,
                               void* stream);
+
+/*
+ * ---- Several tokens per sequence in one step (paged, per-token symmetric format) ----
+ * No counterpart in the reference, which decodes one token of one sequence at a time
+ * (src/nova/kvattn.py:326-327). The new tokens of a batch are packed: token t (t < tokens) is
+ * sequence seq_of[t]'s new token t - cu[seq_of[t]] and stands at position start_dev[seq] + that;
+ * cu: int32 [nseq + 1], ascending; seq_of: int32 [tokens]; start_dev: int64 [nseq]. All three are
+ * read on the device. pages, page_table, num_pages: as for the paged batch above.
+ *
+ * nkv_paged_append_chunks_tok: the stacked projections qkv [tokens][hq + 2 hkv][128] (NKV_F16 /
+ * NKV_BF16 / NKV_F32, rows row_stride elements apart). Each q and k head gets its RMSNorm when
+ * q_gamma / k_gamma ([128], of qkv's type; both or neither NULL) are given, then, when inv_freq (fp32
+ * [64]) is, the rotary embedding at the token's position p: element i < 64 becomes x_i cos - x_(i+64)
+ * sin and element i + 64 x_(i+64) cos + x_i sin, with the cosine and sine of p * inv_freq[i] (reduced in
+ * fp64). All in fp32, rounded once: q to fp16 (token t, head i at q_out + t * q_row_stride + i * 128),
+ * k and v to codes and scales (nkv_quantize_tok's arithmetic) in the row of their position. Tokens whose
+ * page is missing are not stored. q_out may be qkv's own q heads (NKV_F16, the same stride).
+ */
+int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens, uint8_t* pages,
+                                const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                                const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t nseq,
+                                int64_t hq, int64_t hkv, int64_t head_dim, const void* q_gamma, const void* k_gamma,
+                                float eps, const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream);
+
+/*
+ * Causal attention of the new tokens over their sequences' pages (their own keys and values stored before):
+ * out of the token at position p = softmax(q k^T / sqrt(128)) v over tokens [0, p]. q: token t, head i at
+ * q + t * q_token_stride + i * q_head_stride (multiples of 8); out likewise; lse_out [tokens][hq] fp32 or NULL.
+ * Groups without a page take no part; a row with none gives 0 and -inf.
+ * units: int32 [n_units][8], each (sequence, first row, rows, part, parts, partial slot, kind, 0): rows
+ * first .. first + rows - 1 of the sequence's new tokens x (hq / hkv) heads, token-major, over part `part` of
+ * `parts` of the 64-token groups up to the last of them; kind 0: up to 16 rows, 1: up to 32. Each row and part is in one
+ * unit for a result. With parts > 1 a unit writes one partial per row, row r of part p to slot + p * rows + r,
+ * and merges (int32 [n_merges][8]: sequence, first row, rows <= 8, parts, slot, slots from part to part, 0, 0)
+ * join them in a second launch. workspace: nkv_paged_chunks_workspace_bytes(hkv, slots), any contents, one
+ * call's at a time.
+ */
+int64_t nkv_paged_chunks_workspace_bytes(int64_t hkv, int64_t partial_rows);
+int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                              const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                              int64_t num_pages, const int32_t* cu, const int64_t* start_dev, int64_t nseq, int64_t hq,
+                              int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units,
+                              const int32_t* merges, int64_t n_merges, uint16_t* out, int64_t out_token_stride,
+                              int64_t out_head_stride, float* lse_out, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+/*
+ * Cached tokens back as out_dtype, packed: k_out / v_out [tokens][hkv][128], one rounding of the value that the
+ * codes stand for. Per-token symmetric: code * scale. int8t64: code * step + min for the whole groups of the
+ * sequence's length_dev[seq] tokens, the ring's fp16 value after them. A token without a page, or at or after the
+ * length (int8t64), is 0.
+ */
+int nkv_paged_read_tok(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                       const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq,
+                       int64_t hkv, int64_t head_dim, void* k_out, void* v_out, int out_dtype, void* stream);
+int nkv_paged_read_t64(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                       const uint16_t* rings, const int64_t* length_dev, const int32_t* seq_of, const int32_t* cu,
+                       const int64_t* start_dev, int64_t tokens, int64_t nseq, int64_t hkv, int64_t head_dim,
+                       void* k_out, void* v_out, int out_dtype, void* stream);
 
 /*
  * ---- Chunked prefill attention over the int8t64 cache (MFMA) ----

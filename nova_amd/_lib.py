@@ -86,6 +86,19 @@ SIGNATURES = {
     "nkv_paged_quantize_tok": (c_int, [P, c_int, I64, I64, I64, c_int, P, P, I64, I64, P]),
     "nkv_paged_decode_step_tok": (c_int, [P, P, P, I64, I64, P, P, I64, I64, P, I64, I64, I64, I64, P, P, I64, P,
                                           P, P, I64, P]),
+    # qkv, dtype, row_stride, tokens, pages, table, table_stride, num_pages, seq_of, cu, start, nseq, hq, hkv, head_dim,
+    # q_gamma, k_gamma, eps, inv_freq, q_out, q_row_stride, stream
+    "nkv_paged_append_chunks_tok": (c_int, [P, c_int, I64, I64, P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_float,
+                                            P, P, I64, P]),
+    "nkv_paged_chunks_workspace_bytes": (I64, [I64, I64]),
+    # q, q_token_stride, q_head_stride, tokens, pages, table, table_stride, num_pages, cu, start, nseq, hq, hkv, head_dim,
+    # units, n_units, merges, n_merges, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream
+    "nkv_paged_attn_chunks_tok": (c_int, [P, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, P, I64, P,
+                                          I64, I64, P, P, I64, P]),
+    # pages, table, table_stride, num_pages, (rings, length,) seq_of, cu, start, tokens, nseq, hkv, head_dim, k_out, v_out,
+    # dtype, stream
+    "nkv_paged_read_tok": (c_int, [P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_int, P]),
+    "nkv_paged_read_t64": (c_int, [P, P, I64, I64, P, P, P, P, P, I64, I64, I64, I64, P, P, c_int, P]),
     "nkv_prefill_workspace_bytes": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_default_splits": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_cutting": (c_int, [I64, I64, I64, I64, I64, I64, I64, P]),
@@ -112,7 +125,7 @@ SIGNATURES = {
     "nkv_qk_norm_rope": (c_int, [P, I64, I64, I64, P, P, c_float, P, P, P]),
 }
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,167 @@
+"""Plans of the paged caches' calls over several tokens per sequence.
+
+A step of a paged batch may bring any number of tokens for each sequence: a prompt's chunk, a few
+drafted tokens, one decode token, none. The tokens are packed one after another, sequence 0's
+first, as ``[tokens, heads, 128]``. ``SpanPlan`` says which tokens of which sequences a packed
+tensor holds; ``ChunkPlan`` adds how their attention is cut into work units. Plans are read only
+(any number of calls, layers and graphs may share one) and hold the counts fixed, while positions
+come from the cache's device tensor ``pos``, so a captured step follows the sequences as they grow.
+
+``plan_units`` is plain Python on integers, testable without a GPU. The reference decodes one token
+of one sequence (src/nova/kvattn.py:326-327) and has no paged layout.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from . import _lib
+
+D, GT = 128, 64
+CUS = 256        # compute units of an MI355X: one attention workgroup each at a time
+UNIT_INTS = 8    # int32 words of a work unit and of a merge entry
+ROWS16, ROWS32 = 0, 1  # unit kinds
+TILE_ROWS = {ROWS16: 16, ROWS32: 32}  # query rows (tokens x q heads per KV head) of a tile, at most
+MAX_PARTS = 256
+MERGE_ROWS = 8   # rows a merge entry covers
+
+
+@dataclass
+class SpanPlan:
+    """Tokens ``starts[b] .. starts[b] + counts[b] - 1`` of sequences ``0 .. nseq - 1``, packed."""
+
+    counts: list[int]
+    total: int
+    starts: torch.Tensor   # int64 [nseq] on the device
+    cu: torch.Tensor       # int32 [nseq + 1]: where each sequence's tokens begin in the packed tensor
+    seq_of: torch.Tensor   # int32 [total]: the sequence of each packed token
+
+    @property
+    def nseq(self) -> int:
+        return len(self.counts)
+
+
+@dataclass
+class ChunkPlan(SpanPlan):
+    """A step's new tokens: ``starts`` is the cache's ``pos`` itself, ``new`` the counts on the device."""
+
+    new: torch.Tensor = None      # int64 [nseq]
+    units: torch.Tensor = None    # int32 [n, 8]
+    merges: torch.Tensor = None   # int32 [m, 8]
+    ws_bytes: int = 0
+
+
+def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
+    counts = [int(n) for n in counts]
+    if not 0 < len(counts) <= max_seqs:
+        raise ValueError(f"{what} for {len(counts)} sequences; the cache has {max_seqs}")
+    if min(counts) < 0:
+        raise ValueError(f"{what} must not be negative, got {min(counts)}")
+    return counts
+
+
+def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarray, int]:
+    """How the attention of ``counts[b]`` new tokens after ``starts[b]`` is cut.
+
+    Returns ``(units, merges, partial_rows)``, int32 ``[n, 8]`` and ``[m, 8]``. The rows of a KV head
+    (``counts[b] * gq``, token-major) are cut into tiles, a tile's 64-token groups into parts; a
+    unit is one part of one tile: ``(sequence, first row, rows, part, parts, partial slot, kind, 0)``.
+    Cut tiles leave one partial per row and part, which the merge entries ``(sequence, first row,
+    rows, parts, slot, slots from part to part, 0, 0)`` join, eight rows each. The longest units
+    come first."""
+    tiles = []  # (steps, sequence, first row, rows, kind)
+    for b, (start, n) in enumerate(zip(starts, counts)):
+        for row0 in range(0, n * gq, 32):
+            rows = min(32, n * gq - row0)
+            steps = (start + (row0 + rows - 1) // gq) // GT + 1
+            tiles.append((steps, b, row0, rows, ROWS16 if rows <= 16 else ROWS32))
+    target = max(8, -(-sum(t[0] for t in tiles) * hkv // CUS))
+    units, merges, slot = [], [], 0
+    for steps, b, row0, rows, kind in tiles:
+        parts = min(MAX_PARTS, -(-steps // target))
+        for p in range(parts):
+            units.append((-(-steps // parts), b, row0, rows, p, parts, slot, kind, 0))
+        if parts > 1:
+            for r in range(0, rows, MERGE_ROWS):
+                merges.append((b, row0 + r, min(MERGE_ROWS, rows - r), parts, slot + r, rows, 0, 0))
+            slot += parts * rows
+    units.sort(key=lambda u: -u[0])
+    as_ints = lambda rows: np.array(rows, dtype=np.int32).reshape(-1, UNIT_INTS)  # noqa: E731
+    return as_ints([u[1:] for u in units]), as_ints(merges), slot
+
+
+def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:
+    n = np.array(counts, dtype=np.int64)
+    if sum(counts) > 1 << 28:
+        raise ValueError(f"{sum(counts)} tokens in one call; at most 2^28")
+    cu = np.concatenate(([0], np.cumsum(n)))
+    return cu.astype(np.int32), np.repeat(np.arange(len(counts), dtype=np.int32), n)
+
+
+def span_plan(counts: list[int], starts: list[int], device) -> SpanPlan:
+    cu, seq_of = _packed(counts)
+    first = torch.tensor(starts, dtype=torch.int64).to(device)
+    ints = torch.from_numpy(np.concatenate((cu, seq_of))).to(device)
+    return SpanPlan(counts, int(cu[-1]), first, ints[:len(cu)], ints[len(cu):])
+
+
+def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int) -> ChunkPlan:
+    cu, seq_of = _packed(counts)
+    units, merges, rows = plan_units(lengths, counts, gq, hkv)
+    # one copy to the device; the entries are 32 bytes, so that each of them stays aligned
+    ints = torch.from_numpy(np.concatenate((units.ravel(), merges.ravel(), cu, seq_of))).to(pos.device)
+    new = torch.tensor(counts, dtype=torch.int64).to(pos.device)
+    u, m = units.size, units.size + merges.size
+    return ChunkPlan(counts, int(cu[-1]), pos[:len(counts)], ints[m:m + len(cu)], ints[m + len(cu):], new,
+                     ints[:u].view(-1, UNIT_INTS), ints[u:m].view(-1, UNIT_INTS),
+                     int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)))
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of ``device``, whichever device is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_ptr(device))
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, _lib.stream_ptr(device))
+
+
+def heads_of(x: torch.Tensor, name: str, tokens: int, heads: int, device: torch.device) -> None:
+    """``x`` must be fp16 ``[>= tokens, heads, 128]`` on ``device``."""
+    if (x.dim() != 3 or x.shape[0] < tokens or x.shape[1] != heads or x.shape[2] != D or x.dtype != torch.float16
+            or x.device != device):
+        raise ValueError(f"{name} must be fp16 [{tokens}, {heads}, {D}] on {device} (more tokens may follow), "
+                         f"got {tuple(x.shape)} {x.dtype} on {x.device}")
+
+
+def rows_in_place(x: torch.Tensor) -> bool:
+    """Whether the kernels can take ``x`` ``[tokens, heads, 128]`` where it is: rows of 128 elements that start
+    on 16 bytes."""
+    return x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0
+
+
+def _extent(x: torch.Tensor) -> tuple[int, int]:
+    """The bytes from ``x``'s first to behind its last element (no negative strides in torch)."""
+    if x.numel() == 0:
+        return x.data_ptr(), x.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _extent(x), _extent(y)
+    return a0 < b1 and b0 < a1
+
+
+def distinct_rows(x: torch.Tensor) -> bool:
+    """Whether no two elements of ``x`` ``[tokens, heads, 128]`` (unit last stride) share memory: one of the two
+    outer dimensions lies within the other's stride."""
+    (n, h, d), (st, sh, _) = x.shape, x.stride()
+    if x.numel() == 0:
+        return True
+    inner_heads = (h == 1 or sh >= d) and (n == 1 or st >= (h - 1) * sh + d)
+    inner_tokens = (n == 1 or st >= d) and (h == 1 or sh >= (n - 1) * st + d)
+    return inner_heads or inner_tokens

@@ -33,7 +33,7 @@
 //     of a lane share one ruler.
 // The P operand of the PV product is exactly the S^T output layout of two token
 // blocks, so no data moves between the two products.
-#include "nkv_common.h"
+#include "nkv_mfma.h"
 
 #include <algorithm>
 #include <iterator>
@@ -48,12 +48,8 @@ namespace nkv {
 #endif
 
 
-constexpr int D = 128;
-constexpr int GT = 64;              // tokens per ruler group == ring slots
 constexpr int WAVES = NKV_WAVES;    // waves per workgroup
 constexpr int THREADS = 64 * WAVES;
-constexpr int CODE_BYTES = GT * D;                        // one tensor's codes of one group
-constexpr int RULER_BYTES = 4 * D * 2;                    // kst, kmn, vst, vmn of one group
 constexpr int HALF_CODE = 32 * D;                          // one tensor's codes of a half group
 constexpr int HALF_SLOT = 2 * HALF_CODE;                   // K | V codes of a half group
 constexpr int WAVE_LDS = 2 * HALF_SLOT + 2 * RULER_BYTES;  // two slots + two ruler sets
@@ -68,29 +64,14 @@ constexpr int WAVE_LDS_TOK = 2 * HALF_SLOT_TOK;
 constexpr int LDS_BYTES_TOK = WAVES * WAVE_LDS_TOK;        // 130 KiB
 constexpr int DMA_HALF_TOK = 2 * (HALF_CODE / 1024) + 2;
 constexpr int RING_BYTES = GT * D * 2;                    // one fp16 ring tensor of one head
-// paged layout: one page = one 64-token group of one KV head, K codes | V codes | kst | kmn | vst | vmn
-constexpr int PAGE_BYTES = 2 * CODE_BYTES + RULER_BYTES;  // 17 KiB, a multiple of 128
 constexpr int DMA_FIRST_HALF_PAGED = 2 * (HALF_CODE / 1024) + 1;  // the rulers are one 1 KiB load
-// paged per-token symmetric layout: one page = 64 tokens of one KV head, K codes | V codes |
-// K scales (64 fp16) | V scales
-constexpr int PAGE_TOK_BYTES = 2 * CODE_BYTES + 2 * GT * 2;  // 16640, a multiple of 128
 enum Layout : int { CONTIG_T64 = 0, CONTIG_TOK = 1, PAGED_T64 = 2, PAGED_TOK = 3 };
 constexpr float P_SCALE_LOG2 = 15.0f;  // the softmax weights carry a factor 2^15
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-constexpr float NEG_INF = -__builtin_huge_valf();
 
 static_assert(DMA_FIRST_HALF == 12 && DMA_SECOND_HALF == 8 && DMA_HALF_TOK == 10, "loads per half group");
 static_assert(PAGE_BYTES % 128 == 0 && PAGE_TOK_BYTES % 128 == 0, "pages are 128-byte aligned");
 static_assert(LDS_BYTES <= 150 * 1024 && LDS_BYTES_TOK <= 150 * 1024, "LDS of one workgroup");
 
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void lds_void_t;
-typedef int v2i_t __attribute__((vector_size(8)));
-typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
-typedef short v4s_t __attribute__((vector_size(8)));
-typedef __attribute__((address_space(3))) v4s_t lds_v4s_t;
 
 enum TailMode : int { TAIL_NONE = 0, TAIL_MASK = 1, TAIL_SCALARS = 2, TAIL_FUSED = 3 };
 // TAIL_FUSED with `tok`: the new token itself is the tail (its codes written by the prefix kernel).
@@ -206,11 +187,6 @@ __device__ __forceinline__ int parts_used(const AttnArgs& a, int64_t U) {
   return min(a.n_parts, W <= a.part_one ? a.part_few : (W + a.part_add) >> a.part_shift);
 }
 
-// XOR key of the 16-byte chunk positions of LDS row `row` (a token within its group).
-// K reads (16 consecutive rows, one chunk) and V transpose reads (rows 4g + {0..3} of
-// two 16-row blocks, one chunk) both hit 16 distinct bank positions per 16 lanes.
-__device__ __forceinline__ int swz(int row) { return ((row >> 1) & 7) ^ (((row >> 4) & 1) << 2); }
-
 // fp16 ring tensor in LDS: row r (256 B) keeps its 16-byte chunk c at position c ^ (r & 15),
 // so the 16 rows a K operand read touches land on 16 distinct banks.
 __device__ __forceinline__ int ring_chunk_pos(int row, int chunk) { return chunk ^ (row & 15); }
@@ -221,27 +197,6 @@ __device__ __forceinline__ float sum4rows(float v) {
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-
-// Online-softmax state of one wave. m, l: head (lane & 15), log2 domain; m is a reference
-// maximum (at least every score seen so far, times sl2), the weights are 2^(s sl2 - m + 15).
-// acc[cb][i]: head 4*(lane>>4) + i, dim 16*cb + (lane&15), in the same scale.
-struct WaveState {
-  float m, l;
-  float4_t acc[8];
-};
-
-__device__ __forceinline__ void state_init(WaveState& st) {
-  st.m = NEG_INF;
-  st.l = 0.0f;
-#pragma unroll
-  for (int cb = 0; cb < 8; ++cb) st.acc[cb] = float4_t{0.f, 0.f, 0.f, 0.f};
-}
-
-__device__ __forceinline__ float4_t mfma32(half8_t a, half8_t b, float4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ half8_t as_h8(uint4 w) { return __builtin_bit_cast(half8_t, w); }
 
 // 8 codes (bytes of w0, w1) -> fp16(code * st + mn) per element, rulers per element.
 __device__ __forceinline__ half8_t dq8(uint32_t w0, uint32_t w1, uint4 st, uint4 mn) {
@@ -259,16 +214,6 @@ __device__ __forceinline__ half8_t dq8_splat(uint32_t w0, uint32_t w1, half2_t s
   const half2_t c = __builtin_elementwise_fma(codes_to_h2(w1, kSelB01), st, mn);
   const half2_t d = __builtin_elementwise_fma(codes_to_h2(w1, kSelB23), st, mn);
   return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// The thread index for code that runs once per layer (the tails, the chained step's merger):
-// read through an opaque move, so that values derived from it are recomputed where they are used
-// rather than hoisted out of the chained kernel's layer loop and kept live across it (which
-// exhausts the register file there).
-__device__ __forceinline__ int tail_tid() {
-  int t;
-  asm volatile("v_mov_b32 %0, %1" : "=v"(t) : "v"((int)__builtin_amdgcn_workitem_id_x()));
-  return t;
 }
 
 // Q as the B operand of v_mfma_f32_16x16x32_f16: lane (c, g) holds head c's dims
@@ -295,32 +240,6 @@ __device__ __forceinline__ int lane_of() {
 }
 
 // ---------------------------------------------------------------- HBM -> LDS streaming
-
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-  return (uint32_t)(uintptr_t)(const lds_void_t*)p;
-}
-
-// A pointer the wave holds in common, moved to scalar registers.
-__device__ __forceinline__ const void* uniform_ptr(const void* p) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  return reinterpret_cast<const void*>(((uint64_t)hi << 32) | lo);
-}
-
-// One `global_load_lds_dwordx4`: lane L's 16 bytes at sbase + voff land at LDS byte
-// address lds + 16 * L (sbase and lds are wave-uniform).
-__device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t lds) {
-  lds = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
-}
-
-// The same, nontemporal: for the decode prefix's codes and rulers, which a step reads once
-// (about 3-5% faster than the default policy on the 32k decode step).
-__device__ __forceinline__ void dma16_stream(const void* sbase, uint32_t voff, uint32_t lds) {
-  lds = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "s"(lds) : "memory");
-}
 
 // Issue the loads of half `hf` (tokens 32 hf .. 32 hf + 31) of group `grp` of head h: 32
 // K and 32 V code rows (4 + 4 loads) into the slot at `slot` (K codes, then V codes), and
@@ -532,7 +451,6 @@ __device__ __forceinline__ void load_q_lds(const uint16_t* q_lds, int gq, half8_
   }
 }
 
-__device__ __forceinline__ void wait_groups_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---------------------------------------------------------------- one group's attention
 
@@ -815,24 +733,6 @@ __device__ __forceinline__ void pv_qk_half(WaveState& st, const uint8_t* vc, con
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[b][i] = S[b][i];
-}
-
-// fp16(code * scale) for 8 signed codes sharing one fp16 scale, and for 8 codes with one
-// scale each: the product of an 8-bit integer and an fp16 is exact in fp32, so the packed
-// fp16 multiply rounds it once, as fp16(fp32(code) * fp32(scale)) does.
-__device__ __forceinline__ half8_t dq8_sym(uint32_t w0, uint32_t w1, half2_t s) {
-  const half2_t a = scodes_to_h2(w0, kSelB01) * s;
-  const half2_t b = scodes_to_h2(w0, kSelB23) * s;
-  const half2_t c = scodes_to_h2(w1, kSelB01) * s;
-  const half2_t d = scodes_to_h2(w1, kSelB23) * s;
-  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-__device__ __forceinline__ half8_t dq8_sym_v(uint32_t w0, uint32_t w1, uint4 s) {
-  const half2_t a = scodes_to_h2(w0, kSelB01) * as_h2(s.x);
-  const half2_t b = scodes_to_h2(w0, kSelB23) * as_h2(s.y);
-  const half2_t c = scodes_to_h2(w1, kSelB01) * as_h2(s.z);
-  const half2_t d = scodes_to_h2(w1, kSelB23) * as_h2(s.w);
-  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
 // attend_block for 32 tokens of the per-token symmetric format: codes as in attend_block
@@ -3353,7 +3253,6 @@ constexpr int PF_WG_PER_CU = 1;                      // workgroups resident per 
 constexpr int PF_ROWS = PF_WAVES * PF_RB * 16;       // 256 query rows per workgroup
 constexpr int PF_KROW = D + 8;                       // fp16 K tile row stride (halves)
 constexpr int PF_VROW = GT + 16;                     // fp16 V^T tile row stride (halves, 16-byte rows)
-constexpr float PF_TAU = 8.0f;                       // lazy softmax rescaling threshold (log2)
 constexpr int PF_PART = D + 4;                       // floats per row partial: acc[128], m, l, pad
 constexpr int PF_MAX_SHARES = CUS;                   // shares of a head's steps (one workgroup per CU)
 constexpr int PF_STAGE = 2 * GT * D * 2;             // bytes of a stage: an fp16 group, or an int8 one with its rulers
@@ -3432,40 +3331,6 @@ struct PrefillMergeArgs {
   int M, gq, hkv, slots, slot_rows, two_slots, n;
   PrefillMerge t[PF_MAX_SHARES];
 };
-
-// Online softmax of one 16-row block over 64 tokens, from the raw scores S[b][i] (token
-// 16b + 4g + i, row c; -inf where masked): m is a reference maximum in the log2 domain, within
-// PF_TAU below the row's maximum of S * sl2, and P comes out as exp2(S sl2 - m + 15 - PF_TAU)
-// <= 2^15 in two fp16 A operands (tokens of blocks 0,1 and 2,3). The row sums of P are taken on
-// the matrix core by the caller (P times a ones operand, in the accumulator layout), which leaves
-// the VALU the maximum, the exponentials and the conversions; the caller rescales the
-// accumulators and those sums by alpha, only when m moves.
-__device__ __forceinline__ void pf_softmax(WaveState& st, const float (&S)[4][4], float sl2, half8_t (&ph)[2],
-                                           float& alpha_out, bool& moved_out) {
-  float smax = NEG_INF;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) smax = fmaxf(smax, S[b][i]);
-  smax = max4rows(smax);
-  const float m_cand = fmaxf(st.m, smax * sl2);
-  const float m_new = m_cand > st.m + PF_TAU ? m_cand : st.m;
-  const float m_use = m_new == NEG_INF ? 0.0f : m_new;
-  const float alpha = __builtin_amdgcn_exp2f(st.m - m_use);
-  const float off = 15.0f - PF_TAU - m_use;
-  _Float16 p16[2][8];
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(S[b][i], sl2, off));
-#pragma unroll
-  for (int B = 0; B < 2; ++B)
-    ph[B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
-  moved_out = st.m != m_new;
-  alpha_out = alpha;
-  st.m = m_new;
-}
 
 __global__ __launch_bounds__(PF_THREADS, PF_WG_PER_CU) void prefill_chunk_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][PF_STAGE];

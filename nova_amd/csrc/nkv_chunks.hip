@@ -1,0 +1,774 @@
+// The new tokens of a paged batch: a step in which every sequence brings any number of tokens (a prompt's
+// chunk, drafted tokens, one decode token, none), packed one after another.
+//
+// - append_chunks: the head norms and the rotary embedding of the stacked q/k/v projections, and the
+//   quantized store of the keys and values into their pages (per-token symmetric format);
+// - attn_chunks: the new tokens' causal attention over everything their sequence has in its pages;
+// - read: spans of cached tokens back to fp16 / bf16 / fp32, from either page format.
+//
+// Token t of the packed batch belongs to sequence seq_of[t] and is its new token t - cu[seq]; its position is
+// start[seq] + that. Lengths and positions are read on the device, so a captured graph follows them.
+
+#include <algorithm>
+
+#include "nkv_mfma.h"
+
+namespace nkv {
+
+namespace {
+
+// ---------------------------------------------------------------- the packed batch
+
+struct Batch {
+  const int32_t* seq_of;   // [tokens]
+  const int32_t* cu;       // [nseq + 1]
+  const int64_t* start;    // [nseq]
+  const int32_t* table;    // [nseq][table_stride]
+  int64_t table_stride, num_pages;
+  int nseq, hkv;
+};
+
+// The page of group `grp` of sequence b, -1 where the table holds none.
+__device__ __forceinline__ int64_t page_at(const Batch& a, int b, int64_t grp) {
+  if (grp < 0 || grp >= a.table_stride) return -1;
+  const int32_t page = a.table[(int64_t)b * a.table_stride + grp];
+  return page >= 0 && page < a.num_pages ? page : -1;
+}
+
+struct TokenAt {
+  int64_t pos, page;  // position in its sequence; page -1: none
+  int seq;
+};
+
+__device__ __forceinline__ TokenAt token_at(const Batch& a, int64_t t) {
+  const int b = a.seq_of[t];
+  if (b < 0 || b >= a.nseq) return {-1, -1, -1};
+  const int64_t pos = a.start[b] + (t - a.cu[b]);
+  return {pos, page_at(a, b, pos < 0 ? -1 : pos / GT), b};
+}
+
+// ---------------------------------------------------------------- eight values of a row
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<NKV_F16> {
+  static constexpr int SIZE = 2;
+};
+template <>
+struct Elem<NKV_BF16> {
+  static constexpr int SIZE = 2;
+};
+template <>
+struct Elem<NKV_F32> {
+  static constexpr int SIZE = 4;
+};
+
+template <int DT>
+struct Raw8 {  // eight consecutive values as loaded
+  uint4 w[Elem<DT>::SIZE / 2];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::SIZE / 2; ++i) w[i] = *reinterpret_cast<const uint4*>(p + 16 * i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::SIZE / 2; ++i) w[i] = uint4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+    if constexpr (DT == NKV_F32) {
+      const uint32_t u2[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]), v[4 + i] = __uint_as_float(u2[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == NKV_F16) {
+          v[2 * i] = h2f((uint16_t)(u[i] & 0xffffu));
+          v[2 * i + 1] = h2f((uint16_t)(u[i] >> 16));
+        } else {
+          v[2 * i] = bf2f((uint16_t)(u[i] & 0xffffu));
+          v[2 * i + 1] = bf2f((uint16_t)(u[i] >> 16));
+        }
+      }
+    }
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
+  if constexpr (DT == NKV_F32) {
+    *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<float4*>(p + 16) = float4{v[4], v[5], v[6], v[7]};
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = DT == NKV_F16 ? f2h(v[2 * i]) : f2bf(v[2 * i]);
+      const uint32_t hi = DT == NKV_F16 ? f2h(v[2 * i + 1]) : f2bf(v[2 * i + 1]);
+      u[i] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4*>(p) = uint4{u[0], u[1], u[2], u[3]};
+  }
+}
+
+// ---------------------------------------------------------------- append
+
+// Sum over the 16 lanes of each 16-lane row (DPP only; every lane gets it).
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
+  return v;
+}
+
+// The value of lane l ^ 8 of the same 16-lane row (a rotation by 8).
+__device__ __forceinline__ float row16_other_half(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
+}
+
+struct AppendArgs {
+  Batch b;
+  const uint8_t* x;  // [tokens][hq + 2 hkv][128], row stride x_rs elements
+  int64_t x_rs, tokens;
+  uint8_t* pages;
+  const uint8_t* q_gamma;  // [128] of x's type; NULL: no head norms
+  const uint8_t* k_gamma;
+  float eps;
+  const float* inv_freq;   // [64]; NULL: no rotation
+  uint16_t* q_out;         // token t, head i at q_out + t * q_rs + i * 128
+  int64_t q_rs;
+  int hq, heads_per_wg;
+};
+
+// One head row of 128 values to 16 lanes, 8 values each; 16 rows at a time in a workgroup, which takes TOK
+// tokens and heads_per_wg of their hq + 2 hkv heads. Everything in fp32, rounded once (q to fp16, k and v to
+// codes). The angle position * inv_freq is exact in fp64 and reduced there to a part of a turn, so that far
+// positions lose nothing; one lane computes it for each token and frequency, for all heads.
+template <int DT, int TOK>
+__global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
+  __shared__ float2 turn[TOK][D / 2];  // cos, sin
+  __shared__ int64_t row_of[TOK];      // byte offset of the token's row 0 of its page (KV head 0), or -1
+  __shared__ int slot_of[TOK];
+  const int tid = threadIdx.x, j = tid & 15, first = tid >> 4;
+  const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  const int heads = a.hq + 2 * a.b.hkv, h0 = blockIdx.y * a.heads_per_wg;
+  const int nh = min(a.heads_per_wg, heads - h0), nt = (int)min<int64_t>(TOK, a.tokens - t0);
+  const bool norm = a.q_gamma != nullptr, rotate = a.inv_freq != nullptr;
+  constexpr int SIZE = Elem<DT>::SIZE;
+
+  float gq[8], gk[8];
+  if (norm) {
+    Raw8<DT> r;
+    r.load(a.q_gamma + 8 * j * SIZE);
+    r.get(gq);
+    r.load(a.k_gamma + 8 * j * SIZE);
+    r.get(gk);
+  }
+  if (tid < TOK * (D / 2)) {
+    const int k = tid / (D / 2), f = tid % (D / 2);
+    if (k < nt) {
+      const TokenAt at = token_at(a.b, t0 + k);
+      if (f == 0) {
+        row_of[k] = at.page < 0 ? -1 : at.page * a.b.hkv * (int64_t)PAGE_TOK_BYTES;
+        slot_of[k] = (int)(at.pos & (GT - 1));
+      }
+      if (rotate) {
+        const double turns = (double)at.pos * (double)a.inv_freq[f] * 0.15915494309189533577;  // 1 / 2 pi
+        const float part = (float)(turns - __builtin_rint(turns));
+        turn[k][f] = float2{cospif(2.0f * part), sinpif(2.0f * part)};
+      }
+    }
+  }
+  __syncthreads();
+
+  for (int it = first; it < nt * nh; it += 16) {  // (16 lanes agree)
+    const int k = it / nh, h = h0 + it % nh;
+    const int64_t t = t0 + k;
+    Raw8<DT> raw;
+    raw.load(a.x + (t * a.x_rs + (int64_t)h * D + 8 * j) * SIZE);
+    float v[8];
+    raw.get(v);
+    const bool is_q = h < a.hq, is_v = h >= a.hq + a.b.hkv;
+    if (!is_v) {
+      if (norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
+        const float r = 1.0f / sqrtf(row16_sum(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (is_q ? gq[e] : gk[e]);
+      }
+      if (rotate) {
+        // element i < 64 becomes x_i cos - x_(i + 64) sin, element i + 64 x_(i + 64) cos + x_i sin
+        const float side = j < 8 ? -1.0f : 1.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 cs = turn[k][(8 * j + e) & (D / 2 - 1)];
+          v[e] = __builtin_fmaf(v[e], cs.x, side * row16_other_half(v[e]) * cs.y);
+        }
+      }
+    }
+    if (is_q) {
+      store8<NKV_F16>(reinterpret_cast<uint8_t*>(a.q_out + t * a.q_rs + (int64_t)h * D + 8 * j), v);
+    } else if (row_of[k] >= 0) {
+      const int kv = is_v ? h - a.hq - a.b.hkv : h - a.hq, which = is_v ? 1 : 0;
+      float scale;
+      const uint2 codes = sym_quant8<true>(v, scale);
+      uint8_t* page = a.pages + row_of[k] + (int64_t)kv * PAGE_TOK_BYTES;
+      *reinterpret_cast<uint2*>(page + which * CODE_BYTES + slot_of[k] * D + 8 * j) = codes;
+      if (j == 0) *reinterpret_cast<uint16_t*>(page + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot_of[k]) = f2h(scale);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- read
+
+struct ReadArgs {
+  Batch b;
+  int64_t tokens;
+  const uint8_t* pages;
+  const uint16_t* rings;   // int8t64: [nseq][hkv][2][64][128]
+  const int64_t* length;   // int8t64: [nseq] tokens written
+  uint8_t* k_out;          // [tokens][hkv][128]
+  uint8_t* v_out;
+};
+
+constexpr int READ_TOK = 16;
+
+// READ_TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each.
+template <int DT, bool T64>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  __shared__ int64_t page_of[READ_TOK];  // the token's page; -1: none, -2: in its sequence's ring
+  __shared__ int slot_of[READ_TOK], seq_of[READ_TOK];
+  const int tid = threadIdx.x, j = tid & 15;
+  const int64_t t0 = (int64_t)blockIdx.x * READ_TOK;
+  const int nt = (int)min<int64_t>(READ_TOK, a.tokens - t0);
+  if (tid < nt) {
+    const TokenAt at = token_at(a.b, t0 + tid);
+    int64_t page = at.page;
+    if (T64 && at.seq >= 0) {
+      const int64_t len = a.length[at.seq];
+      if (at.pos >= len) page = -1;
+      else if (at.pos >= len / GT * GT) page = -2;
+    }
+    page_of[tid] = page;
+    slot_of[tid] = (int)(at.pos & (GT - 1));
+    seq_of[tid] = at.seq;
+  }
+  __syncthreads();
+  constexpr int SIZE = Elem<DT>::SIZE;
+  const int rows = 2 * a.b.hkv * nt;
+  for (int it = tid >> 4; it < rows; it += 16) {
+    const int k = it % nt, hw = it / nt, h = hw >> 1, which = hw & 1, slot = slot_of[k];
+    const int64_t page = page_of[k];
+    float v[8];
+    if (page == -1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    } else if (T64 && page == -2) {
+      Raw8<NKV_F16> r;
+      r.load(reinterpret_cast<const uint8_t*>(a.rings + ((((int64_t)seq_of[k] * a.b.hkv + h) * 2 + which) * GT + slot) * D + 8 * j));
+      r.get(v);
+    } else {
+      const uint8_t* p = a.pages + (page * a.b.hkv + h) * (T64 ? PAGE_BYTES : PAGE_TOK_BYTES);
+      const uint2 codes = *reinterpret_cast<const uint2*>(p + which * CODE_BYTES + slot * D + 8 * j);
+      if constexpr (T64) {
+        float st[8], mn[8];
+        Raw8<NKV_F16> r;
+        r.load(p + 2 * CODE_BYTES + which * (4 * D) + 16 * j);
+        r.get(st);
+        r.load(p + 2 * CODE_BYTES + which * (4 * D) + 2 * D + 16 * j);
+        r.get(mn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t c = ((e < 4 ? codes.x : codes.y) >> (8 * (e & 3))) & 0xffu;
+          v[e] = __builtin_fmaf((float)c, st[e], mn[e]);  // (the product is exact)
+        }
+      } else {
+        const float s = h2f(*reinterpret_cast<const uint16_t*>(p + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = (float)(int8_t)((e < 4 ? codes.x : codes.y) >> (8 * (e & 3))) * s;
+      }
+    }
+    uint8_t* out = (which ? a.v_out : a.k_out) + (((t0 + k) * a.b.hkv + h) * D + 8 * j) * SIZE;
+    store8<DT>(out, v);
+  }
+}
+
+// ---------------------------------------------------------------- attention
+//
+// The rows of KV head h in sequence b: row R = (new token R / gq, q head h gq + R % gq), gq = hq / hkv. They
+// are cut into tiles; a tile attends the 64-token groups up to its last token (steps 0 .. S - 1), and its
+// steps are cut into parts, unit = one part of one tile. Part p of P takes steps [S p / P, S (p + 1) / P),
+// from the S of the device's lengths: the plan stays valid while sequences grow.
+//
+// Units of up to 32 rows (SMALL): the waves of a workgroup take the part's groups in turn, each wave its own
+// group against all the rows, and their states are merged in LDS at the end. K codes go from memory to the
+// registers of S^T = K Q^T's A operand; V codes and both scales go to LDS, where the transposing read gives
+// the operand of O = P V. K's scale multiplies the scores, V is dequantized. Bound by the page bytes.
+
+constexpr int CH_WAVES = 8, CH_THREADS = 64 * CH_WAVES;
+constexpr int CH_VSLOT = CODE_BYTES + 4 * GT;            // V codes, K scales, V scales: the rest of a page after K
+constexpr int CH_PART = D + 4;                           // floats of a row's partial: acc[128], m, l, pad
+static_assert(CODE_BYTES + CH_VSLOT == PAGE_TOK_BYTES, "a page is K codes and a slot");
+static_assert(16 * CH_PART * 4 <= CH_VSLOT, "a wave's 16 rows fit one of its slots at the merge");
+constexpr int CH_LDS = 2 * CH_WAVES * CH_VSLOT;          // 132 KiB: two slots a wave
+
+enum UnitKind : int { ROWS16 = 0, ROWS32 = 1 };
+
+struct Unit {  // (int32 each, as the plan lays them out)
+  int seq, row0, rows, part, parts, slot, kind, pad;  // slot: partial row of part 0 of the tile
+};
+struct Merge {
+  int seq, row0, rows, parts, slot, stride, pad0, pad1;  // up to 8 rows; part p's partial of row r: slot + p * stride + r
+};
+
+struct ChunkArgs {
+  Batch b;
+  const uint16_t* q;  // token t, head i at q + t * q_ts + i * q_hs
+  int64_t q_ts, q_hs, tokens;
+  const uint8_t* pages;
+  const Unit* units;
+  int n_units, hq, gq;
+  float sl2;
+  uint16_t* out;
+  int64_t o_ts, o_hs;
+  float* lse;  // [tokens][hq] or NULL
+  float* ws;   // partial rows [ws_rows][hkv][CH_PART]
+  int64_t ws_rows;
+};
+
+// Where a tile of sequence b stands.
+struct TileAt {
+  int64_t start, first_token;  // position of the sequence's first new token; packed index of it
+  int rows;                    // rows of the tile (no more than the sequence has)
+  int64_t steps;               // groups up to the tile's last token
+};
+__device__ __forceinline__ TileAt tile_at(const ChunkArgs& a, int seq, int row0, int rows) {
+  TileAt t;
+  const int64_t c0 = a.b.cu[seq], c1 = a.b.cu[seq + 1];
+  const int64_t have = max<int64_t>(0, min(c1, a.tokens) - c0) * a.gq - row0;
+  t.rows = c0 < 0 ? 0 : (int)max<int64_t>(0, min<int64_t>(rows, have));
+  t.start = a.b.start[seq];
+  t.first_token = c0;
+  t.steps = t.rows == 0 || t.start < 0 ? 0 : min((t.start + (row0 + t.rows - 1) / a.gq) / GT + 1, a.b.table_stride);
+  return t;
+}
+
+// Two rows' results in the same LDS or memory layout: 32 lanes a row, 4 dims each.
+struct RowSum {
+  float m, l;
+  float4 acc;
+};
+__device__ __forceinline__ void write_row(const ChunkArgs& a, int h, int64_t token, int head, const RowSum& r, int l32) {
+  const float inv = r.l > 0.0f || r.l != r.l ? 1.0f / r.l : 0.0f;
+  const int i = h * a.gq + head;
+  *reinterpret_cast<uint2*>(a.out + token * a.o_ts + i * a.o_hs + 4 * l32) =
+      uint2{(uint32_t)f2h(r.acc.x * inv) | ((uint32_t)f2h(r.acc.y * inv) << 16),
+            (uint32_t)f2h(r.acc.z * inv) | ((uint32_t)f2h(r.acc.w * inv) << 16)};
+  // the weights carry 2^(15 - PF_TAU)
+  if (a.lse && l32 == 0)
+    a.lse[token * a.hq + i] = r.l == 0.0f ? NEG_INF : (r.m + __builtin_amdgcn_logf(r.l) - (15.0f - PF_TAU)) * LN2;
+}
+
+__device__ __forceinline__ bool finite_h(uint32_t bits) { return (bits & 0x7c00u) != 0x7c00u; }
+
+template <int RB>
+__device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
+  const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);  // tokens the sequence has with the new ones
+  const int64_t s0 = at.steps * u.part / u.parts, s1 = at.steps * (u.part + 1) / u.parts;
+  const uint8_t* pages = a.pages + (int64_t)h * PAGE_TOK_BYTES;
+  const int64_t page_stride = (int64_t)a.b.hkv * PAGE_TOK_BYTES;
+
+  uint4 kn[4][2];  // the next group's K codes: token 16 b + c, bytes 16 g + 64 hh ..
+  auto issue = [&](int64_t page, int sb) {
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride));
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+        kn[b][hh] = *reinterpret_cast<const uint4*>(p + (16 * b + c) * D + 16 * g + 64 * hh);
+    const uint32_t slot = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + (2 * wave + sb) * CH_VSLOT;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // earlier reads of this slot are done
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = 8 * e + (lane >> 3);
+      dma16(p, (uint32_t)(CODE_BYTES + row * D + (((lane & 7) ^ swz(row)) << 4)), slot + 1024 * e);
+    }
+    if (lane < 16) dma16(p, (uint32_t)(2 * CODE_BYTES + 16 * lane), slot + CODE_BYTES);
+  };
+
+  int64_t s = s0 + wave;
+  int64_t page = s < s1 ? page_at(a.b, u.seq, s) : -1;
+  if (page >= 0) issue(page, 0);
+  int64_t next_page = s + CH_WAVES < s1 ? page_at(a.b, u.seq, s + CH_WAVES) : -1;
+
+  half8_t qb[RB][4];
+  int64_t tq[RB];  // the last position that row c attends
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = 16 * rb + c, row = u.row0 + r;
+    const bool ok = r < at.rows;
+    const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
+    tq[rb] = ok ? at.start + tk : -1;
+    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 w = {0, 0, 0, 0};
+      if (ok) w = *reinterpret_cast<const uint4*>(qr + 16 * g + 64 * (k >> 1) + 8 * (k & 1));
+      qb[rb][k] = as_h8(w);
+    }
+  }
+  const int64_t whole = (at.start + u.row0 / a.gq + 1) / GT;  // steps that every row of the tile sees whole
+  const _Float16 one = (_Float16)1.0f;
+  const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
+  WaveState st[RB];
+  float4_t lsum[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    state_init(st[rb]);
+    lsum[rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int sb = 0; s < s1; s += CH_WAVES, sb ^= 1) {
+    const bool here = page >= 0;
+    uint4 kc[4][2];
+    wait_groups_all();
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) kc[b][hh] = kn[b][hh];
+    page = next_page;
+    if (page >= 0) issue(page, sb ^ 1);
+    next_page = s + 2 * CH_WAVES < s1 ? page_at(a.b, u.seq, s + 2 * CH_WAVES) : -1;
+    if (!here) continue;  // a group without a page takes no part
+
+    const uint8_t* slot = lds + (2 * wave + sb) * CH_VSLOT;
+    // the scales of tokens 16 b + 4 g .. + 3, as fp16 pairs
+    uint2 ks[4], vs[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      ks[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * (16 * b + 4 * g));
+      vs[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * GT + 2 * (16 * b + 4 * g));
+    }
+    float S[RB][4][4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      half8_t kop[4];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const half2_t unit = {one, one};
+        kop[2 * hh] = dq8_sym(kc[b][hh].x, kc[b][hh].y, unit);
+        kop[2 * hh + 1] = dq8_sym(kc[b][hh].z, kc[b][hh].w, unit);
+      }
+      const float kscale[4] = {h2f((uint16_t)(ks[b].x & 0xffffu)) * a.sl2, h2f((uint16_t)(ks[b].x >> 16)) * a.sl2,
+                               h2f((uint16_t)(ks[b].y & 0xffffu)) * a.sl2, h2f((uint16_t)(ks[b].y >> 16)) * a.sl2};
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float4_t x = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x = mfma32(kop[k], qb[rb][k], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[rb][b][i] = x[i] * kscale[i];
+      }
+    }
+    if (s >= whole) {
+      // Masked positions: tokens behind a row's own, and the page's rows behind the sequence's last token, which
+      // hold anything. Their weight is 0, but 0 times a V that is not finite is NaN, so such scales become 0;
+      // where a row does attend such a token, its score becomes NaN instead.
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t v16[4] = {vs[b].x & 0xffffu, vs[b].x >> 16, vs[b].y & 0xffffu, vs[b].y >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t tok = s * GT + 16 * b + 4 * g + i;
+          const bool fin = finite_h(v16[i]);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+            S[rb][b][i] = tok > tq[rb] ? NEG_INF : fin ? S[rb][b][i] : __builtin_nanf("");
+          if (!fin || tok >= len) v16[i] = 0;
+        }
+        vs[b] = uint2{v16[0] | (v16[1] << 16), v16[2] | (v16[3] << 16)};
+      }
+    }
+    half8_t ph[RB][2];
+    float alpha[RB];
+    bool moved[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      pf_softmax(st[rb], S[rb], 1.0f, ph[rb], alpha[rb], moved[rb]);
+      if (__builtin_amdgcn_ballot_w64(moved[rb]) != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float ai = shfl(alpha[rb], 4 * g + i);
+#pragma unroll
+          for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb][i] *= ai;
+          lsum[rb][i] *= ai;
+        }
+      }
+    }
+    const int r = c >> 1;
+#pragma unroll
+    for (int B = 0; B < 2; ++B) {
+      const uint4 vscale = {vs[2 * B].x, vs[2 * B].y, vs[2 * B + 1].x, vs[2 * B + 1].y};
+      const int vrow = 16 * (2 * B + (r >> 2)) + 4 * g + (r & 3);
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) {
+        const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_v2i_t*)(const lds_void_t*)(slot + vrow * D + 8 * (c & 1) + ((cb ^ swz(vrow)) << 4))));
+        const half8_t vop = dq8_sym_v(vw.x, vw.y, vscale);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) st[rb].acc[cb] = mfma32(ph[rb][B], vop, st[rb].acc[cb]);
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) lsum[rb] = mfma32(ph[rb][B], ones, lsum[rb]);
+    }
+  }
+
+  // ---- the waves' states into one, row by row
+  wait_groups_all();
+  __syncthreads();  // every wave is done with its slots
+  float* mine = reinterpret_cast<float*>(lds) + wave * (RB * 16 * CH_PART);
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    if (g == 0) mine[(16 * rb + c) * CH_PART + D] = st[rb].m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * rb + 4 * g + i;
+      if (c == 0) mine[r * CH_PART + D + 1] = lsum[rb][i];
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) mine[r * CH_PART + 16 * cb + c] = st[rb].acc[cb][i];
+    }
+  }
+  __syncthreads();
+  const int l32 = tid & 31;
+#pragma unroll
+  for (int p = 0; p < RB; ++p) {
+    const int r = 16 * p + (tid >> 5);
+    if (r >= at.rows) continue;
+    const float* base = reinterpret_cast<const float*>(lds) + r * CH_PART;
+    RowSum sum = {NEG_INF, 0.0f, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int w = 0; w < CH_WAVES; ++w) sum.m = fmaxf(sum.m, base[w * (RB * 16 * CH_PART) + D]);
+    const float mu = sum.m == NEG_INF ? 0.0f : sum.m;
+#pragma unroll
+    for (int w = 0; w < CH_WAVES; ++w) {
+      const float* x = base + w * (RB * 16 * CH_PART);
+      const float wt = __builtin_amdgcn_exp2f(x[D] - mu);
+      const float4 v = *reinterpret_cast<const float4*>(x + 4 * l32);
+      sum.acc.x += v.x * wt; sum.acc.y += v.y * wt; sum.acc.z += v.z * wt; sum.acc.w += v.w * wt;
+      sum.l += x[D + 1] * wt;
+    }
+    const int row = u.row0 + r;
+    if (u.parts == 1) {
+      write_row(a, h, at.first_token + row / a.gq, row % a.gq, sum, l32);
+    } else {
+      const int64_t pr = (int64_t)u.slot + (int64_t)u.part * u.rows + r;
+      if (pr < 0 || pr >= a.ws_rows) continue;
+      float* dst = a.ws + (pr * a.b.hkv + h) * CH_PART;
+      *reinterpret_cast<float4*>(dst + 4 * l32) = sum.acc;
+      if (l32 == 0) *reinterpret_cast<float2*>(dst + D) = float2{sum.m, sum.l};
+    }
+  }
+}
+
+__global__ __launch_bounds__(CH_THREADS, 1) void attn_chunks_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[CH_LDS];
+  const int h = blockIdx.x % a.b.hkv;
+  const Unit u = a.units[blockIdx.x / a.b.hkv];
+  if (u.seq < 0 || u.seq >= a.b.nseq || u.row0 < 0 || u.rows <= 0 || u.rows > 32 || u.part < 0 || u.part >= u.parts) return;
+  if (u.kind == ROWS16 && u.rows <= 16) attend_small<1>(a, u, h, lds);
+  else attend_small<2>(a, u, h, lds);
+}
+
+// The parts of a tile's rows into one: 32 lanes a row, 8 rows a workgroup.
+__global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkArgs a, const Merge* merges) {
+  const int h = blockIdx.x % a.b.hkv;
+  const Merge g = merges[blockIdx.x / a.b.hkv];
+  const int r = threadIdx.x >> 5, l32 = threadIdx.x & 31;
+  if (g.seq < 0 || g.seq >= a.b.nseq || g.row0 < 0) return;
+  const TileAt at = tile_at(a, g.seq, g.row0, g.rows);
+  if (r >= at.rows || g.slot < 0 || g.slot + (int64_t)(g.parts - 1) * g.stride + r >= a.ws_rows) return;  // (32 lanes agree)
+  const float* base = a.ws + (((int64_t)g.slot + r) * a.b.hkv + h) * CH_PART;
+  const int64_t step = (int64_t)g.stride * a.b.hkv * CH_PART;
+  RowSum sum = {NEG_INF, 0.0f, {0.f, 0.f, 0.f, 0.f}};
+  for (int p = l32; p < g.parts; p += 32) sum.m = fmaxf(sum.m, base[p * step + D]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) sum.m = fmaxf(sum.m, __shfl_xor(sum.m, o, 32));
+  const float mu = sum.m == NEG_INF ? 0.0f : sum.m;
+  for (int p = 0; p < g.parts; ++p) {
+    const float* x = base + p * step;
+    const float2 ml = *reinterpret_cast<const float2*>(x + D);
+    const float4 v = *reinterpret_cast<const float4*>(x + 4 * l32);
+    const float wt = __builtin_amdgcn_exp2f(ml.x - mu);
+    sum.acc.x += v.x * wt; sum.acc.y += v.y * wt; sum.acc.z += v.z * wt; sum.acc.w += v.w * wt;
+    sum.l += ml.y * wt;
+  }
+  const int row = g.row0 + r;
+  write_row(a, h, at.first_token + row / a.gq, row % a.gq, sum, l32);
+}
+
+// ---------------------------------------------------------------- host side
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int batch_args(const char* what, Batch& b, const int32_t* seq_of, bool need_seq_of, const int32_t* cu, const int64_t* start,
+               const int32_t* table, int64_t table_stride, int64_t num_pages, int64_t nseq, int64_t hkv, int64_t head_dim,
+               int64_t tokens) {
+  if (head_dim != D) return fail(NKV_ERR_UNSUPPORTED, "%s: head_dim %lld: the HIP kernels are built for head_dim 128", what, (long long)head_dim);
+  if (nseq <= 0 || nseq > 32767 || hkv <= 0 || hkv > 1024 || table_stride <= 0 || num_pages <= 0 || num_pages > (int64_t(1) << 31))
+    return fail(NKV_ERR_INVALID, "%s: bad sizes nseq=%lld hkv=%lld table_stride=%lld num_pages=%lld", what, (long long)nseq,
+                (long long)hkv, (long long)table_stride, (long long)num_pages);
+  if (tokens < 0 || tokens > (int64_t(1) << 28))
+    return fail(NKV_ERR_INVALID, "%s: %lld tokens outside [0, 2^28]", what, (long long)tokens);
+  if (tokens > 0 && ((need_seq_of && !seq_of) || !cu || !start || !table)) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  b = Batch{seq_of, cu, start, table, table_stride, num_pages, (int)nseq, (int)hkv};
+  return NKV_OK;
+}
+
+template <int DT>
+void launch_append(const AppendArgs& a, hipStream_t s) {
+  const int heads = a.hq + 2 * a.b.hkv;
+  AppendArgs c = a;
+  if (a.tokens >= 4 * CUS) {
+    c.heads_per_wg = heads;
+    hipLaunchKernelGGL((append_chunks_kernel<DT, 4>), dim3((unsigned)cdiv(a.tokens, 4)), dim3(256), 0, s, c);
+  } else {
+    c.heads_per_wg = 16;
+    hipLaunchKernelGGL((append_chunks_kernel<DT, 1>), dim3((unsigned)a.tokens, (unsigned)cdiv(heads, 16)), dim3(256), 0, s, c);
+  }
+}
+
+template <bool T64>
+void launch_read(const ReadArgs& a, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.tokens, READ_TOK));
+  if (dtype == NKV_F16) hipLaunchKernelGGL((read_kernel<NKV_F16, T64>), grid, dim3(256), 0, s, a);
+  else if (dtype == NKV_BF16) hipLaunchKernelGGL((read_kernel<NKV_BF16, T64>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((read_kernel<NKV_F32, T64>), grid, dim3(256), 0, s, a);
+}
+
+int read_tokens(const char* what, bool t64, const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                int64_t num_pages, const uint16_t* rings, const int64_t* length_dev, const int32_t* seq_of,
+                const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq, int64_t hkv, int64_t head_dim,
+                void* k_out, void* v_out, int out_dtype, void* stream) {
+  set_error("");
+  ReadArgs a{};
+  if (int rc = batch_args(what, a.b, seq_of, true, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
+    return rc;
+  if (out_dtype != NKV_F16 && out_dtype != NKV_BF16 && out_dtype != NKV_F32)
+    return fail(NKV_ERR_INVALID, "%s: unknown dtype %d", what, out_dtype);
+  if (tokens == 0) return NKV_OK;
+  if (!pages || !k_out || !v_out || (t64 && (!rings || !length_dev))) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(pages) || !al16(k_out) || !al16(v_out) || (t64 && !al16(rings)))
+    return fail(NKV_ERR_UNSUPPORTED, "%s: buffers must be 16-byte aligned", what);
+  a.tokens = tokens;
+  a.pages = pages; a.rings = rings; a.length = length_dev;
+  a.k_out = static_cast<uint8_t*>(k_out); a.v_out = static_cast<uint8_t*>(v_out);
+  if (t64) launch_read<true>(a, out_dtype, static_cast<hipStream_t>(stream));
+  else launch_read<false>(a, out_dtype, static_cast<hipStream_t>(stream));
+  return check_launch(what);
+}
+
+}  // namespace
+
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens,
+                                           uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                                           int64_t num_pages, const int32_t* seq_of, const int32_t* cu,
+                                           const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv,
+                                           int64_t head_dim, const void* q_gamma, const void* k_gamma, float eps,
+                                           const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream) {
+  set_error("");
+  const char* what = "paged_append_chunks_tok";
+  AppendArgs a{};
+  if (int rc = batch_args(what, a.b, seq_of, true, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
+    return rc;
+  if (qkv_dtype != NKV_F16 && qkv_dtype != NKV_BF16 && qkv_dtype != NKV_F32)
+    return fail(NKV_ERR_INVALID, "%s: unknown dtype %d", what, qkv_dtype);
+  if (hq <= 0 || hq > 16 * hkv || hq % hkv) return fail(NKV_ERR_INVALID, "%s: heads hq=%lld hkv=%lld", what, (long long)hq, (long long)hkv);
+  if (row_stride < (hq + 2 * hkv) * D || q_row_stride < hq * D)
+    return fail(NKV_ERR_INVALID, "%s: row strides %lld and %lld for %lld q and %lld KV heads", what, (long long)row_stride,
+                (long long)q_row_stride, (long long)hq, (long long)hkv);
+  if (tokens == 0) return NKV_OK;
+  if (!qkv || !pages || !q_out || (!q_gamma != !k_gamma)) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(qkv) || !al16(pages) || !al16(q_out) || !al16(q_gamma) || !al16(k_gamma) || row_stride % 8 || q_row_stride % 8)
+    return fail(NKV_ERR_UNSUPPORTED, "%s: rows and buffers must be 16-byte aligned", what);
+  a.x = static_cast<const uint8_t*>(qkv); a.x_rs = row_stride; a.tokens = tokens; a.pages = pages;
+  a.q_gamma = static_cast<const uint8_t*>(q_gamma); a.k_gamma = static_cast<const uint8_t*>(k_gamma);
+  a.eps = eps; a.inv_freq = inv_freq; a.q_out = q_out; a.q_rs = q_row_stride; a.hq = (int)hq;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (qkv_dtype == NKV_F16) launch_append<NKV_F16>(a, s);
+  else if (qkv_dtype == NKV_BF16) launch_append<NKV_BF16>(a, s);
+  else launch_append<NKV_F32>(a, s);
+  return check_launch(what);
+}
+
+extern "C" int nkv_paged_read_tok(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                                  const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t tokens,
+                                  int64_t nseq, int64_t hkv, int64_t head_dim, void* k_out, void* v_out, int out_dtype,
+                                  void* stream) {
+  return read_tokens("paged_read_tok", false, pages, page_table, table_stride, num_pages, nullptr, nullptr, seq_of, cu,
+                     start_dev, tokens, nseq, hkv, head_dim, k_out, v_out, out_dtype, stream);
+}
+
+extern "C" int nkv_paged_read_t64(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                                  const uint16_t* rings, const int64_t* length_dev, const int32_t* seq_of,
+                                  const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq, int64_t hkv,
+                                  int64_t head_dim, void* k_out, void* v_out, int out_dtype, void* stream) {
+  return read_tokens("paged_read_t64", true, pages, page_table, table_stride, num_pages, rings, length_dev, seq_of, cu,
+                     start_dev, tokens, nseq, hkv, head_dim, k_out, v_out, out_dtype, stream);
+}
+
+extern "C" int64_t nkv_paged_chunks_workspace_bytes(int64_t hkv, int64_t partial_rows) {
+  return hkv > 0 && partial_rows > 0 ? partial_rows * hkv * CH_PART * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                                         const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                                         int64_t num_pages, const int32_t* cu, const int64_t* start_dev, int64_t nseq,
+                                         int64_t hq, int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units,
+                                         const int32_t* merges, int64_t n_merges, uint16_t* out, int64_t out_token_stride,
+                                         int64_t out_head_stride, float* lse_out, void* workspace, int64_t workspace_bytes,
+                                         void* stream) {
+  set_error("");
+  const char* what = "paged_attn_chunks_tok";
+  ChunkArgs a{};
+  if (int rc = batch_args(what, a.b, nullptr, false, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
+    return rc;
+  if (hq <= 0 || hq > 16 * hkv || hq % hkv) return fail(NKV_ERR_INVALID, "%s: heads hq=%lld hkv=%lld", what, (long long)hq, (long long)hkv);
+  if (n_units < 0 || n_merges < 0 || n_units * hkv > INT32_MAX || n_merges * hkv > INT32_MAX)
+    return fail(NKV_ERR_INVALID, "%s: %lld units and %lld merges of %lld KV heads", what, (long long)n_units,
+                (long long)n_merges, (long long)hkv);
+  if (tokens == 0 || n_units == 0) return NKV_OK;
+  if (!q || !pages || !units || !out || (n_merges && (!merges || !workspace)))
+    return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(q) || !al16(pages) || !al16(out) || !al16(units) || (n_merges && (!al16(merges) || !al16(workspace))) ||
+      q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
+    return fail(NKV_ERR_UNSUPPORTED, "%s: rows and buffers must be 16-byte aligned", what);
+  a.q = q; a.q_ts = q_token_stride; a.q_hs = q_head_stride; a.tokens = tokens; a.pages = pages;
+  a.units = reinterpret_cast<const Unit*>(units); a.n_units = (int)n_units;
+  a.hq = (int)hq; a.gq = (int)(hq / hkv);
+  a.sl2 = LOG2E / sqrtf((float)D);
+  a.out = out; a.o_ts = out_token_stride; a.o_hs = out_head_stride; a.lse = lse_out;
+  a.ws = static_cast<float*>(workspace);
+  a.ws_rows = workspace && workspace_bytes > 0 ? workspace_bytes / (hkv * CH_PART * (int64_t)sizeof(float)) : 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(attn_chunks_kernel, dim3((unsigned)(n_units * hkv)), dim3(CH_THREADS), 0, s, a);
+  if (int rc = check_launch(what)) return rc;
+  if (n_merges) {
+    hipLaunchKernelGGL(merge_chunks_kernel, dim3((unsigned)(n_merges * hkv)), dim3(256), 0, s, a,
+                       reinterpret_cast<const Merge*>(merges));
+    return check_launch(what);
+  }
+  return NKV_OK;
+}

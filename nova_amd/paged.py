@@ -25,6 +25,10 @@ scales (64 fp16) | V scales = 16640 bytes, 128-byte aligned. It keeps no ring; a
 one launch (``nkv_paged_decode_step_tok``) that stores each sequence's new token into its page and
 attends over ``[0, pos_b]``.
 
+Several tokens per sequence in one step, packed (``nova_amd.chunks``): the per-token format's
+``append_chunks`` (head norms, rotary embedding and quantized store) and ``attend_chunks`` (causal
+attention over the pages); ``read`` brings cached tokens of either format back.
+
 Host bookkeeping (``PagePool``: free pages, reservations, lengths; ``plan_parts``: the prefix
 work plan) is plain Python so that its guards are testable without a GPU.
 """
@@ -34,6 +38,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from . import chunks as C
+from .chunks import ChunkPlan, SpanPlan
 from .kvquant import _DT
 
 D = 128
@@ -221,6 +227,51 @@ class PagedKVInt8Cache:
         self.pool.set_length(b, n)
         self.pos[b] = n
 
+    # ---- cached tokens read back
+
+    def plan_read(self, counts: list[int] | None = None, starts: list[int] | None = None) -> SpanPlan:
+        """Which tokens :meth:`read` takes: ``counts[b]`` tokens of sequence ``b`` from ``starts[b]`` (default
+        0) for sequences ``0 .. len(counts) - 1``; by default everything the sequences have."""
+        if counts is None:
+            n = self.max_seqs if starts is None else len(starts)
+            counts = [self._len[b] - (0 if starts is None else int(starts[b])) for b in range(min(n, self.max_seqs))]
+        counts = C.check_counts(counts, self.max_seqs)
+        starts = [0] * len(counts) if starts is None else C.check_counts(starts, self.max_seqs, "starts")
+        if len(starts) != len(counts):
+            raise ValueError(f"{len(starts)} starts for {len(counts)} counts")
+        for b, (s, n) in enumerate(zip(starts, counts)):
+            if s + n > self._len[b]:
+                raise ValueError(f"sequence {b}: tokens {s} .. {s + n - 1} of {self._len[b]}")
+        return C.span_plan(counts, starts, self.pos.device)
+
+    def read(self, plan: SpanPlan, layer: int, dtype: torch.dtype = torch.float16,
+             out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values of ``plan``'s tokens as ``dtype`` (fp16 / bf16 / fp32), packed
+        ``[tokens, H_kv, 128]``, in one launch: the values that the pages' codes stand for, rounded once (in
+        the int8t64 format a sequence's tokens after its last whole group come from its fp16 ring). A token
+        without a page is 0. ``out``: two contiguous tensors to write instead of new ones; rows after the
+        plan's tokens stay as they are."""
+        if dtype not in _DT:
+            raise ValueError(f"unsupported dtype {dtype}")
+        dev, h = self.pos.device, self.num_kv_heads
+        if out is None:
+            out = tuple(torch.empty((plan.total, h, D), dtype=dtype, device=dev) for _ in range(2))
+        for x in out:
+            if (x.dim() != 3 or x.shape[0] < plan.total or x.shape[1:] != (h, D) or x.dtype != dtype or x.device != dev
+                    or not x.is_contiguous() or x.data_ptr() % 16):
+                raise ValueError(f"out must be two contiguous, 16-byte aligned {dtype} tensors [{plan.total}, {h}, {D}] "
+                                 f"on {dev}")
+        if C.overlap(*out):
+            raise ValueError("the two tensors of out overlap")
+        self._read(plan, layer, dtype, *out)
+        return out
+
+    def _read(self, plan: SpanPlan, layer: int, dtype: torch.dtype, k: torch.Tensor, v: torch.Tensor) -> None:
+        C.launch(self.pos.device, "nkv_paged_read_t64", self.pages[layer].data_ptr(), self.page_table.data_ptr(),
+                 self.page_table.stride(0), self.num_pages, self.rings[layer].data_ptr(), self.pos.data_ptr(),
+                 plan.seq_of.data_ptr(), plan.cu.data_ptr(), plan.starts.data_ptr(), plan.total, plan.nseq,
+                 self.num_kv_heads, D, k.data_ptr(), v.data_ptr(), _DT[dtype])
+
     # ---- work plan of the prefix kernel
 
     def plan(self, lengths: list[int] | None = None) -> None:
@@ -334,3 +385,133 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
                   self.seq_parts.data_ptr(), self.total_parts, self.merged.data_ptr(), self.lse.data_ptr(),
                   self.ws.data_ptr(), self.ws.numel() * 4, _lib.stream_ptr(self.pos.device))
         return self.merged[:self.nseq]
+
+    # ---- steps of several tokens per sequence
+
+    def plan_chunks(self, counts: list[int]) -> ChunkPlan:
+        """Plan a step that brings ``counts[b]`` new tokens (0 or more) for each of the sequences
+        ``0 .. len(counts) - 1``, and reserve their pages. The plan stays valid while the sequences grow (the
+        cut of the attention follows their lengths on the device), for any number of layers and steps that
+        bring the same counts; reserve further pages before further steps."""
+        counts = C.check_counts(counts, self.max_seqs)
+        need = [-(-(self._len[b] + n) // GT) - len(self._owned[b]) for b, n in enumerate(counts)]
+        if sum(n for n in need if n > 0) > len(self._free):
+            raise RuntimeError(f"page pool exhausted: the step needs {sum(n for n in need if n > 0)} more pages, "
+                               f"{len(self._free)} are free")
+        for b, n in enumerate(counts):
+            if self._len[b] + n > self.max_pages_per_seq * GT:
+                raise ValueError(f"sequence {b}: {self._len[b]} + {n} tokens exceed max_pages_per_seq "
+                                 f"{self.max_pages_per_seq}")
+        for b, n in enumerate(counts):
+            if n:
+                self.reserve(b, self._len[b] + n)
+        return C.chunk_plan(counts, self._len[:len(counts)], self.pos, self.num_q_heads // self.num_kv_heads,
+                            self.num_kv_heads)
+
+    def append_chunks(self, plan: ChunkPlan, qkv: torch.Tensor, layer: int, q_gamma: torch.Tensor | None = None,
+                      k_gamma: torch.Tensor | None = None, eps: float = 1e-6, inv_freq: torch.Tensor | None = None,
+                      q_out: torch.Tensor | None = None) -> torch.Tensor:
+        """Store the new tokens' keys and values in their pages and return their queries, in one launch.
+
+        ``qkv``: the stacked projections ``[tokens, (H_q + 2 H_kv) * 128]`` (q heads, k heads, v heads; fp16 /
+        bf16 / fp32, unit element stride). With ``q_gamma`` / ``k_gamma`` (``[128]``, of qkv's type) each q and
+        k head gets its RMSNorm, with ``inv_freq`` (fp32 ``[64]``) the rotary embedding at the token's own
+        position (element i with i + 64). All of it in fp32, rounded once: q to fp16, K and V to the codes and
+        scales of ``quantize_tok``. A token whose page is missing is not stored. Returns fp16 ``[tokens, H_q,
+        128]``, or writes ``q_out``, which may be qkv's own q heads; rows after the plan's tokens are neither
+        read nor written."""
+        hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
+        if (qkv.dim() != 2 or qkv.shape[0] < total or qkv.shape[1] != (hq + 2 * hkv) * D or qkv.dtype not in _DT
+                or qkv.device != dev):
+            raise ValueError(f"qkv must be fp16 / bf16 / fp32 [{total}, {(hq + 2 * hkv) * D}] on {dev} (more tokens may "
+                             f"follow), got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
+        if (q_gamma is None) != (k_gamma is None):
+            raise ValueError("q_gamma and k_gamma come together")
+        if q_gamma is not None:
+            for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+                if t.dtype != qkv.dtype or t.numel() != D or not t.is_contiguous() or t.device != dev or t.data_ptr() % 16:
+                    raise ValueError(f"{name} must be a contiguous, 16-byte aligned {qkv.dtype} tensor of {D} elements on {dev}")
+        if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2
+                                     or not inv_freq.is_contiguous() or inv_freq.device != dev):
+            raise ValueError(f"inv_freq must be a contiguous fp32 tensor of {D // 2} elements on {dev}")
+        given = qkv
+        if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16 or (qkv.stride(0) < qkv.shape[1] and qkv.shape[0] > 1):
+            qkv = qkv.contiguous()
+        if q_out is None:
+            q_out = torch.empty((total, hq, D), dtype=torch.float16, device=dev)
+        else:
+            C.heads_of(q_out, "q_out", total, hq, dev)
+            if q_out.stride(1) != D or not C.rows_in_place(q_out) or not C.distinct_rows(q_out):
+                raise ValueError("q_out: a token's heads must be contiguous and its row 16-byte aligned")
+            own_rows = (given is qkv and q_out.data_ptr() == qkv.data_ptr() and q_out.dtype == qkv.dtype
+                        and (q_out.stride(0) == qkv.stride(0) or total <= 1))
+            if not own_rows and C.overlap(q_out, given):
+                raise ValueError("q_out must be qkv's q heads themselves or not overlap qkv")
+        C.launch(dev, "nkv_paged_append_chunks_tok", qkv.data_ptr(), _DT[qkv.dtype], max(qkv.stride(0), qkv.shape[1]), total,
+                 self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
+                 plan.seq_of.data_ptr(), plan.cu.data_ptr(), plan.starts.data_ptr(), plan.nseq, hq, hkv, D,
+                 _lib.ptr(q_gamma), _lib.ptr(k_gamma), float(eps), _lib.ptr(inv_freq), q_out.data_ptr(),
+                 max(q_out.stride(0), hq * D))
+        return q_out
+
+    def attend_chunks(self, plan: ChunkPlan, query: torch.Tensor, layer: int, out: torch.Tensor | None = None,
+                      lse: torch.Tensor | None = None) -> torch.Tensor:
+        """Causal attention of the new tokens over their sequences' pages, the step's own keys and values
+        among them (``append_chunks`` runs first): the token at position p attends ``[0, p]``.
+
+        ``query`` fp16 ``[tokens, H_q, 128]`` (any token and head strides; rows that do not start on 16 bytes are
+        copied). Returns ``out``, fp16 of the same shape (strides as query's), which must not overlap ``query``;
+        ``lse`` (fp32 ``[tokens, H_q]``, contiguous) receives the log-sum-exp of the scaled scores. Groups
+        without a page take no part; a token with none gets 0 and -inf. Rows after the plan's tokens are neither
+        read nor written. Calls may overlap on streams (each has its own scratch memory)."""
+        hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
+        C.heads_of(query, "query", total, hq, dev)
+        if not C.rows_in_place(query):
+            query = query.contiguous()
+        if out is None:
+            out = torch.empty((total, hq, D), dtype=torch.float16, device=dev)
+        else:
+            C.heads_of(out, "out", total, hq, dev)
+            if not C.rows_in_place(out) or not C.distinct_rows(out):
+                raise ValueError("out: rows of 128 elements, apart from each other, must start on 16 bytes")
+            if C.overlap(out, query):
+                raise ValueError("out must not overlap query")
+        if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] < total or lse.shape[1] != hq
+                                or not lse.is_contiguous() or lse.device != dev):
+            raise ValueError(f"lse must be a contiguous fp32 tensor [{total}, {hq}] on {dev}")
+        ws = _lib.scratch(dev, plan.ws_bytes) if plan.ws_bytes else None
+        C.launch(dev, "nkv_paged_attn_chunks_tok", query.data_ptr(), query.stride(0), query.stride(1), total,
+                 self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
+                 plan.cu.data_ptr(), plan.starts.data_ptr(), plan.nseq, hq, hkv, D, plan.units.data_ptr(),
+                 plan.units.shape[0], plan.merges.data_ptr(), plan.merges.shape[0], out.data_ptr(), out.stride(0),
+                 out.stride(1), _lib.ptr(lse), _lib.ptr(ws), plan.ws_bytes)
+        return out
+
+    def advance_chunks(self, plan: ChunkPlan, accepted: list[int] | None = None) -> None:
+        """``pos`` moves past the step's tokens, or past the first ``accepted[b]`` of each sequence's (drafted
+        tokens that were kept; the others' places are written again). Refuses a step whose pages are not
+        reserved."""
+        self.note_chunks(plan, 1, accepted)
+        if accepted is None:
+            self.pos[:plan.nseq].add_(plan.new)
+        else:
+            self.pos[:plan.nseq].add_(torch.tensor([int(n) for n in accepted], dtype=torch.int64).to(self.pos.device))
+
+    def note_chunks(self, plan: ChunkPlan, steps: int = 1, accepted: list[int] | None = None) -> None:
+        """Host bookkeeping of ``steps`` steps that advanced ``pos`` on the device (:meth:`advance_chunks`, or a
+        replayed graph that adds ``plan.new`` to ``pos[:plan.nseq]``)."""
+        moved = plan.counts if accepted is None else C.check_counts(accepted, self.max_seqs, "accepted")
+        if len(moved) != plan.nseq or any(a > n for a, n in zip(moved, plan.counts)):
+            raise ValueError(f"accepted {moved} of a step of {plan.counts}")
+        for b, n in enumerate(moved):
+            if n and (self._len[b] + n * int(steps) - 1) // GT >= len(self._owned[b]):
+                raise RuntimeError(f"sequence {b}: {n * int(steps)} more tokens after {self._len[b]}, but only "
+                                   f"{len(self._owned[b])} pages reserved; reserve() more first")
+        for b, n in enumerate(moved):
+            self.pool.set_length(b, self._len[b] + n * int(steps))
+
+    def _read(self, plan: SpanPlan, layer: int, dtype: torch.dtype, k: torch.Tensor, v: torch.Tensor) -> None:
+        C.launch(self.pos.device, "nkv_paged_read_tok", self.pages[layer].data_ptr(), self.page_table.data_ptr(),
+                 self.page_table.stride(0), self.num_pages, plan.seq_of.data_ptr(), plan.cu.data_ptr(),
+                 plan.starts.data_ptr(), plan.total, plan.nseq, self.num_kv_heads, D, k.data_ptr(), v.data_ptr(),
+                 _DT[dtype])
