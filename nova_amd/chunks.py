@@ -23,9 +23,11 @@ from . import _lib
 D, GT = 128, 64
 CUS = 256        # compute units of an MI355X: one attention workgroup each at a time
 UNIT_INTS = 8    # int32 words of a work unit and of a merge entry
-ROWS16, ROWS32 = 0, 1  # unit kinds
-TILE_ROWS = {ROWS16: 16, ROWS32: 32}  # query rows (tokens x q heads per KV head) of a tile, at most
+ROWS16, ROWS32, ROWS256 = 0, 1, 2  # unit kinds
+TILE_ROWS = {ROWS16: 16, ROWS32: 32, ROWS256: 256}  # query rows (tokens x q heads per KV head) of a tile, at most
 MAX_PARTS = 256
+BIG_FROM = 64    # rows of a sequence from which its tiles are ROWS256
+STEP_COST = {ROWS16: 1, ROWS32: 1, ROWS256: 2}
 MERGE_ROWS = 8   # rows a merge entry covers
 
 
@@ -72,18 +74,21 @@ def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarra
     Cut tiles leave one partial per row and part, which the merge entries ``(sequence, first row,
     rows, parts, slot, slots from part to part, 0, 0)`` join, eight rows each. The longest units
     come first."""
-    tiles = []  # (steps, sequence, first row, rows, kind)
+    tiles = []  # (steps, cost of a step, sequence, first row, rows, kind)
     for b, (start, n) in enumerate(zip(starts, counts)):
-        for row0 in range(0, n * gq, 32):
-            rows = min(32, n * gq - row0)
+        big = n * gq > BIG_FROM
+        size = TILE_ROWS[ROWS256 if big else ROWS32]
+        for row0 in range(0, n * gq, size):
+            rows = min(size, n * gq - row0)
             steps = (start + (row0 + rows - 1) // gq) // GT + 1
-            tiles.append((steps, b, row0, rows, ROWS16 if rows <= 16 else ROWS32))
-    target = max(8, -(-sum(t[0] for t in tiles) * hkv // CUS))
+            kind = ROWS256 if big else ROWS16 if rows <= 16 else ROWS32
+            tiles.append((steps, STEP_COST[kind], b, row0, rows, kind))
+    target = max(8, -(-sum(t[0] * t[1] for t in tiles) * hkv // CUS))
     units, merges, slot = [], [], 0
-    for steps, b, row0, rows, kind in tiles:
-        parts = min(MAX_PARTS, -(-steps // target))
+    for steps, cost, b, row0, rows, kind in tiles:
+        parts = min(MAX_PARTS, -(-steps * cost // target))
         for p in range(parts):
-            units.append((-(-steps // parts), b, row0, rows, p, parts, slot, kind, 0))
+            units.append((-(-steps * cost // parts), b, row0, rows, p, parts, slot, kind, 0))
         if parts > 1:
             for r in range(0, rows, MERGE_ROWS):
                 merges.append((b, row0 + r, min(MERGE_ROWS, rows - r), parts, slot + r, rows, 0, 0))

@@ -9,7 +9,7 @@
 // Token t of the packed batch belongs to sequence seq_of[t] and is its new token t - cu[seq]; its position is
 // start[seq] + that. Lengths and positions are read on the device, so a captured graph follows them.
 
-#include <algorithm>
+#include <type_traits>
 
 #include "nkv_mfma.h"
 
@@ -318,7 +318,7 @@ static_assert(CODE_BYTES + CH_VSLOT == PAGE_TOK_BYTES, "a page is K codes and a 
 static_assert(16 * CH_PART * 4 <= CH_VSLOT, "a wave's 16 rows fit one of its slots at the merge");
 constexpr int CH_LDS = 2 * CH_WAVES * CH_VSLOT;          // 132 KiB: two slots a wave
 
-enum UnitKind : int { ROWS16 = 0, ROWS32 = 1 };
+enum UnitKind : int { ROWS16 = 0, ROWS32 = 1, ROWS256 = 2 };
 
 struct Unit {  // (int32 each, as the plan lays them out)
   int seq, row0, rows, part, parts, slot, kind, pad;  // slot: partial row of part 0 of the tile
@@ -375,6 +375,32 @@ __device__ __forceinline__ void write_row(const ChunkArgs& a, int h, int64_t tok
     a.lse[token * a.hq + i] = r.l == 0.0f ? NEG_INF : (r.m + __builtin_amdgcn_logf(r.l) - (15.0f - PF_TAU)) * LN2;
 }
 
+// The pages of a wave's groups first, first + stride, .., n of them, held 64 at a time, one a lane. (Scalar loads
+// of the table would share their counter with LDS: every wait for an operand would be one for the table, too.)
+struct Pages {
+  const int32_t* row;
+  int64_t num_pages;
+  int stride, n, base;
+  int page;  // lane l: that of group base + l, -1: none
+  __device__ __forceinline__ Pages(const Batch& b, int seq, int64_t first, int stride_, int n_)
+      : row(b.table + (int64_t)seq * b.table_stride + first), num_pages(b.num_pages), stride(stride_), n(n_), base(0) {
+    fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    const int i = base + ((int)threadIdx.x & 63);
+    page = i < n ? row[(int64_t)i * stride] : -1;
+    if (page >= num_pages) page = -1;
+  }
+  // i: not decreasing from call to call
+  __device__ __forceinline__ int at(int i) {
+    if (i >= base + 64) {
+      base = i;
+      fetch();
+    }
+    return __builtin_amdgcn_readlane(page, i - base);
+  }
+};
+
 __device__ __forceinline__ bool finite_h(uint32_t bits) { return (bits & 0x7c00u) != 0x7c00u; }
 
 template <int RB>
@@ -388,7 +414,7 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_TOK_BYTES;
 
   uint4 kn[4][2];  // the next group's K codes: token 16 b + c, bytes 16 g + 64 hh ..
-  auto issue = [&](int64_t page, int sb) {
+  auto issue = [&](int page, int sb) {
     const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride));
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -406,9 +432,10 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   };
 
   int64_t s = s0 + wave;
-  int64_t page = s < s1 ? page_at(a.b, u.seq, s) : -1;
+  const int mine = s < s1 ? (int)((s1 - s + CH_WAVES - 1) / CH_WAVES) : 0;  // groups of this wave
+  Pages pg(a.b, u.seq, s, CH_WAVES, mine);
+  int page = pg.at(0);
   if (page >= 0) issue(page, 0);
-  int64_t next_page = s + CH_WAVES < s1 ? page_at(a.b, u.seq, s + CH_WAVES) : -1;
 
   half8_t qb[RB][4];
   int64_t tq[RB];  // the last position that row c attends
@@ -437,7 +464,8 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     lsum[rb] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int sb = 0; s < s1; s += CH_WAVES, sb ^= 1) {
+  for (int t = 0; t < mine; ++t, s += CH_WAVES) {
+    const int sb = t & 1;
     const bool here = page >= 0;
     uint4 kc[4][2];
     wait_groups_all();
@@ -445,9 +473,8 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) kc[b][hh] = kn[b][hh];
-    page = next_page;
+    page = pg.at(t + 1);
     if (page >= 0) issue(page, sb ^ 1);
-    next_page = s + 2 * CH_WAVES < s1 ? page_at(a.b, u.seq, s + 2 * CH_WAVES) : -1;
     if (!here) continue;  // a group without a page takes no part
 
     const uint8_t* slot = lds + (2 * wave + sb) * CH_VSLOT;
@@ -535,16 +562,16 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   // ---- the waves' states into one, row by row
   wait_groups_all();
   __syncthreads();  // every wave is done with its slots
-  float* mine = reinterpret_cast<float*>(lds) + wave * (RB * 16 * CH_PART);
+  float* state = reinterpret_cast<float*>(lds) + wave * (RB * 16 * CH_PART);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    if (g == 0) mine[(16 * rb + c) * CH_PART + D] = st[rb].m;
+    if (g == 0) state[(16 * rb + c) * CH_PART + D] = st[rb].m;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * rb + 4 * g + i;
-      if (c == 0) mine[r * CH_PART + D + 1] = lsum[rb][i];
+      if (c == 0) state[r * CH_PART + D + 1] = lsum[rb][i];
 #pragma unroll
-      for (int cb = 0; cb < 8; ++cb) mine[r * CH_PART + 16 * cb + c] = st[rb].acc[cb][i];
+      for (int cb = 0; cb < 8; ++cb) state[r * CH_PART + 16 * cb + c] = st[rb].acc[cb][i];
     }
   }
   __syncthreads();
@@ -571,10 +598,302 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
       write_row(a, h, at.first_token + row / a.gq, row % a.gq, sum, l32);
     } else {
       const int64_t pr = (int64_t)u.slot + (int64_t)u.part * u.rows + r;
-      if (pr < 0 || pr >= a.ws_rows) continue;
+      if (pr >= a.ws_rows) continue;
       float* dst = a.ws + (pr * a.b.hkv + h) * CH_PART;
       *reinterpret_cast<float4*>(dst + 4 * l32) = sum.acc;
       if (l32 == 0) *reinterpret_cast<float2*>(dst + D) = float2{sum.m, sum.l};
+    }
+  }
+}
+
+// Units of up to 256 rows (BIG): wave w takes rows 32 w .. 32 w + 31 as two row blocks, and every wave every
+// group. The waves turn a group's codes once into fp16 LDS tiles, fp16(code * scale) as the format defines a value: K
+// row-major (rows of 256 bytes, their 16-byte chunk x at x ^ (row & 15)), V transposed in the tokens' order of P's
+// operand (rows of 128 bytes, chunk x at x ^ (row & 7)).
+// One barrier a step: in step t, before it, the conversion of group t + 1 into the tiles that step t - 1 read and the
+// wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
+constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
+constexpr int BG_KT = BG_STAGES * PAGE_TOK_BYTES, BG_VT = BG_KT + 2 * GT * D * 2, BG_LDS = BG_VT + 2 * GT * D * 2;
+static_assert(BG_LDS <= CH_LDS, "both kinds of unit share the LDS");
+static_assert(BG_ROWS * D * 2 <= BG_LDS, "the output of a tile fits");
+// instruction classes of __builtin_amdgcn_sched_group_barrier
+constexpr int SG_VALU = 0x2, SG_MFMA = 0x8, SG_DSR = 0x100;
+#ifndef BG_VPM
+#define BG_VPM 2
+#endif
+
+__device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
+  const int s0 = (int)(at.steps * u.part / u.parts), n = (int)(at.steps * (u.part + 1) / u.parts) - s0;
+  const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);
+  const uint8_t* pages = a.pages + (int64_t)h * PAGE_TOK_BYTES;
+  const int64_t page_stride = (int64_t)a.b.hkv * PAGE_TOK_BYTES;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+  Pages pg(a.b, u.seq, s0, 1, n);
+  // wave w's loads of a group: K and V rows 8 w .. 8 w + 7, wave 0 the scales, too
+  const int own_loads = wave == 0 ? 3 : 2;
+  int loads = 0;  // in flight of the newest group
+  auto issue = [&](int page, int slot) {
+    loads = 0;
+    if (page < 0) return;
+    loads = own_loads;
+    const void* p = uniform_ptr(pages + page * page_stride);
+    const uint32_t dst = base + slot * PAGE_TOK_BYTES;
+    const int row = 8 * wave + (lane >> 3);
+    const uint32_t off = (uint32_t)(row * D + (((lane & 7) ^ swz(row)) << 4));
+    dma16(p, off, dst + 1024 * wave);
+    dma16(p, off + CODE_BYTES, dst + CODE_BYTES + 1024 * wave);
+    if (wave == 0 && lane < 16) dma16(p, (uint32_t)(2 * CODE_BYTES + 16 * lane), dst + 2 * CODE_BYTES);
+  };
+  // steps that some row of the tile does not see whole: masked places may hold anything there (attend_small)
+  const int tile_whole = (int)((at.start + u.row0 / a.gq + 1) / GT) - s0;
+  // Group t from its stage into its tiles: lane l of wave w takes K row l, dims 16 w .. + 15, and V dims 16 w .. + 15.
+  // `check`: with the rules for masked places; `here`: the group has a page.
+  auto convert = [&](int t, int slot, auto check, bool here) {
+    const uint8_t* sg = lds + slot * PAGE_TOK_BYTES;
+    const uint8_t* sc = sg + 2 * CODE_BYTES;
+    const int r = c >> 1;
+    const uint4 kw = *reinterpret_cast<const uint4*>(sg + lane * D + ((wave ^ swz(lane)) << 4));
+    uint32_t ks = *reinterpret_cast<const uint16_t*>(sc + 2 * lane);
+    u32x2 vw[2];
+    uint2 vs[2][2];
+#pragma unroll
+    for (int B = 0; B < 2; ++B) {
+      const int vrow = 16 * (2 * B + (r >> 2)) + 4 * g + (r & 3);
+      vw[B] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (lds_v2i_t*)(const lds_void_t*)(sg + CODE_BYTES + vrow * D + 8 * (c & 1) + ((wave ^ swz(vrow)) << 4))));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) vs[B][e] = *reinterpret_cast<const uint2*>(sc + 2 * GT + 2 * (32 * B + 16 * e + 4 * g));
+    }
+    if constexpr (decltype(check)::value) {
+      if (!finite_h(*reinterpret_cast<const uint16_t*>(sc + 2 * GT + 2 * lane))) ks = 0x7e00u;  // NaN
+#pragma unroll
+      for (int B = 0; B < 2; ++B)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w[2] = {vs[B][e].x, vs[B][e].y};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t tok = (int64_t)(s0 + t) * GT + 32 * B + 16 * e + 4 * g + i;
+            const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+            if (!here || !finite_h(x) || tok >= len) w[i >> 1] &= (i & 1) ? 0xffffu : 0xffff0000u;
+          }
+          vs[B][e] = uint2{w[0], w[1]};
+        }
+    }
+    uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + lane * (2 * D);
+    uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + (16 * wave + c) * (2 * GT);
+    const half2_t s = as_h2(ks | (ks << 16));
+    const half8_t k0 = dq8_sym(kw.x, kw.y, s), k1 = dq8_sym(kw.z, kw.w, s);
+    *reinterpret_cast<half8_t*>(kt + (((2 * wave) ^ (lane & 15)) << 4)) = k0;
+    *reinterpret_cast<half8_t*>(kt + (((2 * wave + 1) ^ (lane & 15)) << 4)) = k1;
+#pragma unroll
+    for (int B = 0; B < 2; ++B)
+      *reinterpret_cast<half8_t*>(vt + (((4 * B + g) ^ (c & 7)) << 4)) =
+          dq8_sym_v(vw[B].x, vw[B].y, uint4{vs[B][0].x, vs[B][0].y, vs[B][1].x, vs[B][1].y});
+  };
+
+  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
+  issue(p0, 0);
+  issue(p1, 1);
+
+  const int row0 = u.row0 + wave * (BG_RB * 16);  // first row of this wave
+  const int rows = u.row0 + at.rows;
+  half8_t qb[BG_RB][4];
+#pragma unroll
+  for (int rb = 0; rb < BG_RB; ++rb) {
+    const int row = row0 + 16 * rb + c;
+    const bool ok = row < rows;
+    const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
+    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 w = {0, 0, 0, 0};
+      if (ok) w = *reinterpret_cast<const uint4*>(qr + 16 * g + 64 * (k >> 1) + 8 * (k & 1));
+      qb[rb][k] = as_h8(w);
+    }
+  }
+  const _Float16 one = (_Float16)1.0f;
+  const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
+  WaveState st[BG_RB];
+  float4_t lsum[BG_RB];
+#pragma unroll
+  for (int rb = 0; rb < BG_RB; ++rb) {
+    state_init(st[rb]);
+    lsum[rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // this wave's rows attend steps t < mine
+  const int last = min(row0 + BG_RB * 16, rows) - 1;
+  const int mine = row0 < rows ? min(n, (int)((at.start + last / a.gq) / GT) + 1 - s0) : 0;
+
+  half8_t op[16];  // the operands of the products: K's, then V's
+  auto load_k = [&](int t) {
+    const uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + c * (2 * D);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        op[4 * k + b] = *reinterpret_cast<const half8_t*>(kt + 16 * b * (2 * D) + (((2 * g + 8 * (k >> 1) + (k & 1)) ^ c) << 4));
+  };
+  auto load_v = [&](int t) {
+    const uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + c * (2 * GT);
+#pragma unroll
+    for (int B = 0; B < 2; ++B)
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb)
+        op[8 * B + cb] = *reinterpret_cast<const half8_t*>(vt + 16 * cb * (2 * GT) + (((4 * B + g) ^ (c & 7)) << 4));
+  };
+  float4_t S[BG_RB][4];
+  half8_t ph[BG_RB][2];
+  float alpha[BG_RB];
+  bool moved[BG_RB];
+  auto qk = [&](int rb) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        S[rb][b] = mfma32(op[4 * k + b], qb[rb][k], k ? S[rb][b] : float4_t{0.f, 0.f, 0.f, 0.f});
+  };
+  auto softmax = [&](int rb, auto masked, int t) {
+    float sc[4][4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[b][i] = S[rb][b][i];
+    if constexpr (decltype(masked)::value) {
+      const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * g;  // (near the sequence's end: fits)
+      const int tq = (row0 + 16 * rb + c) / a.gq;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (tok0 + 16 * b + i > tq) sc[b][i] = NEG_INF;
+    }
+    pf_softmax(st[rb], sc, a.sl2, ph[rb], alpha[rb], moved[rb]);
+    asm volatile("" : "+v"(ph[rb][0]), "+v"(ph[rb][1]));  // (P is made here, not sunk past the rescale)
+  };
+  auto rescale = [&](int rb) {
+    if (__builtin_amdgcn_ballot_w64(moved[rb]) == 0) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float ai = shfl(alpha[rb], 4 * g + i);
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb][i] *= ai;
+      lsum[rb][i] *= ai;
+    }
+  };
+  auto pv = [&](int rb) {
+#pragma unroll
+    for (int B = 0; B < 2; ++B) {
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb] = mfma32(ph[rb][B], op[8 * B + cb], st[rb].acc[cb]);
+      lsum[rb] = mfma32(ph[rb][B], ones, lsum[rb]);
+    }
+  };
+
+  wait_groups_all();
+  __syncthreads();
+  if (n > 0) convert(0, 0, std::true_type{}, p0 >= 0);
+  __syncthreads();
+  issue(p2, 2);
+  issue(p3, 0);
+  int r1 = 1;  // (t + 1) mod 3
+
+  // One step. `fast`: every row sees groups t and t + 1 whole, and both have a page. A wave issues in order, so
+  // the products of one row block are placed between the softmax instructions of the other: QK(1) beside softmax(0),
+  // PV(0) beside softmax(1), PV(1) beside the conversion.
+  auto step = [&](int t, auto fast_) {
+    constexpr bool fast = decltype(fast_)::value;
+    using masked = std::integral_constant<bool, !fast>;
+    const int p4 = pg.at(t + 4);
+    const bool go = fast || (t < mine && p0 >= 0);
+    if (go) {
+      load_k(t);
+      qk(0);
+      __builtin_amdgcn_sched_barrier(0);
+      qk(1);
+      softmax(0, masked{}, t);
+      if constexpr (fast) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(SG_VALU, BG_VPM, 0);
+        }
+      }
+      rescale(0);
+      load_v(t);
+      pv(0);
+      softmax(1, masked{}, t);
+      if constexpr (fast) {
+        __builtin_amdgcn_sched_group_barrier(SG_DSR, 16, 1);
+#pragma unroll
+        for (int i = 0; i < 18; ++i) {
+          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(SG_VALU, BG_VPM, 1);
+        }
+      }
+      rescale(1);
+    }
+    if constexpr (fast) convert(t + 1, r1, std::false_type{}, true);
+    else if (t + 1 < n) convert(t + 1, r1, std::true_type{}, p1 >= 0);
+    if (go) pv(1);
+    // tile t + 1 is written, tile t is read, group t + 2 has landed
+    if (loads == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
+    else if (loads == 3) asm volatile("s_waitcnt vmcnt(3) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    issue(p4, r1);
+    r1 = r1 == 2 ? 0 : r1 + 1;
+    p0 = p1; p1 = p2; p2 = p3; p3 = p4;
+  };
+  int t = 0;
+  for (; t + 1 < min(n, tile_whole) && p0 >= 0 && p1 >= 0; ++t) step(t, std::true_type{});
+  for (; t < n; ++t) step(t, std::false_type{});
+  wait_groups_all();
+
+  if (u.parts == 1) {
+    // ---- out = acc / l (both x 2^15 - PF_TAU), through LDS so that 16 lanes store a row's 256 bytes (the 2-byte values
+    // at chunk ^ 2 ((row >> 2) & 3))
+    __syncthreads();  // every wave is past its last read of the tiles
+    uint8_t* ow = lds + wave * (BG_RB * 16 * D * 2);
+#pragma unroll
+    for (int rb = 0; rb < BG_RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float l = lsum[rb][i], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, m = shfl(st[rb].m, 4 * g + i);
+        const int r = 16 * rb + 4 * g + i, row = row0 + r;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb)
+          *reinterpret_cast<uint16_t*>(ow + r * (2 * D) + (((2 * cb + (c >> 3)) ^ (((r >> 2) & 3) << 1)) << 4) + 2 * (c & 7)) =
+              f2h(st[rb].acc[cb][i] * inv);
+        if (a.lse && c == 0 && row < rows)
+          a.lse[(at.first_token + row / a.gq) * a.hq + h * a.gq + row % a.gq] =
+              l == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(l) - (15.0f - PF_TAU)) * LN2;
+      }
+#pragma unroll
+    for (int k = 0; k < BG_RB * 4; ++k) {
+      const int r = 4 * k + g, row = row0 + r;
+      const uint4 v = *reinterpret_cast<const uint4*>(ow + r * (2 * D) + ((c ^ (((r >> 2) & 3) << 1)) << 4));
+      if (row < rows)
+        *reinterpret_cast<uint4*>(a.out + (at.first_token + row / a.gq) * a.o_ts + (h * a.gq + row % a.gq) * a.o_hs + 8 * c) = v;
+    }
+  } else {
+    const int64_t pr0 = (int64_t)u.slot + (int64_t)u.part * u.rows + wave * (BG_RB * 16);
+#pragma unroll
+    for (int rb = 0; rb < BG_RB; ++rb) {
+      if (g == 0 && row0 + 16 * rb + c < rows && pr0 + 16 * rb + c < a.ws_rows)
+        a.ws[((pr0 + 16 * rb + c) * a.b.hkv + h) * CH_PART + D] = st[rb].m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * rb + 4 * g + i;
+        if (row0 + r >= rows || pr0 + r >= a.ws_rows) continue;
+        float* dst = a.ws + ((pr0 + r) * a.b.hkv + h) * CH_PART;
+        if (c == 0) dst[D + 1] = lsum[rb][i];
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) dst[16 * cb + c] = st[rb].acc[cb][i];
+      }
     }
   }
 }
@@ -583,8 +902,12 @@ __global__ __launch_bounds__(CH_THREADS, 1) void attn_chunks_kernel(ChunkArgs a)
   __shared__ __attribute__((aligned(16))) uint8_t lds[CH_LDS];
   const int h = blockIdx.x % a.b.hkv;
   const Unit u = a.units[blockIdx.x / a.b.hkv];
-  if (u.seq < 0 || u.seq >= a.b.nseq || u.row0 < 0 || u.rows <= 0 || u.rows > 32 || u.part < 0 || u.part >= u.parts) return;
-  if (u.kind == ROWS16 && u.rows <= 16) attend_small<1>(a, u, h, lds);
+  if (u.seq < 0 || u.seq >= a.b.nseq || u.row0 < 0 || u.rows <= 0 || u.rows > BG_ROWS || u.part < 0 || u.part >= u.parts ||
+      u.slot < 0)
+    return;
+  if (u.kind == ROWS256) attend_big(a, u, h, lds);
+  else if (u.rows > 32) return;
+  else if (u.rows <= 16) attend_small<1>(a, u, h, lds);
   else attend_small<2>(a, u, h, lds);
 }
 
