@@ -96,11 +96,17 @@ struct Raw8 {  // eight consecutive values as loaded
   }
 };
 
-template <int DT>
+template <bool NT>
+__device__ __forceinline__ void store16(uint8_t* p, u32x4_t w) {
+  if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
+  else *reinterpret_cast<u32x4_t*>(p) = w;
+}
+template <int DT, bool NT>
 __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
   if constexpr (DT == NKV_F32) {
-    *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<float4*>(p + 16) = float4{v[4], v[5], v[6], v[7]};
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      store16<NT>(p + 4 * i, u32x4_t{__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])});
   } else {
     uint32_t u[4];
 #pragma unroll
@@ -109,7 +115,7 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
       const uint32_t hi = DT == NKV_F16 ? f2h(v[2 * i + 1]) : f2bf(v[2 * i + 1]);
       u[i] = lo | (hi << 16);
     }
-    *reinterpret_cast<uint4*>(p) = uint4{u[0], u[1], u[2], u[3]};
+    store16<NT>(p, u32x4_t{u[0], u[1], u[2], u[3]});
   }
 }
 
@@ -143,22 +149,31 @@ struct AppendArgs {
   int hq, heads_per_wg;
 };
 
-// One head row of 128 values to 16 lanes, 8 values each; 16 rows at a time in a workgroup, which takes TOK
-// tokens and heads_per_wg of their hq + 2 hkv heads. Everything in fp32, rounded once (q to fp16, k and v to
-// codes). The angle position * inv_freq is exact in fp64 and reduced there to a part of a turn, so that far
-// positions lose nothing; one lane computes it for each token and frequency, for all heads.
-template <int DT, int TOK>
+// A workgroup takes one token and heads_per_wg of its hq + 2 hkv heads: a head row of 128 values to 16 lanes, 8
+// values each, 16 rows at a time. Everything in fp32, rounded once (q to fp16, k and v to codes). The angle position *
+// inv_freq is exact in fp64 and reduced there to a part of a turn, so that far positions lose nothing; one lane
+// computes it for each frequency, for all heads. The rows ahead are loaded while one is worked on, the first ones
+// before the angles and the page are known.
+// Bound by memory: 4112 tokens of 32 q and 8 KV heads (93 MB) in 23 us, 4.0 TB/s. Two or four tokens a workgroup
+// (the angles of four take all its lanes) take as long or longer (4: 25 us; 1029 tokens of 28 + 4 heads 7.3 against
+// 10 us: too few workgroups). NT: nontemporal q stores, for calls whose queries no L2 would hold until they are
+// read (4112 tokens: 2 us less).
+template <int DT, bool NT>
 __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
-  __shared__ float2 turn[TOK][D / 2];  // cos, sin
-  __shared__ int64_t row_of[TOK];      // byte offset of the token's row 0 of its page (KV head 0), or -1
-  __shared__ int slot_of[TOK];
+  __shared__ __attribute__((aligned(16))) float turn[2][D / 2];  // cos, sin
+  __shared__ int64_t row_of;  // byte offset of KV head 0's page, or -1
+  __shared__ int slot_of;
   const int tid = threadIdx.x, j = tid & 15, first = tid >> 4;
-  const int64_t t0 = (int64_t)blockIdx.x * TOK;
-  const int heads = a.hq + 2 * a.b.hkv, h0 = blockIdx.y * a.heads_per_wg;
-  const int nh = min(a.heads_per_wg, heads - h0), nt = (int)min<int64_t>(TOK, a.tokens - t0);
+  const int64_t t = blockIdx.x;
+  const int heads = a.hq + 2 * a.b.hkv, h0 = blockIdx.y * a.heads_per_wg, h1 = min(h0 + a.heads_per_wg, heads);
   const bool norm = a.q_gamma != nullptr, rotate = a.inv_freq != nullptr;
-  constexpr int SIZE = Elem<DT>::SIZE;
+  constexpr int SIZE = Elem<DT>::SIZE, AHEAD = DT == NKV_F32 ? 2 : 4;
 
+  const uint8_t* x = a.x + (t * a.x_rs + 8 * j) * SIZE;
+  Raw8<DT> ahead[AHEAD];
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e)
+    if (h0 + first + 16 * e < h1) ahead[e].load(x + (int64_t)(h0 + first + 16 * e) * (D * SIZE));
   float gq[8], gk[8];
   if (norm) {
     Raw8<DT> r;
@@ -167,59 +182,64 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
     r.load(a.k_gamma + 8 * j * SIZE);
     r.get(gk);
   }
-  if (tid < TOK * (D / 2)) {
-    const int k = tid / (D / 2), f = tid % (D / 2);
-    if (k < nt) {
-      const TokenAt at = token_at(a.b, t0 + k);
-      if (f == 0) {
-        row_of[k] = at.page < 0 ? -1 : at.page * a.b.hkv * (int64_t)PAGE_TOK_BYTES;
-        slot_of[k] = (int)(at.pos & (GT - 1));
-      }
-      if (rotate) {
-        const double turns = (double)at.pos * (double)a.inv_freq[f] * 0.15915494309189533577;  // 1 / 2 pi
-        const float part = (float)(turns - __builtin_rint(turns));
-        turn[k][f] = float2{cospif(2.0f * part), sinpif(2.0f * part)};
-      }
+  if (tid < D / 2) {
+    const TokenAt at = token_at(a.b, t);
+    if (tid == 0) {
+      row_of = at.page < 0 ? -1 : at.page * a.b.hkv * (int64_t)PAGE_TOK_BYTES;
+      slot_of = (int)(at.pos & (GT - 1));
+    }
+    if (rotate) {
+      const double turns = (double)at.pos * (double)a.inv_freq[tid] * 0.15915494309189533577;  // 1 / 2 pi
+      const float part = (float)(turns - __builtin_rint(turns));
+      turn[0][tid] = cospif(2.0f * part);
+      turn[1][tid] = sinpif(2.0f * part);
     }
   }
   __syncthreads();
+  // the lane's angles: elements i and i + 64 share one
+  float cs[8], sn[8];
+  if (rotate) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const float4 c4 = *reinterpret_cast<const float4*>(&turn[0][(8 * j + e) & (D / 2 - 1)]);
+      const float4 s4 = *reinterpret_cast<const float4*>(&turn[1][(8 * j + e) & (D / 2 - 1)]);
+      cs[e] = c4.x, cs[e + 1] = c4.y, cs[e + 2] = c4.z, cs[e + 3] = c4.w;
+      // element i < 64 becomes x_i cos - x_(i + 64) sin, element i + 64 x_(i + 64) cos + x_i sin
+      const float side = j < 8 ? -1.0f : 1.0f;
+      sn[e] = side * s4.x, sn[e + 1] = side * s4.y, sn[e + 2] = side * s4.z, sn[e + 3] = side * s4.w;
+    }
+  }
 
-  for (int it = first; it < nt * nh; it += 16) {  // (16 lanes agree)
-    const int k = it / nh, h = h0 + it % nh;
-    const int64_t t = t0 + k;
-    Raw8<DT> raw;
-    raw.load(a.x + (t * a.x_rs + (int64_t)h * D + 8 * j) * SIZE);
+  for (int h = h0 + first; h < h1; h += 16) {  // (16 lanes agree)
     float v[8];
-    raw.get(v);
+    ahead[0].get(v);
+#pragma unroll
+    for (int e = 0; e + 1 < AHEAD; ++e) ahead[e] = ahead[e + 1];
+    if (h + 16 * AHEAD < h1) ahead[AHEAD - 1].load(x + (int64_t)(h + 16 * AHEAD) * (D * SIZE));
     const bool is_q = h < a.hq, is_v = h >= a.hq + a.b.hkv;
     if (!is_v) {
       if (norm) {
         float ss = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
-        const float r = 1.0f / sqrtf(row16_sum(ss) * (1.0f / D) + a.eps);
+        const float r = rsqrtf(row16_sum(ss) * (1.0f / D) + a.eps);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (is_q ? gq[e] : gk[e]);
       }
       if (rotate) {
-        // element i < 64 becomes x_i cos - x_(i + 64) sin, element i + 64 x_(i + 64) cos + x_i sin
-        const float side = j < 8 ? -1.0f : 1.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 cs = turn[k][(8 * j + e) & (D / 2 - 1)];
-          v[e] = __builtin_fmaf(v[e], cs.x, side * row16_other_half(v[e]) * cs.y);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], cs[e], row16_other_half(v[e]) * sn[e]);
       }
     }
     if (is_q) {
-      store8<NKV_F16>(reinterpret_cast<uint8_t*>(a.q_out + t * a.q_rs + (int64_t)h * D + 8 * j), v);
-    } else if (row_of[k] >= 0) {
+      store8<NKV_F16, NT>(reinterpret_cast<uint8_t*>(a.q_out + t * a.q_rs + (int64_t)h * D + 8 * j), v);
+    } else if (row_of >= 0) {
       const int kv = is_v ? h - a.hq - a.b.hkv : h - a.hq, which = is_v ? 1 : 0;
       float scale;
       const uint2 codes = sym_quant8<true>(v, scale);
-      uint8_t* page = a.pages + row_of[k] + (int64_t)kv * PAGE_TOK_BYTES;
-      *reinterpret_cast<uint2*>(page + which * CODE_BYTES + slot_of[k] * D + 8 * j) = codes;
-      if (j == 0) *reinterpret_cast<uint16_t*>(page + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot_of[k]) = f2h(scale);
+      uint8_t* page = a.pages + row_of + (int64_t)kv * PAGE_TOK_BYTES;
+      *reinterpret_cast<uint2*>(page + which * CODE_BYTES + slot_of * D + 8 * j) = codes;
+      if (j == 0) *reinterpret_cast<uint16_t*>(page + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot_of) = f2h(scale);
     }
   }
 }
@@ -236,16 +256,14 @@ struct ReadArgs {
   uint8_t* v_out;
 };
 
-constexpr int READ_TOK = 16;
-
-// READ_TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each.
-template <int DT, bool T64>
+// TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each, four rows of every lane in flight.
+template <int DT, bool T64, int TOK>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-  __shared__ int64_t page_of[READ_TOK];  // the token's page; -1: none, -2: in its sequence's ring
-  __shared__ int slot_of[READ_TOK], seq_of[READ_TOK];
+  __shared__ int64_t page_of[TOK];  // the token's page; -1: none, -2: in its sequence's ring
+  __shared__ int slot_of[TOK], seq_of[TOK];
   const int tid = threadIdx.x, j = tid & 15;
-  const int64_t t0 = (int64_t)blockIdx.x * READ_TOK;
-  const int nt = (int)min<int64_t>(READ_TOK, a.tokens - t0);
+  const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  const int nt = (int)min<int64_t>(TOK, a.tokens - t0);
   if (tid < nt) {
     const TokenAt at = token_at(a.b, t0 + tid);
     int64_t page = at.page;
@@ -259,43 +277,60 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     seq_of[tid] = at.seq;
   }
   __syncthreads();
-  constexpr int SIZE = Elem<DT>::SIZE;
+  constexpr int SIZE = Elem<DT>::SIZE, FLY = T64 ? 2 : 4;
   const int rows = 2 * a.b.hkv * nt;
-  for (int it = tid >> 4; it < rows; it += 16) {
-    const int k = it % nt, hw = it / nt, h = hw >> 1, which = hw & 1, slot = slot_of[k];
-    const int64_t page = page_of[k];
-    float v[8];
-    if (page == -1) {
+  // item `it`: token it % nt, tensor and KV head it / nt (neighbouring rows of a page, first)
+  for (int it0 = tid >> 4; it0 < rows; it0 += 16 * FLY) {
+    uint2 codes[FLY];
+    uint16_t scale[FLY];
+    Raw8<NKV_F16> st[FLY], mn[FLY];  // (st: the ring's values, too)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    } else if (T64 && page == -2) {
-      Raw8<NKV_F16> r;
-      r.load(reinterpret_cast<const uint8_t*>(a.rings + ((((int64_t)seq_of[k] * a.b.hkv + h) * 2 + which) * GT + slot) * D + 8 * j));
-      r.get(v);
-    } else {
-      const uint8_t* p = a.pages + (page * a.b.hkv + h) * (T64 ? PAGE_BYTES : PAGE_TOK_BYTES);
-      const uint2 codes = *reinterpret_cast<const uint2*>(p + which * CODE_BYTES + slot * D + 8 * j);
-      if constexpr (T64) {
-        float st[8], mn[8];
-        Raw8<NKV_F16> r;
-        r.load(p + 2 * CODE_BYTES + which * (4 * D) + 16 * j);
-        r.get(st);
-        r.load(p + 2 * CODE_BYTES + which * (4 * D) + 2 * D + 16 * j);
-        r.get(mn);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t c = ((e < 4 ? codes.x : codes.y) >> (8 * (e & 3))) & 0xffu;
-          v[e] = __builtin_fmaf((float)c, st[e], mn[e]);  // (the product is exact)
+    for (int f = 0; f < FLY; ++f) {
+      const int it = it0 + 16 * f;
+      if (it >= rows) break;
+      const int k = it % nt, hw = it / nt, h = hw >> 1, which = hw & 1, slot = slot_of[k];
+      const int64_t page = page_of[k];
+      if (T64 && page == -2) {
+        st[f].load(reinterpret_cast<const uint8_t*>(a.rings + ((((int64_t)seq_of[k] * a.b.hkv + h) * 2 + which) * GT + slot) * D + 8 * j));
+      } else if (page >= 0) {
+        const uint8_t* p = a.pages + (page * a.b.hkv + h) * (T64 ? PAGE_BYTES : PAGE_TOK_BYTES);
+        codes[f] = *reinterpret_cast<const uint2*>(p + which * CODE_BYTES + slot * D + 8 * j);
+        if constexpr (T64) {
+          st[f].load(p + 2 * CODE_BYTES + which * (4 * D) + 16 * j);
+          mn[f].load(p + 2 * CODE_BYTES + which * (4 * D) + 2 * D + 16 * j);
+        } else {
+          scale[f] = *reinterpret_cast<const uint16_t*>(p + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot);
         }
-      } else {
-        const float s = h2f(*reinterpret_cast<const uint16_t*>(p + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot));
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          v[e] = (float)(int8_t)((e < 4 ? codes.x : codes.y) >> (8 * (e & 3))) * s;
       }
     }
-    uint8_t* out = (which ? a.v_out : a.k_out) + (((t0 + k) * a.b.hkv + h) * D + 8 * j) * SIZE;
-    store8<DT>(out, v);
+#pragma unroll
+    for (int f = 0; f < FLY; ++f) {
+      const int it = it0 + 16 * f;
+      if (it >= rows) break;
+      const int k = it % nt, hw = it / nt, h = hw >> 1, which = hw & 1;
+      const int64_t page = page_of[k];
+      float v[8];
+      if (page == -1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      } else if (T64 && page == -2) {
+        st[f].get(v);
+      } else if constexpr (T64) {
+        float s8[8], m8[8];
+        st[f].get(s8);
+        mn[f].get(m8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t code = ((e < 4 ? codes[f].x : codes[f].y) >> (8 * (e & 3))) & 0xffu;
+          v[e] = __builtin_fmaf((float)code, s8[e], m8[e]);  // (the product is exact)
+        }
+      } else {
+        const float s = h2f(scale[f]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? codes[f].x : codes[f].y) >> (8 * (e & 3))) * s;
+      }
+      store8<DT, (TOK > 4)>((which ? a.v_out : a.k_out) + (((t0 + k) * a.b.hkv + h) * D + 8 * j) * SIZE, v);
+    }
   }
 }
 
@@ -956,25 +991,30 @@ int batch_args(const char* what, Batch& b, const int32_t* seq_of, bool need_seq_
   return NKV_OK;
 }
 
+// The heads of few tokens are spread over workgroups (12 tokens: 2.9 us, all 48 heads in one 3.6 us).
 template <int DT>
 void launch_append(const AppendArgs& a, hipStream_t s) {
   const int heads = a.hq + 2 * a.b.hkv;
   AppendArgs c = a;
-  if (a.tokens >= 4 * CUS) {
-    c.heads_per_wg = heads;
-    hipLaunchKernelGGL((append_chunks_kernel<DT, 4>), dim3((unsigned)cdiv(a.tokens, 4)), dim3(256), 0, s, c);
-  } else {
-    c.heads_per_wg = 16;
-    hipLaunchKernelGGL((append_chunks_kernel<DT, 1>), dim3((unsigned)a.tokens, (unsigned)cdiv(heads, 16)), dim3(256), 0, s, c);
-  }
+  c.heads_per_wg = a.tokens < CUS ? 16 : heads;
+  const dim3 grid((unsigned)a.tokens, (unsigned)cdiv(heads, c.heads_per_wg));
+  if (a.tokens >= 8 * CUS) hipLaunchKernelGGL((append_chunks_kernel<DT, true>), grid, dim3(256), 0, s, c);
+  else hipLaunchKernelGGL((append_chunks_kernel<DT, false>), grid, dim3(256), 0, s, c);
+}
+
+template <bool T64, int TOK>
+void launch_read_as(const ReadArgs& a, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.tokens, TOK));
+  if (dtype == NKV_F16) hipLaunchKernelGGL((read_kernel<NKV_F16, T64, TOK>), grid, dim3(256), 0, s, a);
+  else if (dtype == NKV_BF16) hipLaunchKernelGGL((read_kernel<NKV_BF16, T64, TOK>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((read_kernel<NKV_F32, T64, TOK>), grid, dim3(256), 0, s, a);
 }
 
 template <bool T64>
 void launch_read(const ReadArgs& a, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv(a.tokens, READ_TOK));
-  if (dtype == NKV_F16) hipLaunchKernelGGL((read_kernel<NKV_F16, T64>), grid, dim3(256), 0, s, a);
-  else if (dtype == NKV_BF16) hipLaunchKernelGGL((read_kernel<NKV_BF16, T64>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((read_kernel<NKV_F32, T64>), grid, dim3(256), 0, s, a);
+  if (a.tokens * a.b.hkv <= 16 * CUS) launch_read_as<T64, 1>(a, dtype, s);
+  else if (a.tokens * a.b.hkv <= 512 * CUS) launch_read_as<T64, 4>(a, dtype, s);
+  else launch_read_as<T64, 16>(a, dtype, s);
 }
 
 int read_tokens(const char* what, bool t64, const uint8_t* pages, const int32_t* page_table, int64_t table_stride,

@@ -255,14 +255,16 @@ class PagedKVInt8Cache:
             raise ValueError(f"unsupported dtype {dtype}")
         dev, h = self.pos.device, self.num_kv_heads
         if out is None:
-            out = tuple(torch.empty((plan.total, h, D), dtype=dtype, device=dev) for _ in range(2))
-        for x in out:
-            if (x.dim() != 3 or x.shape[0] < plan.total or x.shape[1:] != (h, D) or x.dtype != dtype or x.device != dev
-                    or not x.is_contiguous() or x.data_ptr() % 16):
-                raise ValueError(f"out must be two contiguous, 16-byte aligned {dtype} tensors [{plan.total}, {h}, {D}] "
-                                 f"on {dev}")
-        if C.overlap(*out):
-            raise ValueError("the two tensors of out overlap")
+            shape = (plan.total, h, D)
+            out = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        else:
+            for x in out:
+                if (x.dim() != 3 or x.shape[0] < plan.total or x.shape[1:] != (h, D) or x.dtype != dtype or x.device != dev
+                        or not x.is_contiguous() or x.data_ptr() % 16):
+                    raise ValueError(f"out must be two contiguous, 16-byte aligned {dtype} tensors [{plan.total}, {h}, {D}] "
+                                     f"on {dev}")
+            if C.overlap(*out):
+                raise ValueError("the two tensors of out overlap")
         self._read(plan, layer, dtype, *out)
         return out
 
