@@ -613,19 +613,20 @@ int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stri
  * out of the token at position p = softmax(q k^T / sqrt(128)) v over tokens [0, p]. q: token t, head i at
  * q + t * q_token_stride + i * q_head_stride (multiples of 8); out likewise; lse_out [tokens][hq] fp32 or NULL.
  * Groups without a page take no part; a row with none gives 0 and -inf.
- * units: int32 [n_units][8], each (sequence, first row, rows, part, parts, partial slot, kind, 0): rows
+ * units: int32 [n_units][8], each (sequence, first row, rows, part, parts, partial slot, kind, alone): rows
  * first .. first + rows - 1 of the sequence's new tokens x (hq / hkv) heads, token-major, over part `part` of
- * `parts` of the 64-token groups up to the last of them; kind 0: up to 16 rows, 1: up to 32. Each row and part is in one
- * unit for a result. With parts > 1 a unit writes one partial per row, row r of part p to slot + p * rows + r,
- * and merges (int32 [n_merges][8]: sequence, first row, rows <= 8, parts, slot, slots from part to part, 0, 0)
- * join them in a second launch. workspace: nkv_paged_chunks_workspace_bytes(hkv, slots), any contents, one
+ * `parts` of the 64-token groups up to the last of them; kind 0: up to 16 rows, 1: up to 32, 2: up to 256; alone: 1
+ * for the only tile of its sequence. wide: nonzero
+ * when a unit has more than 32 rows (kind 2). Each row and part is in one unit for a result. With parts > 1 a unit writes one partial per row, row r of part p to slot + p * rows + r,
+ * and merges (int32 [n_merges][8]: cu[sequence], first row, rows <= 8, parts, slot, slots from part to part,
+ * 0, 0) join them in a second launch. workspace: nkv_paged_chunks_workspace_bytes(hkv, slots), any contents, one
  * call's at a time.
  */
 int64_t nkv_paged_chunks_workspace_bytes(int64_t hkv, int64_t partial_rows);
 int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
                               const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
                               int64_t num_pages, const int32_t* cu, const int64_t* start_dev, int64_t nseq, int64_t hq,
-                              int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units,
+                              int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units, int wide,
                               const int32_t* merges, int64_t n_merges, uint16_t* out, int64_t out_token_stride,
                               int64_t out_head_stride, float* lse_out, void* workspace, int64_t workspace_bytes,
                               void* stream);

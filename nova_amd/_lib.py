@@ -92,9 +92,9 @@ SIGNATURES = {
                                             P, P, I64, P]),
     "nkv_paged_chunks_workspace_bytes": (I64, [I64, I64]),
     # q, q_token_stride, q_head_stride, tokens, pages, table, table_stride, num_pages, cu, start, nseq, hq, hkv, head_dim,
-    # units, n_units, merges, n_merges, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream
-    "nkv_paged_attn_chunks_tok": (c_int, [P, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, P, I64, P,
-                                          I64, I64, P, P, I64, P]),
+    # units, n_units, wide, merges, n_merges, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream
+    "nkv_paged_attn_chunks_tok": (c_int, [P, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, c_int, P, I64,
+                                          P, I64, I64, P, P, I64, P]),
     # pages, table, table_stride, num_pages, (rings, length,) seq_of, cu, start, tokens, nseq, hkv, head_dim, k_out, v_out,
     # dtype, stream
     "nkv_paged_read_tok": (c_int, [P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_int, P]),

@@ -54,6 +54,7 @@ class ChunkPlan(SpanPlan):
     units: torch.Tensor = None    # int32 [n, 8]
     merges: torch.Tensor = None   # int32 [m, 8]
     ws_bytes: int = 0
+    wide: bool = False            # some unit is ROWS256
 
 
 def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
@@ -70,9 +71,10 @@ def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarra
 
     Returns ``(units, merges, partial_rows)``, int32 ``[n, 8]`` and ``[m, 8]``. The rows of a KV head
     (``counts[b] * gq``, token-major) are cut into tiles, a tile's 64-token groups into parts; a
-    unit is one part of one tile: ``(sequence, first row, rows, part, parts, partial slot, kind, 0)``.
-    Cut tiles leave one partial per row and part, which the merge entries ``(sequence, first row,
-    rows, parts, slot, slots from part to part, 0, 0)`` join, eight rows each. The longest units
+    unit is one part of one tile: ``(sequence, first row, rows, part, parts, partial slot, kind, alone)``,
+    alone: 1 for the only tile of its sequence.
+    Cut tiles leave one partial per row and part, which the merge entries ``(sequence's first packed
+    token, first row, rows, parts, slot, slots from part to part, 0, 0)`` join, eight rows each. The longest units
     come first."""
     tiles = []  # (steps, cost of a step, sequence, first row, rows, kind)
     for b, (start, n) in enumerate(zip(starts, counts)):
@@ -83,15 +85,20 @@ def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarra
             steps = (start + (row0 + rows - 1) // gq) // GT + 1
             kind = ROWS256 if big else ROWS16 if rows <= 16 else ROWS32
             tiles.append((steps, STEP_COST[kind], b, row0, rows, kind))
-    target = max(8, -(-sum(t[0] * t[1] for t in tiles) * hkv // CUS))
+    import os
+    wide = any(t[5] == ROWS256 for t in tiles)
+    w = 8 if wide else 4
+    target = max(8, -(-sum(t[0] * t[1] for t in tiles) * hkv // (CUS if wide else 2 * CUS)))
+    if os.environ.get("TGT"): target = int(os.environ["TGT"])
+    first = np.concatenate(([0], np.cumsum(counts))).tolist()  # each sequence's first packed token
     units, merges, slot = [], [], 0
     for steps, cost, b, row0, rows, kind in tiles:
-        parts = min(MAX_PARTS, -(-steps * cost // target))
+        parts = min(MAX_PARTS, -(-steps * cost // target)) if wide and kind == ROWS256 else min(MAX_PARTS, -(-(-(-steps // w)) // max(1, target // w)))
         for p in range(parts):
-            units.append((-(-steps * cost // parts), b, row0, rows, p, parts, slot, kind, 0))
+            units.append((-(-steps * cost // parts), b, row0, rows, p, parts, slot, kind, int(rows == counts[b] * gq)))
         if parts > 1:
             for r in range(0, rows, MERGE_ROWS):
-                merges.append((b, row0 + r, min(MERGE_ROWS, rows - r), parts, slot + r, rows, 0, 0))
+                merges.append((first[b], row0 + r, min(MERGE_ROWS, rows - r), parts, slot + r, rows, 0, 0))
             slot += parts * rows
     units.sort(key=lambda u: -u[0])
     as_ints = lambda rows: np.array(rows, dtype=np.int32).reshape(-1, UNIT_INTS)  # noqa: E731
@@ -122,7 +129,7 @@ def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int
     u, m = units.size, units.size + merges.size
     return ChunkPlan(counts, int(cu[-1]), pos[:len(counts)], ints[m:m + len(cu)], ints[m + len(cu):], new,
                      ints[:u].view(-1, UNIT_INTS), ints[u:m].view(-1, UNIT_INTS),
-                     int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)))
+                     int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)), bool((units[:, 6] == ROWS256).any()))
 
 
 def launch(device: torch.device, name: str, *args) -> None:

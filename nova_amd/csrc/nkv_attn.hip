@@ -191,13 +191,6 @@ __device__ __forceinline__ int parts_used(const AttnArgs& a, int64_t U) {
 // so the 16 rows a K operand read touches land on 16 distinct banks.
 __device__ __forceinline__ int ring_chunk_pos(int row, int chunk) { return chunk ^ (row & 15); }
 
-__device__ __forceinline__ float sum4rows(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // 8 codes (bytes of w0, w1) -> fp16(code * st + mn) per element, rulers per element.
 __device__ __forceinline__ half8_t dq8(uint32_t w0, uint32_t w1, uint4 st, uint4 mn) {
   const half2_t a = __builtin_elementwise_fma(codes_to_h2(w0, kSelB01), as_h2(st.x), as_h2(mn.x));

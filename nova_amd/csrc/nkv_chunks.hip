@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 // Units of up to 32 rows (SMALL): the waves of a workgroup take the part's groups in turn, each wave its own
 // group against all the rows, and their states are merged in LDS at the end. K codes go from memory to the
 // registers of S^T = K Q^T's A operand; V codes and both scales go to LDS, where the transposing read gives
-// the operand of O = P V. K's scale multiplies the scores, V is dequantized. Bound by the page bytes.
+// the operand of O = P V. K's scale multiplies the scores and V's the weights, so that the codes are exact operands.
 
 constexpr int CH_WAVES = 8, CH_THREADS = 64 * CH_WAVES;
 constexpr int CH_VSLOT = CODE_BYTES + 4 * GT;            // V codes, K scales, V scales: the rest of a page after K
@@ -356,10 +356,11 @@ constexpr int CH_LDS = 2 * CH_WAVES * CH_VSLOT;          // 132 KiB: two slots a
 enum UnitKind : int { ROWS16 = 0, ROWS32 = 1, ROWS256 = 2 };
 
 struct Unit {  // (int32 each, as the plan lays them out)
-  int seq, row0, rows, part, parts, slot, kind, pad;  // slot: partial row of part 0 of the tile
+  int seq, row0, rows, part, parts, slot, kind, alone;  // slot: partial row of part 0 of the tile; alone: of its sequence
 };
 struct Merge {
-  int seq, row0, rows, parts, slot, stride, pad0, pad1;  // up to 8 rows; part p's partial of row r: slot + p * stride + r
+  int first, row0, rows, parts, slot, stride, pad0, pad1;  // first: the sequence's first packed token; up to 8 rows;
+                                                           // part p's partial of row r: slot + p * stride + r
 };
 
 struct ChunkArgs {
@@ -438,48 +439,90 @@ struct Pages {
 
 __device__ __forceinline__ bool finite_h(uint32_t bits) { return (bits & 0x7c00u) != 0x7c00u; }
 
-template <int RB>
+// Eight signed codes as the fp16 values 2^-24 (code + 128): denormals, which the matrix core takes as they are, so
+// that a code becomes an operand with a byte's move alone.
+__device__ __forceinline__ half8_t tiny8(uint32_t w0, uint32_t w1) {
+  w0 ^= 0x80808080u;
+  w1 ^= 0x80808080u;
+  return as_h8(uint4{perm(0u, w0, 0x0c010c00u), perm(0u, w0, 0x0c030c02u), perm(0u, w1, 0x0c010c00u), perm(0u, w1, 0x0c030c02u)});
+}
+
+__device__ __forceinline__ _Float16 half_at(uint2 w, int i) {
+  const half2_t h = as_h2(i < 2 ? w.x : w.y);
+  return i & 1 ? h.y : h.x;
+}
+
+// The state of a row block: m, the reference maximum (log2 domain), and l, the sum of weights over the lane's tokens,
+// of row c; acc 2^-24 times the sum of P (code + 128), psum the sum of P, of rows 4 g + i, P = weight times V's scale.
+// A weight is 2^(s - m + SM_TOP - SM_TAU), at most 2^SM_TOP, so that P stays below 2^6 times the largest scale,
+// 65504 / 127.
+constexpr float SM_TAU = 4.0f, SM_TOP = 6.0f;
+struct SmallState {
+  float m, l;
+  float4_t psum, acc[8];
+};
+
+// W: waves of the workgroup.
+template <int RB, int W>
 __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
-  const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);  // tokens the sequence has with the new ones
-  const int64_t s0 = at.steps * u.part / u.parts, s1 = at.steps * (u.part + 1) / u.parts;
+  const int fresh = a.b.cu[u.seq + 1] - a.b.cu[u.seq];  // the sequence's new tokens
+  constexpr bool LATE = RB > 1;  // K's next loads after this group's scores: no registers for both
+  // (whole rounds of the waves, so that no wave idles in a part's last one)
+  const int64_t rounds = (at.steps + W - 1) / W;
+  const int64_t s0 = rounds * u.part / u.parts * W, s1 = min(rounds * (u.part + 1) / u.parts * W, at.steps);
   const uint8_t* pages = a.pages + (int64_t)h * PAGE_TOK_BYTES;
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_TOK_BYTES;
 
   uint4 kn[4][2];  // the next group's K codes: token 16 b + c, bytes 16 g + 64 hh ..
-  auto issue = [&](int page, int sb) {
-    const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride));
+  // The pages of a sequence with one tile are read once in the launch, and not kept in the caches (nontemporal); those
+  // of several tiles are left there for the others.
+  auto issue_k = [&](int page) {
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride)) + c * D + 16 * g;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-        kn[b][hh] = *reinterpret_cast<const uint4*>(p + (16 * b + c) * D + 16 * g + 64 * hh);
+      for (int hh = 0; hh < 2; ++hh) {
+        const u32x4_t* from = reinterpret_cast<const u32x4_t*>(p + 16 * b * D + 64 * hh);
+        const u32x4_t x = u.alone ? __builtin_nontemporal_load(from) : *from;
+        kn[b][hh] = uint4{x.x, x.y, x.z, x.w};
+      }
+  };
+  auto issue_v = [&](int page, int sb) {
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride));
     const uint32_t slot = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + (2 * wave + sb) * CH_VSLOT;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // earlier reads of this slot are done
+    auto load = [&](auto dma) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int row = 8 * e + (lane >> 3);
-      dma16(p, (uint32_t)(CODE_BYTES + row * D + (((lane & 7) ^ swz(row)) << 4)), slot + 1024 * e);
-    }
-    if (lane < 16) dma16(p, (uint32_t)(2 * CODE_BYTES + 16 * lane), slot + CODE_BYTES);
+      for (int e = 0; e < 8; ++e) {
+        const int row = 8 * e + (lane >> 3);
+        dma(p, (uint32_t)(CODE_BYTES + row * D + (((lane & 7) ^ swz(row)) << 4)), slot + 1024 * e);
+      }
+      if (lane < 16) dma(p, (uint32_t)(2 * CODE_BYTES + 16 * lane), slot + CODE_BYTES);
+    };
+    if (u.alone) load([](const void* b, uint32_t off, uint32_t to) { dma16_stream(b, off, to); });
+    else load([](const void* b, uint32_t off, uint32_t to) { dma16(b, off, to); });
   };
 
   int64_t s = s0 + wave;
-  const int mine = s < s1 ? (int)((s1 - s + CH_WAVES - 1) / CH_WAVES) : 0;  // groups of this wave
-  Pages pg(a.b, u.seq, s, CH_WAVES, mine);
+  const int mine = s < s1 ? (int)((s1 - s + W - 1) / W) : 0;  // groups of this wave
+  Pages pg(a.b, u.seq, s, W, mine);
   int page = pg.at(0);
-  if (page >= 0) issue(page, 0);
+  if (page >= 0) {
+    issue_k(page);
+    issue_v(page, 0);
+  }
 
   half8_t qb[RB][4];
-  int64_t tq[RB];  // the last position that row c attends
+  int tq[RB];  // the token of row c: the last one that it attends
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int r = 16 * rb + c, row = u.row0 + r;
     const bool ok = r < at.rows;
     const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
-    tq[rb] = ok ? at.start + tk : -1;
+    tq[rb] = tk;
     const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -491,15 +534,27 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   const int64_t whole = (at.start + u.row0 / a.gq + 1) / GT;  // steps that every row of the tile sees whole
   const _Float16 one = (_Float16)1.0f;
   const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
-  WaveState st[RB];
-  float4_t lsum[RB];
+  // Q K^T with codes as 2^-24 (code + 128): the accumulators start at the offset's share, -128 2^-24 sum(q)
+  float4_t start[RB];
+  SmallState st[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    state_init(st[rb]);
-    lsum[rb] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += (float)qb[rb][k][e];
+    sum = sum4rows(sum) * (-128.0f * 0x1p-24f);
+    start[rb] = float4_t{sum, sum, sum, sum};
+    st[rb].m = NEG_INF;
+    st[rb].l = 0.0f;
+    st[rb].psum = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
+  const float sl2 = a.sl2 * 0x1p24f;
 
-  for (int t = 0; t < mine; ++t, s += CH_WAVES) {
+  for (int t = 0; t < mine; ++t, s += W) {
     const int sb = t & 1;
     const bool here = page >= 0;
     uint4 kc[4][2];
@@ -509,88 +564,111 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) kc[b][hh] = kn[b][hh];
     page = pg.at(t + 1);
-    if (page >= 0) issue(page, sb ^ 1);
+    if (page >= 0) {
+      issue_v(page, sb ^ 1);
+      if (!LATE || !here) issue_k(page);
+    }
     if (!here) continue;  // a group without a page takes no part
 
     const uint8_t* slot = lds + (2 * wave + sb) * CH_VSLOT;
-    // the scales of tokens 16 b + 4 g .. + 3, as fp16 pairs
+    // the scales of tokens 16 b + 4 g .. + 3, as the lane's scores have them
     uint2 ks[4], vs[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       ks[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * (16 * b + 4 * g));
       vs[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * GT + 2 * (16 * b + 4 * g));
     }
-    float S[RB][4][4];
+    float S[RB][4][4];  // scores, times 2^-24
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       half8_t kop[4];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        const half2_t unit = {one, one};
-        kop[2 * hh] = dq8_sym(kc[b][hh].x, kc[b][hh].y, unit);
-        kop[2 * hh + 1] = dq8_sym(kc[b][hh].z, kc[b][hh].w, unit);
+        kop[2 * hh] = tiny8(kc[b][hh].x, kc[b][hh].y);
+        kop[2 * hh + 1] = tiny8(kc[b][hh].z, kc[b][hh].w);
       }
-      const float kscale[4] = {h2f((uint16_t)(ks[b].x & 0xffffu)) * a.sl2, h2f((uint16_t)(ks[b].x >> 16)) * a.sl2,
-                               h2f((uint16_t)(ks[b].y & 0xffffu)) * a.sl2, h2f((uint16_t)(ks[b].y >> 16)) * a.sl2};
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        float4_t x = float4_t{0.f, 0.f, 0.f, 0.f};
+        float4_t x = start[rb];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x = mfma32(kop[k], qb[rb][k], x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[rb][b][i] = x[i] * kscale[i];
+        for (int i = 0; i < 4; ++i) S[rb][b][i] = __builtin_fmaf(x[i], (float)half_at(ks[b], i), 0.0f);
       }
     }
+    if (LATE && page >= 0) issue_k(page);
     if (s >= whole) {
       // Masked positions: tokens behind a row's own, and the page's rows behind the sequence's last token, which
       // hold anything. Their weight is 0, but 0 times a V that is not finite is NaN, so such scales become 0;
-      // where a row does attend such a token, its score becomes NaN instead.
+      // where a row does attend such a token, its score becomes NaN instead. (Positions count from the sequence's
+      // first new token: they fit there.)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
+        int tok = (int)(s * GT - at.start) + 16 * b + 4 * g;
+        asm volatile("" : "+v"(tok), "+v"(vs[b].x), "+v"(vs[b].y));  // (all of it in this branch: few groups come here)
         uint32_t v16[4] = {vs[b].x & 0xffffu, vs[b].x >> 16, vs[b].y & 0xffffu, vs[b].y >> 16};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int64_t tok = s * GT + 16 * b + 4 * g + i;
           const bool fin = finite_h(v16[i]);
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb)
-            S[rb][b][i] = tok > tq[rb] ? NEG_INF : fin ? S[rb][b][i] : __builtin_nanf("");
-          if (!fin || tok >= len) v16[i] = 0;
+          for (int rb = 0; rb < RB; ++rb) S[rb][b][i] = tok + i > tq[rb] ? NEG_INF : fin ? S[rb][b][i] : __builtin_nanf("");
+          if (!fin || tok + i >= fresh) v16[i] = 0;
         }
         vs[b] = uint2{v16[0] | (v16[1] << 16), v16[2] | (v16[3] << 16)};
       }
     }
     half8_t ph[RB][2];
-    float alpha[RB];
-    bool moved[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      pf_softmax(st[rb], S[rb], 1.0f, ph[rb], alpha[rb], moved[rb]);
-      if (__builtin_amdgcn_ballot_w64(moved[rb]) != 0) {
+      SmallState& x = st[rb];
+      float top = NEG_INF;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, S[rb][b][i]);
+      top = fmaxf(x.m, max4rows(top) * sl2);
+      const float m = top > x.m + SM_TAU ? top : x.m, mu = m == NEG_INF ? 0.0f : m;
+      const bool moved = x.m != m;
+      const float alpha = __builtin_amdgcn_exp2f(x.m - mu), off = SM_TOP - SM_TAU - mu;
+      x.m = m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      _Float16 p16[2][8];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float ai = shfl(alpha[rb], 4 * g + i);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[rb][b][i], sl2, off));
+          sum[i] += p;
+          p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_fmaf(p, (float)half_at(vs[b], i), 0.0f);
+        }
 #pragma unroll
-          for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb][i] *= ai;
-          lsum[rb][i] *= ai;
+      for (int B = 0; B < 2; ++B)
+        ph[rb][B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
+      x.l = __builtin_fmaf(x.l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      if (__builtin_amdgcn_ballot_w64(moved) != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float ai = shfl(alpha, 4 * g + i);
+#pragma unroll
+          for (int cb = 0; cb < 8; ++cb) x.acc[cb][i] *= ai;
+          x.psum[i] *= ai;
         }
       }
     }
     const int r = c >> 1;
 #pragma unroll
     for (int B = 0; B < 2; ++B) {
-      const uint4 vscale = {vs[2 * B].x, vs[2 * B].y, vs[2 * B + 1].x, vs[2 * B + 1].y};
       const int vrow = 16 * (2 * B + (r >> 2)) + 4 * g + (r & 3);
 #pragma unroll
       for (int cb = 0; cb < 8; ++cb) {
         const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (lds_v2i_t*)(const lds_void_t*)(slot + vrow * D + 8 * (c & 1) + ((cb ^ swz(vrow)) << 4))));
-        const half8_t vop = dq8_sym_v(vw.x, vw.y, vscale);
+        const half8_t vop = tiny8(vw.x, vw.y);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) st[rb].acc[cb] = mfma32(ph[rb][B], vop, st[rb].acc[cb]);
       }
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) lsum[rb] = mfma32(ph[rb][B], ones, lsum[rb]);
+      for (int rb = 0; rb < RB; ++rb) st[rb].psum = mfma32(ph[rb][B], ones, st[rb].psum);
     }
   }
 
@@ -600,28 +678,36 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   float* state = reinterpret_cast<float*>(lds) + wave * (RB * 16 * CH_PART);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    if (g == 0) state[(16 * rb + c) * CH_PART + D] = st[rb].m;
+    // weights in the scale of the other tiles: 2^(15 - PF_TAU) at the reference maximum
+    constexpr float UNIT = 0x1p5f;
+    static_assert(15.0f - PF_TAU == SM_TOP - SM_TAU + 5.0f, "scale of the partials");
+    const float l = sum4rows(st[rb].l) * UNIT;
+    if (g == 0) {
+      state[(16 * rb + c) * CH_PART + D] = st[rb].m;
+      state[(16 * rb + c) * CH_PART + D + 1] = l;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * rb + 4 * g + i;
-      if (c == 0) state[r * CH_PART + D + 1] = lsum[rb][i];
+      const float offset = -128.0f * UNIT * st[rb].psum[i];
 #pragma unroll
-      for (int cb = 0; cb < 8; ++cb) state[r * CH_PART + 16 * cb + c] = st[rb].acc[cb][i];
+      for (int cb = 0; cb < 8; ++cb)
+        state[r * CH_PART + 16 * cb + c] = __builtin_fmaf(st[rb].acc[cb][i], 0x1p24f * UNIT, offset);
     }
   }
   __syncthreads();
   const int l32 = tid & 31;
 #pragma unroll
-  for (int p = 0; p < RB; ++p) {
-    const int r = 16 * p + (tid >> 5);
+  for (int p = 0; p < RB * 8 / W; ++p) {
+    const int r = 2 * W * p + (tid >> 5);
     if (r >= at.rows) continue;
     const float* base = reinterpret_cast<const float*>(lds) + r * CH_PART;
     RowSum sum = {NEG_INF, 0.0f, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int w = 0; w < CH_WAVES; ++w) sum.m = fmaxf(sum.m, base[w * (RB * 16 * CH_PART) + D]);
+    for (int w = 0; w < W; ++w) sum.m = fmaxf(sum.m, base[w * (RB * 16 * CH_PART) + D]);
     const float mu = sum.m == NEG_INF ? 0.0f : sum.m;
 #pragma unroll
-    for (int w = 0; w < CH_WAVES; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float* x = base + w * (RB * 16 * CH_PART);
       const float wt = __builtin_amdgcn_exp2f(x[D] - mu);
       const float4 v = *reinterpret_cast<const float4*>(x + 4 * l32);
@@ -942,35 +1028,68 @@ __global__ __launch_bounds__(CH_THREADS, 1) void attn_chunks_kernel(ChunkArgs a)
     return;
   if (u.kind == ROWS256) attend_big(a, u, h, lds);
   else if (u.rows > 32) return;
-  else if (u.rows <= 16) attend_small<1>(a, u, h, lds);
-  else attend_small<2>(a, u, h, lds);
+  else if (u.rows <= 16) attend_small<1, CH_WAVES>(a, u, h, lds);
+  else attend_small<2, CH_WAVES>(a, u, h, lds);
 }
 
-// The parts of a tile's rows into one: 32 lanes a row, 8 rows a workgroup.
+// A launch without units of more than 32 rows: workgroups of four waves, two on a CU, so that one's start and end (a
+// chain of loads that wait for each other, the merge of its waves) pass beside the other's stream.
+constexpr int SM_WAVES = 4;
+__global__ __launch_bounds__(64 * SM_WAVES, 2) void attn_small_chunks_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * SM_WAVES * CH_VSLOT];
+  const int h = blockIdx.x % a.b.hkv;
+  const Unit u = a.units[blockIdx.x / a.b.hkv];
+  if (u.seq < 0 || u.seq >= a.b.nseq || u.row0 < 0 || u.rows <= 0 || u.rows > 32 || u.part < 0 || u.part >= u.parts || u.slot < 0)
+    return;
+  if (u.rows <= 16) attend_small<1, SM_WAVES>(a, u, h, lds);
+  else attend_small<2, SM_WAVES>(a, u, h, lds);
+}
+
+// The parts of a tile's rows into one: 32 lanes a row, 8 rows a workgroup. The entry holds all that it needs, and the
+// columns of 8 parts are in flight beside the weights' loads: two waits for memory in a row for up to 8 parts.
 __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkArgs a, const Merge* merges) {
   const int h = blockIdx.x % a.b.hkv;
   const Merge g = merges[blockIdx.x / a.b.hkv];
-  const int r = threadIdx.x >> 5, l32 = threadIdx.x & 31;
-  if (g.seq < 0 || g.seq >= a.b.nseq || g.row0 < 0) return;
-  const TileAt at = tile_at(a, g.seq, g.row0, g.rows);
-  if (r >= at.rows || g.slot < 0 || g.slot + (int64_t)(g.parts - 1) * g.stride + r >= a.ws_rows) return;  // (32 lanes agree)
+  const int r = threadIdx.x >> 5, l32 = threadIdx.x & 31, row = g.row0 + r;
+  const int64_t token = (int64_t)g.first + row / a.gq;
+  if (r >= g.rows || g.first < 0 || g.row0 < 0 || token >= a.tokens || g.slot < 0 || g.stride < 0 ||
+      g.slot + (int64_t)(g.parts - 1) * g.stride + r >= a.ws_rows)
+    return;  // (32 lanes agree)
   const float* base = a.ws + (((int64_t)g.slot + r) * a.b.hkv + h) * CH_PART;
   const int64_t step = (int64_t)g.stride * a.b.hkv * CH_PART;
   RowSum sum = {NEG_INF, 0.0f, {0.f, 0.f, 0.f, 0.f}};
-  for (int p = l32; p < g.parts; p += 32) sum.m = fmaxf(sum.m, base[p * step + D]);
+  constexpr int FLY = 8;
+  float4 v[FLY];
+  auto columns = [&](int p0) {
+#pragma unroll
+    for (int e = 0; e < FLY; ++e) v[e] = *reinterpret_cast<const float4*>(base + min(p0 + e, g.parts - 1) * step + 4 * l32);
+  };
+  columns(0);
+  float2 ml = {NEG_INF, 0.0f};
+  if (l32 < g.parts) ml = *reinterpret_cast<const float2*>(base + l32 * step + D);
+  sum.m = ml.x;
+  for (int p = l32 + 32; p < g.parts; p += 32) sum.m = fmaxf(sum.m, base[p * step + D]);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) sum.m = fmaxf(sum.m, __shfl_xor(sum.m, o, 32));
   const float mu = sum.m == NEG_INF ? 0.0f : sum.m;
-  for (int p = 0; p < g.parts; ++p) {
-    const float* x = base + p * step;
-    const float2 ml = *reinterpret_cast<const float2*>(x + D);
-    const float4 v = *reinterpret_cast<const float4*>(x + 4 * l32);
+  for (int p0 = 0; p0 < g.parts; p0 += FLY) {
+    if (p0) columns(p0);
+    if (p0 % 32 == 0 && p0) {
+      ml = float2{NEG_INF, 0.0f};
+      if (p0 + l32 < g.parts) ml = *reinterpret_cast<const float2*>(base + (p0 + l32) * step + D);
+    }
     const float wt = __builtin_amdgcn_exp2f(ml.x - mu);
-    sum.acc.x += v.x * wt; sum.acc.y += v.y * wt; sum.acc.z += v.z * wt; sum.acc.w += v.w * wt;
-    sum.l += ml.y * wt;
+#pragma unroll
+    for (int e = 0; e < FLY; ++e) {
+      const int from = (p0 + e) & 31;
+      const float we = __shfl(wt, from, 32), le = __shfl(ml.y, from, 32);
+      if (p0 + e < g.parts) {
+        sum.acc.x += v[e].x * we; sum.acc.y += v[e].y * we; sum.acc.z += v[e].z * we; sum.acc.w += v[e].w * we;
+        sum.l += le * we;
+      }
+    }
   }
-  const int row = g.row0 + r;
-  write_row(a, h, at.first_token + row / a.gq, row % a.gq, sum, l32);
+  write_row(a, h, token, row % a.gq, sum, l32);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1099,7 +1218,7 @@ extern "C" int64_t nkv_paged_chunks_workspace_bytes(int64_t hkv, int64_t partial
 extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
                                          const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
                                          int64_t num_pages, const int32_t* cu, const int64_t* start_dev, int64_t nseq,
-                                         int64_t hq, int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units,
+                                         int64_t hq, int64_t hkv, int64_t head_dim, const int32_t* units, int64_t n_units, int wide,
                                          const int32_t* merges, int64_t n_merges, uint16_t* out, int64_t out_token_stride,
                                          int64_t out_head_stride, float* lse_out, void* workspace, int64_t workspace_bytes,
                                          void* stream) {
@@ -1126,7 +1245,9 @@ extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stri
   a.ws = static_cast<float*>(workspace);
   a.ws_rows = workspace && workspace_bytes > 0 ? workspace_bytes / (hkv * CH_PART * (int64_t)sizeof(float)) : 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(attn_chunks_kernel, dim3((unsigned)(n_units * hkv)), dim3(CH_THREADS), 0, s, a);
+  const dim3 grid((unsigned)(n_units * hkv));
+  if (wide) hipLaunchKernelGGL(attn_chunks_kernel, grid, dim3(CH_THREADS), 0, s, a);
+  else hipLaunchKernelGGL(attn_small_chunks_kernel, grid, dim3(64 * SM_WAVES), 0, s, a);
   if (int rc = check_launch(what)) return rc;
   if (n_merges) {
     hipLaunchKernelGGL(merge_chunks_kernel, dim3((unsigned)(n_merges * hkv)), dim3(256), 0, s, a,

@@ -33,6 +33,13 @@ typedef __attribute__((address_space(3))) v4s_t lds_v4s_t;
 // two 16-row blocks, one chunk) both hit 16 distinct bank positions per 16 lanes.
 __device__ __forceinline__ int swz(int row) { return ((row >> 1) & 7) ^ (((row >> 4) & 1) << 2); }
 
+__device__ __forceinline__ float sum4rows(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // Online-softmax state of one wave. m, l: head (lane & 15), log2 domain; m is a reference
 // maximum (at least every score seen so far, times sl2), the weights are 2^(s sl2 - m + 15).
 // acc[cb][i]: head 4*(lane>>4) + i, dim 16*cb + (lane&15), in the same scale.

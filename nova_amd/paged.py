@@ -485,7 +485,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         C.launch(dev, "nkv_paged_attn_chunks_tok", query.data_ptr(), query.stride(0), query.stride(1), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
                  plan.cu.data_ptr(), plan.starts.data_ptr(), plan.nseq, hq, hkv, D, plan.units.data_ptr(),
-                 plan.units.shape[0], plan.merges.data_ptr(), plan.merges.shape[0], out.data_ptr(), out.stride(0),
+                 plan.units.shape[0], plan.wide, plan.merges.data_ptr(), plan.merges.shape[0], out.data_ptr(), out.stride(0),
                  out.stride(1), _lib.ptr(lse), _lib.ptr(ws), plan.ws_bytes)
         return out
 

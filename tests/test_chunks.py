@@ -38,8 +38,8 @@ def test_units_cover_each_row_and_part_once(starts, counts, gq, hkv):
     units, merges, slots = C.plan_units(starts, counts, gq, hkv)
     assert units.dtype == merges.dtype == np.int32 and units.shape[1] == merges.shape[1] == C.UNIT_INTS
     tiles = {}
-    for seq, row0, rows, part, parts, slot, kind, pad in units.tolist():
-        assert 0 <= part < parts <= C.MAX_PARTS and pad == 0 and rows <= C.TILE_ROWS[kind]
+    for seq, row0, rows, part, parts, slot, kind, alone in units.tolist():
+        assert 0 <= part < parts <= C.MAX_PARTS and rows <= C.TILE_ROWS[kind] and alone == (rows == counts[seq] * gq)
         tiles.setdefault((seq, row0, rows, parts, slot, kind), []).append(part)
     seen = {}
     for (seq, row0, rows, parts, slot, kind), got in tiles.items():
@@ -53,8 +53,9 @@ def test_units_cover_each_row_and_part_once(starts, counts, gq, hkv):
         if parts > 1:
             used += range(slot, slot + parts * rows)
     assert sorted(used) == list(range(slots))
-    want = {(seq, row0 + r, parts, slot + r, rows) for seq, row0, rows, parts, slot, _ in tiles if parts > 1 for r in range(rows)}
-    got = [(seq, row0 + r, parts, slot + r, stride) for seq, row0, rows, parts, slot, stride, _, _ in merges.tolist()
+    first = np.concatenate(([0], np.cumsum(counts)))
+    want = {(first[seq], row0 + r, parts, slot + r, rows) for seq, row0, rows, parts, slot, _ in tiles if parts > 1 for r in range(rows)}
+    got = [(f, row0 + r, parts, slot + r, stride) for f, row0, rows, parts, slot, stride, _, _ in merges.tolist()
            for r in range(rows)]
     assert len(got) == len(set(got)) and set(got) == want
     assert all(rows <= C.MERGE_ROWS for rows in merges[:, 2])
@@ -99,7 +100,7 @@ def _append(lib, **kw):
 
 def _attend(lib, **kw):
     a = dict(q=PTR, q_ts=4096, q_hs=128, tokens=4, pages=PTR, table=PTR, ts=4, np=8, cu=PTR, start=PTR, nseq=2, hq=32, hkv=8,
-             d=128, units=PTR, n_units=1, merges=None, n_merges=0, out=PTR, o_ts=4096, o_hs=128, lse=None, ws=None, ws_bytes=0,
+             d=128, units=PTR, n_units=1, wide=0, merges=None, n_merges=0, out=PTR, o_ts=4096, o_hs=128, lse=None, ws=None, ws_bytes=0,
              stream=None)
     a.update(kw)
     return lib.nkv_paged_attn_chunks_tok(*a.values())
