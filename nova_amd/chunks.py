@@ -25,10 +25,20 @@ CUS = 256        # compute units of an MI355X: one attention workgroup each at a
 UNIT_INTS = 8    # int32 words of a work unit and of a merge entry
 ROWS16, ROWS32, ROWS256 = 0, 1, 2  # unit kinds
 TILE_ROWS = {ROWS16: 16, ROWS32: 32, ROWS256: 256}  # query rows (tokens x q heads per KV head) of a tile, at most
-MAX_PARTS = 256
-BIG_FROM = 64    # rows of a sequence from which its tiles are ROWS256
-STEP_COST = {ROWS16: 1, ROWS32: 1, ROWS256: 2}
 MERGE_ROWS = 8   # rows a merge entry covers
+MAX_PARTS = 256
+# Rows of a sequence from which its tiles are ROWS256 (32 query and 8 KV heads; as ROWS256 / as ROWS32):
+#   64 rows over 32000 tokens 54 / 42 us, 96 rows 55 / 56 us, 8 times 128 rows over 4000 tokens 55 / 58 us, 256 rows 64 / 89 us
+BIG_FROM = 64
+# 64-token groups of a small unit's part, at least: 32 rows over 4000 tokens 20 us (8: 25), 4 times one token over
+# 2000 10.9 us (8: 12.3; 1: 10.9)
+SMALL_PART = 4
+# prices of a cut in us: a step of a wide tile, a group of a small one with the card full of them, a unit's start and end,
+# the second launch, a partial row written and read. The cut that they choose is within 10% of the best of CUTS for every
+# batch of the comment above, prompts of 512 and 4096 tokens, chunks of 256 to 2048 over 8192 to 32000, 1 to 64
+# sequences of one token over 2000 to 131000.
+STEP_US, GROUP_US, UNIT_US, MERGE_US, PARTIAL_US = 2.4, 0.75, 7.0, 5.0, 0.0002
+CUTS = (1, 1.5, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256)
 
 
 @dataclass
@@ -72,37 +82,59 @@ def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarra
     Returns ``(units, merges, partial_rows)``, int32 ``[n, 8]`` and ``[m, 8]``. The rows of a KV head
     (``counts[b] * gq``, token-major) are cut into tiles, a tile's 64-token groups into parts; a
     unit is one part of one tile: ``(sequence, first row, rows, part, parts, partial slot, kind, alone)``,
-    alone: 1 for the only tile of its sequence.
-    Cut tiles leave one partial per row and part, which the merge entries ``(sequence's first packed
-    token, first row, rows, parts, slot, slots from part to part, 0, 0)`` join, eight rows each. The longest units
-    come first."""
-    tiles = []  # (steps, cost of a step, sequence, first row, rows, kind)
-    for b, (start, n) in enumerate(zip(starts, counts)):
-        big = n * gq > BIG_FROM
-        size = TILE_ROWS[ROWS256 if big else ROWS32]
-        for row0 in range(0, n * gq, size):
-            rows = min(size, n * gq - row0)
-            steps = (start + (row0 + rows - 1) // gq) // GT + 1
-            kind = ROWS256 if big else ROWS16 if rows <= 16 else ROWS32
-            tiles.append((steps, STEP_COST[kind], b, row0, rows, kind))
-    import os
-    wide = any(t[5] == ROWS256 for t in tiles)
-    w = 8 if wide else 4
-    target = max(8, -(-sum(t[0] * t[1] for t in tiles) * hkv // (CUS if wide else 2 * CUS)))
-    if os.environ.get("TGT"): target = int(os.environ["TGT"])
-    first = np.concatenate(([0], np.cumsum(counts))).tolist()  # each sequence's first packed token
-    units, merges, slot = [], [], 0
-    for steps, cost, b, row0, rows, kind in tiles:
-        parts = min(MAX_PARTS, -(-steps * cost // target)) if wide and kind == ROWS256 else min(MAX_PARTS, -(-(-(-steps // w)) // max(1, target // w)))
-        for p in range(parts):
-            units.append((-(-steps * cost // parts), b, row0, rows, p, parts, slot, kind, int(rows == counts[b] * gq)))
-        if parts > 1:
-            for r in range(0, rows, MERGE_ROWS):
-                merges.append((first[b], row0 + r, min(MERGE_ROWS, rows - r), parts, slot + r, rows, 0, 0))
-            slot += parts * rows
-    units.sort(key=lambda u: -u[0])
-    as_ints = lambda rows: np.array(rows, dtype=np.int32).reshape(-1, UNIT_INTS)  # noqa: E731
-    return as_ints([u[1:] for u in units]), as_ints(merges), slot
+    alone 1 for the only tile of its sequence. Cut tiles leave one partial per row and part, which the
+    merge entries ``(sequence's first packed token, first row, rows, parts, slot, slots from part to part,
+    0, 0)`` join, eight rows each. The longest units come first."""
+    rows = np.array(counts, dtype=np.int64) * gq
+    wide = bool((rows > BIG_FROM).any())
+    size = np.where(rows > BIG_FROM, TILE_ROWS[ROWS256], TILE_ROWS[ROWS32])
+    n_tiles = -(-rows // size)
+    seq = np.repeat(np.arange(len(rows)), n_tiles)
+    if not len(seq):
+        return np.zeros((0, UNIT_INTS), np.int32), np.zeros((0, UNIT_INTS), np.int32), 0
+    row0 = (np.arange(len(seq)) - np.repeat(np.cumsum(n_tiles) - n_tiles, n_tiles)) * size[seq]
+    have = np.minimum(size[seq], rows[seq] - row0)
+    kind = np.where(size[seq] == TILE_ROWS[ROWS256], ROWS256, np.where(have <= TILE_ROWS[ROWS16], ROWS16, ROWS32))
+    steps = (np.array(starts, dtype=np.int64)[seq] + (row0 + have - 1) // gq) // GT + 1
+    parts = _parts(steps, kind, have, hkv, wide)
+    # one entry a unit
+    tile = np.repeat(np.arange(len(seq)), parts)
+    part = np.arange(len(tile)) - np.repeat(np.cumsum(parts) - parts, parts)
+    slots = np.where(parts > 1, parts * have, 0)
+    slot = np.cumsum(slots) - slots
+    cost = (steps * np.where(kind == ROWS256, STEP_US, GROUP_US) / parts)[tile]
+    alone = (n_tiles[seq] == 1).astype(np.int64)
+    units = np.stack([seq[tile], row0[tile], have[tile], part, parts[tile], slot[tile], kind[tile], alone[tile]], 1)
+    units = units[np.argsort(-cost, kind="stable")]
+    # the cut tiles' rows, eight a merge entry
+    cut = np.nonzero(parts > 1)[0]
+    n_merges = -(-have[cut] // MERGE_ROWS)
+    t = np.repeat(cut, n_merges)
+    r = (np.arange(len(t)) - np.repeat(np.cumsum(n_merges) - n_merges, n_merges)) * MERGE_ROWS
+    first = (np.cumsum(counts) - np.array(counts))[seq]  # the sequence's first packed token
+    zero = np.zeros_like(t)
+    merges = np.stack([first[t], row0[t] + r, np.minimum(MERGE_ROWS, have[t] - r), parts[t], slot[t] + r, have[t], zero, zero], 1)
+    return units.astype(np.int32), merges.astype(np.int32), int(slots.sum())
+
+
+def _parts(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide: bool) -> np.ndarray:
+    """Into how many parts each tile is cut: the cut with the least estimated time among those whose parts take at
+    most the longest tile's time divided by 1, 1.5, 2, 3, .. A launch takes as long as its longest unit, or all of them
+    over the workgroups that run at once, plus the partials' traffic and second launch."""
+    small = kind != ROWS256
+    waves, slots = (8, CUS) if wide else (4, 2 * CUS)
+    rounds = -(-steps // waves)  # of a small unit: its waves take a group each
+    most = np.minimum(MAX_PARTS, np.where(small, np.maximum(1, steps // SMALL_PART), steps))
+    us = np.where(small, rounds * (waves * GROUP_US), steps * STEP_US)
+    best = None
+    for k in CUTS:
+        parts = np.clip(np.ceil(us * (k / us.max())).astype(np.int64), 1, most)
+        unit = np.where(small, -(-rounds // parts) * (waves * GROUP_US), us / parts) + UNIT_US
+        partials = int((np.where(parts > 1, parts * rows, 0)).sum()) * hkv
+        time = max(unit.max(), float((unit * parts).sum()) * hkv / slots) + (MERGE_US + partials * PARTIAL_US if partials else 0.0)
+        if best is None or time < best[0]:
+            best = time, parts
+    return best[1]
 
 
 def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:

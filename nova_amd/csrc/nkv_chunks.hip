@@ -130,6 +130,14 @@ __device__ __forceinline__ float row16_sum(float v) {
   return v;
 }
 
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false)));
+  return v;
+}
+
 // The value of lane l ^ 8 of the same 16-lane row (a rotation by 8).
 __device__ __forceinline__ float row16_other_half(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
@@ -395,7 +403,10 @@ __device__ __forceinline__ TileAt tile_at(const ChunkArgs& a, int seq, int row0,
   return t;
 }
 
-// Two rows' results in the same LDS or memory layout: 32 lanes a row, 4 dims each.
+constexpr float W_TAU = 4.0f;  // (RowState)
+
+// A row's sums, 32 lanes a row, 4 dims each: l of the weights 2^(score - m), scores in the log2 domain, acc of weight
+// times V.
 struct RowSum {
   float m, l;
   float4 acc;
@@ -406,9 +417,7 @@ __device__ __forceinline__ void write_row(const ChunkArgs& a, int h, int64_t tok
   *reinterpret_cast<uint2*>(a.out + token * a.o_ts + i * a.o_hs + 4 * l32) =
       uint2{(uint32_t)f2h(r.acc.x * inv) | ((uint32_t)f2h(r.acc.y * inv) << 16),
             (uint32_t)f2h(r.acc.z * inv) | ((uint32_t)f2h(r.acc.w * inv) << 16)};
-  // the weights carry 2^(15 - PF_TAU)
-  if (a.lse && l32 == 0)
-    a.lse[token * a.hq + i] = r.l == 0.0f ? NEG_INF : (r.m + __builtin_amdgcn_logf(r.l) - (15.0f - PF_TAU)) * LN2;
+  if (a.lse && l32 == 0) a.lse[token * a.hq + i] = r.l == 0.0f ? NEG_INF : (r.m + __builtin_amdgcn_logf(r.l)) * LN2;
 }
 
 // The pages of a wave's groups first, first + stride, .., n of them, held 64 at a time, one a lane. (Scalar loads
@@ -452,15 +461,121 @@ __device__ __forceinline__ _Float16 half_at(uint2 w, int i) {
   return i & 1 ? h.y : h.x;
 }
 
-// The state of a row block: m, the reference maximum (log2 domain), and l, the sum of weights over the lane's tokens,
-// of row c; acc 2^-24 times the sum of P (code + 128), psum the sum of P, of rows 4 g + i, P = weight times V's scale.
-// A weight is 2^(s - m + SM_TOP - SM_TAU), at most 2^SM_TOP, so that P stays below 2^6 times the largest scale,
-// 65504 / 127.
-constexpr float SM_TAU = 4.0f, SM_TOP = 6.0f;
-struct SmallState {
-  float m, l;
+// Eight signed codes as fp16 whole numbers.
+__device__ __forceinline__ half8_t whole8(uint32_t w0, uint32_t w1) {
+  const half2_t a = scodes_to_h2(w0, kSelB01), b = scodes_to_h2(w0, kSelB23);
+  const half2_t c = scodes_to_h2(w1, kSelB01), d = scodes_to_h2(w1, kSelB23);
+  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// The state of a row block. Weights are at most 2^top: with the largest V scale so far (as bits at most vs, which has
+// all of its exponent) P = weight times scale is 65504 at most, and no lower than that asks, so that small V lose
+// nothing to fp16's denormals. Of row c: off, what turns a score (log2 domain) into a weight's exponent, and l, the sum
+// of weights over the lane's tokens. Of rows 4 g + i: acc, the sum of P code (small units: 2^-24 P (code + 128), and
+// psum that of P). A row's largest score so far has an exponent of top - W_TAU at least; before its first score off is
+// NO_SCORE, with which any score passes top.
+constexpr float NO_SCORE = 3e38f;
+struct RowState {
+  float top;  // (the wave's lanes agree on top and vs)
+  uint32_t vs;
+  float off, l;
   float4_t psum, acc[8];
 };
+__device__ __forceinline__ void state_init(RowState& x) {
+  x.top = 30.0f;
+  x.vs = 0x3ff;
+  x.off = NO_SCORE;
+  x.l = 0.0f;
+  x.psum = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int cb = 0; cb < 8; ++cb) x.acc[cb] = float4_t{0.f, 0.f, 0.f, 0.f};
+}
+// The score (log2 domain) whose weight is 1; -inf: no token yet.
+__device__ __forceinline__ float reference(const RowState& x) { return x.off == NO_SCORE ? NEG_INF : -x.off; }
+
+// Whether a group has a V scale (its bits, one token's a lane) that lowers top.
+__device__ __forceinline__ bool larger_scale(const RowState& x, uint32_t vs) {
+  return __builtin_amdgcn_ballot_w64((vs & 0x7fffu) > x.vs) != 0;
+}
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+
+// Where the accumulators of Q K^T start: the share of the codes' offset, -128 2^-24 sum(q), of row c.
+__device__ __forceinline__ float4_t offset_share(const half8_t (&qb)[4]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += (float)qb[k][e];
+  sum = sum4rows(sum) * (-128.0f * 0x1p-24f);
+  return float4_t{sum, sum, sum, sum};
+}
+
+// The online softmax of a row block over 64 tokens. exponent(b, i, off): the weight's exponent of token 16 b + 4 g + i
+// and row c, its score plus off (-inf where masked); vs: the tokens' V scales; ph: the weights times those, in fp16, as
+// the operands of O = P V. The weights are taken with the off there is, without a maximum; only if an exponent passes
+// top, or the group has a larger V scale than top allows (`larger`, of the
+// wave; scale(): the lane's token's), is off moved, what was summed up scaled, and the pass made again.
+template <class F, class V>
+__device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& exponent, const uint2 (&vs)[4], half8_t (&ph)[2], int g) {
+  float top, sum[4];
+  auto pass = [&]() {
+    top = NEG_INF;
+    sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+    _Float16 p16[2][8];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = exponent(b, i, x.off), p = __builtin_amdgcn_exp2f(e);
+        top = fmaxf(top, e);
+        sum[i] += p;
+        p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_fmaf(p, (float)half_at(vs[b], i), 0.0f);
+      }
+#pragma unroll
+    for (int B = 0; B < 2; ++B)
+      ph[B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
+  };
+  pass();
+  asm volatile("" : "+v"(ph[0]), "+v"(ph[1]));  // (P is made here, not sunk past the branch)
+  // (one comparison for both; a group without a score for the wave has no use for its scales)
+  if (__builtin_amdgcn_ballot_w64(top > (larger ? NEG_INF : x.top)) != 0) {
+    float by = 0.0f;
+    if (larger) {
+      const float all = max4rows(row16_max((float)(scale() & 0x7fffu)));
+      const uint32_t m = max((uint32_t)__builtin_amdgcn_readfirstlane((int)all), x.vs);  // (the other row block may be ahead)
+      const float to = 30.0f - (float)(m >> 10);  // 2^15 over the power of two in the scale
+      by = x.top - to;
+      x.top = uniform(to);
+      x.vs = m | 0x3ffu;
+    }
+    const bool first = x.off == NO_SCORE;
+    float off = first ? 0.0f : x.off, t = NEG_INF;
+    asm volatile("" : "+v"(off));  // (all of it in this branch: few groups come here)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t = fmaxf(t, exponent(b, i, off));
+    t = max4rows(t);
+    const float moved = t - (x.top - W_TAU);
+    const float delta = first ? moved : fmaxf(t > x.top ? moved : 0.0f, by);
+    const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-delta);
+    x.off = first && t == NEG_INF ? NO_SCORE : off - delta;
+    x.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float ai = shfl(alpha, 4 * g + i);
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) x.acc[cb][i] *= ai;
+      x.psum[i] *= ai;
+    }
+    pass();
+  }
+  x.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// Element (row 4 g + i, dim 16 cb + c) of the weighted sum of V.
+__device__ __forceinline__ float value_sum(const RowState& x, int cb, int i) {
+  return __builtin_fmaf(x.acc[cb][i], 0x1p24f, -128.0f * x.psum[i]);
+}
 
 // W: waves of the workgroup.
 template <int RB, int W>
@@ -495,6 +610,7 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     const uint32_t slot = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + (2 * wave + sb) * CH_VSLOT;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // earlier reads of this slot are done
     auto load = [&](auto dma) {
+      const int lane = tail_tid() & 63;  // (opaque: the offsets are made again at each use, for want of registers)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int row = 8 * e + (lane >> 3);
@@ -534,23 +650,12 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   const int64_t whole = (at.start + u.row0 / a.gq + 1) / GT;  // steps that every row of the tile sees whole
   const _Float16 one = (_Float16)1.0f;
   const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
-  // Q K^T with codes as 2^-24 (code + 128): the accumulators start at the offset's share, -128 2^-24 sum(q)
   float4_t start[RB];
-  SmallState st[RB];
+  RowState st[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += (float)qb[rb][k][e];
-    sum = sum4rows(sum) * (-128.0f * 0x1p-24f);
-    start[rb] = float4_t{sum, sum, sum, sum};
-    st[rb].m = NEG_INF;
-    st[rb].l = 0.0f;
-    st[rb].psum = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb] = float4_t{0.f, 0.f, 0.f, 0.f};
+    start[rb] = offset_share(qb[rb]);
+    state_init(st[rb]);
   }
   const float sl2 = a.sl2 * 0x1p24f;
 
@@ -578,7 +683,14 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
       ks[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * (16 * b + 4 * g));
       vs[b] = *reinterpret_cast<const uint2*>(slot + CODE_BYTES + 2 * GT + 2 * (16 * b + 4 * g));
     }
-    float S[RB][4][4];  // scores, times 2^-24
+    // (places behind the sequence's last token hold anything)
+    auto own_scale = [&]() -> uint32_t {
+      const int l = tail_tid() & 63;
+      const uint32_t v = *reinterpret_cast<const uint16_t*>(slot + CODE_BYTES + 2 * GT + 2 * l);
+      return s >= whole && (int)(s * GT - at.start) + l >= fresh ? 0u : v;
+    };
+    const bool larger = larger_scale(st[0], own_scale());
+    float S[RB][4][4];  // scores, times 2^-24, in the natural domain
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       half8_t kop[4];
@@ -619,50 +731,17 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     }
     half8_t ph[RB][2];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      SmallState& x = st[rb];
-      float top = NEG_INF;
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, S[rb][b][i]);
-      top = fmaxf(x.m, max4rows(top) * sl2);
-      const float m = top > x.m + SM_TAU ? top : x.m, mu = m == NEG_INF ? 0.0f : m;
-      const bool moved = x.m != m;
-      const float alpha = __builtin_amdgcn_exp2f(x.m - mu), off = SM_TOP - SM_TAU - mu;
-      x.m = m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      _Float16 p16[2][8];
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[rb][b][i], sl2, off));
-          sum[i] += p;
-          p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_fmaf(p, (float)half_at(vs[b], i), 0.0f);
-        }
-#pragma unroll
-      for (int B = 0; B < 2; ++B)
-        ph[rb][B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
-      x.l = __builtin_fmaf(x.l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-      if (__builtin_amdgcn_ballot_w64(moved) != 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float ai = shfl(alpha, 4 * g + i);
-#pragma unroll
-          for (int cb = 0; cb < 8; ++cb) x.acc[cb][i] *= ai;
-          x.psum[i] *= ai;
-        }
-      }
-    }
-    const int r = c >> 1;
+    for (int rb = 0; rb < RB; ++rb)
+      weigh(st[rb], larger, own_scale,
+            [&](int b, int i, float off) { return __builtin_fmaf(S[rb][b][i], sl2, off); }, vs, ph[rb], g);
+    const int vl = tail_tid() & 63, vc = vl & 1, vr = (vl & 15) >> 1, vg = vl >> 4;
 #pragma unroll
     for (int B = 0; B < 2; ++B) {
-      const int vrow = 16 * (2 * B + (r >> 2)) + 4 * g + (r & 3);
+      const int vrow = 16 * (2 * B + (vr >> 2)) + 4 * vg + (vr & 3);
 #pragma unroll
       for (int cb = 0; cb < 8; ++cb) {
         const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_v2i_t*)(const lds_void_t*)(slot + vrow * D + 8 * (c & 1) + ((cb ^ swz(vrow)) << 4))));
+            (lds_v2i_t*)(const lds_void_t*)(slot + vrow * D + 8 * vc + ((cb ^ swz(vrow)) << 4))));
         const half8_t vop = tiny8(vw.x, vw.y);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) st[rb].acc[cb] = mfma32(ph[rb][B], vop, st[rb].acc[cb]);
@@ -678,22 +757,15 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   float* state = reinterpret_cast<float*>(lds) + wave * (RB * 16 * CH_PART);
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    // weights in the scale of the other tiles: 2^(15 - PF_TAU) at the reference maximum
-    constexpr float UNIT = 0x1p5f;
-    static_assert(15.0f - PF_TAU == SM_TOP - SM_TAU + 5.0f, "scale of the partials");
-    const float l = sum4rows(st[rb].l) * UNIT;
+    const float l = sum4rows(st[rb].l);
     if (g == 0) {
-      state[(16 * rb + c) * CH_PART + D] = st[rb].m;
+      state[(16 * rb + c) * CH_PART + D] = reference(st[rb]);
       state[(16 * rb + c) * CH_PART + D + 1] = l;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * rb + 4 * g + i;
-      const float offset = -128.0f * UNIT * st[rb].psum[i];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int cb = 0; cb < 8; ++cb)
-        state[r * CH_PART + 16 * cb + c] = __builtin_fmaf(st[rb].acc[cb][i], 0x1p24f * UNIT, offset);
-    }
+      for (int cb = 0; cb < 8; ++cb) state[(16 * rb + 4 * g + i) * CH_PART + 16 * cb + c] = value_sum(st[rb], cb, i);
   }
   __syncthreads();
   const int l32 = tid & 31;
@@ -728,20 +800,16 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 }
 
 // Units of up to 256 rows (BIG): wave w takes rows 32 w .. 32 w + 31 as two row blocks, and every wave every
-// group. The waves turn a group's codes once into fp16 LDS tiles, fp16(code * scale) as the format defines a value: K
-// row-major (rows of 256 bytes, their 16-byte chunk x at x ^ (row & 15)), V transposed in the tokens' order of P's
-// operand (rows of 128 bytes, chunk x at x ^ (row & 7)).
+// group. The waves turn a group's codes once into fp16 LDS tiles (whole8): K row-major (rows of 256 bytes, their
+// 16-byte chunk x at x ^ (row & 15)), V transposed in the tokens' order of P's operand (rows of 128 bytes, chunk x at
+// x ^ (row & 7)), the scales beside.
 // One barrier a step: in step t, before it, the conversion of group t + 1 into the tiles that step t - 1 read and the
 // wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
 constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
-constexpr int BG_KT = BG_STAGES * PAGE_TOK_BYTES, BG_VT = BG_KT + 2 * GT * D * 2, BG_LDS = BG_VT + 2 * GT * D * 2;
+constexpr int BG_KT = BG_STAGES * PAGE_TOK_BYTES, BG_VT = BG_KT + 2 * GT * D * 2;
+constexpr int BG_SC = BG_VT + 2 * GT * D * 2, BG_LDS = BG_SC + 2 * 6 * GT;  // a tile's scales: K's in fp32, V's
 static_assert(BG_LDS <= CH_LDS, "both kinds of unit share the LDS");
 static_assert(BG_ROWS * D * 2 <= BG_LDS, "the output of a tile fits");
-// instruction classes of __builtin_amdgcn_sched_group_barrier
-constexpr int SG_VALU = 0x2, SG_MFMA = 0x8, SG_DSR = 0x100;
-#ifndef BG_VPM
-#define BG_VPM 2
-#endif
 
 __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -754,12 +822,11 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
   Pages pg(a.b, u.seq, s0, 1, n);
   // wave w's loads of a group: K and V rows 8 w .. 8 w + 7, wave 0 the scales, too
-  const int own_loads = wave == 0 ? 3 : 2;
   int loads = 0;  // in flight of the newest group
   auto issue = [&](int page, int slot) {
     loads = 0;
     if (page < 0) return;
-    loads = own_loads;
+    loads = wave == 0 ? 3 : 2;
     const void* p = uniform_ptr(pages + page * page_stride);
     const uint32_t dst = base + slot * PAGE_TOK_BYTES;
     const int row = 8 * wave + (lane >> 3);
@@ -770,50 +837,36 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   };
   // steps that some row of the tile does not see whole: masked places may hold anything there (attend_small)
   const int tile_whole = (int)((at.start + u.row0 / a.gq + 1) / GT) - s0;
-  // Group t from its stage into its tiles: lane l of wave w takes K row l, dims 16 w .. + 15, and V dims 16 w .. + 15.
-  // `check`: with the rules for masked places; `here`: the group has a page.
+  // Group t from its stage into its tiles: lane l of wave w takes K row l, dims 16 w .. + 15, and V dims 16 w .. + 15;
+  // and the scales, with the rules for masked places where `check`. `here`: the group has a page.
   auto convert = [&](int t, int slot, auto check, bool here) {
     const uint8_t* sg = lds + slot * PAGE_TOK_BYTES;
-    const uint8_t* sc = sg + 2 * CODE_BYTES;
-    const int r = c >> 1;
+    const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4, r = c >> 1;
     const uint4 kw = *reinterpret_cast<const uint4*>(sg + lane * D + ((wave ^ swz(lane)) << 4));
-    uint32_t ks = *reinterpret_cast<const uint16_t*>(sc + 2 * lane);
-    u32x2 vw[2];
-    uint2 vs[2][2];
-#pragma unroll
-    for (int B = 0; B < 2; ++B) {
-      const int vrow = 16 * (2 * B + (r >> 2)) + 4 * g + (r & 3);
-      vw[B] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-          (lds_v2i_t*)(const lds_void_t*)(sg + CODE_BYTES + vrow * D + 8 * (c & 1) + ((wave ^ swz(vrow)) << 4))));
-#pragma unroll
-      for (int e = 0; e < 2; ++e) vs[B][e] = *reinterpret_cast<const uint2*>(sc + 2 * GT + 2 * (32 * B + 16 * e + 4 * g));
-    }
+    const int vrow = 16 * (r >> 2) + 4 * g + (r & 3);  // and 32 further, swizzled alike
+    const uint8_t* vp = sg + CODE_BYTES + vrow * D + 8 * (c & 1) + ((wave ^ swz(vrow)) << 4);
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(sg + 2 * CODE_BYTES);
+    uint32_t ks = sc[lane], vs = sc[GT + lane];
     if constexpr (decltype(check)::value) {
-      if (!finite_h(*reinterpret_cast<const uint16_t*>(sc + 2 * GT + 2 * lane))) ks = 0x7e00u;  // NaN
-#pragma unroll
-      for (int B = 0; B < 2; ++B)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w[2] = {vs[B][e].x, vs[B][e].y};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t tok = (int64_t)(s0 + t) * GT + 32 * B + 16 * e + 4 * g + i;
-            const uint32_t x = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            if (!here || !finite_h(x) || tok >= len) w[i >> 1] &= (i & 1) ? 0xffffu : 0xffff0000u;
-          }
-          vs[B][e] = uint2{w[0], w[1]};
-        }
+      if (!finite_h(vs)) ks = 0x7e00u, vs = 0;  // NaN
+      if (!here || (int64_t)(s0 + t) * GT + lane >= len) vs = 0;
     }
-    uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + lane * (2 * D);
-    uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + (16 * wave + c) * (2 * GT);
-    const half2_t s = as_h2(ks | (ks << 16));
-    const half8_t k0 = dq8_sym(kw.x, kw.y, s), k1 = dq8_sym(kw.z, kw.w, s);
-    *reinterpret_cast<half8_t*>(kt + (((2 * wave) ^ (lane & 15)) << 4)) = k0;
-    *reinterpret_cast<half8_t*>(kt + (((2 * wave + 1) ^ (lane & 15)) << 4)) = k1;
+    u32x2 vw[2];
 #pragma unroll
     for (int B = 0; B < 2; ++B)
-      *reinterpret_cast<half8_t*>(vt + (((4 * B + g) ^ (c & 7)) << 4)) =
-          dq8_sym_v(vw[B].x, vw[B].y, uint4{vs[B][0].x, vs[B][0].y, vs[B][1].x, vs[B][1].y});
+      vw[B] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t*)(const lds_void_t*)(vp + 32 * D * B)));
+    uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + lane * (2 * D);
+    uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + (16 * wave + c) * (2 * GT);
+    const int kx = ((2 * wave) ^ (lane & 15)) << 4, vx = (g ^ (c & 7)) << 4;
+    *reinterpret_cast<half8_t*>(kt + kx) = whole8(kw.x, kw.y);
+    *reinterpret_cast<half8_t*>(kt + (kx ^ 16)) = whole8(kw.z, kw.w);
+    *reinterpret_cast<half8_t*>(vt + vx) = whole8(vw[0].x, vw[0].y);
+    *reinterpret_cast<half8_t*>(vt + (vx ^ 64)) = whole8(vw[1].x, vw[1].y);
+    // (every wave writes the scales, the same ones: a branch would end the block that the products are mixed with)
+    uint8_t* to = lds + BG_SC + (t & 1) * (6 * GT);
+    *reinterpret_cast<float*>(to + 4 * lane) = h2f((uint16_t)ks) * a.sl2;
+    *reinterpret_cast<uint16_t*>(to + 4 * GT + 2 * lane) = (uint16_t)vs;
+    return vs;
   };
 
   int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
@@ -836,21 +889,18 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
       qb[rb][k] = as_h8(w);
     }
   }
-  const _Float16 one = (_Float16)1.0f;
-  const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
-  WaveState st[BG_RB];
-  float4_t lsum[BG_RB];
+  RowState st[BG_RB];  // (codes are whole numbers here: acc is the sum of P code, psum stays 0)
 #pragma unroll
-  for (int rb = 0; rb < BG_RB; ++rb) {
-    state_init(st[rb]);
-    lsum[rb] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int rb = 0; rb < BG_RB; ++rb) state_init(st[rb]);
+  bool larger = false;  // the next group has a larger V scale
   // this wave's rows attend steps t < mine
   const int last = min(row0 + BG_RB * 16, rows) - 1;
   const int mine = row0 < rows ? min(n, (int)((at.start + last / a.gq) / GT) + 1 - s0) : 0;
 
   half8_t op[16];  // the operands of the products: K's, then V's
+  // (here and below, an opaque lane: the offsets made of it are made again at each use, for want of registers)
   auto load_k = [&](int t) {
+    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
     const uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + c * (2 * D);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -859,6 +909,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
         op[4 * k + b] = *reinterpret_cast<const half8_t*>(kt + 16 * b * (2 * D) + (((2 * g + 8 * (k >> 1) + (k & 1)) ^ c) << 4));
   };
   auto load_v = [&](int t) {
+    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
     const uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + c * (2 * GT);
 #pragma unroll
     for (int B = 0; B < 2; ++B)
@@ -868,8 +919,6 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   };
   float4_t S[BG_RB][4];
   half8_t ph[BG_RB][2];
-  float alpha[BG_RB];
-  bool moved[BG_RB];
   auto qk = [&](int rb) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -878,45 +927,35 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
         S[rb][b] = mfma32(op[4 * k + b], qb[rb][k], k ? S[rb][b] : float4_t{0.f, 0.f, 0.f, 0.f});
   };
   auto softmax = [&](int rb, auto masked, int t) {
-    float sc[4][4];
+    // the scales of tokens 16 b + 4 g .. + 3, K's with the softmax's factor (read again by each row block: kept for
+    // both, they would not fit)
+    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
+    const uint8_t* scales = lds + BG_SC + (t & 1) * (6 * GT) + 16 * g;
+    float4_t ks[4];
+    uint2 vs[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[b][i] = S[rb][b][i];
-    if constexpr (decltype(masked)::value) {
-      const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * g;  // (near the sequence's end: fits)
-      const int tq = (row0 + 16 * rb + c) / a.gq;
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (tok0 + 16 * b + i > tq) sc[b][i] = NEG_INF;
+    for (int b = 0; b < 4; ++b) {
+      ks[b] = *reinterpret_cast<const float4_t*>(scales + 64 * b);
+      vs[b] = *reinterpret_cast<const uint2*>(scales + 4 * GT + 32 * b - 8 * g);
     }
-    pf_softmax(st[rb], sc, a.sl2, ph[rb], alpha[rb], moved[rb]);
-    asm volatile("" : "+v"(ph[rb][0]), "+v"(ph[rb][1]));  // (P is made here, not sunk past the rescale)
-  };
-  auto rescale = [&](int rb) {
-    if (__builtin_amdgcn_ballot_w64(moved[rb]) == 0) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float ai = shfl(alpha[rb], 4 * g + i);
-#pragma unroll
-      for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb][i] *= ai;
-      lsum[rb][i] *= ai;
-    }
+    const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * g;  // (masked: near the sequence's end, it fits)
+    const int tq = (row0 + 16 * rb + c) / a.gq;
+    weigh(st[rb], larger, [&]() { return *reinterpret_cast<const uint16_t*>(scales - 16 * g + 4 * GT + 2 * l); },
+          [&](int b, int i, float off) {
+      const float e = __builtin_fmaf(S[rb][b][i], ks[b][i], off);
+      return decltype(masked)::value && tok0 + 16 * b + i > tq ? NEG_INF : e;
+    }, vs, ph[rb], g);
   };
   auto pv = [&](int rb) {
 #pragma unroll
-    for (int B = 0; B < 2; ++B) {
+    for (int B = 0; B < 2; ++B)
 #pragma unroll
       for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb] = mfma32(ph[rb][B], op[8 * B + cb], st[rb].acc[cb]);
-      lsum[rb] = mfma32(ph[rb][B], ones, lsum[rb]);
-    }
   };
 
   wait_groups_all();
   __syncthreads();
-  if (n > 0) convert(0, 0, std::true_type{}, p0 >= 0);
+  if (n > 0) larger = larger_scale(st[0], convert(0, 0, std::true_type{}, p0 >= 0));
   __syncthreads();
   issue(p2, 2);
   issue(p3, 0);
@@ -936,30 +975,15 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
       __builtin_amdgcn_sched_barrier(0);
       qk(1);
       softmax(0, masked{}, t);
-      if constexpr (fast) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(SG_VALU, BG_VPM, 0);
-        }
-      }
-      rescale(0);
       load_v(t);
       pv(0);
       softmax(1, masked{}, t);
-      if constexpr (fast) {
-        __builtin_amdgcn_sched_group_barrier(SG_DSR, 16, 1);
-#pragma unroll
-        for (int i = 0; i < 18; ++i) {
-          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 1);
-          __builtin_amdgcn_sched_group_barrier(SG_VALU, BG_VPM, 1);
-        }
-      }
-      rescale(1);
     }
-    if constexpr (fast) convert(t + 1, r1, std::false_type{}, true);
-    else if (t + 1 < n) convert(t + 1, r1, std::true_type{}, p1 >= 0);
+    uint32_t vs = 0;
+    if constexpr (fast) vs = convert(t + 1, r1, std::false_type{}, true);
+    else if (t + 1 < n) vs = convert(t + 1, r1, std::true_type{}, p1 >= 0);
     if (go) pv(1);
+    larger = larger_scale(st[0], vs);
     // tile t + 1 is written, tile t is read, group t + 2 has landed
     if (loads == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
     else if (loads == 3) asm volatile("s_waitcnt vmcnt(3) lgkmcnt(0)" ::: "memory");
@@ -973,9 +997,12 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   for (; t + 1 < min(n, tile_whole) && p0 >= 0 && p1 >= 0; ++t) step(t, std::true_type{});
   for (; t < n; ++t) step(t, std::false_type{});
   wait_groups_all();
+  float rl[BG_RB];  // row c's sum of weights
+#pragma unroll
+  for (int rb = 0; rb < BG_RB; ++rb) rl[rb] = sum4rows(st[rb].l);
 
   if (u.parts == 1) {
-    // ---- out = acc / l (both x 2^15 - PF_TAU), through LDS so that 16 lanes store a row's 256 bytes (the 2-byte values
+    // ---- out = the sum of V / l, through LDS so that 16 lanes store a row's 256 bytes (the 2-byte values
     // at chunk ^ 2 ((row >> 2) & 3))
     __syncthreads();  // every wave is past its last read of the tiles
     uint8_t* ow = lds + wave * (BG_RB * 16 * D * 2);
@@ -983,7 +1010,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     for (int rb = 0; rb < BG_RB; ++rb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float l = lsum[rb][i], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, m = shfl(st[rb].m, 4 * g + i);
+        const float l = shfl(rl[rb], 4 * g + i), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, m = shfl(reference(st[rb]), 4 * g + i);
         const int r = 16 * rb + 4 * g + i, row = row0 + r;
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb)
@@ -991,7 +1018,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
               f2h(st[rb].acc[cb][i] * inv);
         if (a.lse && c == 0 && row < rows)
           a.lse[(at.first_token + row / a.gq) * a.hq + h * a.gq + row % a.gq] =
-              l == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(l) - (15.0f - PF_TAU)) * LN2;
+              l == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
       }
 #pragma unroll
     for (int k = 0; k < BG_RB * 4; ++k) {
@@ -1005,13 +1032,12 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
 #pragma unroll
     for (int rb = 0; rb < BG_RB; ++rb) {
       if (g == 0 && row0 + 16 * rb + c < rows && pr0 + 16 * rb + c < a.ws_rows)
-        a.ws[((pr0 + 16 * rb + c) * a.b.hkv + h) * CH_PART + D] = st[rb].m;
+        *reinterpret_cast<float2*>(a.ws + ((pr0 + 16 * rb + c) * a.b.hkv + h) * CH_PART + D) = float2{reference(st[rb]), rl[rb]};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 16 * rb + 4 * g + i;
         if (row0 + r >= rows || pr0 + r >= a.ws_rows) continue;
         float* dst = a.ws + ((pr0 + r) * a.b.hkv + h) * CH_PART;
-        if (c == 0) dst[D + 1] = lsum[rb][i];
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb) dst[16 * cb + c] = st[rb].acc[cb][i];
       }

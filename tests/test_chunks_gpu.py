@@ -265,6 +265,13 @@ ATTEND = [
     ([100, 333], [40, 64], 8, 1),
     ([0, 129], [65, 130], 7, 7),
     ([4000], [9], 12, 4),
+    # 64 rows of a sequence and fewer are tiles of 32, more are tiles of 256
+    ([900], [64], 1, 1),
+    ([900, 30], [65, 64], 1, 1),
+    ([500], [255], 1, 1),
+    ([500], [257], 1, 1),
+    ([5000, 700, 60], [40, 2, 17], 16, 2),
+    ([9000], [33], 2, 1),
 ]
 
 
@@ -353,6 +360,101 @@ def test_groups_without_a_page_take_no_part():
         want, _, tol = _attend64(q[i:i + 1].double().cpu().numpy(), k[keep[:n]], v[keep[:n]], n - 1, 2)
         assert (np.abs(out[i] - want[0]) <= tol[0]).all()
     assert (out[5:] == 0).all() and bool((lse[5:] == -float("inf")).all())
+
+
+@pytest.mark.parametrize("counts", [[3, 2], [40, 70]])
+def test_masked_places_of_few_rows_and_of_many(counts):
+    lens, hq, hkv = [60, 150], 4, 1
+    cache = _held_with_step(lens, counts, hq, hkv, 144)
+    plan = cache.plan_chunks(counts)
+    q = _randn((plan.total, hq, D), 145).cuda()
+    want = cache.attend_chunks(plan, q, 0).clone()
+    halves = cache.pages[0].view(torch.float16)
+    for b, n in enumerate(counts):  # everything behind each sequence's last token
+        end = lens[b] + n
+        page = int(cache.page_table[b, (end - 1) // GT])
+        for bad in (float("inf"), float("nan"), 60000.0):
+            for which in (0, 1):
+                halves[page, :, 8192 + 64 * which + (end - 1) % GT + 1:8192 + 64 * which + 64] = bad
+            assert torch.equal(cache.attend_chunks(plan, q, 0), want)
+
+
+@pytest.mark.parametrize("lens,counts,hq,hkv", [([0, 130], [1, 2], 4, 2), ([500], [9], 4, 1), ([0, 200], [90, 40], 4, 2), ([1500], [70], 2, 1)])
+@pytest.mark.parametrize("scales", [(2.0 ** -24, 2.0 ** -20), (2.0 ** -17, 2.0 ** -16), (2.0 ** -24, 500.0), (500.0, 2.0 ** -22)])
+def test_values_of_any_size(lens, counts, hq, hkv, scales):
+    """Values so small that their scales are fp16 denormals, and sequences whose values grow or shrink by many
+    powers of two from the first to the last token, lose nothing that the bound does not allow."""
+    cache = _held_with_step(lens, counts, hq, hkv, 146)
+    halves = cache.pages[0].view(torch.float16)
+    first, last = (np.log2(x) for x in scales)
+    for b, n in enumerate(counts):
+        end = lens[b] + n
+        s = torch.from_numpy(2.0 ** (first + (last - first) * np.arange(end) / max(1, end - 1))).half().cuda()
+        for g in range(-(-end // GT)):
+            part = s[g * GT:(g + 1) * GT]
+            halves[int(cache.page_table[b, g]), :, 8192 + 64:8192 + 64 + len(part)] = part
+    plan = cache.plan_chunks(counts)
+    q = _randn((plan.total, hq, D), 147, 1.5).cuda()
+    lse = torch.empty(plan.total, hq, device="cuda")
+    _check_attention(cache, 0, plan, q, cache.attend_chunks(plan, q, 0, lse=lse), lse, lens)
+
+
+def test_scores_that_grow_by_much():
+    """Keys whose scores rise by hundreds from group to group: what was summed before vanishes, and the
+    last tokens hold all of the weight."""
+    for counts in ([2, 1], [70, 30]):
+        lens, hq, hkv = [700, 300], 4, 1
+        cache = _held_with_step(lens, counts, hq, hkv, 148)
+        halves = cache.pages[0].view(torch.float16)
+        for b in range(2):
+            for g in range(-(-(lens[b] + counts[b]) // GT)):
+                halves[int(cache.page_table[b, g]), :, 8192:8192 + 64] = 2.0 ** (g - 6)
+        plan = cache.plan_chunks(counts)
+        q = _randn((plan.total, hq, D), 149, 1.0).cuda()
+        out = cache.attend_chunks(plan, q, 0)
+        _check_attention(cache, 0, plan, q, out, None, lens)
+
+
+def test_many_rows_over_missing_pages():
+    lens, counts, hq, hkv = [700, 130], [40, 70], 8, 2
+    cache = _held_with_step(lens, counts, hq, hkv, 150)
+    plan = cache.plan_chunks(counts)
+    assert plan.wide
+    q = _randn((110, hq, D), 151).cuda()
+    k, v = _values(cache, 0, 0, 740)
+    cache.page_table[0, 0] = -1
+    cache.page_table[0, 4:6] = 1 << 20
+    cache.page_table[1].fill_(-1)
+    lse = torch.empty(110, hq, device="cuda")
+    out = cache.attend_chunks(plan, q, 0, lse=lse).double().cpu().numpy()
+    keep = np.r_[64:256, 384:740]
+    for i in range(40):
+        n = int((keep < 701 + i).sum())
+        want, _, tol = _attend64(q[i:i + 1].double().cpu().numpy(), k[keep[:n]], v[keep[:n]], n - 1, 4)
+        assert (np.abs(out[i] - want[0]) <= tol[0]).all()
+    assert (out[40:] == 0).all() and bool((lse[40:] == -float("inf")).all())
+
+
+@pytest.mark.parametrize("counts", [[3, 1], [80, 40]])
+def test_a_plan_outlives_its_lengths(counts):
+    """A plan made at one length serves others, shorter (some parts have nothing to do) and longer."""
+    hq, hkv = 4, 1
+    made = [2500, 900]
+    cache = _held_with_step(made, counts, hq, hkv, 152)
+    plan = cache.plan_chunks(counts)
+    assert plan.ws_bytes > 0
+    q = _randn((plan.total, hq, D), 153, 1.5).cuda()
+    for lens in ([0, 0], [1, 700], [63, 65], [2499, 130]):
+        cache.pos[:2] = torch.tensor(lens)
+        lse = torch.empty(plan.total, hq, device="cuda")
+        _check_attention(cache, 0, plan, q, cache.attend_chunks(plan, q, 0, lse=lse), lse, lens)
+    late = _held_with_step(made, counts, hq, hkv, 152)
+    late.pos[:2] = torch.tensor([3, 70])
+    for b, n in enumerate((3, 70)):
+        late.pool.set_length(b, n)
+    early = late.plan_chunks(counts)
+    late.pos[:2] = torch.tensor(made)
+    _check_attention(late, 0, early, q, late.attend_chunks(early, q, 0), None, made)
 
 
 def test_one_token_each_agrees_with_the_decode_step():
@@ -568,6 +670,44 @@ def test_a_captured_step_follows_the_sequences():
         for w, g in zip(want, got):
             assert torch.equal(w, g), i
         assert torch.equal(a.pages[0], b.pages[0]) and torch.equal(a.pos, b.pos) and a._len == b._len
+
+
+def test_a_captured_step_of_many_rows_follows_the_sequences():
+    """As above, with rows of every kind, and two graphs of one plan replayed side by side on two streams."""
+    hq, hkv, counts, lens, steps = 8, 2, [40, 1, 9, 0], [0, 1000, 70, 5], 4
+    a, b = (_cache(lens, [n * (steps + 1) for n in counts], hq, hkv, 160) for _ in range(2))
+    pa, pb = a.plan_chunks(counts), b.plan_chunks(counts)
+    assert pa.wide and pa.ws_bytes > 0
+    x = torch.empty(pa.total, 12 * D, dtype=torch.float16, device="cuda")
+    q2 = torch.empty(pa.total, hq, D, dtype=torch.float16, device="cuda")
+
+    def step(c, p):
+        q = c.append_chunks(p, x, 0)
+        return q, c.attend_chunks(p, q, 0)
+
+    graphs, outs = [], []
+    for f in (lambda: step(b, pb), lambda: (q2, b.attend_chunks(pb, q2, 0))):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(f())
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for i in range(steps):
+        x.copy_(_randn(x.shape, 161 + i))
+        q2.copy_(_randn(q2.shape, 171 + i))
+        want = step(a, pa)
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        other = a.attend_chunks(pa, q2, 0)
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            graphs[0].replay()
+            with torch.cuda.stream(side):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(want[0], outs[0][0]) and torch.equal(want[1], outs[0][1]) and torch.equal(other, outs[1][1])
+        for c, p in ((a, pa), (b, pb)):
+            c.advance_chunks(p)
 
 
 def test_two_streams_share_a_plan():
