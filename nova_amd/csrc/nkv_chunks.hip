@@ -403,7 +403,7 @@ __device__ __forceinline__ TileAt tile_at(const ChunkArgs& a, int seq, int row0,
   return t;
 }
 
-constexpr float W_TAU = 4.0f;  // (RowState)
+constexpr float W_TAU = 4.0f;  // (RowState; log2 of the weights that a lane sums at a time)
 
 // A row's sums, 32 lanes a row, 4 dims each: l of the weights 2^(score - m), scores in the log2 domain, acc of weight
 // times V.
@@ -476,13 +476,14 @@ __device__ __forceinline__ half8_t whole8(uint32_t w0, uint32_t w1) {
 // NO_SCORE, with which any score passes top.
 constexpr float NO_SCORE = 3e38f;
 struct RowState {
-  float top;  // (the wave's lanes agree on top and vs)
+  float top, cap;  // (the wave's lanes agree on top, cap = 2^top, and vs)
   uint32_t vs;
   float off, l;
   float4_t psum, acc[8];
 };
 __device__ __forceinline__ void state_init(RowState& x) {
   x.top = 30.0f;
+  x.cap = 0x1p30f;
   x.vs = 0x3ff;
   x.off = NO_SCORE;
   x.l = 0.0f;
@@ -512,33 +513,32 @@ __device__ __forceinline__ float4_t offset_share(const half8_t (&qb)[4]) {
 
 // The online softmax of a row block over 64 tokens. exponent(b, i, off): the weight's exponent of token 16 b + 4 g + i
 // and row c, its score plus off (-inf where masked); vs: the tokens' V scales; ph: the weights times those, in fp16, as
-// the operands of O = P V. The weights are taken with the off there is, without a maximum; only if an exponent passes
-// top, or the group has a larger V scale than top allows (`larger`, of the
+// the operands of O = P V. The weights are taken with the off there is, without a maximum; only if a lane's sum passes
+// 2^top (16 weights of 2^(top - W_TAU) do not), or the group has a larger V scale than top allows (`larger`, of the
 // wave; scale(): the lane's token's), is off moved, what was summed up scaled, and the pass made again.
 template <class F, class V>
 __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& exponent, const uint2 (&vs)[4], half8_t (&ph)[2], int g) {
-  float top, sum[4];
+  float sum;
   auto pass = [&]() {
-    top = NEG_INF;
-    sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+    float part[4];
     _Float16 p16[2][8];
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = exponent(b, i, x.off), p = __builtin_amdgcn_exp2f(e);
-        top = fmaxf(top, e);
-        sum[i] += p;
+        const float p = __builtin_amdgcn_exp2f(exponent(b, i, x.off));
+        part[i] = b ? part[i] + p : p;
         p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_fmaf(p, (float)half_at(vs[b], i), 0.0f);
       }
+    sum = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
     for (int B = 0; B < 2; ++B)
       ph[B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
   };
   pass();
   asm volatile("" : "+v"(ph[0]), "+v"(ph[1]));  // (P is made here, not sunk past the branch)
-  // (one comparison for both; a group without a score for the wave has no use for its scales)
-  if (__builtin_amdgcn_ballot_w64(top > (larger ? NEG_INF : x.top)) != 0) {
+  // (one comparison for both)
+  if (__builtin_amdgcn_ballot_w64(sum > (larger ? -1.0f : x.cap)) != 0) {
     float by = 0.0f;
     if (larger) {
       const float all = max4rows(row16_max((float)(scale() & 0x7fffu)));
@@ -546,6 +546,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
       const float to = 30.0f - (float)(m >> 10);  // 2^15 over the power of two in the scale
       by = x.top - to;
       x.top = uniform(to);
+      x.cap = uniform(__builtin_amdgcn_exp2f(to));
       x.vs = m | 0x3ffu;
     }
     const bool first = x.off == NO_SCORE;
@@ -557,7 +558,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
       for (int i = 0; i < 4; ++i) t = fmaxf(t, exponent(b, i, off));
     t = max4rows(t);
     const float moved = t - (x.top - W_TAU);
-    const float delta = first ? moved : fmaxf(t > x.top ? moved : 0.0f, by);
+    const float delta = first ? moved : fmaxf(moved, by);
     const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-delta);
     x.off = first && t == NEG_INF ? NO_SCORE : off - delta;
     x.l *= alpha;
@@ -570,7 +571,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
     }
     pass();
   }
-  x.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  x.l += sum;
 }
 // Element (row 4 g + i, dim 16 cb + c) of the weighted sum of V.
 __device__ __forceinline__ float value_sum(const RowState& x, int cb, int i) {
@@ -806,8 +807,10 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 // One barrier a step: in step t, before it, the conversion of group t + 1 into the tiles that step t - 1 read and the
 // wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
 constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
-constexpr int BG_KT = BG_STAGES * PAGE_TOK_BYTES, BG_VT = BG_KT + 2 * GT * D * 2;
-constexpr int BG_SC = BG_VT + 2 * GT * D * 2, BG_LDS = BG_SC + 2 * 6 * GT;  // a tile's scales: K's in fp32, V's
+constexpr int BG_TILE = GT * D * 2, BG_SCALES = 8 * GT;  // a tile's scales, 32 bytes for 4 tokens: K's in fp32, V's, 0
+constexpr int BG_KT = 2 * BG_SCALES, BG_VT = BG_KT + 2 * BG_TILE;  // scales, K tiles, V tiles, stages: what is read most
+constexpr int BG_ST = BG_VT + 2 * BG_TILE;                         // in the range of an instruction's offset
+constexpr int BG_LDS = BG_ST + BG_STAGES * PAGE_TOK_BYTES;
 static_assert(BG_LDS <= CH_LDS, "both kinds of unit share the LDS");
 static_assert(BG_ROWS * D * 2 <= BG_LDS, "the output of a tile fits");
 
@@ -819,7 +822,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);
   const uint8_t* pages = a.pages + (int64_t)h * PAGE_TOK_BYTES;
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_TOK_BYTES;
-  const uint32_t base = __builtin_amdgcn_readfirstlane(lds_addr(lds));
+  const uint32_t stages = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + BG_ST;
   Pages pg(a.b, u.seq, s0, 1, n);
   // wave w's loads of a group: K and V rows 8 w .. 8 w + 7, wave 0 the scales, too
   int loads = 0;  // in flight of the newest group
@@ -828,7 +831,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     if (page < 0) return;
     loads = wave == 0 ? 3 : 2;
     const void* p = uniform_ptr(pages + page * page_stride);
-    const uint32_t dst = base + slot * PAGE_TOK_BYTES;
+    const uint32_t dst = stages + slot * PAGE_TOK_BYTES;
     const int row = 8 * wave + (lane >> 3);
     const uint32_t off = (uint32_t)(row * D + (((lane & 7) ^ swz(row)) << 4));
     dma16(p, off, dst + 1024 * wave);
@@ -840,7 +843,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   // Group t from its stage into its tiles: lane l of wave w takes K row l, dims 16 w .. + 15, and V dims 16 w .. + 15;
   // and the scales, with the rules for masked places where `check`. `here`: the group has a page.
   auto convert = [&](int t, int slot, auto check, bool here) {
-    const uint8_t* sg = lds + slot * PAGE_TOK_BYTES;
+    const uint8_t* sg = lds + BG_ST + slot * PAGE_TOK_BYTES;
     const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4, r = c >> 1;
     const uint4 kw = *reinterpret_cast<const uint4*>(sg + lane * D + ((wave ^ swz(lane)) << 4));
     const int vrow = 16 * (r >> 2) + 4 * g + (r & 3);  // and 32 further, swizzled alike
@@ -855,17 +858,17 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
 #pragma unroll
     for (int B = 0; B < 2; ++B)
       vw[B] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t*)(const lds_void_t*)(vp + 32 * D * B)));
-    uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + lane * (2 * D);
-    uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + (16 * wave + c) * (2 * GT);
+    uint8_t* kt = lds + BG_KT + (t & 1) * BG_TILE + lane * (2 * D);
+    uint8_t* vt = lds + BG_VT + (t & 1) * BG_TILE + (16 * wave + c) * (2 * GT);
     const int kx = ((2 * wave) ^ (lane & 15)) << 4, vx = (g ^ (c & 7)) << 4;
     *reinterpret_cast<half8_t*>(kt + kx) = whole8(kw.x, kw.y);
     *reinterpret_cast<half8_t*>(kt + (kx ^ 16)) = whole8(kw.z, kw.w);
     *reinterpret_cast<half8_t*>(vt + vx) = whole8(vw[0].x, vw[0].y);
     *reinterpret_cast<half8_t*>(vt + (vx ^ 64)) = whole8(vw[1].x, vw[1].y);
     // (every wave writes the scales, the same ones: a branch would end the block that the products are mixed with)
-    uint8_t* to = lds + BG_SC + (t & 1) * (6 * GT);
-    *reinterpret_cast<float*>(to + 4 * lane) = h2f((uint16_t)ks) * a.sl2;
-    *reinterpret_cast<uint16_t*>(to + 4 * GT + 2 * lane) = (uint16_t)vs;
+    uint8_t* to = lds + (t & 1) * BG_SCALES + 32 * (lane >> 2);
+    *reinterpret_cast<float*>(to + 4 * (lane & 3)) = h2f((uint16_t)ks) * a.sl2;
+    *reinterpret_cast<uint16_t*>(to + 16 + 2 * (lane & 3)) = (uint16_t)vs;
     return vs;
   };
 
@@ -898,24 +901,24 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   const int mine = row0 < rows ? min(n, (int)((at.start + last / a.gq) / GT) + 1 - s0) : 0;
 
   half8_t op[16];  // the operands of the products: K's, then V's
-  // (here and below, an opaque lane: the offsets made of it are made again at each use, for want of registers)
-  auto load_k = [&](int t) {
-    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
-    const uint8_t* kt = lds + BG_KT + (t & 1) * (GT * D * 2) + c * (2 * D);
+  // where this lane reads the tiles and scales of step t: kept, opaque to the compiler so that it makes the few others
+  // (an exclusive or each) at their use, for want of registers
+  uint32_t ka = c * (2 * D) + (((2 * g) ^ c) << 4), va = c * (2 * GT) + ((g ^ (c & 7)) << 4), sa = 32 * g;
+  auto load_k = [&]() {
+    asm volatile("" : "+v"(ka));
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        op[4 * k + b] = *reinterpret_cast<const half8_t*>(kt + 16 * b * (2 * D) + (((2 * g + 8 * (k >> 1) + (k & 1)) ^ c) << 4));
+        op[4 * k + b] = *reinterpret_cast<const half8_t*>(lds + (ka ^ (128 * (k >> 1) + 16 * (k & 1))) + (BG_KT + 16 * b * (2 * D)));
   };
-  auto load_v = [&](int t) {
-    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
-    const uint8_t* vt = lds + BG_VT + (t & 1) * (GT * D * 2) + c * (2 * GT);
+  auto load_v = [&]() {
+    asm volatile("" : "+v"(va));
 #pragma unroll
     for (int B = 0; B < 2; ++B)
 #pragma unroll
       for (int cb = 0; cb < 8; ++cb)
-        op[8 * B + cb] = *reinterpret_cast<const half8_t*>(vt + 16 * cb * (2 * GT) + (((4 * B + g) ^ (c & 7)) << 4));
+        op[8 * B + cb] = *reinterpret_cast<const half8_t*>(lds + (va ^ (64 * B)) + (BG_VT + 16 * cb * (2 * GT)));
   };
   float4_t S[BG_RB][4];
   half8_t ph[BG_RB][2];
@@ -929,22 +932,22 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
   auto softmax = [&](int rb, auto masked, int t) {
     // the scales of tokens 16 b + 4 g .. + 3, K's with the softmax's factor (read again by each row block: kept for
     // both, they would not fit)
-    const int l = tail_tid() & 63, c = l & 15, g = l >> 4;
-    const uint8_t* scales = lds + BG_SC + (t & 1) * (6 * GT) + 16 * g;
+    asm volatile("" : "+v"(sa));
     float4_t ks[4];
     uint2 vs[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      ks[b] = *reinterpret_cast<const float4_t*>(scales + 64 * b);
-      vs[b] = *reinterpret_cast<const uint2*>(scales + 4 * GT + 32 * b - 8 * g);
+      ks[b] = *reinterpret_cast<const float4_t*>(lds + sa + 128 * b);
+      vs[b] = *reinterpret_cast<const uint2*>(lds + sa + (128 * b + 16));
     }
-    const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * g;  // (masked: near the sequence's end, it fits)
-    const int tq = (row0 + 16 * rb + c) / a.gq;
-    weigh(st[rb], larger, [&]() { return *reinterpret_cast<const uint16_t*>(scales - 16 * g + 4 * GT + 2 * l); },
+    const int l = tail_tid() & 63;
+    const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * (l >> 4);  // (masked: near the sequence's end, it fits)
+    const int tq = (row0 + 16 * rb + (l & 15)) / a.gq;
+    weigh(st[rb], larger, [&]() { return *reinterpret_cast<const uint16_t*>(lds + (t & 1) * BG_SCALES + 32 * (l >> 2) + 16 + 2 * (l & 3)); },
           [&](int b, int i, float off) {
       const float e = __builtin_fmaf(S[rb][b][i], ks[b][i], off);
       return decltype(masked)::value && tok0 + 16 * b + i > tq ? NEG_INF : e;
-    }, vs, ph[rb], g);
+    }, vs, ph[rb], l >> 4);
   };
   auto pv = [&](int rb) {
 #pragma unroll
@@ -970,12 +973,11 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     const int p4 = pg.at(t + 4);
     const bool go = fast || (t < mine && p0 >= 0);
     if (go) {
-      load_k(t);
+      load_k();
       qk(0);
-      __builtin_amdgcn_sched_barrier(0);
       qk(1);
       softmax(0, masked{}, t);
-      load_v(t);
+      load_v();
       pv(0);
       softmax(1, masked{}, t);
     }
@@ -992,6 +994,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     issue(p4, r1);
     r1 = r1 == 2 ? 0 : r1 + 1;
     p0 = p1; p1 = p2; p2 = p3; p3 = p4;
+    ka ^= BG_TILE; va ^= BG_TILE; sa ^= BG_SCALES;
   };
   int t = 0;
   for (; t + 1 < min(n, tile_whole) && p0 >= 0 && p1 >= 0; ++t) step(t, std::true_type{});
