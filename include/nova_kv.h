@@ -590,8 +590,8 @@ int nkv_paged_decode_step_tok(const uint16_t* q, const uint16_t* k_new, const ui
  * No counterpart in the reference, which decodes one token of one sequence at a time
  * (src/nova/kvattn.py:326-327). The new tokens of a batch are packed: token t (t < tokens) is
  * sequence seq_of[t]'s new token t - cu[seq_of[t]] and stands at position start_dev[seq] + that;
- * cu: int32 [nseq + 1], ascending; seq_of: int32 [tokens]; start_dev: int64 [nseq]. All three are
- * read on the device. pages, page_table, num_pages: as for the paged batch above.
+ * cu: int32 [nseq + 1], ascending; seq_of: int32 [tokens]; start_dev: int64 [nseq]; less than 2^24 tokens
+ * a call. All three are read on the device. pages, page_table, num_pages: as for the paged batch above.
  *
  * nkv_paged_append_chunks_tok: the stacked projections qkv [tokens][hq + 2 hkv][128] (NKV_F16 /
  * NKV_BF16 / NKV_F32, rows row_stride elements apart). Each q and k head gets its RMSNorm when
@@ -616,11 +616,11 @@ int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stri
  * units: int32 [n_units][8], each (sequence, first row, rows, part, parts, partial slot, kind, alone): rows
  * first .. first + rows - 1 of the sequence's new tokens x (hq / hkv) heads, token-major, over part `part` of
  * `parts` of the 64-token groups up to the last of them; kind 0: up to 16 rows, 1: up to 32, 2: up to 256; alone: 1
- * for the only tile of its sequence. wide: nonzero
- * when a unit has more than 32 rows (kind 2). Each row and part is in one unit for a result. With parts > 1 a unit writes one partial per row, row r of part p to slot + p * rows + r,
+ * for the only tile of its sequence. wide: nonzero when a unit has more than 32 rows (kind 2). Every row and part of
+ * the result is in one unit. With parts > 1 a unit writes one partial per row, row r of part p to slot + p * rows + r,
  * and merges (int32 [n_merges][8]: cu[sequence], first row, rows <= 8, parts, slot, slots from part to part,
- * 0, 0) join them in a second launch. workspace: nkv_paged_chunks_workspace_bytes(hkv, slots), any contents, one
- * call's at a time.
+ * 0, 0) join them in a second launch. units and merges must be on 16 bytes; less than 2^23 workgroups (units or merges
+ * times hkv). workspace: nkv_paged_chunks_workspace_bytes(hkv, slots), any contents, one call's at a time.
  */
 int64_t nkv_paged_chunks_workspace_bytes(int64_t hkv, int64_t partial_rows);
 int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,

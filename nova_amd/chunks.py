@@ -43,7 +43,8 @@ CUTS = (1, 1.5, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256)
 
 @dataclass
 class SpanPlan:
-    """Tokens ``starts[b] .. starts[b] + counts[b] - 1`` of sequences ``0 .. nseq - 1``, packed."""
+    """Tokens ``starts[b] .. starts[b] + counts[b] - 1`` of sequences ``0 .. nseq - 1``, packed. A captured graph reads
+    the plan's tensors: keep the plan as long as the graph."""
 
     counts: list[int]
     total: int
@@ -139,8 +140,8 @@ def _parts(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide
 
 def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:
     n = np.array(counts, dtype=np.int64)
-    if sum(counts) > 1 << 28:
-        raise ValueError(f"{sum(counts)} tokens in one call; at most 2^28")
+    if sum(counts) >= 1 << 24:
+        raise ValueError(f"{sum(counts)} tokens in one call; less than 2^24 are possible")
     cu = np.concatenate(([0], np.cumsum(n)))
     return cu.astype(np.int32), np.repeat(np.arange(len(counts), dtype=np.int32), n)
 
@@ -171,6 +172,13 @@ def launch(device: torch.device, name: str, *args) -> None:
         return
     with torch.cuda.device(device):
         _lib.call(name, *args, _lib.stream_ptr(device))
+
+
+def of_cache(plan: SpanPlan, pos: torch.Tensor, max_seqs: int) -> None:
+    """A chunk plan follows the lengths of the cache that made it; a span plan must at least fit the cache."""
+    if plan.starts.device != pos.device or plan.nseq > max_seqs or (
+            isinstance(plan, ChunkPlan) and plan.starts.data_ptr() != pos.data_ptr()):
+        raise ValueError("the plan was made by another cache")
 
 
 def heads_of(x: torch.Tensor, name: str, tokens: int, heads: int, device: torch.device) -> None:

@@ -162,10 +162,10 @@ struct AppendArgs {
 // inv_freq is exact in fp64 and reduced there to a part of a turn, so that far positions lose nothing; one lane
 // computes it for each frequency, for all heads. The rows ahead are loaded while one is worked on, the first ones
 // before the angles and the page are known.
-// Bound by memory: 4112 tokens of 32 q and 8 KV heads (93 MB) in 23 us, 4.0 TB/s. Two or four tokens a workgroup
-// (the angles of four take all its lanes) take as long or longer (4: 25 us; 1029 tokens of 28 + 4 heads 7.3 against
-// 10 us: too few workgroups). NT: nontemporal q stores, for calls whose queries no L2 would hold until they are
-// read (4112 tokens: 2 us less).
+// Bound by memory: 4112 tokens of 32 q and 8 KV heads (93 MB) in 20.6 us, 4.5 TB/s (a large copy reaches 4.9); four
+// tokens a workgroup without the loads ahead took 25.8 us. 1029 bf16 tokens of 28 q and 4 KV heads 7.3
+// us; 12 tokens 3.7 us, the time of the chain sequence, position and table, angles, rows. NT: nontemporal q stores, for
+// calls whose queries no L2 would hold until they are read (4112 tokens: 20.6 against 21.4 us).
 template <int DT, bool NT>
 __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) float turn[2][D / 2];  // cos, sin
@@ -264,7 +264,9 @@ struct ReadArgs {
   uint8_t* v_out;
 };
 
-// TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each, four rows of every lane in flight.
+// TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each, four rows of every lane in flight (two of
+// int8t64, whose steps and minima are 32 bytes a lane more). Bound by memory: 70000 tokens of 8 KV heads to bf16 (431 MB)
+// in 92 us, 4.7 TB/s; 275 tokens 3.0 us, a chain of three loads.
 template <int DT, bool T64, int TOK>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   __shared__ int64_t page_of[TOK];  // the token's page; -1: none, -2: in its sequence's ring
@@ -349,10 +351,14 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 // steps are cut into parts, unit = one part of one tile. Part p of P takes steps [S p / P, S (p + 1) / P),
 // from the S of the device's lengths: the plan stays valid while sequences grow.
 //
-// Units of up to 32 rows (SMALL): the waves of a workgroup take the part's groups in turn, each wave its own
+// softmax(q K^T / sqrt(128)) V with K = code * scale and V likewise: K's scale multiplies the scores and V's the
+// weights, so that the codes are exact operands, and only P (weight times V's scale) and the output are rounded to fp16.
+//
+// Units of up to 32 rows (small): the waves of a workgroup take the part's groups in turn, each wave its own
 // group against all the rows, and their states are merged in LDS at the end. K codes go from memory to the
 // registers of S^T = K Q^T's A operand; V codes and both scales go to LDS, where the transposing read gives
-// the operand of O = P V. K's scale multiplies the scores and V's the weights, so that the codes are exact operands.
+// the operand of O = P V. Bound by memory: one token of each of 32 sequences of 64 to 8155 tokens (274 MB) in 50 us
+// and 4 for the merge, 5.5 TB/s; 64 sequences of 2048 in 45 us, 6.1 TB/s.
 
 constexpr int CH_WAVES = 8, CH_THREADS = 64 * CH_WAVES;
 constexpr int CH_VSLOT = CODE_BYTES + 4 * GT;            // V codes, K scales, V scales: the rest of a page after K
@@ -800,12 +806,20 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   }
 }
 
-// Units of up to 256 rows (BIG): wave w takes rows 32 w .. 32 w + 31 as two row blocks, and every wave every
+// Units of up to 256 rows (big): wave w takes rows 32 w .. 32 w + 31 as two row blocks, and every wave every
 // group. The waves turn a group's codes once into fp16 LDS tiles (whole8): K row-major (rows of 256 bytes, their
 // 16-byte chunk x at x ^ (row & 15)), V transposed in the tokens' order of P's operand (rows of 128 bytes, chunk x at
-// x ^ (row & 7)), the scales beside.
+// x ^ (row & 7)), the scales beside. (These swizzles read without conflicts: 5 cycles a wave's 16 bytes a lane, padded
+// rows of 272 and 144 bytes take 8.)
 // One barrier a step: in step t, before it, the conversion of group t + 1 into the tiles that step t - 1 read and the
 // wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
+// Bound by the vector and matrix instructions' issue: a step of a wave has 64 matrix (16 cycles each on the SIMD that
+// two waves share), 32 exponentials and about 200 other instructions; 2048 tokens over 14336, 32 q and 8 KV heads (515
+// GFLOP) in 592 us, 870 TFLOP/s, where a large fp16 matrix product of the library reaches 1092; 2.3 us a step, and a
+// unit of one step takes 15 us (8 of them its queries' and outputs' traffic when 256 units run). Keys and values rounded
+// to fp16 instead of exact codes: 578 us, and twice the error. Slower were: waves of 64 rows, for want of registers;
+// the conversion at the start of the step in half of the waves (600 us); the largest score taken before the weights
+// (622 us).
 constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
 constexpr int BG_TILE = GT * D * 2, BG_SCALES = 8 * GT;  // a tile's scales, 32 bytes for 4 tokens: K's in fp32, V's, 0
 constexpr int BG_KT = 2 * BG_SCALES, BG_VT = BG_KT + 2 * BG_TILE;  // scales, K tiles, V tiles, stages: what is read most
@@ -1075,13 +1089,14 @@ __global__ __launch_bounds__(64 * SM_WAVES, 2) void attn_small_chunks_kernel(Chu
 }
 
 // The parts of a tile's rows into one: 32 lanes a row, 8 rows a workgroup. The entry holds all that it needs, and the
-// columns of 8 parts are in flight beside the weights' loads: two waits for memory in a row for up to 8 parts.
+// columns of 8 parts are in flight beside the weights' loads: two waits for memory in a row for up to 8 parts. 2.7 us
+// for few rows, 7 us for 45760 partial rows (24 MB, 3.4 TB/s).
 __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkArgs a, const Merge* merges) {
   const int h = blockIdx.x % a.b.hkv;
   const Merge g = merges[blockIdx.x / a.b.hkv];
   const int r = threadIdx.x >> 5, l32 = threadIdx.x & 31, row = g.row0 + r;
   const int64_t token = (int64_t)g.first + row / a.gq;
-  if (r >= g.rows || g.first < 0 || g.row0 < 0 || token >= a.tokens || g.slot < 0 || g.stride < 0 ||
+  if (r >= g.rows || g.first < 0 || g.row0 < 0 || token >= a.tokens || g.slot < 0 || g.stride < 0 || g.parts <= 0 ||
       g.slot + (int64_t)(g.parts - 1) * g.stride + r >= a.ws_rows)
     return;  // (32 lanes agree)
   const float* base = a.ws + (((int64_t)g.slot + r) * a.b.hkv + h) * CH_PART;
@@ -1132,14 +1147,15 @@ int batch_args(const char* what, Batch& b, const int32_t* seq_of, bool need_seq_
   if (nseq <= 0 || nseq > 32767 || hkv <= 0 || hkv > 1024 || table_stride <= 0 || num_pages <= 0 || num_pages > (int64_t(1) << 31))
     return fail(NKV_ERR_INVALID, "%s: bad sizes nseq=%lld hkv=%lld table_stride=%lld num_pages=%lld", what, (long long)nseq,
                 (long long)hkv, (long long)table_stride, (long long)num_pages);
-  if (tokens < 0 || tokens > (int64_t(1) << 28))
-    return fail(NKV_ERR_INVALID, "%s: %lld tokens outside [0, 2^28]", what, (long long)tokens);
+  if (tokens < 0 || tokens >= (int64_t(1) << 24))  // (a launch has less than 2^32 threads)
+    return fail(NKV_ERR_INVALID, "%s: %lld tokens outside [0, 2^24)", what, (long long)tokens);
   if (tokens > 0 && ((need_seq_of && !seq_of) || !cu || !start || !table)) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
   b = Batch{seq_of, cu, start, table, table_stride, num_pages, (int)nseq, (int)hkv};
   return NKV_OK;
 }
 
-// The heads of few tokens are spread over workgroups (12 tokens: 2.9 us, all 48 heads in one 3.6 us).
+// The heads of few tokens are spread over workgroups (12 tokens: 3.7 us, all 48 heads in one 4.6 us), those of many
+// are not (1029 tokens: 7.3 us, spread 8.6 us; 4112 tokens 20.6 and 25.8 us: each workgroup makes the angles).
 template <int DT>
 void launch_append(const AppendArgs& a, hipStream_t s) {
   const int heads = a.hq + 2 * a.b.hkv;
@@ -1158,6 +1174,9 @@ void launch_read_as(const ReadArgs& a, int dtype, hipStream_t s) {
   else hipLaunchKernelGGL((read_kernel<NKV_F32, T64, TOK>), grid, dim3(256), 0, s, a);
 }
 
+// Few tokens want all the workgroups that there are, many tokens few waits for the chain at a workgroup's start. Tokens a
+// workgroup 1 / 4 / 16, 8 KV heads: 275 tokens 3.3 / 4.5 / 9.5 us, 5418 tokens of int8t64 16.1 / 14.4 / 19.6 us, 70000
+// tokens 16: 98 us, 4: 101 us. Stores of the long ones pass the caches (store8).
 template <bool T64>
 void launch_read(const ReadArgs& a, int dtype, hipStream_t s) {
   if (a.tokens * a.b.hkv <= 16 * CUS) launch_read_as<T64, 1>(a, dtype, s);
@@ -1257,7 +1276,8 @@ extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stri
   if (int rc = batch_args(what, a.b, nullptr, false, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
     return rc;
   if (hq <= 0 || hq > 16 * hkv || hq % hkv) return fail(NKV_ERR_INVALID, "%s: heads hq=%lld hkv=%lld", what, (long long)hq, (long long)hkv);
-  if (n_units < 0 || n_merges < 0 || n_units * hkv > INT32_MAX || n_merges * hkv > INT32_MAX)
+  constexpr int64_t MOST = (int64_t(1) << 23) - 1;  // workgroups: a launch has less than 2^32 threads
+  if (n_units < 0 || n_merges < 0 || n_units > MOST / hkv || n_merges > MOST / hkv)
     return fail(NKV_ERR_INVALID, "%s: %lld units and %lld merges of %lld KV heads", what, (long long)n_units,
                 (long long)n_merges, (long long)hkv);
   if (tokens == 0 || n_units == 0) return NKV_OK;

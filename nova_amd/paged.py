@@ -253,6 +253,7 @@ class PagedKVInt8Cache:
         plan's tokens stay as they are."""
         if dtype not in _DT:
             raise ValueError(f"unsupported dtype {dtype}")
+        C.of_cache(plan, self.pos, self.max_seqs)
         dev, h = self.pos.device, self.num_kv_heads
         if out is None:
             shape = (plan.total, h, D)
@@ -423,6 +424,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         128]``, or writes ``q_out``, which may be qkv's own q heads; rows after the plan's tokens are neither
         read nor written."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
+        C.of_cache(plan, self.pos, self.max_seqs)
         if (qkv.dim() != 2 or qkv.shape[0] < total or qkv.shape[1] != (hq + 2 * hkv) * D or qkv.dtype not in _DT
                 or qkv.device != dev):
             raise ValueError(f"qkv must be fp16 / bf16 / fp32 [{total}, {(hq + 2 * hkv) * D}] on {dev} (more tokens may "
@@ -467,6 +469,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         without a page take no part; a token with none gets 0 and -inf. Rows after the plan's tokens are neither
         read nor written. Calls may overlap on streams (each has its own scratch memory)."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
+        C.of_cache(plan, self.pos, self.max_seqs)
         C.heads_of(query, "query", total, hq, dev)
         if not C.rows_in_place(query):
             query = query.contiguous()
@@ -502,6 +505,9 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
     def note_chunks(self, plan: ChunkPlan, steps: int = 1, accepted: list[int] | None = None) -> None:
         """Host bookkeeping of ``steps`` steps that advanced ``pos`` on the device (:meth:`advance_chunks`, or a
         replayed graph that adds ``plan.new`` to ``pos[:plan.nseq]``)."""
+        C.of_cache(plan, self.pos, self.max_seqs)
+        if steps < 0:
+            raise ValueError(f"{steps} steps")
         moved = plan.counts if accepted is None else C.check_counts(accepted, self.max_seqs, "accepted")
         if len(moved) != plan.nseq or any(a > n for a, n in zip(moved, plan.counts)):
             raise ValueError(f"accepted {moved} of a step of {plan.counts}")

@@ -65,8 +65,8 @@ def test_packing():
     cu, seq_of = C._packed([3, 0, 1, 2])
     assert cu.tolist() == [0, 3, 3, 4, 6] and seq_of.tolist() == [0, 0, 0, 2, 3, 3]
     assert cu.dtype == seq_of.dtype == np.int32
-    with pytest.raises(ValueError, match="2\\^28"):
-        C._packed([1 << 29])  # (refused before the tokens are listed)
+    with pytest.raises(ValueError, match="2\\^24"):
+        C._packed([1 << 24])  # (refused before the tokens are listed)
 
 
 def test_counts_are_checked():
@@ -121,7 +121,7 @@ def _read_t64(lib, **kw):
 
 
 SHARED = [(dict(nseq=0), INVALID), (dict(nseq=1 << 15), INVALID), (dict(hkv=0), INVALID), (dict(ts=0), INVALID), (dict(np=0), INVALID),
-          (dict(tokens=-1), INVALID), (dict(tokens=1 << 29), INVALID), (dict(d=64), UNSUPPORTED), (dict(table=None), INVALID),
+          (dict(tokens=-1), INVALID), (dict(tokens=1 << 24), INVALID), (dict(d=64), UNSUPPORTED), (dict(table=None), INVALID),
           (dict(cu=None), INVALID), (dict(start=None), INVALID), (dict(pages=None), INVALID), (dict(pages=PTR + 8), UNSUPPORTED),
           (dict(tokens=0, cu=None), OK)]
 
@@ -138,7 +138,7 @@ def test_append_refusals(lib, kw, rc):
 
 @pytest.mark.parametrize("kw,rc", SHARED + [
     (dict(q=None), INVALID), (dict(units=None), INVALID), (dict(out=None), INVALID), (dict(hq=30), INVALID), (dict(n_units=-1), INVALID),
-    (dict(n_units=1 << 31), INVALID), (dict(n_merges=1), INVALID), (dict(n_merges=1, merges=PTR), INVALID),
+    (dict(n_units=1 << 20), INVALID), (dict(n_merges=1 << 62, merges=PTR, ws=PTR, ws_bytes=1 << 40), INVALID), (dict(n_merges=1), INVALID), (dict(n_merges=1, merges=PTR), INVALID),
     (dict(q_ts=4), UNSUPPORTED), (dict(q_hs=4), UNSUPPORTED), (dict(o_ts=4), UNSUPPORTED), (dict(o_hs=4), UNSUPPORTED),
     (dict(out=PTR + 2), UNSUPPORTED), (dict(n_units=0), OK)])
 def test_attend_refusals(lib, kw, rc):

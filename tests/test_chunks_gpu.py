@@ -338,7 +338,7 @@ def test_masked_places_may_hold_anything():
             halves[last, :, 8192 + 64 * which + 2:8192 + 64 * which + 64] = bad
         mid = int(cache2.page_table[1, 1])    # tokens 64 .. 127: position 110 is the chunk's eleventh token
         halves[mid, 0, 8192 + 64 + 110 - 64] = bad
-        got = cache2.attend_chunks(plan, q, 0)
+        got = cache2.attend_chunks(cache2.plan_chunks(counts), q, 0)
         assert torch.equal(got[:70], want[:70])
         assert torch.equal(got[70:80], want[70:80]) and torch.equal(got[:, 4:], want[:, 4:])
         assert bool(got[80:, :4].isnan().all())
@@ -523,6 +523,21 @@ def test_refusals():
     for out in ((k, k), (k, k[:10]), (k, k.float()), (k, torch.empty(11, 2, 2 * D, dtype=torch.float16, device="cuda")[..., ::2])):
         with pytest.raises(ValueError):
             cache.read(span, 0, out=out)
+
+
+def test_plans_of_other_caches_are_refused():
+    a, b = _cache([10, 20], [100, 100], 8, 2, 64), _cache([10, 20], [100, 100], 8, 2, 64)
+    small = _cache([40], [10], 8, 2, 65)
+    plan, span = a.plan_chunks([3, 4]), a.plan_read([5, 6])
+    qkv, q = _randn((7, 12 * D), 66).cuda(), _randn((7, 8, D), 67).cuda()
+    for call in (lambda: b.append_chunks(plan, qkv, 0), lambda: b.attend_chunks(plan, q, 0), lambda: b.read(plan, 0),
+                 lambda: b.advance_chunks(plan), lambda: small.read(span, 0)):
+        with pytest.raises(ValueError, match="another cache"):
+            call()
+    with pytest.raises(ValueError, match="steps"):
+        a.note_chunks(plan, -1)
+    k, v = a.read(span, 0)
+    assert all(torch.equal(x, y) for x, y in zip((k, v), b.read(span, 0)))  # (a span of tokens that b has, too)
 
 
 def test_steps_of_no_tokens():
