@@ -814,7 +814,7 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 // One barrier a step: in step t, before it, the conversion of group t + 1 into the tiles that step t - 1 read and the
 // wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
 // Bound by the vector and matrix instructions' issue: a step of a wave has 64 matrix (16 cycles each on the SIMD that
-// two waves share), 32 exponentials and about 200 other instructions; 2048 tokens over 14336, 32 q and 8 KV heads (515
+// two waves share), 32 exponentials and about 215 other instructions; 2048 tokens over 14336, 32 q and 8 KV heads (515
 // GFLOP) in 592 us, 870 TFLOP/s, where a large fp16 matrix product of the library reaches 1092; 2.3 us a step, and a
 // unit of one step takes 15 us (8 of them its queries' and outputs' traffic when 256 units run). Keys and values rounded
 // to fp16 instead of exact codes: 578 us, and twice the error. Slower were: waves of 64 rows, for want of registers;
