@@ -197,15 +197,19 @@ def l2_handover(enable: bool = True) -> int:
 def call(name: str, *args) -> None:
     """Call ``name``; raise ``ValueError`` (invalid argument), ``NotImplementedError``
     (unsupported here) or ``NovaKVError`` (HIP failure) on a nonzero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(load(), name)(*args)
     if rc != NKV_OK:
-        msg = lib.nkv_last_error().decode("utf-8", "replace")
-        if rc == NKV_ERR_INVALID:
-            raise ValueError(f"{name}: {msg}")
-        if rc == NKV_ERR_UNSUPPORTED:
-            raise NotImplementedError(f"{name}: {msg}")
-        raise NovaKVError(rc, f"{name}: {msg}")
+        fail(name, rc)
+
+
+def fail(name: str, rc: int) -> None:
+    """Raise what the nonzero status ``rc`` of ``name`` stands for."""
+    msg = load().nkv_last_error().decode("utf-8", "replace")
+    if rc == NKV_ERR_INVALID:
+        raise ValueError(f"{name}: {msg}")
+    if rc == NKV_ERR_UNSUPPORTED:
+        raise NotImplementedError(f"{name}: {msg}")
+    raise NovaKVError(rc, f"{name}: {msg}")
 
 
 def stream_ptr(device: torch.device | None = None) -> int:

@@ -48,13 +48,15 @@ class SpanPlan:
 
     counts: list[int]
     total: int
+    pos: torch.Tensor      # the positions of the cache that made the plan
     starts: torch.Tensor   # int64 [nseq] on the device
     cu: torch.Tensor       # int32 [nseq + 1]: where each sequence's tokens begin in the packed tensor
     seq_of: torch.Tensor   # int32 [total]: the sequence of each packed token
 
-    @property
-    def nseq(self) -> int:
-        return len(self.counts)
+    def __post_init__(self):
+        self.nseq = len(self.counts)
+        self.where = self.cu.data_ptr(), self.starts.data_ptr()  # (the plan's own memory: the addresses stay)
+        self.seq_ptr = self.seq_of.data_ptr()
 
 
 @dataclass
@@ -66,6 +68,10 @@ class ChunkPlan(SpanPlan):
     merges: torch.Tensor = None   # int32 [m, 8]
     ws_bytes: int = 0
     wide: bool = False            # some unit is ROWS256
+
+    def __post_init__(self):
+        super().__post_init__()
+        self.work = self.units.data_ptr(), self.units.shape[0], self.wide, self.merges.data_ptr(), self.merges.shape[0]
 
 
 def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
@@ -146,11 +152,11 @@ def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:
     return cu.astype(np.int32), np.repeat(np.arange(len(counts), dtype=np.int32), n)
 
 
-def span_plan(counts: list[int], starts: list[int], device) -> SpanPlan:
+def span_plan(counts: list[int], starts: list[int], pos: torch.Tensor) -> SpanPlan:
     cu, seq_of = _packed(counts)
-    first = torch.tensor(starts, dtype=torch.int64).to(device)
-    ints = torch.from_numpy(np.concatenate((cu, seq_of))).to(device)
-    return SpanPlan(counts, int(cu[-1]), first, ints[:len(cu)], ints[len(cu):])
+    first = torch.tensor(starts, dtype=torch.int64).to(pos.device)
+    ints = torch.from_numpy(np.concatenate((cu, seq_of))).to(pos.device)
+    return SpanPlan(counts, int(cu[-1]), pos, first, ints[:len(cu)], ints[len(cu):])
 
 
 def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int) -> ChunkPlan:
@@ -160,39 +166,42 @@ def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int
     ints = torch.from_numpy(np.concatenate((units.ravel(), merges.ravel(), cu, seq_of))).to(pos.device)
     new = torch.tensor(counts, dtype=torch.int64).to(pos.device)
     u, m = units.size, units.size + merges.size
-    return ChunkPlan(counts, int(cu[-1]), pos[:len(counts)], ints[m:m + len(cu)], ints[m + len(cu):], new,
+    return ChunkPlan(counts, int(cu[-1]), pos, pos[:len(counts)], ints[m:m + len(cu)], ints[m + len(cu):], new,
                      ints[:u].view(-1, UNIT_INTS), ints[u:m].view(-1, UNIT_INTS),
                      int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)), bool((units[:, 6] == ROWS256).any()))
 
 
 def launch(device: torch.device, name: str, *args) -> None:
-    """``_lib.call`` on the current stream of ``device``, whichever device is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _lib.stream_ptr(device))
+    """``_lib.call`` on the current stream of ``device`` (a tensor's, so it has an index), whichever device is
+    current."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():  # (current_device() without the check that CUDA is set up, and below)
+        rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            _lib.fail(name, rc)
         return
     with torch.cuda.device(device):
         _lib.call(name, *args, _lib.stream_ptr(device))
 
 
-def of_cache(plan: SpanPlan, pos: torch.Tensor, max_seqs: int) -> None:
-    """A chunk plan follows the lengths of the cache that made it; a span plan must at least fit the cache."""
-    if plan.starts.device != pos.device or plan.nseq > max_seqs or (
-            isinstance(plan, ChunkPlan) and plan.starts.data_ptr() != pos.data_ptr()):
+def of_cache(plan: SpanPlan, pos: torch.Tensor) -> None:
+    if plan.pos is not pos:
         raise ValueError("the plan was made by another cache")
 
 
 def heads_of(x: torch.Tensor, name: str, tokens: int, heads: int, device: torch.device) -> None:
     """``x`` must be fp16 ``[>= tokens, heads, 128]`` on ``device``."""
-    if (x.dim() != 3 or x.shape[0] < tokens or x.shape[1] != heads or x.shape[2] != D or x.dtype != torch.float16
-            or x.device != device):
+    shape = x.shape
+    if len(shape) != 3 or shape[0] < tokens or shape[1:] != (heads, D) or x.dtype != torch.float16 or x.device != device:
         raise ValueError(f"{name} must be fp16 [{tokens}, {heads}, {D}] on {device} (more tokens may follow), "
-                         f"got {tuple(x.shape)} {x.dtype} on {x.device}")
+                         f"got {tuple(shape)} {x.dtype} on {x.device}")
 
 
 def rows_in_place(x: torch.Tensor) -> bool:
     """Whether the kernels can take ``x`` ``[tokens, heads, 128]`` where it is: rows of 128 elements that start
     on 16 bytes."""
-    return x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0
+    token, head, element = x.stride()
+    return element == 1 and token % 8 == 0 and head % 8 == 0 and x.data_ptr() % 16 == 0
 
 
 def _extent(x: torch.Tensor) -> tuple[int, int]:

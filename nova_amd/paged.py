@@ -242,7 +242,7 @@ class PagedKVInt8Cache:
         for b, (s, n) in enumerate(zip(starts, counts)):
             if s + n > self._len[b]:
                 raise ValueError(f"sequence {b}: tokens {s} .. {s + n - 1} of {self._len[b]}")
-        return C.span_plan(counts, starts, self.pos.device)
+        return C.span_plan(counts, starts, self.pos)
 
     def read(self, plan: SpanPlan, layer: int, dtype: torch.dtype = torch.float16,
              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -253,11 +253,11 @@ class PagedKVInt8Cache:
         plan's tokens stay as they are."""
         if dtype not in _DT:
             raise ValueError(f"unsupported dtype {dtype}")
-        C.of_cache(plan, self.pos, self.max_seqs)
+        C.of_cache(plan, self.pos)
         dev, h = self.pos.device, self.num_kv_heads
         if out is None:
-            shape = (plan.total, h, D)
-            out = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+            k = torch.empty((plan.total, h, D), dtype=dtype, device=dev)
+            out = k, torch.empty_like(k)
         else:
             for x in out:
                 if (x.dim() != 3 or x.shape[0] < plan.total or x.shape[1:] != (h, D) or x.dtype != dtype or x.device != dev
@@ -272,8 +272,8 @@ class PagedKVInt8Cache:
     def _read(self, plan: SpanPlan, layer: int, dtype: torch.dtype, k: torch.Tensor, v: torch.Tensor) -> None:
         C.launch(self.pos.device, "nkv_paged_read_t64", self.pages[layer].data_ptr(), self.page_table.data_ptr(),
                  self.page_table.stride(0), self.num_pages, self.rings[layer].data_ptr(), self.pos.data_ptr(),
-                 plan.seq_of.data_ptr(), plan.cu.data_ptr(), plan.starts.data_ptr(), plan.total, plan.nseq,
-                 self.num_kv_heads, D, k.data_ptr(), v.data_ptr(), _DT[dtype])
+                 plan.seq_ptr, *plan.where, plan.total, plan.nseq, self.num_kv_heads, D, k.data_ptr(), v.data_ptr(),
+                 _DT[dtype])
 
     # ---- work plan of the prefix kernel
 
@@ -424,38 +424,38 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         128]``, or writes ``q_out``, which may be qkv's own q heads; rows after the plan's tokens are neither
         read nor written."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
-        C.of_cache(plan, self.pos, self.max_seqs)
-        if (qkv.dim() != 2 or qkv.shape[0] < total or qkv.shape[1] != (hq + 2 * hkv) * D or qkv.dtype not in _DT
-                or qkv.device != dev):
-            raise ValueError(f"qkv must be fp16 / bf16 / fp32 [{total}, {(hq + 2 * hkv) * D}] on {dev} (more tokens may "
-                             f"follow), got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
+        C.of_cache(plan, self.pos)
+        shape, dtype, width = qkv.shape, qkv.dtype, (hq + 2 * hkv) * D
+        if len(shape) != 2 or shape[0] < total or shape[1] != width or dtype not in _DT or qkv.device != dev:
+            raise ValueError(f"qkv must be fp16 / bf16 / fp32 [{total}, {width}] on {dev} (more tokens may "
+                             f"follow), got {tuple(shape)} {dtype} on {qkv.device}")
         if (q_gamma is None) != (k_gamma is None):
             raise ValueError("q_gamma and k_gamma come together")
         if q_gamma is not None:
             for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
-                if t.dtype != qkv.dtype or t.numel() != D or not t.is_contiguous() or t.device != dev or t.data_ptr() % 16:
-                    raise ValueError(f"{name} must be a contiguous, 16-byte aligned {qkv.dtype} tensor of {D} elements on {dev}")
+                if t.dtype != dtype or t.numel() != D or not t.is_contiguous() or t.device != dev or t.data_ptr() % 16:
+                    raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dtype} tensor of {D} elements on {dev}")
         if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2
                                      or not inv_freq.is_contiguous() or inv_freq.device != dev):
             raise ValueError(f"inv_freq must be a contiguous fp32 tensor of {D // 2} elements on {dev}")
-        given = qkv
-        if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16 or (qkv.stride(0) < qkv.shape[1] and qkv.shape[0] > 1):
+        given, (row, element) = qkv, qkv.stride()
+        if element != 1 or row % 8 or qkv.data_ptr() % 16 or (row < width and shape[0] > 1):
             qkv = qkv.contiguous()
+            row = width
         if q_out is None:
             q_out = torch.empty((total, hq, D), dtype=torch.float16, device=dev)
         else:
             C.heads_of(q_out, "q_out", total, hq, dev)
             if q_out.stride(1) != D or not C.rows_in_place(q_out) or not C.distinct_rows(q_out):
                 raise ValueError("q_out: a token's heads must be contiguous and its row 16-byte aligned")
-            own_rows = (given is qkv and q_out.data_ptr() == qkv.data_ptr() and q_out.dtype == qkv.dtype
-                        and (q_out.stride(0) == qkv.stride(0) or total <= 1))
+            own_rows = (given is qkv and q_out.data_ptr() == qkv.data_ptr() and q_out.dtype == dtype
+                        and (q_out.stride(0) == row or total <= 1))
             if not own_rows and C.overlap(q_out, given):
                 raise ValueError("q_out must be qkv's q heads themselves or not overlap qkv")
-        C.launch(dev, "nkv_paged_append_chunks_tok", qkv.data_ptr(), _DT[qkv.dtype], max(qkv.stride(0), qkv.shape[1]), total,
+        C.launch(dev, "nkv_paged_append_chunks_tok", qkv.data_ptr(), _DT[dtype], max(row, width), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
-                 plan.seq_of.data_ptr(), plan.cu.data_ptr(), plan.starts.data_ptr(), plan.nseq, hq, hkv, D,
-                 _lib.ptr(q_gamma), _lib.ptr(k_gamma), float(eps), _lib.ptr(inv_freq), q_out.data_ptr(),
-                 max(q_out.stride(0), hq * D))
+                 plan.seq_ptr, *plan.where, plan.nseq, hq, hkv, D, _lib.ptr(q_gamma), _lib.ptr(k_gamma), eps,
+                 _lib.ptr(inv_freq), q_out.data_ptr(), max(q_out.stride(0), hq * D))
         return q_out
 
     def attend_chunks(self, plan: ChunkPlan, query: torch.Tensor, layer: int, out: torch.Tensor | None = None,
@@ -469,7 +469,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         without a page take no part; a token with none gets 0 and -inf. Rows after the plan's tokens are neither
         read nor written. Calls may overlap on streams (each has its own scratch memory)."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
-        C.of_cache(plan, self.pos, self.max_seqs)
+        C.of_cache(plan, self.pos)
         C.heads_of(query, "query", total, hq, dev)
         if not C.rows_in_place(query):
             query = query.contiguous()
@@ -487,9 +487,8 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         ws = _lib.scratch(dev, plan.ws_bytes) if plan.ws_bytes else None
         C.launch(dev, "nkv_paged_attn_chunks_tok", query.data_ptr(), query.stride(0), query.stride(1), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
-                 plan.cu.data_ptr(), plan.starts.data_ptr(), plan.nseq, hq, hkv, D, plan.units.data_ptr(),
-                 plan.units.shape[0], plan.wide, plan.merges.data_ptr(), plan.merges.shape[0], out.data_ptr(), out.stride(0),
-                 out.stride(1), _lib.ptr(lse), _lib.ptr(ws), plan.ws_bytes)
+                 *plan.where, plan.nseq, hq, hkv, D, *plan.work, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), _lib.ptr(ws),
+                 plan.ws_bytes)
         return out
 
     def advance_chunks(self, plan: ChunkPlan, accepted: list[int] | None = None) -> None:
@@ -505,7 +504,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
     def note_chunks(self, plan: ChunkPlan, steps: int = 1, accepted: list[int] | None = None) -> None:
         """Host bookkeeping of ``steps`` steps that advanced ``pos`` on the device (:meth:`advance_chunks`, or a
         replayed graph that adds ``plan.new`` to ``pos[:plan.nseq]``)."""
-        C.of_cache(plan, self.pos, self.max_seqs)
+        C.of_cache(plan, self.pos)
         if steps < 0:
             raise ValueError(f"{steps} steps")
         moved = plan.counts if accepted is None else C.check_counts(accepted, self.max_seqs, "accepted")
@@ -520,6 +519,5 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
 
     def _read(self, plan: SpanPlan, layer: int, dtype: torch.dtype, k: torch.Tensor, v: torch.Tensor) -> None:
         C.launch(self.pos.device, "nkv_paged_read_tok", self.pages[layer].data_ptr(), self.page_table.data_ptr(),
-                 self.page_table.stride(0), self.num_pages, plan.seq_of.data_ptr(), plan.cu.data_ptr(),
-                 plan.starts.data_ptr(), plan.total, plan.nseq, self.num_kv_heads, D, k.data_ptr(), v.data_ptr(),
-                 _DT[dtype])
+                 self.page_table.stride(0), self.num_pages, plan.seq_ptr, *plan.where, plan.total, plan.nseq,
+                 self.num_kv_heads, D, k.data_ptr(), v.data_ptr(), _DT[dtype])

@@ -531,13 +531,11 @@ def test_plans_of_other_caches_are_refused():
     plan, span = a.plan_chunks([3, 4]), a.plan_read([5, 6])
     qkv, q = _randn((7, 12 * D), 66).cuda(), _randn((7, 8, D), 67).cuda()
     for call in (lambda: b.append_chunks(plan, qkv, 0), lambda: b.attend_chunks(plan, q, 0), lambda: b.read(plan, 0),
-                 lambda: b.advance_chunks(plan), lambda: small.read(span, 0)):
+                 lambda: b.advance_chunks(plan), lambda: small.read(span, 0), lambda: b.read(span, 0)):
         with pytest.raises(ValueError, match="another cache"):
             call()
     with pytest.raises(ValueError, match="steps"):
         a.note_chunks(plan, -1)
-    k, v = a.read(span, 0)
-    assert all(torch.equal(x, y) for x, y in zip((k, v), b.read(span, 0)))  # (a span of tokens that b has, too)
 
 
 def test_steps_of_no_tokens():
