@@ -440,7 +440,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
             raise ValueError(f"inv_freq must be a contiguous fp32 tensor of {D // 2} elements on {dev}")
         given, (row, element) = qkv, qkv.stride()
         if element != 1 or row % 8 or qkv.data_ptr() % 16 or (row < width and shape[0] > 1):
-            qkv = qkv.contiguous()
+            qkv = qkv.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps rows that start between)
             row = width
         if q_out is None:
             q_out = torch.empty((total, hq, D), dtype=torch.float16, device=dev)
@@ -454,7 +454,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
                 raise ValueError("q_out must be qkv's q heads themselves or not overlap qkv")
         C.launch(dev, "nkv_paged_append_chunks_tok", qkv.data_ptr(), _DT[dtype], max(row, width), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
-                 plan.seq_ptr, *plan.where, plan.nseq, hq, hkv, D, _lib.ptr(q_gamma), _lib.ptr(k_gamma), eps,
+                 plan.seq_ptr, *plan.where, plan.nseq, hq, hkv, D, _lib.ptr(q_gamma), _lib.ptr(k_gamma), float(eps),
                  _lib.ptr(inv_freq), q_out.data_ptr(), max(q_out.stride(0), hq * D))
         return q_out
 
@@ -472,7 +472,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         C.of_cache(plan, self.pos)
         C.heads_of(query, "query", total, hq, dev)
         if not C.rows_in_place(query):
-            query = query.contiguous()
+            query = query.clone(memory_format=torch.contiguous_format)
         if out is None:
             out = torch.empty((total, hq, D), dtype=torch.float16, device=dev)
         else:

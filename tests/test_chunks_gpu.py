@@ -238,6 +238,22 @@ def test_append_in_place_and_strided():
     assert torch.equal(a.pages[0], c.pages[0])
 
 
+def test_rows_that_start_between_are_copied():
+    """Contiguous tensors whose first element is not on 16 bytes."""
+    cache = _held_with_step([70, 10], [30, 5], 8, 2, 22)
+    plan = cache.plan_chunks([30, 5])
+    qkv = _randn((35, 12 * D), 23).cuda()
+    q = cache.append_chunks(plan, qkv, 0)
+    pages, out = cache.pages[0].clone(), cache.attend_chunks(plan, q, 0)
+    odd = torch.empty(35 * 12 * D + 3, dtype=torch.float16, device="cuda")[3:].view(35, 12 * D)
+    odd.copy_(qkv)
+    assert odd.is_contiguous() and torch.equal(cache.append_chunks(plan, odd, 0, eps=np.float32(1e-6)), q)
+    assert torch.equal(cache.pages[0], pages)
+    odd_q = torch.empty(35 * 8 * D + 1, dtype=torch.float16, device="cuda")[1:].view(35, 8, D)
+    odd_q.copy_(q)
+    assert torch.equal(cache.attend_chunks(plan, odd_q, 0), out)
+
+
 def test_append_skips_tokens_without_a_page():
     cache = _cache([10, 50], [200, 30], 4, 2, 30)
     plan = cache.plan_chunks([200, 30])
@@ -397,6 +413,21 @@ def test_values_of_any_size(lens, counts, hq, hkv, scales):
     q = _randn((plan.total, hq, D), 147, 1.5).cuda()
     lse = torch.empty(plan.total, hq, device="cuda")
     _check_attention(cache, 0, plan, q, cache.attend_chunks(plan, q, 0, lse=lse), lse, lens)
+
+
+@pytest.mark.parametrize("counts", [[3, 4], [40, 30]])
+def test_a_query_that_is_not_finite_spoils_its_own_row(counts):
+    lens, hq, hkv = [300, 90], 4, 1
+    cache = _held_with_step(lens, counts, hq, hkv, 154)
+    plan = cache.plan_chunks(counts)
+    q = _randn((plan.total, hq, D), 155).cuda()
+    want = cache.attend_chunks(plan, q, 0)
+    bad = q.clone()
+    bad[1, 2, 7], bad[plan.total - 1, 0, 100], bad[0, 3, 5] = float("nan"), float("inf"), -float("inf")
+    got = cache.attend_chunks(plan, bad, 0)
+    rows = torch.zeros(plan.total, hq, dtype=torch.bool, device="cuda")
+    rows[1, 2] = rows[plan.total - 1, 0] = rows[0, 3] = True
+    assert torch.equal(got[~rows], want[~rows]) and bool(got[rows].isnan().all())
 
 
 def test_scores_that_grow_by_much():
