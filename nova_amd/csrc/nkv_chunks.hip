@@ -545,6 +545,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
   asm volatile("" : "+v"(ph[0]), "+v"(ph[1]));  // (P is made here, not sunk past the branch)
   // (one comparison for both)
   if (__builtin_amdgcn_ballot_w64(sum > (larger ? -1.0f : x.cap)) != 0) {
+    const bool own = max4rows(sum) > x.cap;  // (a row's result does not hang on its neighbours')
     float by = 0.0f;
     if (larger) {
       const float all = max4rows(row16_max((float)(scale() & 0x7fffu)));
@@ -564,7 +565,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
       for (int i = 0; i < 4; ++i) t = fmaxf(t, exponent(b, i, off));
     t = max4rows(t);
     const float moved = t - (x.top - W_TAU);
-    const float delta = first ? moved : fmaxf(moved, by);
+    const float delta = first ? moved : fmaxf(own ? moved : 0.0f, by);
     const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-delta);
     x.off = first && t == NEG_INF ? NO_SCORE : off - delta;
     x.l *= alpha;
