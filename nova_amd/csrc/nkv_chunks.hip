@@ -633,12 +633,6 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
   int64_t s = s0 + wave;
   const int mine = s < s1 ? (int)((s1 - s + W - 1) / W) : 0;  // groups of this wave
   Pages pg(a.b, u.seq, s, W, mine);
-  int page = pg.at(0);
-  if (page >= 0) {
-    issue_k(page);
-    issue_v(page, 0);
-  }
-
   half8_t qb[RB][4];
   int tq[RB];  // the token of row c: the last one that it attends
 #pragma unroll
@@ -655,6 +649,12 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
       qb[rb][k] = as_h8(w);
     }
   }
+  int page = pg.at(0);
+  if (page >= 0) {
+    issue_k(page);
+    issue_v(page, 0);
+  }
+
   const int64_t whole = (at.start + u.row0 / a.gq + 1) / GT;  // steps that every row of the tile sees whole
   const _Float16 one = (_Float16)1.0f;
   const half8_t ones = half8_t{one, one, one, one, one, one, one, one};
@@ -887,13 +887,9 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     return vs;
   };
 
-  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
-  issue(p0, 0);
-  issue(p1, 1);
-
   const int row0 = u.row0 + wave * (BG_RB * 16);  // first row of this wave
   const int rows = u.row0 + at.rows;
-  half8_t qb[BG_RB][4];
+  half8_t qb[BG_RB][4];  // (loaded beside the page ids)
 #pragma unroll
   for (int rb = 0; rb < BG_RB; ++rb) {
     const int row = row0 + 16 * rb + c;
@@ -907,6 +903,10 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
       qb[rb][k] = as_h8(w);
     }
   }
+  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
+  issue(p0, 0);
+  issue(p1, 1);
+
   RowState st[BG_RB];  // (codes are whole numbers here: acc is the sum of P code, psum stays 0)
 #pragma unroll
   for (int rb = 0; rb < BG_RB; ++rb) state_init(st[rb]);
