@@ -816,11 +816,12 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 // wait for the loads of group t + 2; after it the loads of group t + 4 into the stage of group t + 1.
 // Bound by the vector and matrix instructions' issue: a step of a wave has 64 matrix (16 cycles each on the SIMD that
 // two waves share), 32 exponentials and about 215 other instructions; 2048 tokens over 14336, 32 q and 8 KV heads (515
-// GFLOP) in 592 us, 870 TFLOP/s, where a large fp16 matrix product of the library reaches 1092; 2.3 us a step, and a
+// GFLOP) in 591 us, 872 TFLOP/s, where a large fp16 matrix product of the library reaches 1092; 2.3 us a step, and a
 // unit of one step takes 15 us (8 of them its queries' and outputs' traffic when 256 units run). Keys and values rounded
 // to fp16 instead of exact codes: 578 us, and twice the error. Slower were: waves of 64 rows, for want of registers;
 // the conversion at the start of the step in half of the waves (600 us); the largest score taken before the weights
-// (622 us).
+// (622 us). And this is about as much as the card's power allows: 32 x 32 x 16 products (half as many, twice the
+// accumulators' traffic) took 1.31 million cycles instead of 1.44, and 606 us, at 2.15 GHz instead of 2.4.
 constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
 constexpr int BG_TILE = GT * D * 2, BG_SCALES = 8 * GT;  // a tile's scales, 32 bytes for 4 tokens: K's in fp32, V's, 0
 constexpr int BG_KT = 2 * BG_SCALES, BG_VT = BG_KT + 2 * BG_TILE;  // scales, K tiles, V tiles, stages: what is read most
