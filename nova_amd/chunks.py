@@ -133,15 +133,13 @@ def _parts(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide
     rounds = -(-steps // waves)  # of a small unit: its waves take a group each
     most = np.minimum(MAX_PARTS, np.where(small, np.maximum(1, steps // SMALL_PART), steps))
     us = np.where(small, rounds * (waves * GROUP_US), steps * STEP_US)
-    best = None
-    for k in CUTS:
-        parts = np.clip(np.ceil(us * (k / us.max())).astype(np.int64), 1, most)
-        unit = np.where(small, -(-rounds // parts) * (waves * GROUP_US), us / parts) + UNIT_US
-        partials = int((np.where(parts > 1, parts * rows, 0)).sum()) * hkv
-        time = max(unit.max(), float((unit * parts).sum()) * hkv / slots) + (MERGE_US + partials * PARTIAL_US if partials else 0.0)
-        if best is None or time < best[0]:
-            best = time, parts
-    return best[1]
+    # (far more tiles than slots are not cut)
+    cuts = np.array(CUTS if len(steps) * hkv < 16 * slots else CUTS[:1])[:, None]
+    parts = np.clip(np.ceil(us * (cuts / us.max())).astype(np.int64), 1, most)
+    unit = np.where(small, -(-rounds // parts) * (waves * GROUP_US), us / parts) + UNIT_US
+    partials = (np.where(parts > 1, parts, 0) @ rows) * hkv
+    time = np.maximum(unit.max(1), (unit * parts).sum(1) * (hkv / slots)) + np.where(partials > 0, MERGE_US + partials * PARTIAL_US, 0.0)
+    return parts[time.argmin()]
 
 
 def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:
