@@ -383,7 +383,7 @@ struct ChunkArgs {
   int64_t q_ts, q_hs, tokens;
   const uint8_t* pages;
   const Unit* units;
-  int n_units, hq, gq;
+  int hq, gq;
   float sl2;
   uint16_t* out;
   int64_t o_ts, o_hs;
@@ -523,7 +523,8 @@ __device__ __forceinline__ float4_t offset_share(const half8_t (&qb)[4]) {
 // 2^top (16 weights of 2^(top - W_TAU) do not), or the group has a larger V scale than top allows (`larger`, of the
 // wave; scale(): the lane's token's), is off moved, what was summed up scaled, and the pass made again.
 template <class F, class V>
-__device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& exponent, const uint2 (&vs)[4], half8_t (&ph)[2], int g) {
+__device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& exponent, const uint2 (&vs)[4],
+                                      half8_t (&ph)[2], int g) {
   float sum;
   auto pass = [&]() {
     float part[4];
@@ -549,7 +550,8 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
     float by = 0.0f;
     if (larger) {
       const float all = max4rows(row16_max((float)(scale() & 0x7fffu)));
-      const uint32_t m = max((uint32_t)__builtin_amdgcn_readfirstlane((int)all), x.vs);  // (the other row block may be ahead)
+      // (this row block may be ahead of the one that `larger` was taken from)
+      const uint32_t m = max((uint32_t)__builtin_amdgcn_readfirstlane((int)all), x.vs);
       const float to = 30.0f - (float)(m >> 10);  // 2^15 over the power of two in the scale
       by = x.top - to;
       x.top = uniform(to);
@@ -926,7 +928,8 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        op[4 * k + b] = *reinterpret_cast<const half8_t*>(lds + (ka ^ (128 * (k >> 1) + 16 * (k & 1))) + (BG_KT + 16 * b * (2 * D)));
+        op[4 * k + b] = *reinterpret_cast<const half8_t*>(lds + (ka ^ (128 * (k >> 1) + 16 * (k & 1))) +
+                                                          (BG_KT + 16 * b * (2 * D)));
   };
   auto load_v = [&]() {
     asm volatile("" : "+v"(va));
@@ -959,8 +962,8 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     const int l = tail_tid() & 63;
     const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * (l >> 4);  // (masked: near the sequence's end, it fits)
     const int tq = (row0 + 16 * rb + (l & 15)) / a.gq;
-    weigh(st[rb], larger, [&]() { return *reinterpret_cast<const uint16_t*>(lds + (t & 1) * BG_SCALES + 32 * (l >> 2) + 16 + 2 * (l & 3)); },
-          [&](int b, int i, float off) {
+    auto scale = [&]() { return *reinterpret_cast<const uint16_t*>(lds + (t & 1) * BG_SCALES + 32 * (l >> 2) + 16 + 2 * (l & 3)); };
+    weigh(st[rb], larger, scale, [&](int b, int i, float off) {
       const float e = __builtin_fmaf(S[rb][b][i], ks[b][i], off);
       return decltype(masked)::value && tok0 + 16 * b + i > tq ? NEG_INF : e;
     }, vs, ph[rb], l >> 4);
@@ -1029,7 +1032,8 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     for (int rb = 0; rb < BG_RB; ++rb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float l = shfl(rl[rb], 4 * g + i), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f, m = shfl(reference(st[rb]), 4 * g + i);
+        const float l = shfl(rl[rb], 4 * g + i), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float m = shfl(reference(st[rb]), 4 * g + i);
         const int r = 16 * rb + 4 * g + i, row = row0 + r;
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb)
@@ -1289,7 +1293,7 @@ extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stri
       q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
     return fail(NKV_ERR_UNSUPPORTED, "%s: rows and buffers must be 16-byte aligned", what);
   a.q = q; a.q_ts = q_token_stride; a.q_hs = q_head_stride; a.tokens = tokens; a.pages = pages;
-  a.units = reinterpret_cast<const Unit*>(units); a.n_units = (int)n_units;
+  a.units = reinterpret_cast<const Unit*>(units);
   a.hq = (int)hq; a.gq = (int)(hq / hkv);
   a.sl2 = LOG2E / sqrtf((float)D);
   a.out = out; a.o_ts = out_token_stride; a.o_hs = out_head_stride; a.lse = lse_out;
