@@ -476,10 +476,11 @@ __device__ __forceinline__ half8_t whole8(uint32_t w0, uint32_t w1) {
 
 // The state of a row block. Weights are at most 2^top: with the largest V scale so far (as bits at most vs, which has
 // all of its exponent) P = weight times scale is 65504 at most, and no lower than that asks, so that small V lose
-// nothing to fp16's denormals. Of row c: off, what turns a score (log2 domain) into a weight's exponent, and l, the sum
-// of weights over the lane's tokens. Of rows 4 g + i: acc, the sum of P code (small units: 2^-24 P (code + 128), and
-// psum that of P). A row's largest score so far has an exponent of top - W_TAU at least; before its first score off is
-// NO_SCORE, with which any score passes top.
+// nothing to fp16's denormals. In a group that some row does not see whole, the largest scale differs from row to row:
+// there each row goes by those that it attends, for that group, and top stays. Of row c: off, what turns a score (log2
+// domain) into a weight's exponent, and l, the sum of weights over the lane's tokens. Of rows 4 g + i: acc, the sum of
+// P code (small units: 2^-24 P (code + 128), and psum that of P). A row's largest score so far has an exponent of its
+// top - W_TAU at least; before its first score off is NO_SCORE, with which any score passes top.
 constexpr float NO_SCORE = 3e38f;
 struct RowState {
   float top, cap;  // (the wave's lanes agree on top, cap = 2^top, and vs)
@@ -500,6 +501,15 @@ __device__ __forceinline__ void state_init(RowState& x) {
 // The score (log2 domain) whose weight is 1; -inf: no token yet.
 __device__ __forceinline__ float reference(const RowState& x) { return x.off == NO_SCORE ? NEG_INF : -x.off; }
 
+// The bits of the largest of the V scales (one token's a lane) up to token `reach` of the group.
+__device__ __forceinline__ uint32_t largest_up_to(uint32_t vs, int reach) {
+  int m = (int)(vs & 0x7fffu);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) m = max(m, __shfl_up(m, o));
+  m = __shfl(m, min(max(reach, 0), 63));
+  return reach < 0 ? 0u : (uint32_t)m;
+}
+
 // Whether a group has a V scale (its bits, one token's a lane) that lowers top.
 __device__ __forceinline__ bool larger_scale(const RowState& x, uint32_t vs) {
   return __builtin_amdgcn_ballot_w64((vs & 0x7fffu) > x.vs) != 0;
@@ -518,13 +528,15 @@ __device__ __forceinline__ float4_t offset_share(const half8_t (&qb)[4]) {
 }
 
 // The online softmax of a row block over 64 tokens. exponent(b, i, off): the weight's exponent of token 16 b + 4 g + i
-// and row c, its score plus off (-inf where masked); vs: the tokens' V scales; ph: the weights times those, in fp16, as
-// the operands of O = P V. The weights are taken with the off there is, without a maximum; only if a lane's sum passes
-// 2^top (16 weights of 2^(top - W_TAU) do not), or the group has a larger V scale than top allows (`larger`, of the
-// wave; scale(): the lane's token's), is off moved, what was summed up scaled, and the pass made again.
-template <class F, class V>
-__device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& exponent, const uint2 (&vs)[4],
-                                      half8_t (&ph)[2], int g) {
+// and row c, its score plus off (-inf where masked); vs: the tokens' V scales; ph: the weights times those, in fp16,
+// as the operands of O = P V. The weights are taken with the off there is, without a maximum; only if a lane's sum
+// passes 2^top (16 weights of 2^(top - W_TAU) do not), or the group has a larger V scale than top allows (`larger`, of
+// the wave; scale(): the lane's token's), is off moved, what was summed up scaled, and the pass made again. masked:
+// some row does not see the group whole; reach(): the last token that row c attends, counted in the group (any
+// integer).
+template <class M, class F, class V, class R>
+__device__ __forceinline__ void weigh(RowState& x, bool larger, M masked, V&& scale, R&& reach, F&& exponent,
+                                      const uint2 (&vs)[4], half8_t (&ph)[2], int g) {
   float sum;
   auto pass = [&]() {
     float part[4];
@@ -546,9 +558,14 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
   asm volatile("" : "+v"(ph[0]), "+v"(ph[1]));  // (P is made here, not sunk past the branch)
   // (one comparison for both)
   if (__builtin_amdgcn_ballot_w64(sum > (larger ? -1.0f : x.cap)) != 0) {
-    const bool own = max4rows(sum) > x.cap;  // (a row's result does not hang on its neighbours')
-    float by = 0.0f;
-    if (larger) {
+    float cap = x.cap, top = x.top, by = 0.0f;
+    if (masked && larger) {
+      const uint32_t m = max(largest_up_to(scale(), reach()), x.vs);
+      top = 30.0f - (float)(m >> 10);
+      cap = __builtin_amdgcn_exp2f(top);
+    }
+    const bool own = max4rows(sum) > cap;  // (a row's result does not hang on its neighbours')
+    if (!masked && larger) {
       const float all = max4rows(row16_max((float)(scale() & 0x7fffu)));
       // (this row block may be ahead of the one that `larger` was taken from)
       const uint32_t m = max((uint32_t)__builtin_amdgcn_readfirstlane((int)all), x.vs);
@@ -557,6 +574,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
       x.top = uniform(to);
       x.cap = uniform(__builtin_amdgcn_exp2f(to));
       x.vs = m | 0x3ffu;
+      top = x.top;
     }
     const bool first = x.off == NO_SCORE;
     float off = first ? 0.0f : x.off, t = NEG_INF;
@@ -566,7 +584,7 @@ __device__ __forceinline__ void weigh(RowState& x, bool larger, V&& scale, F&& e
 #pragma unroll
       for (int i = 0; i < 4; ++i) t = fmaxf(t, exponent(b, i, off));
     t = max4rows(t);
-    const float moved = t - (x.top - W_TAU);
+    const float moved = t - (top - W_TAU);
     const float delta = first ? moved : fmaxf(own ? moved : 0.0f, by);
     const float alpha = first ? 1.0f : __builtin_amdgcn_exp2f(-delta);
     x.off = first && t == NEG_INF ? NO_SCORE : off - delta;
@@ -697,7 +715,7 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     auto own_scale = [&]() -> uint32_t {
       const int l = tail_tid() & 63;
       const uint32_t v = *reinterpret_cast<const uint16_t*>(slot + CODE_BYTES + 2 * GT + 2 * l);
-      return s >= whole && (int)(s * GT - at.start) + l >= fresh ? 0u : v;
+      return s >= whole && (!finite_h(v) || (int)(s * GT - at.start) + l >= fresh) ? 0u : v;
     };
     const bool larger = larger_scale(st[0], own_scale());
     float S[RB][4][4];  // scores, times 2^-24, in the natural domain
@@ -742,7 +760,8 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
     half8_t ph[RB][2];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
-      weigh(st[rb], larger, own_scale,
+      weigh(st[rb], larger, s >= whole, own_scale,
+            [&]() { return tq[rb] - (int)(s * GT - at.start); },
             [&](int b, int i, float off) { return __builtin_fmaf(S[rb][b][i], sl2, off); }, vs, ph[rb], g);
     const int vl = tail_tid() & 63, vc = vl & 1, vr = (vl & 15) >> 1, vg = vl >> 4;
 #pragma unroll
@@ -963,7 +982,9 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 4 * (l >> 4);  // (masked: near the sequence's end, it fits)
     const int tq = (row0 + 16 * rb + (l & 15)) / a.gq;
     auto scale = [&]() { return *reinterpret_cast<const uint16_t*>(lds + (t & 1) * BG_SCALES + 32 * (l >> 2) + 16 + 2 * (l & 3)); };
-    weigh(st[rb], larger, scale, [&](int b, int i, float off) {
+    auto reach = [&]() { return tq - (int)((int64_t)(s0 + t) * GT - at.start); };
+    const bool part = decltype(masked)::value && __builtin_amdgcn_readfirstlane(reach()) < GT - 1;  // (the first row's)
+    weigh(st[rb], larger, part, scale, reach, [&](int b, int i, float off) {
       const float e = __builtin_fmaf(S[rb][b][i], ks[b][i], off);
       return decltype(masked)::value && tok0 + 16 * b + i > tq ? NEG_INF : e;
     }, vs, ph[rb], l >> 4);
@@ -1027,6 +1048,7 @@ __device__ __forceinline__ void attend_big(const ChunkArgs& a, const Unit& u, in
     // ---- out = the sum of V / l, through LDS so that 16 lanes store a row's 256 bytes (the 2-byte values
     // at chunk ^ 2 ((row >> 2) & 3))
     __syncthreads();  // every wave is past its last read of the tiles
+    const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4;  // (made again, for want of registers in the loop)
     uint8_t* ow = lds + wave * (BG_RB * 16 * D * 2);
 #pragma unroll
     for (int rb = 0; rb < BG_RB; ++rb)

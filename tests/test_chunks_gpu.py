@@ -791,3 +791,53 @@ def test_pages_beyond_four_gigabytes():
     k, _ = cache.read(plan, 0)
     assert np.array_equal(k.cpu().numpy(), _values(cache, 0, 0, n)[0].astype(np.float16))
     assert int(cache.pages[0][:pages - 2].count_nonzero()) == 0
+
+
+# ---------------------------------------------------------------- tokens that a row does not attend
+
+
+@pytest.mark.parametrize("small", [2.0 ** -9, 2.0 ** -12, 2.0 ** -20])
+@pytest.mark.parametrize("lens,counts,hq,hkv", [
+    ([10], [4], 4, 1),      # 16 rows
+    ([30], [8], 8, 2),      # 16 and 16 rows of two heads
+    ([70], [9], 3, 1),      # 27 rows
+    ([128], [16], 4, 1),    # two tiles of 32 rows
+    ([300, 7], [6, 20], 4, 1),
+    ([20], [40], 4, 1),     # a wide tile in one group
+    ([0], [130], 2, 1),     # a wide tile that begins with masked places, and one of 4 rows
+    ([500, 33], [70, 5], 2, 1),
+])
+def test_a_later_tokens_scale_changes_nothing_before_it(lens, counts, hq, hkv, small):
+    """V scales that are large or not finite, in tokens of the same step: the rows before such a token give the bits
+    that they give beside an ordinary one, within the bound of the values that they attend."""
+    cache = _held_with_step(lens, counts, hq, hkv, 180)
+    halves = cache.pages[0].view(torch.float16)
+    for b in range(len(lens)):
+        for g in range(-(-(lens[b] + counts[b]) // GT)):
+            halves[int(cache.page_table[b, g]), :, 8192 + 64:] = small
+    plan = cache.plan_chunks(counts)
+    q = _randn((plan.total, hq, D), 181, 1.5).cuda()
+    want = cache.attend_chunks(plan, q, 0).clone()
+    q64, gq, at = q.double().cpu().numpy(), hq // hkv, 0
+    for b, n in enumerate(counts):
+        for j in sorted({1, n * 3 // 4, n - 1}):
+            k, v = _values(cache, 0, b, lens[b] + j)
+            exact, _, tol = _attend64(q64[at:at + j], k, v, lens[b], gq)
+            page, place = int(cache.page_table[b, (lens[b] + j) // GT]), (lens[b] + j) % GT
+            for bad in (float("inf"), float("nan"), -float("inf"), 60000.0, 500.0, -500.0):
+                print(f"case sequence {b} token {j} scale {bad}", flush=True)
+                halves[page, :, 8192 + 64 + place] = bad
+                got = cache.attend_chunks(plan, q, 0)
+                err = np.abs(got[at:at + j].double().cpu().numpy() - exact)
+                assert (err <= tol).all(), f"off by {(err / tol).max():.2f} of the bound"
+                others = torch.ones(plan.total, dtype=torch.bool, device="cuda")
+                others[at + j:at + n] = False
+                assert torch.equal(got[others], want[others])
+                if abs(bad) == 500.0:
+                    k2, v2 = _values(cache, 0, b, lens[b] + n)
+                    late, _, tol2 = _attend64(q64[at + j:at + n], k2, v2, lens[b] + j, gq)
+                    assert (np.abs(got[at + j:at + n].double().cpu().numpy() - late) <= tol2).all()
+                elif not np.isfinite(bad):
+                    assert not bool(got[at + j:at + n].isfinite().any())
+            halves[page, :, 8192 + 64 + place] = small
+        at += n
