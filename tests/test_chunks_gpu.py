@@ -841,3 +841,32 @@ def test_a_later_tokens_scale_changes_nothing_before_it(lens, counts, hq, hkv, s
                     assert not bool(got[at + j:at + n].isfinite().any())
             halves[page, :, 8192 + 64 + place] = small
         at += n
+
+
+@pytest.mark.parametrize("tokens", [131072, 1 << 20])
+@pytest.mark.parametrize("n", [1, 20])
+def test_sums_over_long_contexts_keep_their_precision(n, tokens):
+    """A plan made while the sequence was short leaves all of a long context to one unit of four waves. Queries of zero
+    give every token the same weight, a power of two, so that nothing but the sums' roundings is left: values of one
+    code, +1 or -1, times a scale of each head, come out as they are. Half a step of the sum of P times a code and of
+    the sum of P, for each of their additions (up to four in a matrix instruction, which takes 32 tokens), with the
+    codes' offset of 128 in them for at most 16 groups; a lane's sum of weights, one addition a group; the output."""
+    hkv = 8
+    cache = PagedKVInt8TokCache(1, hkv, D, hkv, max_seqs=1, num_pages=8, max_pages_per_seq=tokens // GT)
+    plan = cache.plan_chunks([n])
+    assert len(plan.units) == 1 and not plan.wide
+    cache.page_table[0] = torch.arange(tokens // GT, dtype=torch.int32) % 8
+    scales = torch.tensor([0.02, 0.0123, 0.7, 1.001, 0.333, 0.00731, 0.05, 0.11]).half()
+    sign = torch.where(torch.arange(D) % 2 == 0, 1, -1).to(torch.int8)
+    pool = cache.pages[0]
+    pool[:, :, 8192:16384] = sign.repeat(GT).view(torch.uint8).cuda()
+    pool.view(torch.float16)[:, :, 8192:8192 + GT] = 1.0
+    pool.view(torch.float16)[:, :, 8192 + GT:] = scales.cuda()[:, None]
+    cache.pos[0] = tokens - n
+    out = cache.attend_chunks(plan, torch.zeros(n, hkv, D, dtype=torch.float16, device="cuda"), 0).double().cpu().numpy()
+    want = scales.double().numpy()[:, None] * sign.double().numpy()
+    groups, held = tokens // GT // 4, 16  # of a wave; that the offset's share stays for
+    adds = 4 * (groups + 2 * held * GT + 2 * held * GT) + groups / 2 + groups / held + 16
+    err = np.abs(out - want) / np.abs(want)
+    print(f"off by {err.max() / U16:.2f} half steps of fp16, allowed {1 + adds * 2.0 ** -24 / U16:.2f}", flush=True)
+    assert (err <= U16 + adds * 2.0 ** -24).all()
