@@ -187,6 +187,14 @@ def of_cache(plan: SpanPlan, pos: torch.Tensor) -> None:
         raise ValueError("the plan was made by another cache")
 
 
+def step_of_cache(plan: SpanPlan, pos: torch.Tensor) -> None:
+    """``plan`` must be a step's plan (``plan_chunks``) of the cache: one of ``plan_read`` names cached tokens, which a
+    step would overwrite."""
+    of_cache(plan, pos)
+    if not isinstance(plan, ChunkPlan):
+        raise ValueError("the plan was made by plan_read; a step takes one of plan_chunks")
+
+
 def heads_of(x: torch.Tensor, name: str, tokens: int, heads: int, device: torch.device) -> None:
     """``x`` must be fp16 ``[>= tokens, heads, 128]`` on ``device``."""
     shape = x.shape

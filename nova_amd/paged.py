@@ -424,7 +424,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         128]``, or writes ``q_out``, which may be qkv's own q heads; rows after the plan's tokens are neither
         read nor written."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
-        C.of_cache(plan, self.pos)
+        C.step_of_cache(plan, self.pos)
         shape, dtype, width = qkv.shape, qkv.dtype, (hq + 2 * hkv) * D
         if len(shape) != 2 or shape[0] < total or shape[1] != width or dtype not in _DT or qkv.device != dev:
             raise ValueError(f"qkv must be fp16 / bf16 / fp32 [{total}, {width}] on {dev} (more tokens may "
@@ -469,7 +469,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         without a page take no part; a token with none gets 0 and -inf. Rows after the plan's tokens are neither
         read nor written. Calls may overlap on streams (each has its own scratch memory)."""
         hq, hkv, dev, total = self.num_q_heads, self.num_kv_heads, self.pos.device, plan.total
-        C.of_cache(plan, self.pos)
+        C.step_of_cache(plan, self.pos)
         C.heads_of(query, "query", total, hq, dev)
         if not C.rows_in_place(query):
             query = query.clone(memory_format=torch.contiguous_format)
@@ -504,7 +504,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
     def note_chunks(self, plan: ChunkPlan, steps: int = 1, accepted: list[int] | None = None) -> None:
         """Host bookkeeping of ``steps`` steps that advanced ``pos`` on the device (:meth:`advance_chunks`, or a
         replayed graph that adds ``plan.new`` to ``pos[:plan.nseq]``)."""
-        C.of_cache(plan, self.pos)
+        C.step_of_cache(plan, self.pos)
         if steps < 0:
             raise ValueError(f"{steps} steps")
         moved = plan.counts if accepted is None else C.check_counts(accepted, self.max_seqs, "accepted")

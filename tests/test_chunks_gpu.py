@@ -870,3 +870,18 @@ def test_sums_over_long_contexts_keep_their_precision(n, tokens):
     err = np.abs(out - want) / np.abs(want)
     print(f"off by {err.max() / U16:.2f} half steps of fp16, allowed {1 + adds * 2.0 ** -24 / U16:.2f}", flush=True)
     assert (err <= U16 + adds * 2.0 ** -24).all()
+
+
+def test_plans_to_read_are_no_steps():
+    cache = _cache([70, 20], [10, 10], 8, 2, 190)
+    span = cache.plan_read([5, 6], [60, 0])
+    qkv, q = _randn((11, 12 * D), 191).cuda(), _randn((11, 8, D), 192).cuda()
+    before, lens = cache.pages[0].clone(), list(cache._len)
+    for call in (lambda: cache.append_chunks(span, qkv, 0), lambda: cache.attend_chunks(span, q, 0),
+                 lambda: cache.advance_chunks(span), lambda: cache.advance_chunks(span, [1, 1]), lambda: cache.note_chunks(span)):
+        with pytest.raises(ValueError, match="plan_read"):
+            call()
+    assert torch.equal(cache.pages[0], before) and cache._len == lens and cache.pos.tolist() == lens
+    plan = cache.plan_chunks([3, 2])  # a step's plan reads what the step stored
+    cache.append_chunks(plan, qkv[:5], 0)
+    assert cache.read(plan, 0)[0].shape == (5, 2, D)
