@@ -885,3 +885,84 @@ def test_plans_to_read_are_no_steps():
     plan = cache.plan_chunks([3, 2])  # a step's plan reads what the step stored
     cache.append_chunks(plan, qkv[:5], 0)
     assert cache.read(plan, 0)[0].shape == (5, 2, D)
+
+
+# ---------------------------------------------------------------- the forms that the call's size chooses
+
+
+@pytest.mark.parametrize("lens,counts,hq,hkv,dtype,norm,rope,pad", [
+    # from 256 tokens all heads of a token in one workgroup; more than 64 of them (32 of fp32) in several rounds of loads
+    ([30], [300], 64, 8, torch.float16, True, True, 1),
+    ([3], [260], 72, 8, torch.bfloat16, True, True, 0),
+    ([0], [300], 40, 4, torch.float32, True, True, 0),
+    # from 2048 tokens the queries pass the caches
+    ([0, 100], [2000, 61], 32, 8, torch.float16, True, True, 2),
+    ([5], [2100], 4, 2, torch.bfloat16, False, True, 0),
+    ([0], [2050], 8, 2, torch.float32, True, False, 0),
+])
+def test_append_of_many_tokens(lens, counts, hq, hkv, dtype, norm, rope, pad):
+    test_append_against_64_bits(lens, counts, hq, hkv, dtype, norm, rope, pad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cls", [PagedKVInt8TokCache, PagedKVInt8Cache])
+@pytest.mark.parametrize("lens,counts,starts,hkv", [
+    ([700, 129, 333], None, None, 8),                            # four tokens a workgroup, the last one less
+    ([2000, 1500, 64], [1900, 0, 63], [37, 1, 1], 3),
+    ([9000, 77, 8000], None, None, 8),                           # sixteen, the last one less
+    ([5000, 16000, 700], [4801, 15900, 3], [199, 50, 640], 7)])
+def test_read_of_many_tokens(lens, counts, starts, hkv, cls, dtype):
+    cache = _cache(lens, [3] * len(lens), hkv, hkv, 200, cls=cls)
+    plan = cache.plan_read(counts, starts)
+    counts = lens if counts is None else counts
+    starts = [0] * len(lens) if starts is None else starts
+    assert plan.total * hkv > 4096
+    print(f"case read {cls.__name__} {lens} {dtype}: {plan.total} tokens", flush=True)
+    room = tuple(torch.full((plan.total + 3, hkv, D), 5.0, dtype=dtype, device="cuda") for _ in range(2))
+    cache.read(plan, 0, dtype, out=room)
+    assert all(bool((x[plan.total:] == 5.0).all()) for x in room)
+    at = 0
+    for b, (first, n) in enumerate(zip(starts, counts)):
+        end = first + n
+        pages = cache.pages[0][cache.page_table[b, :-(-end // GT)].long()]
+        for got, which in zip(room, (0, 1)):
+            codes = pages[:, :, 8192 * which:8192 * (which + 1)]
+            if cls is PagedKVInt8TokCache:
+                scales = pages[:, :, 16384 + 128 * which:16384 + 128 * (which + 1)].contiguous().view(torch.float16)
+                x = codes.contiguous().view(torch.int8).unflatten(2, (GT, D)).float() * scales[..., None].float()  # (exact)
+            else:
+                step, low = pages[:, :, 16384 + 512 * which:16384 + 512 * (which + 1)].contiguous().view(torch.float16).split(D, 2)
+                x = (codes.unflatten(2, (GT, D)).double() * step[:, :, None].double() + low[:, :, None].double()).float()
+            x = x.transpose(1, 2).flatten(0, 1)
+            if cls is PagedKVInt8Cache and end > lens[b] // GT * GT:
+                left = lens[b] - lens[b] // GT * GT
+                x[lens[b] // GT * GT:][:left] = cache.rings[0][b, :, which, :left].transpose(0, 1).float()
+            assert torch.equal(got[at:at + n], x[first:end].to(dtype)), (b, which)
+        at += n
+
+
+@pytest.mark.parametrize("lens,counts,hq", [
+    ([20500], [3], 16),             # four waves of 81 groups each, rows in tiles of 32 and 16
+    ([20500], [1], 2),
+    ([6100, 36000], [70, 3], 2),    # a wide tile over 96 groups, and eight waves of 71 groups beside it
+    ([36000, 10], [9, 300], 3),
+])
+def test_waves_of_more_groups_than_page_ids_at_once(lens, counts, hq):
+    """A plan made while the sequences were short cuts nothing: each wave takes more groups than it holds page ids for.
+    Each query is one and a half times a key of its own, spread over all groups, so that this token has most of the weight.
+    (A lane's and an accumulator's additions stay within the 256 of the bound.)"""
+    cache = _held_with_step(lens, counts, hq, 1, 210)
+    for b in range(len(lens)):
+        cache.pool.set_length(b, 0)
+    plan = cache.plan_chunks(counts)
+    units = plan.units.cpu()
+    assert bool((units[units[:, 0] == int(np.argmax(lens)), 4] == 1).all())
+    q, at = torch.empty(plan.total, hq, D, dtype=torch.float16), 0
+    for b, n in enumerate(counts):
+        k, _ = _values(cache, 0, b, lens[b] + n)
+        token = (np.arange(n * hq) * (lens[b] / (n * hq)) + 31).astype(np.int64) % (lens[b] + 1)
+        q[at:at + n] = torch.from_numpy(1.5 * k[token, 0]).half().view(n, hq, D)
+        at += n
+    lse = torch.empty(plan.total, hq, device="cuda")
+    out = cache.attend_chunks(plan, q.cuda(), 0, lse=lse)
+    _check_attention(cache, 0, plan, q, out, lse, lens)
