@@ -72,6 +72,8 @@ static_assert(DMA_FIRST_HALF == 12 && DMA_SECOND_HALF == 8 && DMA_HALF_TOK == 10
 static_assert(PAGE_BYTES % 128 == 0 && PAGE_TOK_BYTES % 128 == 0, "pages are 128-byte aligned");
 static_assert(LDS_BYTES <= 150 * 1024 && LDS_BYTES_TOK <= 150 * 1024, "LDS of one workgroup");
 
+typedef short v4s_t __attribute__((vector_size(8)));
+typedef __attribute__((address_space(3))) v4s_t lds_v4s_t;
 
 enum TailMode : int { TAIL_NONE = 0, TAIL_MASK = 1, TAIL_SCALARS = 2, TAIL_FUSED = 3 };
 // TAIL_FUSED with `tok`: the new token itself is the tail (its codes written by the prefix kernel).
@@ -190,6 +192,21 @@ __device__ __forceinline__ int parts_used(const AttnArgs& a, int64_t U) {
 // fp16 ring tensor in LDS: row r (256 B) keeps its 16-byte chunk c at position c ^ (r & 15),
 // so the 16 rows a K operand read touches land on 16 distinct banks.
 __device__ __forceinline__ int ring_chunk_pos(int row, int chunk) { return chunk ^ (row & 15); }
+
+// Online-softmax state of one wave. m, l: head (lane & 15), log2 domain; m is a reference
+// maximum (at least every score seen so far, times sl2), the weights are 2^(s sl2 - m + 15).
+// acc[cb][i]: head 4*(lane>>4) + i, dim 16*cb + (lane&15), in the same scale.
+struct WaveState {
+  float m, l;
+  float4_t acc[8];
+};
+
+__device__ __forceinline__ void state_init(WaveState& st) {
+  st.m = NEG_INF;
+  st.l = 0.0f;
+#pragma unroll
+  for (int cb = 0; cb < 8; ++cb) st.acc[cb] = float4_t{0.f, 0.f, 0.f, 0.f};
+}
 
 // 8 codes (bytes of w0, w1) -> fp16(code * st + mn) per element, rulers per element.
 __device__ __forceinline__ half8_t dq8(uint32_t w0, uint32_t w1, uint4 st, uint4 mn) {
@@ -726,6 +743,24 @@ __device__ __forceinline__ void pv_qk_half(WaveState& st, const uint8_t* vc, con
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[b][i] = S[b][i];
+}
+
+// fp16(code * scale) for 8 signed codes sharing one fp16 scale, and for 8 codes with one
+// scale each: the product of an 8-bit integer and an fp16 is exact in fp32, so the packed
+// fp16 multiply rounds it once, as fp16(fp32(code) * fp32(scale)) does.
+__device__ __forceinline__ half8_t dq8_sym(uint32_t w0, uint32_t w1, half2_t s) {
+  const half2_t a = scodes_to_h2(w0, kSelB01) * s;
+  const half2_t b = scodes_to_h2(w0, kSelB23) * s;
+  const half2_t c = scodes_to_h2(w1, kSelB01) * s;
+  const half2_t d = scodes_to_h2(w1, kSelB23) * s;
+  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+__device__ __forceinline__ half8_t dq8_sym_v(uint32_t w0, uint32_t w1, uint4 s) {
+  const half2_t a = scodes_to_h2(w0, kSelB01) * as_h2(s.x);
+  const half2_t b = scodes_to_h2(w0, kSelB23) * as_h2(s.y);
+  const half2_t c = scodes_to_h2(w1, kSelB01) * as_h2(s.z);
+  const half2_t d = scodes_to_h2(w1, kSelB23) * as_h2(s.w);
+  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
 // attend_block for 32 tokens of the per-token symmetric format: codes as in attend_block
@@ -3246,6 +3281,7 @@ constexpr int PF_WG_PER_CU = 1;                      // workgroups resident per 
 constexpr int PF_ROWS = PF_WAVES * PF_RB * 16;       // 256 query rows per workgroup
 constexpr int PF_KROW = D + 8;                       // fp16 K tile row stride (halves)
 constexpr int PF_VROW = GT + 16;                     // fp16 V^T tile row stride (halves, 16-byte rows)
+constexpr float PF_TAU = 8.0f;                       // lazy softmax rescaling threshold (log2)
 constexpr int PF_PART = D + 4;                       // floats per row partial: acc[128], m, l, pad
 constexpr int PF_MAX_SHARES = CUS;                   // shares of a head's steps (one workgroup per CU)
 constexpr int PF_STAGE = 2 * GT * D * 2;             // bytes of a stage: an fp16 group, or an int8 one with its rulers
@@ -3324,6 +3360,40 @@ struct PrefillMergeArgs {
   int M, gq, hkv, slots, slot_rows, two_slots, n;
   PrefillMerge t[PF_MAX_SHARES];
 };
+
+// Online softmax of one 16-row block over 64 tokens, from the raw scores S[b][i] (token
+// 16b + 4g + i, row c; -inf where masked): m is a reference maximum in the log2 domain, within
+// PF_TAU below the row's maximum of S * sl2, and P comes out as exp2(S sl2 - m + 15 - PF_TAU)
+// <= 2^15 in two fp16 A operands (tokens of blocks 0,1 and 2,3). The row sums of P are taken on
+// the matrix core by the caller (P times a ones operand, in the accumulator layout), which leaves
+// the VALU the maximum, the exponentials and the conversions; the caller rescales the
+// accumulators and those sums by alpha, only when m moves.
+__device__ __forceinline__ void pf_softmax(WaveState& st, const float (&S)[4][4], float sl2, half8_t (&ph)[2],
+                                           float& alpha_out, bool& moved_out) {
+  float smax = NEG_INF;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) smax = fmaxf(smax, S[b][i]);
+  smax = max4rows(smax);
+  const float m_cand = fmaxf(st.m, smax * sl2);
+  const float m_new = m_cand > st.m + PF_TAU ? m_cand : st.m;
+  const float m_use = m_new == NEG_INF ? 0.0f : m_new;
+  const float alpha = __builtin_amdgcn_exp2f(st.m - m_use);
+  const float off = 15.0f - PF_TAU - m_use;
+  _Float16 p16[2][8];
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      p16[b >> 1][4 * (b & 1) + i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(S[b][i], sl2, off));
+#pragma unroll
+  for (int B = 0; B < 2; ++B)
+    ph[B] = half8_t{p16[B][0], p16[B][1], p16[B][2], p16[B][3], p16[B][4], p16[B][5], p16[B][6], p16[B][7]};
+  moved_out = st.m != m_new;
+  alpha_out = alpha;
+  st.m = m_new;
+}
 
 __global__ __launch_bounds__(PF_THREADS, PF_WG_PER_CU) void prefill_chunk_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][PF_STAGE];
