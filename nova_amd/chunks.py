@@ -27,11 +27,12 @@ ROWS16, ROWS32, ROWS256 = 0, 1, 2  # unit kinds
 TILE_ROWS = {ROWS16: 16, ROWS32: 32, ROWS256: 256}  # query rows (tokens x q heads per KV head) of a tile, at most
 MERGE_ROWS = 8   # rows a merge entry covers
 MAX_PARTS = 256
-# Rows of a sequence from which its tiles are ROWS256 (32 query and 8 KV heads; as ROWS256 / as ROWS32):
-#   64 rows over 32000 tokens 54 / 42 us, 96 rows 55 / 56 us, 8 times 128 rows over 4000 tokens 55 / 58 us, 256 rows 64 / 89 us
+# Rows of a sequence from which its tiles are ROWS256 (32 query and 8 KV heads; all as ROWS256 / as ROWS32): 64 rows over
+# 32000 tokens 52 / 32 us, 96 rows 52 / 49, 8 times 128 rows over 4000 tokens 53 / 42, 256 rows 62 / 65. (Set when the
+# small units were slower, at 42, 56, 58 and 89 us: up to about 200 rows they are now the faster ones.)
 BIG_FROM = 64
-# 64-token groups of a small unit's part, at least: 32 rows over 4000 tokens 20 us (8: 25), 4 times one token over
-# 2000 10.9 us (8: 12.3; 1: 10.9)
+# 64-token groups of a small unit's part, at least: 32 rows over 4000 tokens 16.4 us (8: 18.8; 1: 15.7), 4 times one
+# token over 2000 12.4 us (8: 13.4; 1: 12.4)
 SMALL_PART = 4
 # prices of a cut in us: a step of a wide tile, a group of a small one with the card full of them, a unit's start and end,
 # the second launch, a partial row written and read. The cut that they choose is within 10% of the best of CUTS for every

@@ -164,8 +164,8 @@ struct AppendArgs {
 // before the angles and the page are known.
 // Bound by memory: 4112 tokens of 32 q and 8 KV heads (93 MB) in 20.6 us, 4.5 TB/s (a large copy reaches 4.9); four
 // tokens a workgroup without the loads ahead took 25.8 us. 1029 bf16 tokens of 28 q and 4 KV heads 7.3
-// us; 12 tokens 3.7 us, the time of the chain sequence, position and table, angles, rows. NT: nontemporal q stores, for
-// calls whose queries no L2 would hold until they are read (4112 tokens: 20.6 against 21.4 us).
+// us (21 MB, 2.9 TB/s: a workgroup's chain takes about as long as its data); 12 tokens 3.7 us, the time of the chain
+// sequence, position and table, angles, rows. NT: nontemporal q stores.
 template <int DT, bool NT>
 __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) float turn[2][D / 2];  // cos, sin
@@ -857,8 +857,7 @@ __device__ __forceinline__ void attend_small(const ChunkArgs& a, const Unit& u, 
 // unit of one step takes 15 us (8 of them its queries' and outputs' traffic when 256 units run). Keys and values rounded
 // to fp16 instead of exact codes: 578 us, and twice the error. Slower were: waves of 64 rows, for want of registers;
 // the conversion at the start of the step in half of the waves (600 us); the largest score taken before the weights
-// (622 us). And this is about as much as the card's power allows: 32 x 32 x 16 products (half as many, twice the
-// accumulators' traffic) took 1.31 million cycles instead of 1.44, and 606 us, at 2.15 GHz instead of 2.4.
+// (622 us); 32 x 32 x 16 products (606 us: half as many, twice the accumulators' traffic).
 constexpr int BG_RB = 2, BG_ROWS = CH_WAVES * BG_RB * 16, BG_STAGES = 3;
 constexpr int BG_TILE = GT * D * 2, BG_SCALES = 8 * GT;  // a tile's scales, 32 bytes for 4 tokens: K's in fp32, V's, 0
 constexpr int BG_KT = 2 * BG_SCALES, BG_VT = BG_KT + 2 * BG_TILE;  // scales, K tiles, V tiles, stages: what is read most
@@ -1199,7 +1198,11 @@ int batch_args(const char* what, Batch& b, const int32_t* seq_of, bool need_seq_
 }
 
 // The heads of few tokens are spread over workgroups (12 tokens: 3.7 us, all 48 heads in one 4.6 us), those of many
-// are not (1029 tokens: 7.3 us, spread 8.6 us; 4112 tokens 20.6 and 25.8 us: each workgroup makes the angles).
+// are not (1029 tokens: 7.3 us, spread 8.6 us; 4112 tokens 20.6 and 25.8 us: each workgroup makes the angles). From 2048
+// tokens the queries are stored past the caches (us nontemporal / ordinary, 32 q and 8 KV heads): 2048 tokens 12.0 /
+// 12.8, 4112 20.1 / 20.7; 8 and 2 heads, 4112 tokens 9.6 / 10.3; 4 and 2, 16000 26.1 / 26.5. With a kernel that reads
+// the queries next, both: 19.7 / 20.1, 31.9 / 31.1, 14.9 / 16.1, 33.3 / 32.6. Few tokens gain nothing (300: 5.1 / 5.1).
+// In between it would gain, too (1029 tokens 7.9 / 8.9, with the reader 12.7 / 15.0).
 template <int DT>
 void launch_append(const AppendArgs& a, hipStream_t s) {
   const int heads = a.hq + 2 * a.b.hkv;
