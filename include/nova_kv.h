@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define NKV_ABI_VERSION 13
+#define NKV_ABI_VERSION 14
 
 #define NKV_OK 0
 #define NKV_ERR_INVALID 1     /* argument outside what the reference accepts */
@@ -810,6 +810,62 @@ int nkv_swiglu_gemv(const uint16_t* x, const uint16_t* gamma, float eps, const u
  */
 int nkv_qk_norm_rope(uint16_t* qkv, int64_t hq, int64_t hkv, int64_t head_dim, const uint16_t* q_gamma,
                      const uint16_t* k_gamma, float eps, const float* inv_freq, const int64_t* pos, void* stream);
+
+/* ---------------------------------------------------------------- 4 bits
+ *
+ * One format for weights and for a paged cache (no counterpart in the reference). 32 consecutive values of a row
+ * share a scale: with amax their largest magnitude, s = max(amax / 7, 2^-24) in fp32, rounded to 8 significant bits
+ * (to nearest, ties to even) and held in fp16 (infinite where 7 s passes 65504, NaN for a group with a NaN);
+ * code = clamp(rint(x / s), -7, 7), value = code * s, which fp16 holds exactly. Byte i of a row holds code + 8 of value
+ * 2 i in its low half and that of value 2 i + 1 in its high half: n / 2 bytes a row of n values, n a multiple of 32.
+ *
+ * nkv_quantize_q4: x [rows][n] of x_dtype (contiguous, 16-byte aligned) to codes [rows][n / 2] (16-byte aligned) and
+ * scales [rows][n / 32]; nkv_dequantize_q4: back to out_dtype, one rounding of code * s.
+ */
+int nkv_quantize_q4(const void* x, int x_dtype, int64_t rows, int64_t n, uint8_t* codes, uint16_t* scales, void* stream);
+int nkv_dequantize_q4(const uint8_t* codes, const uint16_t* scales, int64_t rows, int64_t n, void* out, int out_dtype,
+                      void* stream);
+
+/*
+ * Products of a few tokens with 4-bit weights, beside nkv_gemv and nkv_swiglu_gemv: x [tokens][in_features], gamma
+ * [in_features], residual and y [tokens][out_features], all of one dtype (NKV_F16 or NKV_BF16), contiguous; codes
+ * [out_features][in_features / 2], scales [out_features][in_features / 32]; x, gamma and codes 16-byte aligned.
+ * y[t][o] = sum_i W[o][i] xn[t][i] (+ residual[t][o]) with xn = x when gamma is NULL, else x * rsqrt(mean(x^2) + eps) *
+ * gamma. xn is rounded once to 11 bits (as an operand), everything else is fp32 with one rounding of y. residual may be
+ * NULL; y may be residual itself, but must not overlap it otherwise, nor x, gamma or the weight.
+ * SwiGLU: act[t][j] = silu(g) * u, g = row j and u = row intermediate + j of the [2 * intermediate][in_features]
+ * weight times xn. in_features a multiple of 32, at most 2^20; out_features (intermediate) less than 2^27; at most 2^20 - 16 tokens.
+ */
+int nkv_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
+                const uint16_t* scales, int64_t out_features, int64_t in_features, const void* residual, void* y,
+                void* stream);
+int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
+                       const uint16_t* scales, int64_t intermediate, int64_t in_features, void* act, void* stream);
+
+/*
+ * The paged cache in 4 bits: a page is 64 tokens of one KV head, 9216 bytes: K codes [64][64 bytes], V codes, K scales,
+ * V scales (256 fp16 each; token t, channels 32 r .. + 31: K at ((4 (t / 16) + t % 4) * 4 + r) * 4 + t / 4 % 4, V at
+ * 64 r + t / 8 * 8 + 2 (t % 4) + t / 4 % 2). pages, tables, batches and plans as for the per-token symmetric pages:
+ * nkv_paged_quantize_q4 as nkv_paged_quantize_tok, nkv_paged_append_chunks_q4 as nkv_paged_append_chunks_tok,
+ * nkv_paged_attn_chunks_q4 as nkv_paged_attn_chunks_tok, nkv_paged_read_q4 as nkv_paged_read_tok. In the attention keys
+ * and values are exact operands; the softmax's weights and the output are rounded to fp16.
+ */
+int nkv_paged_quantize_q4(const void* x, int x_dtype, int64_t x_head_stride, int64_t hkv, int64_t n, int which,
+                          uint8_t* pages, const int32_t* table_row, int64_t first_token, int64_t num_pages, void* stream);
+int nkv_paged_append_chunks_q4(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens, uint8_t* pages,
+                               const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                               const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t nseq,
+                               int64_t hq, int64_t hkv, int64_t head_dim, const void* q_gamma, const void* k_gamma,
+                               float eps, const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream);
+int nkv_paged_attn_chunks_q4(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
+                             const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                             const int32_t* cu, const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv,
+                             int64_t head_dim, const int32_t* units, int64_t n_units, int wide, const int32_t* merges,
+                             int64_t n_merges, uint16_t* out, int64_t out_token_stride, int64_t out_head_stride,
+                             float* lse_out, void* workspace, int64_t workspace_bytes, void* stream);
+int nkv_paged_read_q4(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                      const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq,
+                      int64_t hkv, int64_t head_dim, void* k_out, void* v_out, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

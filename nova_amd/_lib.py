@@ -43,6 +43,17 @@ _STEP_STATIC = _STEP[:23] + _STEP[25:]
 # lse, workspace, workspace_bytes, n_parts, stream
 _STEP_TOK = [P, P, P, I64, P, P, P, P, P, P, I64, I64, I64, I64, P, P, P, I64, I64, P]
 
+# qkv, dtype, row_stride, tokens, pages, table, table_stride, num_pages, seq_of, cu, start, nseq, hq, hkv, head_dim,
+# q_gamma, k_gamma, eps, inv_freq, q_out, q_row_stride, stream
+_APPEND_CHUNKS = [P, c_int, I64, I64, P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_float, P, P, I64, P]
+# q, q_token_stride, q_head_stride, tokens, pages, table, table_stride, num_pages, cu, start, nseq, hq, hkv, head_dim,
+# units, n_units, wide, merges, n_merges, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream
+_ATTN_CHUNKS = [P, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, c_int, P, I64, P, I64, I64, P, P, I64, P]
+# pages, table, table_stride, num_pages, seq_of, cu, start, tokens, nseq, hkv, head_dim, k_out, v_out, dtype, stream
+_READ = [P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_int, P]
+# x, x_dtype, head_stride, hkv, n, which, pages, table_row, first_token, num_pages, stream
+_PAGED_QUANTIZE = [P, c_int, I64, I64, I64, c_int, P, P, I64, I64, P]
+
 SIGNATURES = {
     "nkv_abi_version": (c_int, []),
     "nkv_last_error": (ctypes.c_char_p, []),
@@ -86,19 +97,20 @@ SIGNATURES = {
     "nkv_paged_quantize_tok": (c_int, [P, c_int, I64, I64, I64, c_int, P, P, I64, I64, P]),
     "nkv_paged_decode_step_tok": (c_int, [P, P, P, I64, I64, P, P, I64, I64, P, I64, I64, I64, I64, P, P, I64, P,
                                           P, P, I64, P]),
-    # qkv, dtype, row_stride, tokens, pages, table, table_stride, num_pages, seq_of, cu, start, nseq, hq, hkv, head_dim,
-    # q_gamma, k_gamma, eps, inv_freq, q_out, q_row_stride, stream
-    "nkv_paged_append_chunks_tok": (c_int, [P, c_int, I64, I64, P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_float,
-                                            P, P, I64, P]),
+    "nkv_paged_append_chunks_tok": (c_int, _APPEND_CHUNKS),
+    "nkv_paged_append_chunks_q4": (c_int, _APPEND_CHUNKS),
     "nkv_paged_chunks_workspace_bytes": (I64, [I64, I64]),
-    # q, q_token_stride, q_head_stride, tokens, pages, table, table_stride, num_pages, cu, start, nseq, hq, hkv, head_dim,
-    # units, n_units, wide, merges, n_merges, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream
-    "nkv_paged_attn_chunks_tok": (c_int, [P, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P, I64, c_int, P, I64,
-                                          P, I64, I64, P, P, I64, P]),
-    # pages, table, table_stride, num_pages, (rings, length,) seq_of, cu, start, tokens, nseq, hkv, head_dim, k_out, v_out,
-    # dtype, stream
-    "nkv_paged_read_tok": (c_int, [P, P, I64, I64, P, P, P, I64, I64, I64, I64, P, P, c_int, P]),
-    "nkv_paged_read_t64": (c_int, [P, P, I64, I64, P, P, P, P, P, I64, I64, I64, I64, P, P, c_int, P]),
+    "nkv_paged_attn_chunks_tok": (c_int, _ATTN_CHUNKS),
+    "nkv_paged_attn_chunks_q4": (c_int, _ATTN_CHUNKS),
+    "nkv_paged_read_tok": (c_int, _READ),
+    "nkv_paged_read_q4": (c_int, _READ),
+    "nkv_paged_read_t64": (c_int, _READ[:4] + [P, P] + _READ[4:]),  # (rings and length after num_pages)
+    "nkv_paged_quantize_q4": (c_int, _PAGED_QUANTIZE),
+    "nkv_quantize_q4": (c_int, [P, c_int, I64, I64, P, P, P]),
+    "nkv_dequantize_q4": (c_int, [P, P, I64, I64, P, c_int, P]),
+    # x, dtype, tokens, gamma, eps, codes, scales, out_features, in_features, (residual,) y, stream
+    "nkv_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, P, I64, I64, P, P, P]),
+    "nkv_swiglu_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, P, I64, I64, P, P]),
     "nkv_prefill_workspace_bytes": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_default_splits": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_cutting": (c_int, [I64, I64, I64, I64, I64, I64, I64, P]),
@@ -125,7 +137,7 @@ SIGNATURES = {
     "nkv_qk_norm_rope": (c_int, [P, I64, I64, I64, P, P, c_float, P, P, P]),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lib = None
 _lock = threading.Lock()

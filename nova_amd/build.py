@@ -23,7 +23,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libnova_kv.so"
-SOURCES = ("nkv_quant.hip", "nkv_attn.hip", "nkv_gemv.hip", "nkv_chunks.hip")
+SOURCES = ("nkv_quant.hip", "nkv_attn.hip", "nkv_gemv.hip", "nkv_chunks.hip", "nkv_q4.hip", "nkv_q4_gemv.hip")
 ARCH = "gfx950"
 
 COMMON_FLAGS = [

@@ -84,7 +84,7 @@ def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
     return counts
 
 
-def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarray, int]:
+def plan_units(starts, counts, gq: int, hkv: int, big_from: int = BIG_FROM) -> tuple[np.ndarray, np.ndarray, int]:
     """How the attention of ``counts[b]`` new tokens after ``starts[b]`` is cut.
 
     Returns ``(units, merges, partial_rows)``, int32 ``[n, 8]`` and ``[m, 8]``. The rows of a KV head
@@ -94,8 +94,8 @@ def plan_units(starts, counts, gq: int, hkv: int) -> tuple[np.ndarray, np.ndarra
     merge entries ``(sequence's first packed token, first row, rows, parts, slot, slots from part to part,
     0, 0)`` join, eight rows each. The longest units come first."""
     rows = np.array(counts, dtype=np.int64) * gq
-    wide = bool((rows > BIG_FROM).any())
-    size = np.where(rows > BIG_FROM, TILE_ROWS[ROWS256], TILE_ROWS[ROWS32])
+    wide = bool((rows > big_from).any())
+    size = np.where(rows > big_from, TILE_ROWS[ROWS256], TILE_ROWS[ROWS32])
     n_tiles = -(-rows // size)
     seq = np.repeat(np.arange(len(rows)), n_tiles)
     if not len(seq):
@@ -158,9 +158,9 @@ def span_plan(counts: list[int], starts: list[int], pos: torch.Tensor) -> SpanPl
     return SpanPlan(counts, int(cu[-1]), pos, first, ints[:len(cu)], ints[len(cu):])
 
 
-def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int) -> ChunkPlan:
+def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int, big_from: int = BIG_FROM) -> ChunkPlan:
     cu, seq_of = _packed(counts)
-    units, merges, rows = plan_units(lengths, counts, gq, hkv)
+    units, merges, rows = plan_units(lengths, counts, gq, hkv, big_from)
     # one copy to the device; the entries are 32 bytes, so that each of them stays aligned
     ints = torch.from_numpy(np.concatenate((units.ravel(), merges.ravel(), cu, seq_of))).to(pos.device)
     new = torch.tensor(counts, dtype=torch.int64).to(pos.device)

@@ -2,146 +2,28 @@
 // chunk, drafted tokens, one decode token, none), packed one after another.
 //
 // - append_chunks: the head norms and the rotary embedding of the stacked q/k/v projections, and the
-//   quantized store of the keys and values into their pages (per-token symmetric format);
-// - attn_chunks: the new tokens' causal attention over everything their sequence has in its pages;
-// - read: spans of cached tokens back to fp16 / bf16 / fp32, from either page format.
-//
-// Token t of the packed batch belongs to sequence seq_of[t] and is its new token t - cu[seq]; its position is
-// start[seq] + that. Lengths and positions are read on the device, so a captured graph follows them.
+//   quantized store of the keys and values into their pages (per-token symmetric or 4-bit format);
+// - attn_chunks: the new tokens' causal attention over everything their sequence has in its pages (per-token
+//   symmetric format; over 4-bit pages: nkv_q4.hip);
+// - read: spans of cached tokens back to fp16 / bf16 / fp32, from any page format.
 
 #include <type_traits>
 
-#include "nkv_mfma.h"
+#include "nkv_paged.h"
+#include "nkv_q4.h"
 
 namespace nkv {
 
 namespace {
 
-// ---------------------------------------------------------------- the packed batch
-
-struct Batch {
-  const int32_t* seq_of;   // [tokens]
-  const int32_t* cu;       // [nseq + 1]
-  const int64_t* start;    // [nseq]
-  const int32_t* table;    // [nseq][table_stride]
-  int64_t table_stride, num_pages;
-  int nseq, hkv;
-};
-
-// The page of group `grp` of sequence b, -1 where the table holds none.
-__device__ __forceinline__ int64_t page_at(const Batch& a, int b, int64_t grp) {
-  if (grp < 0 || grp >= a.table_stride) return -1;
-  const int32_t page = a.table[(int64_t)b * a.table_stride + grp];
-  return page >= 0 && page < a.num_pages ? page : -1;
-}
-
-struct TokenAt {
-  int64_t pos, page;  // position in its sequence; page -1: none
-  int seq;
-};
-
-__device__ __forceinline__ TokenAt token_at(const Batch& a, int64_t t) {
-  const int b = a.seq_of[t];
-  if (b < 0 || b >= a.nseq) return {-1, -1, -1};
-  const int64_t pos = a.start[b] + (t - a.cu[b]);
-  return {pos, page_at(a, b, pos < 0 ? -1 : pos / GT), b};
-}
-
-// ---------------------------------------------------------------- eight values of a row
-
-template <int DT>
-struct Elem;
-template <>
-struct Elem<NKV_F16> {
-  static constexpr int SIZE = 2;
-};
-template <>
-struct Elem<NKV_BF16> {
-  static constexpr int SIZE = 2;
-};
-template <>
-struct Elem<NKV_F32> {
-  static constexpr int SIZE = 4;
-};
-
-template <int DT>
-struct Raw8 {  // eight consecutive values as loaded
-  uint4 w[Elem<DT>::SIZE / 2];
-  __device__ __forceinline__ void load(const uint8_t* p) {
-#pragma unroll
-    for (int i = 0; i < Elem<DT>::SIZE / 2; ++i) w[i] = *reinterpret_cast<const uint4*>(p + 16 * i);
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < Elem<DT>::SIZE / 2; ++i) w[i] = uint4{0, 0, 0, 0};
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
-    if constexpr (DT == NKV_F32) {
-      const uint32_t u2[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]), v[4 + i] = __uint_as_float(u2[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (DT == NKV_F16) {
-          v[2 * i] = h2f((uint16_t)(u[i] & 0xffffu));
-          v[2 * i + 1] = h2f((uint16_t)(u[i] >> 16));
-        } else {
-          v[2 * i] = bf2f((uint16_t)(u[i] & 0xffffu));
-          v[2 * i + 1] = bf2f((uint16_t)(u[i] >> 16));
-        }
-      }
-    }
-  }
-};
-
-template <bool NT>
-__device__ __forceinline__ void store16(uint8_t* p, u32x4_t w) {
-  if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
-  else *reinterpret_cast<u32x4_t*>(p) = w;
-}
-template <int DT, bool NT>
-__device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
-  if constexpr (DT == NKV_F32) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4)
-      store16<NT>(p + 4 * i, u32x4_t{__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])});
-  } else {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = DT == NKV_F16 ? f2h(v[2 * i]) : f2bf(v[2 * i]);
-      const uint32_t hi = DT == NKV_F16 ? f2h(v[2 * i + 1]) : f2bf(v[2 * i + 1]);
-      u[i] = lo | (hi << 16);
-    }
-    store16<NT>(p, u32x4_t{u[0], u[1], u[2], u[3]});
-  }
-}
-
 // ---------------------------------------------------------------- append
-
-// Sum over the 16 lanes of each 16-lane row (DPP only; every lane gets it).
-__device__ __forceinline__ float row16_sum(float v) {
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
-  return v;
-}
-
-__device__ __forceinline__ float row16_max(float v) {
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false)));
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false)));
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false)));
-  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false)));
-  return v;
-}
 
 // The value of lane l ^ 8 of the same 16-lane row (a rotation by 8).
 __device__ __forceinline__ float row16_other_half(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
 }
+
+enum Format : int { TOK, T64, Q4 };  // a page's
 
 struct AppendArgs {
   Batch b;
@@ -166,7 +48,7 @@ struct AppendArgs {
 // tokens a workgroup without the loads ahead took 25.8 us. 1029 bf16 tokens of 28 q and 4 KV heads 7.3
 // us (21 MB, 2.9 TB/s: a workgroup's chain takes about as long as its data); 12 tokens 3.7 us, the time of the chain
 // sequence, position and table, angles, rows. NT: nontemporal q stores.
-template <int DT, bool NT>
+template <int DT, bool NT, Format F>
 __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) float turn[2][D / 2];  // cos, sin
   __shared__ int64_t row_of;  // byte offset of KV head 0's page, or -1
@@ -176,6 +58,7 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
   const int heads = a.hq + 2 * a.b.hkv, h0 = blockIdx.y * a.heads_per_wg, h1 = min(h0 + a.heads_per_wg, heads);
   const bool norm = a.q_gamma != nullptr, rotate = a.inv_freq != nullptr;
   constexpr int SIZE = Elem<DT>::SIZE, AHEAD = DT == NKV_F32 ? 2 : 4;
+  constexpr int PAGE = F == Q4 ? PAGE_Q4_BYTES : PAGE_TOK_BYTES;
 
   const uint8_t* x = a.x + (t * a.x_rs + 8 * j) * SIZE;
   Raw8<DT> ahead[AHEAD];
@@ -193,7 +76,7 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
   if (tid < D / 2) {
     const TokenAt at = token_at(a.b, t);
     if (tid == 0) {
-      row_of = at.page < 0 ? -1 : at.page * a.b.hkv * (int64_t)PAGE_TOK_BYTES;
+      row_of = at.page < 0 ? -1 : at.page * a.b.hkv * (int64_t)PAGE;
       slot_of = (int)(at.pos & (GT - 1));
     }
     if (rotate) {
@@ -243,11 +126,21 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
       store8<NKV_F16, NT>(reinterpret_cast<uint8_t*>(a.q_out + t * a.q_rs + (int64_t)h * D + 8 * j), v);
     } else if (row_of >= 0) {
       const int kv = is_v ? h - a.hq - a.b.hkv : h - a.hq, which = is_v ? 1 : 0;
-      float scale;
-      const uint2 codes = sym_quant8<true>(v, scale);
-      uint8_t* page = a.pages + row_of + (int64_t)kv * PAGE_TOK_BYTES;
-      *reinterpret_cast<uint2*>(page + which * CODE_BYTES + slot_of * D + 8 * j) = codes;
-      if (j == 0) *reinterpret_cast<uint16_t*>(page + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot_of) = f2h(scale);
+      uint8_t* page = a.pages + row_of + (int64_t)kv * PAGE;
+      if constexpr (F == Q4) {
+        uint16_t scale;
+        const uint32_t codes = q4_quant8(v, scale);
+        *reinterpret_cast<uint32_t*>(page + which * Q4_CODES + slot_of * Q4_ROW + 4 * j) = codes;
+        if (j % 4 == 0) {
+          const int to = which ? v_scale_at(slot_of, j / 4) : k_scale_at(slot_of, j / 4);
+          *reinterpret_cast<uint16_t*>(page + 2 * Q4_CODES + which * Q4_SCALES + 2 * to) = scale;
+        }
+      } else {
+        float scale;
+        const uint2 codes = sym_quant8<true>(v, scale);
+        *reinterpret_cast<uint2*>(page + which * CODE_BYTES + slot_of * D + 8 * j) = codes;
+        if (j == 0) *reinterpret_cast<uint16_t*>(page + 2 * CODE_BYTES + which * (2 * GT) + 2 * slot_of) = f2h(scale);
+      }
     }
   }
 }
@@ -267,17 +160,17 @@ struct ReadArgs {
 // TOK tokens of one workgroup; 16 lanes to a row of 128, 8 values each, four rows of every lane in flight (two of
 // int8t64, whose steps and minima are 32 bytes a lane more). Bound by memory: 70000 tokens of 8 KV heads to bf16 (431 MB)
 // in 92 us, 4.7 TB/s; 275 tokens 3.0 us, a chain of three loads.
-template <int DT, bool T64, int TOK>
+template <int DT, Format F, int N>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-  __shared__ int64_t page_of[TOK];  // the token's page; -1: none, -2: in its sequence's ring
-  __shared__ int slot_of[TOK], seq_of[TOK];
+  __shared__ int64_t page_of[N];  // the token's page; -1: none, -2: in its sequence's ring
+  __shared__ int slot_of[N], seq_of[N];
   const int tid = threadIdx.x, j = tid & 15;
-  const int64_t t0 = (int64_t)blockIdx.x * TOK;
-  const int nt = (int)min<int64_t>(TOK, a.tokens - t0);
+  const int64_t t0 = (int64_t)blockIdx.x * N;
+  const int nt = (int)min<int64_t>(N, a.tokens - t0);
   if (tid < nt) {
     const TokenAt at = token_at(a.b, t0 + tid);
     int64_t page = at.page;
-    if (T64 && at.seq >= 0) {
+    if (F == T64 && at.seq >= 0) {
       const int64_t len = a.length[at.seq];
       if (at.pos >= len) page = -1;
       else if (at.pos >= len / GT * GT) page = -2;
@@ -287,7 +180,8 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     seq_of[tid] = at.seq;
   }
   __syncthreads();
-  constexpr int SIZE = Elem<DT>::SIZE, FLY = T64 ? 2 : 4;
+  constexpr int SIZE = Elem<DT>::SIZE, FLY = F == T64 ? 2 : 4;
+  constexpr int PAGE = F == T64 ? PAGE_BYTES : F == Q4 ? PAGE_Q4_BYTES : PAGE_TOK_BYTES;
   const int rows = 2 * a.b.hkv * nt;
   // item `it`: token it % nt, tensor and KV head it / nt (neighbouring rows of a page, first)
   for (int it0 = tid >> 4; it0 < rows; it0 += 16 * FLY) {
@@ -300,12 +194,18 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
       if (it >= rows) break;
       const int k = it % nt, hw = it / nt, h = hw >> 1, which = hw & 1, slot = slot_of[k];
       const int64_t page = page_of[k];
-      if (T64 && page == -2) {
+      if (F == T64 && page == -2) {
         st[f].load(reinterpret_cast<const uint8_t*>(a.rings + ((((int64_t)seq_of[k] * a.b.hkv + h) * 2 + which) * GT + slot) * D + 8 * j));
       } else if (page >= 0) {
-        const uint8_t* p = a.pages + (page * a.b.hkv + h) * (T64 ? PAGE_BYTES : PAGE_TOK_BYTES);
+        const uint8_t* p = a.pages + (page * a.b.hkv + h) * PAGE;
+        if constexpr (F == Q4) {
+          codes[f].x = *reinterpret_cast<const uint32_t*>(p + which * Q4_CODES + slot * Q4_ROW + 4 * j);
+          const int from = which ? v_scale_at(slot, j / 4) : k_scale_at(slot, j / 4);
+          scale[f] = *reinterpret_cast<const uint16_t*>(p + 2 * Q4_CODES + which * Q4_SCALES + 2 * from);
+          continue;
+        }
         codes[f] = *reinterpret_cast<const uint2*>(p + which * CODE_BYTES + slot * D + 8 * j);
-        if constexpr (T64) {
+        if constexpr (F == T64) {
           st[f].load(p + 2 * CODE_BYTES + which * (4 * D) + 16 * j);
           mn[f].load(p + 2 * CODE_BYTES + which * (4 * D) + 2 * D + 16 * j);
         } else {
@@ -323,9 +223,9 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
       if (page == -1) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      } else if (T64 && page == -2) {
+      } else if (F == T64 && page == -2) {
         st[f].get(v);
-      } else if constexpr (T64) {
+      } else if constexpr (F == T64) {
         float s8[8], m8[8];
         st[f].get(s8);
         mn[f].get(m8);
@@ -334,22 +234,21 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
           const uint32_t code = ((e < 4 ? codes[f].x : codes[f].y) >> (8 * (e & 3))) & 0xffu;
           v[e] = __builtin_fmaf((float)code, s8[e], m8[e]);  // (the product is exact)
         }
+      } else if constexpr (F == Q4) {
+        const float s = h2f(scale[f]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = q4_value(codes[f].x, e, s);
       } else {
         const float s = h2f(scale[f]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? codes[f].x : codes[f].y) >> (8 * (e & 3))) * s;
       }
-      store8<DT, (TOK > 4)>((which ? a.v_out : a.k_out) + (((t0 + k) * a.b.hkv + h) * D + 8 * j) * SIZE, v);
+      store8<DT, (N > 4)>((which ? a.v_out : a.k_out) + (((t0 + k) * a.b.hkv + h) * D + 8 * j) * SIZE, v);
     }
   }
 }
 
 // ---------------------------------------------------------------- attention
-//
-// The rows of KV head h in sequence b: row R = (new token R / gq, q head h gq + R % gq), gq = hq / hkv. They
-// are cut into tiles; a tile attends the 64-token groups up to its last token (steps 0 .. S - 1), and its
-// steps are cut into parts, unit = one part of one tile. Part p of P takes steps [S p / P, S (p + 1) / P),
-// from the S of the device's lengths: the plan stays valid while sequences grow.
 //
 // softmax(q K^T / sqrt(128)) V with K = code * scale and V likewise: K's scale multiplies the scores and V's the
 // weights, so that the codes are exact operands, and only P (weight times V's scale) and the output are rounded to fp16.
@@ -362,97 +261,11 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 
 constexpr int CH_WAVES = 8, CH_THREADS = 64 * CH_WAVES;
 constexpr int CH_VSLOT = CODE_BYTES + 4 * GT;            // V codes, K scales, V scales: the rest of a page after K
-constexpr int CH_PART = D + 4;                           // floats of a row's partial: acc[128], m, l, pad
 static_assert(CODE_BYTES + CH_VSLOT == PAGE_TOK_BYTES, "a page is K codes and a slot");
 static_assert(16 * CH_PART * 4 <= CH_VSLOT, "a wave's 16 rows fit one of its slots at the merge");
 constexpr int CH_LDS = 2 * CH_WAVES * CH_VSLOT;          // 132 KiB: two slots a wave
 
-enum UnitKind : int { ROWS16 = 0, ROWS32 = 1, ROWS256 = 2 };
-
-struct Unit {  // (int32 each, as the plan lays them out)
-  int seq, row0, rows, part, parts, slot, kind, alone;  // slot: partial row of part 0 of the tile; alone: of its sequence
-};
-struct Merge {
-  int first, row0, rows, parts, slot, stride, pad0, pad1;  // first: the sequence's first packed token; up to 8 rows;
-                                                           // part p's partial of row r: slot + p * stride + r
-};
-
-struct ChunkArgs {
-  Batch b;
-  const uint16_t* q;  // token t, head i at q + t * q_ts + i * q_hs
-  int64_t q_ts, q_hs, tokens;
-  const uint8_t* pages;
-  const Unit* units;
-  int hq, gq;
-  float sl2;
-  uint16_t* out;
-  int64_t o_ts, o_hs;
-  float* lse;  // [tokens][hq] or NULL
-  float* ws;   // partial rows [ws_rows][hkv][CH_PART]
-  int64_t ws_rows;
-};
-
-// Where a tile of sequence b stands.
-struct TileAt {
-  int64_t start, first_token;  // position of the sequence's first new token; packed index of it
-  int rows;                    // rows of the tile (no more than the sequence has)
-  int64_t steps;               // groups up to the tile's last token
-};
-__device__ __forceinline__ TileAt tile_at(const ChunkArgs& a, int seq, int row0, int rows) {
-  TileAt t;
-  const int64_t c0 = a.b.cu[seq], c1 = a.b.cu[seq + 1];
-  const int64_t have = max<int64_t>(0, min(c1, a.tokens) - c0) * a.gq - row0;
-  t.rows = c0 < 0 ? 0 : (int)max<int64_t>(0, min<int64_t>(rows, have));
-  t.start = a.b.start[seq];
-  t.first_token = c0;
-  t.steps = t.rows == 0 || t.start < 0 ? 0 : min((t.start + (row0 + t.rows - 1) / a.gq) / GT + 1, a.b.table_stride);
-  return t;
-}
-
 constexpr float W_TAU = 4.0f;  // (RowState; log2 of the weights that a lane sums at a time)
-
-// A row's sums, 32 lanes a row, 4 dims each: l of the weights 2^(score - m), scores in the log2 domain, acc of weight
-// times V.
-struct RowSum {
-  float m, l;
-  float4 acc;
-};
-__device__ __forceinline__ void write_row(const ChunkArgs& a, int h, int64_t token, int head, const RowSum& r, int l32) {
-  const float inv = r.l > 0.0f || r.l != r.l ? 1.0f / r.l : 0.0f;
-  const int i = h * a.gq + head;
-  *reinterpret_cast<uint2*>(a.out + token * a.o_ts + i * a.o_hs + 4 * l32) =
-      uint2{(uint32_t)f2h(r.acc.x * inv) | ((uint32_t)f2h(r.acc.y * inv) << 16),
-            (uint32_t)f2h(r.acc.z * inv) | ((uint32_t)f2h(r.acc.w * inv) << 16)};
-  if (a.lse && l32 == 0) a.lse[token * a.hq + i] = r.l == 0.0f ? NEG_INF : (r.m + __builtin_amdgcn_logf(r.l)) * LN2;
-}
-
-// The pages of a wave's groups first, first + stride, .., n of them, held 64 at a time, one a lane. (Scalar loads
-// of the table would share their counter with LDS: every wait for an operand would be one for the table, too.)
-struct Pages {
-  const int32_t* row;
-  int64_t num_pages;
-  int stride, n, base;
-  int page;  // lane l: that of group base + l, -1: none
-  __device__ __forceinline__ Pages(const Batch& b, int seq, int64_t first, int stride_, int n_)
-      : row(b.table + (int64_t)seq * b.table_stride + first), num_pages(b.num_pages), stride(stride_), n(n_), base(0) {
-    fetch();
-  }
-  __device__ __forceinline__ void fetch() {
-    const int i = base + ((int)threadIdx.x & 63);
-    page = i < n ? row[(int64_t)i * stride] : -1;
-    if (page >= num_pages) page = -1;
-  }
-  // i: not decreasing from call to call
-  __device__ __forceinline__ int at(int i) {
-    if (i >= base + 64) {
-      base = i;
-      fetch();
-    }
-    return __builtin_amdgcn_readlane(page, i - base);
-  }
-};
-
-__device__ __forceinline__ bool finite_h(uint32_t bits) { return (bits & 0x7c00u) != 0x7c00u; }
 
 // Eight signed codes as the fp16 values 2^-24 (code + 128): denormals, which the matrix core takes as they are, so
 // that a code becomes an operand with a byte's move alone.
@@ -1181,57 +994,41 @@ __global__ __launch_bounds__(256) void merge_chunks_kernel(ChunkArgs a, const Me
 
 // ---------------------------------------------------------------- host side
 
-bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-int batch_args(const char* what, Batch& b, const int32_t* seq_of, bool need_seq_of, const int32_t* cu, const int64_t* start,
-               const int32_t* table, int64_t table_stride, int64_t num_pages, int64_t nseq, int64_t hkv, int64_t head_dim,
-               int64_t tokens) {
-  if (head_dim != D) return fail(NKV_ERR_UNSUPPORTED, "%s: head_dim %lld: the HIP kernels are built for head_dim 128", what, (long long)head_dim);
-  if (nseq <= 0 || nseq > 32767 || hkv <= 0 || hkv > 1024 || table_stride <= 0 || num_pages <= 0 || num_pages > (int64_t(1) << 31))
-    return fail(NKV_ERR_INVALID, "%s: bad sizes nseq=%lld hkv=%lld table_stride=%lld num_pages=%lld", what, (long long)nseq,
-                (long long)hkv, (long long)table_stride, (long long)num_pages);
-  if (tokens < 0 || tokens >= (int64_t(1) << 24))  // (a launch has less than 2^32 threads)
-    return fail(NKV_ERR_INVALID, "%s: %lld tokens outside [0, 2^24)", what, (long long)tokens);
-  if (tokens > 0 && ((need_seq_of && !seq_of) || !cu || !start || !table)) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  b = Batch{seq_of, cu, start, table, table_stride, num_pages, (int)nseq, (int)hkv};
-  return NKV_OK;
-}
-
 // The heads of few tokens are spread over workgroups (12 tokens: 3.7 us, all 48 heads in one 4.6 us), those of many
 // are not (1029 tokens: 7.3 us, spread 8.6 us; 4112 tokens 20.6 and 25.8 us: each workgroup makes the angles). From 2048
 // tokens the queries are stored past the caches (us nontemporal / ordinary, 32 q and 8 KV heads): 2048 tokens 12.0 /
 // 12.8, 4112 20.1 / 20.7; 8 and 2 heads, 4112 tokens 9.6 / 10.3; 4 and 2, 16000 26.1 / 26.5. With a kernel that reads
 // the queries next, both: 19.7 / 20.1, 31.9 / 31.1, 14.9 / 16.1, 33.3 / 32.6. Few tokens gain nothing (300: 5.1 / 5.1).
 // In between it would gain, too (1029 tokens 7.9 / 8.9, with the reader 12.7 / 15.0).
-template <int DT>
-void launch_append(const AppendArgs& a, hipStream_t s) {
+template <int DT, Format F>
+void launch_append_as(const AppendArgs& a, hipStream_t s) {
   const int heads = a.hq + 2 * a.b.hkv;
   AppendArgs c = a;
   c.heads_per_wg = a.tokens < CUS ? 16 : heads;
   const dim3 grid((unsigned)a.tokens, (unsigned)cdiv(heads, c.heads_per_wg));
-  if (a.tokens >= 8 * CUS) hipLaunchKernelGGL((append_chunks_kernel<DT, true>), grid, dim3(256), 0, s, c);
-  else hipLaunchKernelGGL((append_chunks_kernel<DT, false>), grid, dim3(256), 0, s, c);
+  if (a.tokens >= 8 * CUS) hipLaunchKernelGGL((append_chunks_kernel<DT, true, F>), grid, dim3(256), 0, s, c);
+  else hipLaunchKernelGGL((append_chunks_kernel<DT, false, F>), grid, dim3(256), 0, s, c);
 }
 
-template <bool T64, int TOK>
+template <Format F, int N>
 void launch_read_as(const ReadArgs& a, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv(a.tokens, TOK));
-  if (dtype == NKV_F16) hipLaunchKernelGGL((read_kernel<NKV_F16, T64, TOK>), grid, dim3(256), 0, s, a);
-  else if (dtype == NKV_BF16) hipLaunchKernelGGL((read_kernel<NKV_BF16, T64, TOK>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((read_kernel<NKV_F32, T64, TOK>), grid, dim3(256), 0, s, a);
+  const dim3 grid((unsigned)cdiv(a.tokens, N));
+  if (dtype == NKV_F16) hipLaunchKernelGGL((read_kernel<NKV_F16, F, N>), grid, dim3(256), 0, s, a);
+  else if (dtype == NKV_BF16) hipLaunchKernelGGL((read_kernel<NKV_BF16, F, N>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((read_kernel<NKV_F32, F, N>), grid, dim3(256), 0, s, a);
 }
 
 // Few tokens want all the workgroups that there are, many tokens few waits for the chain at a workgroup's start. Tokens a
 // workgroup 1 / 4 / 16, 8 KV heads: 275 tokens 3.3 / 4.5 / 9.5 us, 5418 tokens of int8t64 16.1 / 14.4 / 19.6 us, 70000
 // tokens 16: 98 us, 4: 101 us. Stores of the long ones pass the caches (store8).
-template <bool T64>
+template <Format F>
 void launch_read(const ReadArgs& a, int dtype, hipStream_t s) {
-  if (a.tokens * a.b.hkv <= 16 * CUS) launch_read_as<T64, 1>(a, dtype, s);
-  else if (a.tokens * a.b.hkv <= 512 * CUS) launch_read_as<T64, 4>(a, dtype, s);
-  else launch_read_as<T64, 16>(a, dtype, s);
+  if (a.tokens * a.b.hkv <= 16 * CUS) launch_read_as<F, 1>(a, dtype, s);
+  else if (a.tokens * a.b.hkv <= 512 * CUS) launch_read_as<F, 4>(a, dtype, s);
+  else launch_read_as<F, 16>(a, dtype, s);
 }
 
-int read_tokens(const char* what, bool t64, const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+int read_tokens(const char* what, Format f, const uint8_t* pages, const int32_t* page_table, int64_t table_stride,
                 int64_t num_pages, const uint16_t* rings, const int64_t* length_dev, const int32_t* seq_of,
                 const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq, int64_t hkv, int64_t head_dim,
                 void* k_out, void* v_out, int out_dtype, void* stream) {
@@ -1242,31 +1039,31 @@ int read_tokens(const char* what, bool t64, const uint8_t* pages, const int32_t*
   if (out_dtype != NKV_F16 && out_dtype != NKV_BF16 && out_dtype != NKV_F32)
     return fail(NKV_ERR_INVALID, "%s: unknown dtype %d", what, out_dtype);
   if (tokens == 0) return NKV_OK;
-  if (!pages || !k_out || !v_out || (t64 && (!rings || !length_dev))) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  if (!al16(pages) || !al16(k_out) || !al16(v_out) || (t64 && !al16(rings)))
+  if (!pages || !k_out || !v_out || (f == T64 && (!rings || !length_dev))) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(pages) || !al16(k_out) || !al16(v_out) || (f == T64 && !al16(rings)))
     return fail(NKV_ERR_UNSUPPORTED, "%s: buffers must be 16-byte aligned", what);
   a.tokens = tokens;
   a.pages = pages; a.rings = rings; a.length = length_dev;
   a.k_out = static_cast<uint8_t*>(k_out); a.v_out = static_cast<uint8_t*>(v_out);
-  if (t64) launch_read<true>(a, out_dtype, static_cast<hipStream_t>(stream));
-  else launch_read<false>(a, out_dtype, static_cast<hipStream_t>(stream));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (f == T64) launch_read<T64>(a, out_dtype, s);
+  else if (f == Q4) launch_read<Q4>(a, out_dtype, s);
+  else launch_read<TOK>(a, out_dtype, s);
   return check_launch(what);
 }
 
-}  // namespace
+template <Format F>
+void launch_append(const AppendArgs& a, int dtype, hipStream_t s) {
+  if (dtype == NKV_F16) launch_append_as<NKV_F16, F>(a, s);
+  else if (dtype == NKV_BF16) launch_append_as<NKV_BF16, F>(a, s);
+  else launch_append_as<NKV_F32, F>(a, s);
+}
 
-}  // namespace nkv
-
-using namespace nkv;
-
-extern "C" int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens,
-                                           uint8_t* pages, const int32_t* page_table, int64_t table_stride,
-                                           int64_t num_pages, const int32_t* seq_of, const int32_t* cu,
-                                           const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv,
-                                           int64_t head_dim, const void* q_gamma, const void* k_gamma, float eps,
-                                           const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream) {
+int append_tokens(const char* what, Format f, const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens, uint8_t* pages, const int32_t* page_table,
+                  int64_t table_stride, int64_t num_pages, const int32_t* seq_of, const int32_t* cu,
+                  const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv, int64_t head_dim, const void* q_gamma,
+                  const void* k_gamma, float eps, const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream) {
   set_error("");
-  const char* what = "paged_append_chunks_tok";
   AppendArgs a{};
   if (int rc = batch_args(what, a.b, seq_of, true, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
     return rc;
@@ -1284,17 +1081,58 @@ extern "C" int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64
   a.q_gamma = static_cast<const uint8_t*>(q_gamma); a.k_gamma = static_cast<const uint8_t*>(k_gamma);
   a.eps = eps; a.inv_freq = inv_freq; a.q_out = q_out; a.q_rs = q_row_stride; a.hq = (int)hq;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (qkv_dtype == NKV_F16) launch_append<NKV_F16>(a, s);
-  else if (qkv_dtype == NKV_BF16) launch_append<NKV_BF16>(a, s);
-  else launch_append<NKV_F32>(a, s);
+  if (f == Q4) launch_append<Q4>(a, qkv_dtype, s);
+  else launch_append<TOK>(a, qkv_dtype, s);
   return check_launch(what);
+}
+
+}  // namespace
+
+int launch_merges(const char* what, const ChunkArgs& a, const Merge* merges, int64_t n_merges, hipStream_t s) {
+  if (n_merges == 0) return NKV_OK;
+  hipLaunchKernelGGL(merge_chunks_kernel, dim3((unsigned)(n_merges * a.b.hkv)), dim3(256), 0, s, a, merges);
+  return check_launch(what);
+}
+
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" int nkv_paged_append_chunks_tok(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens,
+                                           uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                                           int64_t num_pages, const int32_t* seq_of, const int32_t* cu,
+                                           const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv,
+                                           int64_t head_dim, const void* q_gamma, const void* k_gamma, float eps,
+                                           const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream) {
+  return append_tokens("paged_append_chunks_tok", TOK, qkv, qkv_dtype, row_stride, tokens, pages, page_table, table_stride,
+                       num_pages, seq_of, cu, start_dev, nseq, hq, hkv, head_dim, q_gamma, k_gamma, eps, inv_freq, q_out,
+                       q_row_stride, stream);
+}
+
+extern "C" int nkv_paged_append_chunks_q4(const void* qkv, int qkv_dtype, int64_t row_stride, int64_t tokens,
+                                           uint8_t* pages, const int32_t* page_table, int64_t table_stride,
+                                           int64_t num_pages, const int32_t* seq_of, const int32_t* cu,
+                                           const int64_t* start_dev, int64_t nseq, int64_t hq, int64_t hkv,
+                                           int64_t head_dim, const void* q_gamma, const void* k_gamma, float eps,
+                                           const float* inv_freq, uint16_t* q_out, int64_t q_row_stride, void* stream) {
+  return append_tokens("paged_append_chunks_q4", Q4, qkv, qkv_dtype, row_stride, tokens, pages, page_table, table_stride,
+                       num_pages, seq_of, cu, start_dev, nseq, hq, hkv, head_dim, q_gamma, k_gamma, eps, inv_freq, q_out,
+                       q_row_stride, stream);
 }
 
 extern "C" int nkv_paged_read_tok(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
                                   const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t tokens,
                                   int64_t nseq, int64_t hkv, int64_t head_dim, void* k_out, void* v_out, int out_dtype,
                                   void* stream) {
-  return read_tokens("paged_read_tok", false, pages, page_table, table_stride, num_pages, nullptr, nullptr, seq_of, cu,
+  return read_tokens("paged_read_tok", TOK, pages, page_table, table_stride, num_pages, nullptr, nullptr, seq_of, cu,
+                     start_dev, tokens, nseq, hkv, head_dim, k_out, v_out, out_dtype, stream);
+}
+
+extern "C" int nkv_paged_read_q4(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, int64_t num_pages,
+                                 const int32_t* seq_of, const int32_t* cu, const int64_t* start_dev, int64_t tokens,
+                                 int64_t nseq, int64_t hkv, int64_t head_dim, void* k_out, void* v_out, int out_dtype,
+                                 void* stream) {
+  return read_tokens("paged_read_q4", Q4, pages, page_table, table_stride, num_pages, nullptr, nullptr, seq_of, cu,
                      start_dev, tokens, nseq, hkv, head_dim, k_out, v_out, out_dtype, stream);
 }
 
@@ -1302,7 +1140,7 @@ extern "C" int nkv_paged_read_t64(const uint8_t* pages, const int32_t* page_tabl
                                   const uint16_t* rings, const int64_t* length_dev, const int32_t* seq_of,
                                   const int32_t* cu, const int64_t* start_dev, int64_t tokens, int64_t nseq, int64_t hkv,
                                   int64_t head_dim, void* k_out, void* v_out, int out_dtype, void* stream) {
-  return read_tokens("paged_read_t64", true, pages, page_table, table_stride, num_pages, rings, length_dev, seq_of, cu,
+  return read_tokens("paged_read_t64", T64, pages, page_table, table_stride, num_pages, rings, length_dev, seq_of, cu,
                      start_dev, tokens, nseq, hkv, head_dim, k_out, v_out, out_dtype, stream);
 }
 
@@ -1317,38 +1155,18 @@ extern "C" int nkv_paged_attn_chunks_tok(const uint16_t* q, int64_t q_token_stri
                                          const int32_t* merges, int64_t n_merges, uint16_t* out, int64_t out_token_stride,
                                          int64_t out_head_stride, float* lse_out, void* workspace, int64_t workspace_bytes,
                                          void* stream) {
-  set_error("");
   const char* what = "paged_attn_chunks_tok";
   ChunkArgs a{};
-  if (int rc = batch_args(what, a.b, nullptr, false, cu, start_dev, page_table, table_stride, num_pages, nseq, hkv, head_dim, tokens))
+  bool any = false;
+  if (int rc = chunk_args(what, a, any, q, q_token_stride, q_head_stride, tokens, pages, page_table, table_stride, num_pages, cu,
+                          start_dev, nseq, hq, hkv, head_dim, units, n_units, merges, n_merges, out, out_token_stride,
+                          out_head_stride, lse_out, workspace, workspace_bytes))
     return rc;
-  if (hq <= 0 || hq > 16 * hkv || hq % hkv) return fail(NKV_ERR_INVALID, "%s: heads hq=%lld hkv=%lld", what, (long long)hq, (long long)hkv);
-  constexpr int64_t MOST = (int64_t(1) << 23) - 1;  // workgroups: a launch has less than 2^32 threads
-  if (n_units < 0 || n_merges < 0 || n_units > MOST / hkv || n_merges > MOST / hkv)
-    return fail(NKV_ERR_INVALID, "%s: %lld units and %lld merges of %lld KV heads", what, (long long)n_units,
-                (long long)n_merges, (long long)hkv);
-  if (tokens == 0 || n_units == 0) return NKV_OK;
-  if (!q || !pages || !units || !out || (n_merges && (!merges || !workspace)))
-    return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  if (!al16(q) || !al16(pages) || !al16(out) || !al16(units) || (n_merges && (!al16(merges) || !al16(workspace))) ||
-      q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
-    return fail(NKV_ERR_UNSUPPORTED, "%s: rows and buffers must be 16-byte aligned", what);
-  a.q = q; a.q_ts = q_token_stride; a.q_hs = q_head_stride; a.tokens = tokens; a.pages = pages;
-  a.units = reinterpret_cast<const Unit*>(units);
-  a.hq = (int)hq; a.gq = (int)(hq / hkv);
-  a.sl2 = LOG2E / sqrtf((float)D);
-  a.out = out; a.o_ts = out_token_stride; a.o_hs = out_head_stride; a.lse = lse_out;
-  a.ws = static_cast<float*>(workspace);
-  a.ws_rows = workspace && workspace_bytes > 0 ? workspace_bytes / (hkv * CH_PART * (int64_t)sizeof(float)) : 0;
+  if (!any) return NKV_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(n_units * hkv));
   if (wide) hipLaunchKernelGGL(attn_chunks_kernel, grid, dim3(CH_THREADS), 0, s, a);
   else hipLaunchKernelGGL(attn_small_chunks_kernel, grid, dim3(64 * SM_WAVES), 0, s, a);
   if (int rc = check_launch(what)) return rc;
-  if (n_merges) {
-    hipLaunchKernelGGL(merge_chunks_kernel, dim3((unsigned)(n_merges * hkv)), dim3(256), 0, s, a,
-                       reinterpret_cast<const Merge*>(merges));
-    return check_launch(what);
-  }
-  return NKV_OK;
+  return launch_merges(what, a, reinterpret_cast<const Merge*>(merges), n_merges, s);
 }

@@ -1,0 +1,91 @@
+// The 4-bit format of weights and cache (gfx950, wave64).
+//
+// 32 consecutive values of a row share a scale: with amax their largest magnitude, s = max(amax / 7, 2^-24) rounded to 8
+// significant bits and held in fp16, code = clamp(rint(x / s), -7, 7), value = code * s. A code has 3 significant bits
+// beside its sign and the scale 8, so that every value is an fp16 number (denormals among them: their codes' multiples of
+// 2^-24, too): the matrix cores' fp16 operands are the values themselves, with no rounding. A scale whose sevenfold passes
+// fp16's range is infinite, that of a group with a NaN is NaN.
+// Packed: nibble e of a 32-bit word holds code e + 8, of values 8 w .. 8 w + 7 of the row; a row of n values is n / 2 bytes.
+//
+// A page of the cache is 64 tokens of one KV head: K codes [64][64 bytes], V codes, K scales, V scales (256 fp16 each). The
+// scales lie as the attention's lanes take them (k_scale_at, v_scale_at).
+#pragma once
+
+#include "nkv_mfma.h"
+
+namespace nkv {
+
+constexpr uint32_t kBias1024h = 0x64006400u;  // fp16 1024, twice
+constexpr int Q4_GROUP = 32;
+constexpr int Q4_ROW = D / 2;                      // bytes of a token's codes
+constexpr int Q4_CODES = GT * Q4_ROW;              // one tensor's codes of a page
+constexpr int Q4_SCALES = GT * (D / Q4_GROUP) * 2;  // one tensor's scales
+constexpr int PAGE_Q4_BYTES = 2 * (Q4_CODES + Q4_SCALES);
+static_assert(PAGE_Q4_BYTES == 9216 && PAGE_Q4_BYTES % 128 == 0, "a page is a multiple of 128 bytes");
+
+// Where the scale of token t (0 .. 63 of its page), channels 32 grp .. + 31, stands among its tensor's. In the products
+// lane c + 16 g of tile b holds token 16 (c / 4) + 4 b + c % 4 of K, so that its scores are of tokens 16 g + 4 b ..
+// + 3 and the 16 tokens of a lane's scores follow each other.
+// K: the four tiles' scales of lane c + 16 grp follow each other.
+__host__ __device__ __forceinline__ constexpr int k_scale_at(int t, int grp) {
+  return ((4 * (t >> 4) + (t & 3)) * 4 + grp) * 4 + ((t >> 2) & 3);
+}
+// V: tokens r and r + 4 of eight follow each other, as the two halves of a register do after unpack4.
+__host__ __device__ __forceinline__ constexpr int v_scale_at(int t, int grp) {
+  return grp * GT + (t & ~7) + 2 * (t & 3) + ((t >> 2) & 1);
+}
+
+// The scale's bits for a group whose largest magnitude has the bits `amax` (of fp32; NaN above infinity).
+__device__ __forceinline__ uint16_t q4_scale(uint32_t amax) {
+  if (amax > 0x7f800000u) return 0x7e00u;
+  const float s = bf2f(f2bf(fmaxf(__fdiv_rn(__uint_as_float(amax), 7.0f), 0x1p-24f)));
+  return 7.0f * s <= 65504.0f ? f2h(s) : 0x7c00u;
+}
+
+// Eight values of a lane; the four lanes 4 k .. 4 k + 3 hold a group. The packed codes, and the scale's bits in all four.
+// (The quotient as a product unless it is near a half, as sym_code does.)
+__device__ __forceinline__ uint32_t q4_quant8(const float (&v)[8], uint16_t& scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));
+  scale = q4_scale(m);
+  const float s = h2f(scale), inv = __builtin_amdgcn_rcpf(s);
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = __fmul_rn(v[e], inv);
+    float r = __builtin_rintf(q);
+    if (__builtin_fabsf(q - r) > 0.5f - 0x1p-12f) r = __builtin_rintf(__fdiv_rn(v[e], s));
+    w |= (uint32_t)((int)fminf(fmaxf(r, -7.0f), 7.0f) + 8) << (4 * e);
+  }
+  return w;
+}
+
+// Value e of a packed word (fp32).
+__device__ __forceinline__ float q4_value(uint32_t w, int e, float s) { return (float)((int)((w >> (4 * e)) & 15u) - 8) * s; }
+
+// The eight values of a packed word as fp16, in the order 0 4 1 5 2 6 3 7 of its nibbles; s: their scales (a pair's two
+// halves may differ). A nibble becomes the mantissa's end of 1024 + n, or the middle of 1024 + 16 n: exact throughout.
+__device__ __forceinline__ half8_t unpack4(uint32_t w, const half2_t (&s)[4]) {
+  const half2_t lo = {(_Float16)-1032.0f, (_Float16)-1032.0f}, hi = {(_Float16)-72.0f, (_Float16)-72.0f};
+  const half2_t by = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const uint32_t x = w >> 8;
+  const half2_t a = (as_h2((w & 0x000f000fu) | kBias1024h) + lo) * s[0];
+  const half2_t b = (as_h2((w & 0x00f000f0u) | kBias1024h) * by + hi) * s[1];
+  const half2_t c = (as_h2((x & 0x000f000fu) | kBias1024h) + lo) * s[2];
+  const half2_t d = (as_h2((x & 0x00f000f0u) | kBias1024h) * by + hi) * s[3];
+  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+__device__ __forceinline__ half8_t unpack4(uint32_t w, half2_t s) {
+  const half2_t four[4] = {s, s, s, s};
+  return unpack4(w, four);
+}
+// Eight consecutive fp16 values in unpack4's order.
+__device__ __forceinline__ half8_t paired(uint4 w) {
+  return as_h8(uint4{perm(w.z, w.x, 0x05040100u), perm(w.z, w.x, 0x07060302u), perm(w.w, w.y, 0x05040100u),
+                     perm(w.w, w.y, 0x07060302u)});
+}
+
+}  // namespace nkv

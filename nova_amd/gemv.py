@@ -14,6 +14,9 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .chunks import launch, overlap
+from .kvquant import _DT
+from .q4 import Q4Weight
 
 
 def _vec(t: torch.Tensor, name: str, n: int | None = None) -> None:
@@ -83,3 +86,63 @@ def qk_norm_rope_(qkv: torch.Tensor, hq: int, hkv: int, q_gamma: torch.Tensor, k
     _lib.call("nkv_qk_norm_rope", qkv.data_ptr(), hq, hkv, d, q_gamma.data_ptr(), k_gamma.data_ptr(), float(eps),
               inv_freq.data_ptr(), pos.data_ptr(), _lib.stream_ptr(qkv.device))
     return qkv
+
+
+# ---- 4-bit weights (``nova_amd.q4``), one token or a few
+
+
+def _q4_args(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None, n_out: int, out: torch.Tensor | None,
+             residual: torch.Tensor | None = None) -> tuple[int, torch.Tensor]:
+    """The checked arguments of a product: the number of tokens and the output."""
+    if not isinstance(w, Q4Weight):
+        raise ValueError("w must be a Q4Weight (nova_amd.q4.quantize_q4)")
+    n_in, dev = w.shape[1], w.codes.device
+    if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() == 0 or x.shape[-1] != n_in or x.device != dev:
+        raise ValueError(f"x must be fp16 / bf16 [.., {n_in}] on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        raise ValueError("x must be contiguous and 16-byte aligned")
+    if gamma is not None and (gamma.dtype != x.dtype or gamma.shape != (n_in,) or gamma.device != dev
+                              or not gamma.is_contiguous() or gamma.data_ptr() % 16):
+        raise ValueError(f"gamma must be a contiguous, 16-byte aligned {x.dtype} tensor of {n_in} elements on {dev}")
+    shape = (*x.shape[:-1], n_out)
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != shape or residual.device != dev
+                                 or not residual.is_contiguous()):
+        raise ValueError(f"residual must be a contiguous {x.dtype} tensor {list(shape)} on {dev}")
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        if out.dtype != x.dtype or out.shape != shape or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {x.dtype} tensor {list(shape)} on {dev}")
+        for name, t in (("x", x), ("gamma", gamma), ("w's codes", w.codes), ("w's scales", w.scales)):
+            if t is not None and overlap(out, t):
+                raise ValueError(f"out must not overlap {name}")
+        if residual is not None and residual.data_ptr() != out.data_ptr() and overlap(out, residual):
+            raise ValueError("out must be residual itself or not overlap it")
+    return x.numel() // n_in, out
+
+
+def rms_gemv_q4(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``W @ rms_norm(x) (+ residual)`` for each token of ``x`` ``[.., in]`` (fp16 or bf16, contiguous) with a 4-bit
+    weight; ``gamma=None`` skips the norm. Returns ``[.., out]`` of x's type; ``out`` may be ``residual``.
+
+    The normalized input is rounded once, to 11 bits, as the matrix cores' operand; all else is fp32 with one
+    rounding of the result. Made for one token to a few dozen (each 16 tokens read the weight again, from the caches
+    where it fits them)."""
+    tokens, out = _q4_args(x, w, gamma, w.shape[0], out, residual)
+    launch(x.device, "nkv_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps), w.codes.data_ptr(),
+           w.scales.data_ptr(), *w.shape, _lib.ptr(residual), out.data_ptr())
+    return out
+
+
+def swiglu_gemv_q4(x: torch.Tensor, w_gate_up: Q4Weight, gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``silu(G @ xn) * (U @ xn)`` for each token with the 4-bit ``w_gate_up = cat([G, U])`` of
+    ``[2 * intermediate, in]`` and ``xn = rms_norm(x)`` (``gamma=None``: ``x``), as :func:`rms_gemv_q4`."""
+    if not isinstance(w_gate_up, Q4Weight) or w_gate_up.shape[0] % 2:
+        raise ValueError("w_gate_up must be a Q4Weight [2 * intermediate, in_features] (nova_amd.q4.quantize_q4)")
+    inter = w_gate_up.shape[0] // 2
+    tokens, out = _q4_args(x, w_gate_up, gamma, inter, out)
+    launch(x.device, "nkv_swiglu_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps),
+           w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), inter, w_gate_up.shape[1], out.data_ptr())
+    return out

@@ -46,6 +46,7 @@ D = 128
 GT = 64
 PAGE_BYTES = 2 * GT * D + 4 * D * 2
 PAGE_BYTES_TOK = 2 * GT * D + 2 * GT * 2
+PAGE_BYTES_Q4 = 2 * (GT * D // 2 + GT * (D // 32) * 2)
 CODE_BYTES = GT * D
 MAX_PARTS_PER_SEQ = 256  # partials the tail's merge holds for one sequence
 CUS = 256  # compute units of an MI355X: one workgroup each at a time
@@ -360,10 +361,12 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
 
     page_bytes = PAGE_BYTES_TOK
     has_rings = False
+    _calls = {name: f"nkv_paged_{name}_tok" for name in ("quantize", "append_chunks", "attn_chunks", "read")}
+    _big_from = C.BIG_FROM
 
     def prefill(self, b: int, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store a prompt of n tokens (``[1, H_kv, n, 128]``) for sequence ``b``: every token
-        quantized by the HIP quantizer straight into its page (``nkv_paged_quantize_tok``)."""
+        quantized by the HIP quantizer straight into its page (``nkv_paged_quantize_tok`` / ``_q4``)."""
         n = self._check_prompt(key, value)
         h = self.num_kv_heads
         self.reserve(b, n + 1)
@@ -371,7 +374,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
             row = self.page_table[b]
             for which, x in enumerate((key, value)):
                 xc = x if x.stride(3) == 1 and x.stride(2) == D and x.data_ptr() % 16 == 0 else x.contiguous()
-                _lib.call("nkv_paged_quantize_tok", xc.data_ptr(), _DT[x.dtype], xc.stride(1), h, n, which,
+                _lib.call(self._calls["quantize"], xc.data_ptr(), _DT[x.dtype], xc.stride(1), h, n, which,
                           self.pages[layer].data_ptr(), row.data_ptr(), 0, self.num_pages, _lib.stream_ptr(row.device))
         self.pool.set_length(b, n)
         self.pos[b] = n
@@ -412,7 +415,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
             if n:
                 self.reserve(b, self._len[b] + n)
         return C.chunk_plan(counts, self._len[:len(counts)], self.pos, self.num_q_heads // self.num_kv_heads,
-                            self.num_kv_heads)
+                            self.num_kv_heads, self._big_from)
 
     def append_chunks(self, plan: ChunkPlan, qkv: torch.Tensor, layer: int, q_gamma: torch.Tensor | None = None,
                       k_gamma: torch.Tensor | None = None, eps: float = 1e-6, inv_freq: torch.Tensor | None = None,
@@ -455,7 +458,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
                         and (q_out.stride(0) == row or total <= 1))
             if not own_rows and C.overlap(q_out, given):
                 raise ValueError("q_out must be qkv's q heads themselves or not overlap qkv")
-        C.launch(dev, "nkv_paged_append_chunks_tok", qkv.data_ptr(), _DT[dtype], max(row, width), total,
+        C.launch(dev, self._calls["append_chunks"], qkv.data_ptr(), _DT[dtype], max(row, width), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
                  plan.seq_ptr, *plan.where, plan.nseq, hq, hkv, D, _lib.ptr(q_gamma), _lib.ptr(k_gamma), float(eps),
                  _lib.ptr(inv_freq), q_out.data_ptr(), max(q_out.stride(0), hq * D))
@@ -489,7 +492,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
                                 or not lse.is_contiguous() or lse.device != dev):
             raise ValueError(f"lse must be a contiguous fp32 tensor [{total}, {hq}] on {dev}")
         ws = _lib.scratch(dev, plan.ws_bytes) if plan.ws_bytes else None
-        C.launch(dev, "nkv_paged_attn_chunks_tok", query.data_ptr(), query.stride(0), query.stride(1), total,
+        C.launch(dev, self._calls["attn_chunks"], query.data_ptr(), query.stride(0), query.stride(1), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
                  *plan.where, plan.nseq, hq, hkv, D, *plan.work, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), _lib.ptr(ws),
                  plan.ws_bytes)
@@ -522,6 +525,27 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
             self.pool.set_length(b, self._len[b] + n * int(steps))
 
     def _read(self, plan: SpanPlan, layer: int, dtype: torch.dtype, k: torch.Tensor, v: torch.Tensor) -> None:
-        C.launch(self.pos.device, "nkv_paged_read_tok", self.pages[layer].data_ptr(), self.page_table.data_ptr(),
+        C.launch(self.pos.device, self._calls["read"], self.pages[layer].data_ptr(), self.page_table.data_ptr(),
                  self.page_table.stride(0), self.num_pages, plan.seq_ptr, *plan.where, plan.total, plan.nseq,
                  self.num_kv_heads, D, k.data_ptr(), v.data_ptr(), _DT[dtype])
+
+
+class PagedKVQ4Cache(PagedKVInt8TokCache):
+    """A batch of ragged sequences in 4 bits (the format of ``nova_amd.q4``: 32 channels of a token share a scale),
+    in pages of 64 tokens of one KV head: K codes ``[64, 64]`` bytes, V codes, K scales, V scales (256 fp16 each, in the
+    order that ``nkv_paged_attn_chunks_q4`` takes them), 9216 bytes; the per-token int8 format has 16640. Prompts go in
+    by ``prefill`` or ``append_chunks``, every step (a decode step is one of counts ``[1, 1, ..]``) by ``plan_chunks``,
+    ``append_chunks``, ``attend_chunks`` and ``advance_chunks``, cached tokens come back by ``plan_read`` and ``read``."""
+
+    page_bytes = PAGE_BYTES_Q4
+    _calls = {name: f"nkv_paged_{name}_q4" for name in PagedKVInt8TokCache._calls}
+    _big_from = 1 << 62
+
+    def plan(self, lengths: list[int] | None = None) -> None:
+        raise NotImplementedError("the 4-bit cache steps by plan_chunks")
+
+    def decode_step(self, key: torch.Tensor, value: torch.Tensor, query: torch.Tensor, layer: int) -> torch.Tensor:
+        raise NotImplementedError("the 4-bit cache decodes by plan_chunks([1, ..]), append_chunks and attend_chunks")
+
+    def attend(self, query: torch.Tensor, layer: int) -> torch.Tensor:
+        raise NotImplementedError("the 4-bit cache attends by attend_chunks")

@@ -1,0 +1,150 @@
+"""Host side of the 4-bit format (CPU): what the entry points refuse before any launch, the layouts of the header."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nova_amd import _lib
+from nova_amd import gemv as G
+from nova_amd import q4
+from nova_amd.paged import PAGE_BYTES_Q4
+
+OK, INVALID, UNSUPPORTED = _lib.NKV_OK, _lib.NKV_ERR_INVALID, _lib.NKV_ERR_UNSUPPORTED
+PTR = 1 << 20  # never followed: each call fails, or has nothing to do
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load(require_gpu=False)
+
+
+def _quantize(lib, **kw):
+    a = dict(x=PTR, dtype=0, rows=4, n=64, codes=PTR, scales=PTR, stream=None)
+    a.update(kw)
+    return lib.nkv_quantize_q4(*a.values())
+
+
+def _dequantize(lib, **kw):
+    a = dict(codes=PTR, scales=PTR, rows=4, n=64, x=PTR, dtype=0, stream=None)
+    a.update(kw)
+    return lib.nkv_dequantize_q4(*a.values())
+
+
+@pytest.mark.parametrize("call", [_quantize, _dequantize])
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=3), INVALID), (dict(rows=-1), INVALID), (dict(n=0), INVALID), (dict(n=48), INVALID), (dict(n=-32), INVALID),
+    (dict(rows=1 << 40), INVALID), (dict(x=None), INVALID), (dict(codes=None), INVALID), (dict(scales=None), INVALID),
+    (dict(x=PTR + 8), UNSUPPORTED), (dict(codes=PTR + 4), UNSUPPORTED), (dict(rows=0, x=None), OK)])
+def test_quantizer_refusals(lib, call, kw, rc):
+    assert call(lib, **kw) == rc
+    assert rc == OK or lib.nkv_last_error()
+
+
+def _gemv(lib, **kw):
+    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, codes=PTR, scales=PTR, out=64, n_in=64, residual=None, y=PTR, stream=None)
+    a.update(kw)
+    return lib.nkv_gemv_q4(*a.values())
+
+
+def _swiglu(lib, **kw):
+    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, codes=PTR, scales=PTR, out=64, n_in=64, y=PTR, stream=None)
+    a.update(kw)
+    return lib.nkv_swiglu_gemv_q4(*a.values())
+
+
+@pytest.mark.parametrize("call", [_gemv, _swiglu])
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=2), INVALID), (dict(dtype=-1), INVALID), (dict(tokens=-1), INVALID), (dict(tokens=1 << 20), INVALID),
+    (dict(out=0), INVALID), (dict(out=1 << 27), INVALID), (dict(n_in=0), INVALID), (dict(n_in=40), INVALID),
+    (dict(n_in=(1 << 20) + 32), INVALID), (dict(x=None), INVALID), (dict(codes=None), INVALID), (dict(scales=None), INVALID),
+    (dict(y=None), INVALID), (dict(x=PTR + 2), UNSUPPORTED), (dict(codes=PTR + 8), UNSUPPORTED), (dict(gamma=PTR + 2), UNSUPPORTED),
+    (dict(tokens=0, x=None), OK)])
+def test_product_refusals(lib, call, kw, rc):
+    assert call(lib, **kw) == rc
+    assert rc == OK or lib.nkv_last_error()
+
+
+def _paged_quantize(lib, **kw):
+    a = dict(x=PTR, dtype=0, hs=64 * 128, hkv=2, n=64, which=0, pages=PTR, row=PTR, first=0, np=4, stream=None)
+    a.update(kw)
+    return lib.nkv_paged_quantize_q4(*a.values())
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=3), INVALID), (dict(hkv=0), INVALID), (dict(n=-1), INVALID), (dict(which=2), INVALID), (dict(first=-1), INVALID),
+    (dict(np=0), INVALID), (dict(x=None), INVALID), (dict(pages=None), INVALID), (dict(row=None), INVALID),
+    (dict(x=PTR + 8), UNSUPPORTED), (dict(pages=PTR + 8), UNSUPPORTED), (dict(hs=63 * 128), UNSUPPORTED),
+    (dict(hs=64 * 128 + 4), UNSUPPORTED), (dict(n=0, x=None), OK)])
+def test_paged_quantizer_refusals(lib, kw, rc):
+    assert _paged_quantize(lib, **kw) == rc
+    assert rc == OK or lib.nkv_last_error()
+
+
+def _append(lib, **kw):
+    a = dict(qkv=PTR, dtype=0, rs=48 * 128, tokens=4, pages=PTR, table=PTR, ts=4, np=8, seq_of=PTR, cu=PTR, start=PTR, nseq=2,
+             hq=32, hkv=8, d=128, qg=PTR, kg=PTR, eps=1e-6, inv=PTR, q=PTR, q_rs=32 * 128, stream=None)
+    a.update(kw)
+    return lib.nkv_paged_append_chunks_q4(*a.values())
+
+
+def _attend(lib, **kw):
+    a = dict(q=PTR, q_ts=4096, q_hs=128, tokens=4, pages=PTR, table=PTR, ts=4, np=8, cu=PTR, start=PTR, nseq=2, hq=32, hkv=8,
+             d=128, units=PTR, n_units=1, wide=0, merges=None, n_merges=0, out=PTR, o_ts=4096, o_hs=128, lse=None, ws=None, ws_bytes=0,
+             stream=None)
+    a.update(kw)
+    return lib.nkv_paged_attn_chunks_q4(*a.values())
+
+
+def _read(lib, **kw):
+    a = dict(pages=PTR, table=PTR, ts=4, np=8, seq_of=PTR, cu=PTR, start=PTR, tokens=4, nseq=2, hkv=8, d=128, k=PTR, v=PTR, dtype=0,
+             stream=None)
+    a.update(kw)
+    return lib.nkv_paged_read_q4(*a.values())
+
+
+SHARED = [(dict(nseq=0), INVALID), (dict(nseq=1 << 15), INVALID), (dict(hkv=0), INVALID), (dict(ts=0), INVALID), (dict(np=0), INVALID),
+          (dict(tokens=-1), INVALID), (dict(tokens=1 << 24), INVALID), (dict(d=64), UNSUPPORTED), (dict(table=None), INVALID),
+          (dict(cu=None), INVALID), (dict(start=None), INVALID), (dict(pages=None), INVALID), (dict(pages=PTR + 8), UNSUPPORTED),
+          (dict(tokens=0, cu=None), OK)]
+OWN = {_append: [(dict(qkv=None), INVALID), (dict(dtype=3), INVALID), (dict(hq=30), INVALID), (dict(rs=47 * 128), INVALID),
+                 (dict(rs=48 * 128 + 4), UNSUPPORTED), (dict(qg=None), INVALID), (dict(q=PTR + 2), UNSUPPORTED)],
+       _attend: [(dict(q=None), INVALID), (dict(units=None), INVALID), (dict(hq=136), INVALID), (dict(n_units=1 << 20), INVALID),
+                 (dict(n_merges=1, merges=PTR), INVALID), (dict(q_ts=4), UNSUPPORTED), (dict(out=PTR + 2), UNSUPPORTED),
+                 (dict(n_units=0), OK)],
+       _read: [(dict(seq_of=None), INVALID), (dict(dtype=7), INVALID), (dict(k=None), INVALID), (dict(v=PTR + 4), UNSUPPORTED)]}
+
+
+@pytest.mark.parametrize("call", list(OWN))
+def test_paged_refusals(lib, call):
+    for kw, rc in SHARED + OWN[call]:
+        assert call(lib, **kw) == rc, kw
+        assert rc == OK or lib.nkv_last_error()
+
+
+def test_weights_of_the_host_are_refused():
+    with pytest.raises(ValueError):
+        q4.quantize_q4(torch.zeros(4, 64))
+    with pytest.raises(ValueError):
+        q4.Q4Weight(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.float16))
+    with pytest.raises(ValueError):
+        G.rms_gemv_q4(torch.zeros(64, dtype=torch.float16), torch.zeros(4, 64))
+    with pytest.raises(ValueError):
+        G.swiglu_gemv_q4(torch.zeros(64, dtype=torch.float16), torch.zeros(4, 64))
+
+
+def test_scale_places_are_one_each():
+    """The header's places of a page's 256 scales, each taken once."""
+    k = [((4 * (t // 16) + t % 4) * 4 + r) * 4 + t // 4 % 4 for t in range(64) for r in range(4)]
+    v = [64 * r + t // 8 * 8 + 2 * (t % 4) + t // 4 % 2 for t in range(64) for r in range(4)]
+    assert sorted(k) == sorted(v) == list(range(256))
+    assert PAGE_BYTES_Q4 == 2 * (64 * 64 + 512) == 9216
+
+
+def test_values_are_fp16_numbers():
+    """A scale of 8 significant bits (denormal: what fp16 keeps of them) times a code is an fp16 number."""
+    m = torch.arange(128, 256, dtype=torch.float64) / 128
+    s = (m[:, None] * 2.0 ** torch.arange(-24, 14, dtype=torch.float64)).to(torch.float16)
+    s = s[7 * s.double() <= 65504].double()
+    for c in range(8):
+        assert torch.equal((c * s).to(torch.float16).double(), c * s)
