@@ -338,13 +338,254 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
   }
 }
 
+// Units of up to 256 rows ("wide"): wave w takes rows 32 w .. 32 w + 31 as two row blocks, and every wave every page. A page's
+// codes come to one of three stages in LDS; its operands are made once for all waves, a sixteenth of K's and of V's by each, and
+// laid out as the products take them, 16 bytes a lane: tile t & 1 while the other one is read. One barrier a step: in step
+// t, before it, the conversion of page t + 1 into the tile that step t - 1 read and the wait for the loads of page t + 2;
+// after it the loads of page t + 4 into the stage of page t + 1.
+constexpr int WD_RB = 2, WD_ROWS = Q4_WAVES * WD_RB * 16, WD_STAGES = 3;
+constexpr int WD_TILE = GT * D * 2;                   // an operand tile: [16][64 lanes][16 bytes]
+constexpr int WD_VT = 2 * WD_TILE, WD_ST = 4 * WD_TILE;  // K tiles, V tiles, stages
+constexpr int WD_LDS = WD_ST + WD_STAGES * PAGE_Q4_BYTES;
+static_assert(WD_ROWS * D * 2 <= WD_LDS && 2 * Q4_WAVES * Q4_SLOT <= WD_LDS, "the output of a tile, and the small units, fit");
+
+__device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
+  const int s0 = (int)(at.steps * u.part / u.parts), n = (int)(at.steps * (u.part + 1) / u.parts) - s0;
+  const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);
+  const uint8_t* pages = a.pages + (int64_t)h * PAGE_Q4_BYTES;
+  const int64_t page_stride = (int64_t)a.b.hkv * PAGE_Q4_BYTES;
+  const uint32_t stages = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + WD_ST;
+  Pages pg(a.b, u.seq, s0, 1, n);
+  // wave w's loads of a page: 16 rows of K's (0 .. 3) or V's codes, wave 0 the scales, too. The 16-byte chunks of a row are
+  // moved by a key, so that the conversion's reads fall on different banks: K's by row / 16, V's by row / 4.
+  int loads = 0;  // in flight of the newest page
+  auto issue = [&](int page, int slot) {
+    loads = 0;
+    if (page < 0) return;
+    loads = wave == 0 ? 2 : 1;
+    const void* p = uniform_ptr(pages + page * page_stride);
+    const uint32_t dst = stages + slot * PAGE_Q4_BYTES;
+    const int key = wave < 4 ? wave : lane >> 4;
+    dma16(p, (uint32_t)(1024 * wave + (lane >> 2) * Q4_ROW + (((lane & 3) ^ key) << 4)), dst + 1024 * wave);
+    if (wave == 0) dma16(p, (uint32_t)(2 * Q4_CODES + 16 * lane), dst + 2 * Q4_CODES);
+  };
+  // steps that some row of the tile does not see whole: masked places may hold anything there (attend4_small)
+  const int tile_whole = (int)((at.start + u.row0 / a.gq + 1) / GT) - s0;
+  // Page t from its stage into its tiles; with the rules for masked places where `check` (a token whose V is not finite
+  // gets a K that is not). Wave w: K's tile b = w / 2, channels 32 g + 16 (w % 2) .. + 15; V's channels 16 w .. + 15.
+  auto convert = [&](int t, int slot, auto check) {
+    const uint8_t* sg = lds + WD_ST + slot * PAGE_Q4_BYTES;
+    const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4, b = wave >> 1;
+    const int krow = 16 * (c >> 2) + 4 * b + (c & 3), vrow = 16 * g + c;
+    const uint2 kw = *reinterpret_cast<const uint2*>(sg + krow * Q4_ROW + ((g ^ (c >> 2)) << 4) + 8 * (wave & 1));
+    const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+        (lds_v2i_t*)(const lds_void_t*)(sg + Q4_CODES + vrow * Q4_ROW + 8 * (wave & 1) + (((wave >> 1) ^ (c >> 2)) << 4))));
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(sg + 2 * Q4_CODES);
+    uint32_t ks = sc[(4 * c + g) * 4 + b];
+    const uint4* vp = reinterpret_cast<const uint4*>(sc + Q4_SCALES / 2 + (wave >> 1) * GT + 16 * g);
+    const uint4 v0 = vp[0], v1 = vp[1];
+    uint32_t vs[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    if constexpr (decltype(check)::value) {
+#pragma unroll
+      for (int grp = 0; grp < 4; ++grp)
+        if ((sc[Q4_SCALES / 2 + v_scale_at(krow, grp)] & 0x7fffu) > Q4_LARGEST) ks = 0x7e00u;
+      const int left = (int)min<int64_t>(GT, len - (int64_t)(s0 + t) * GT);  // tokens that the page has
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // the pair of tokens 16 g + 8 (e / 4) + e % 4 and 4 further
+        const int tok = 16 * g + 8 * (e >> 2) + (e & 3);
+        if ((vs[e] & 0x7fffu) > Q4_LARGEST || tok >= left) vs[e] &= 0xffff0000u;
+        if (((vs[e] >> 16) & 0x7fffu) > Q4_LARGEST || tok + 4 >= left) vs[e] &= 0xffffu;
+      }
+    }
+    const half2_t k2 = twice(ks);
+    const half2_t va[4] = {as_h2(vs[0]), as_h2(vs[1]), as_h2(vs[2]), as_h2(vs[3])};
+    const half2_t vb[4] = {as_h2(vs[4]), as_h2(vs[5]), as_h2(vs[6]), as_h2(vs[7])};
+    uint8_t* kt = lds + (t & 1) * WD_TILE + 16 * lane + 2048 * wave;  // (operand 4 b + k of wave 2 b + k / 2)
+    uint8_t* vt = lds + WD_VT + (t & 1) * WD_TILE + 16 * lane + 1024 * wave;
+    *reinterpret_cast<half8_t*>(kt) = unpack4(kw.x, k2);
+    *reinterpret_cast<half8_t*>(kt + 1024) = unpack4(kw.y, k2);
+    *reinterpret_cast<half8_t*>(vt) = unpack4(vw.x, va);
+    *reinterpret_cast<half8_t*>(vt + 8192) = unpack4(vw.y, vb);
+  };
+
+  const int row0 = u.row0 + wave * (WD_RB * 16);  // first row of this wave
+  const int rows = u.row0 + at.rows;
+  half8_t qb[WD_RB][4];
+#pragma unroll
+  for (int rb = 0; rb < WD_RB; ++rb) {
+    const int row = row0 + 16 * rb + c;
+    const bool ok = row < rows;
+    const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
+    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs + 32 * g;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 w = {0, 0, 0, 0};
+      if (ok) w = *reinterpret_cast<const uint4*>(qr + 8 * k);
+      qb[rb][k] = paired(w);
+    }
+  }
+  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
+  issue(p0, 0);
+  issue(p1, 1);
+  Sum4 st[WD_RB];
+#pragma unroll
+  for (int rb = 0; rb < WD_RB; ++rb) init(st[rb]);
+  // this wave's rows attend steps t < mine
+  const int last = min(row0 + WD_RB * 16, rows) - 1;
+  const int mine = row0 < rows ? min(n, (int)((at.start + last / a.gq) / GT) + 1 - s0) : 0;
+
+  half8_t op[16];  // the operands of the products: K's, then V's
+  const uint8_t* tile = lds + 16 * lane;
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) op[4 * k + b] = *reinterpret_cast<const half8_t*>(tile + (t & 1) * WD_TILE + 1024 * (4 * b + k));
+  };
+  auto load_v = [&](int t) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) op[e] = *reinterpret_cast<const half8_t*>(tile + (t & 1) * WD_TILE + WD_VT + 1024 * e);
+  };
+  float4_t S[WD_RB][4];
+  half8_t ph[WD_RB][2];
+  auto qk = [&](int rb) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        S[rb][b] = mfma32(op[4 * k + b], qb[rb][k], k ? S[rb][b] : float4_t{0.f, 0.f, 0.f, 0.f});
+  };
+  auto softmax = [&](int rb, auto masked, int t) {
+    const int l = tail_tid() & 63;
+    if constexpr (decltype(masked)::value) {
+      const int tok0 = (int)((int64_t)(s0 + t) * GT - at.start) + 16 * (l >> 4);  // (near the sequence's end, it fits)
+      const int tq = (row0 + 16 * rb + (l & 15)) / a.gq;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (tok0 + 4 * b + i > tq) S[rb][b][i] = NEG_INF;
+    }
+    weigh(st[rb], S[rb], a.sl2, ph[rb], l >> 4);
+  };
+  auto pv = [&](int rb) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int cb = 0; cb < 8; ++cb) st[rb].acc[cb] = mfma32(ph[rb][w], op[8 * w + cb], st[rb].acc[cb]);
+  };
+
+  wait_groups_all();
+  __syncthreads();
+  if (n > 0) convert(0, 0, std::true_type{});
+  __syncthreads();
+  issue(p2, 2);
+  issue(p3, 0);
+  int r1 = 1;  // (t + 1) mod 3
+
+  // One step. `fast`: every row sees pages t and t + 1 whole, and both are there.
+  auto step = [&](int t, auto fast_) {
+    constexpr bool fast = decltype(fast_)::value;
+    using masked = std::integral_constant<bool, !fast>;
+    const int p4 = pg.at(t + 4);
+    const bool go = fast || (t < mine && p0 >= 0);
+    if (go) {
+      load_k(t);
+      qk(0);
+      qk(1);
+      softmax(0, masked{}, t);
+      load_v(t);
+      pv(0);
+      softmax(1, masked{}, t);
+    }
+    if constexpr (fast) convert(t + 1, r1, std::false_type{});
+    else if (t + 1 < n) convert(t + 1, r1, std::true_type{});
+    if (go) pv(1);
+    // tile t + 1 is written, tile t is read, page t + 2 has landed
+    if (loads == 1) asm volatile("s_waitcnt vmcnt(1) lgkmcnt(0)" ::: "memory");
+    else if (loads == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    issue(p4, r1);
+    r1 = r1 == 2 ? 0 : r1 + 1;
+    p0 = p1; p1 = p2; p2 = p3; p3 = p4;
+  };
+  int t = 0;
+  for (; t + 1 < min(n, tile_whole) && p0 >= 0 && p1 >= 0; ++t) step(t, std::true_type{});
+  for (; t < n; ++t) step(t, std::false_type{});
+  wait_groups_all();
+  float rl[WD_RB];  // row c's sum of weights
+#pragma unroll
+  for (int rb = 0; rb < WD_RB; ++rb) rl[rb] = sum4rows(st[rb].l);
+
+  if (u.parts == 1) {
+    // out = the sum of V / l, through LDS so that 16 lanes store a row's 256 bytes (the 2-byte values at chunk ^ 2 ((row >> 2) & 3))
+    __syncthreads();  // every wave is past its last read of the tiles
+    const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4;
+    uint8_t* ow = lds + wave * (WD_RB * 16 * D * 2);
+#pragma unroll
+    for (int rb = 0; rb < WD_RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float l = shfl(rl[rb], 4 * g + i), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float m = shfl(reference(st[rb]), 4 * g + i);
+        const int r = 16 * rb + 4 * g + i, row = row0 + r;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb)
+          *reinterpret_cast<uint16_t*>(ow + r * (2 * D) + (((2 * cb + (c >> 3)) ^ (((r >> 2) & 3) << 1)) << 4) + 2 * (c & 7)) =
+              f2h(st[rb].acc[cb][i] * inv);
+        if (a.lse && c == 0 && row < rows)
+          a.lse[(at.first_token + row / a.gq) * a.hq + h * a.gq + row % a.gq] =
+              l == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
+      }
+#pragma unroll
+    for (int k = 0; k < WD_RB * 4; ++k) {
+      const int r = 4 * k + g, row = row0 + r;
+      const uint4 v = *reinterpret_cast<const uint4*>(ow + r * (2 * D) + ((c ^ (((r >> 2) & 3) << 1)) << 4));
+      if (row < rows)
+        *reinterpret_cast<uint4*>(a.out + (at.first_token + row / a.gq) * a.o_ts + (h * a.gq + row % a.gq) * a.o_hs + 8 * c) = v;
+    }
+  } else {
+    const int64_t pr0 = (int64_t)u.slot + (int64_t)u.part * u.rows + wave * (WD_RB * 16);
+#pragma unroll
+    for (int rb = 0; rb < WD_RB; ++rb) {
+      if (g == 0 && row0 + 16 * rb + c < rows && pr0 + 16 * rb + c < a.ws_rows)
+        *reinterpret_cast<float2*>(a.ws + ((pr0 + 16 * rb + c) * a.b.hkv + h) * CH_PART + D) = float2{reference(st[rb]), rl[rb]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * rb + 4 * g + i;
+        if (row0 + r >= rows || pr0 + r >= a.ws_rows) continue;
+        float* dst = a.ws + ((pr0 + r) * a.b.hkv + h) * CH_PART;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) dst[16 * cb + c] = st[rb].acc[cb][i];
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ bool unit_ok(const ChunkArgs& a, const Unit& u, int most) {
+  return u.seq >= 0 && u.seq < a.b.nseq && u.row0 >= 0 && u.rows > 0 && u.rows <= most && u.part >= 0 && u.part < u.parts && u.slot >= 0;
+}
+
+__global__ __launch_bounds__(Q4_THREADS, 1) void attn_q4_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[WD_LDS];
+  const int h = blockIdx.x % a.b.hkv;
+  const Unit u = a.units[blockIdx.x / a.b.hkv];
+  if (!unit_ok(a, u, u.kind == ROWS256 ? WD_ROWS : 32)) return;
+  if (u.kind == ROWS256) attend4_wide(a, u, h, lds);
+  else if (u.rows <= 16) attend4_small<1, Q4_WAVES>(a, u, h, lds);
+  else attend4_small<2, Q4_WAVES>(a, u, h, lds);
+}
+
 constexpr int Q4_SMALL = 4;  // waves of a workgroup in a launch of small units alone
 __global__ __launch_bounds__(64 * Q4_SMALL, 2) void attn_q4_small_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Q4_SMALL * Q4_SLOT];
   const int h = blockIdx.x % a.b.hkv;
   const Unit u = a.units[blockIdx.x / a.b.hkv];
-  if (u.seq < 0 || u.seq >= a.b.nseq || u.row0 < 0 || u.rows <= 0 || u.rows > 32 || u.part < 0 || u.part >= u.parts || u.slot < 0)
-    return;
+  if (!unit_ok(a, u, 32)) return;
   if (u.rows <= 16) attend4_small<1, Q4_SMALL>(a, u, h, lds);
   else attend4_small<2, Q4_SMALL>(a, u, h, lds);
 }
@@ -451,7 +692,8 @@ extern "C" int nkv_paged_attn_chunks_q4(const uint16_t* q, int64_t q_token_strid
   if (!any) return NKV_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(n_units * hkv));
-  hipLaunchKernelGGL(attn_q4_small_kernel, grid, dim3(64 * Q4_SMALL), 0, s, a);
+  if (wide) hipLaunchKernelGGL(attn_q4_kernel, grid, dim3(Q4_THREADS), 0, s, a);
+  else hipLaunchKernelGGL(attn_q4_small_kernel, grid, dim3(64 * Q4_SMALL), 0, s, a);
   if (int rc = check_launch(what)) return rc;
   return launch_merges(what, a, reinterpret_cast<const Merge*>(merges), n_merges, s);
 }

@@ -539,7 +539,6 @@ class PagedKVQ4Cache(PagedKVInt8TokCache):
 
     page_bytes = PAGE_BYTES_Q4
     _calls = {name: f"nkv_paged_{name}_q4" for name in PagedKVInt8TokCache._calls}
-    _big_from = 1 << 62
 
     def plan(self, lengths: list[int] | None = None) -> None:
         raise NotImplementedError("the 4-bit cache steps by plan_chunks")
