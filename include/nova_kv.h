@@ -816,31 +816,40 @@ int nkv_qk_norm_rope(uint16_t* qkv, int64_t hq, int64_t hkv, int64_t head_dim, c
  * One format for weights and for a paged cache (no counterpart in the reference). 32 consecutive values of a row
  * share a scale: with amax their largest magnitude, s = max(amax / 7, 2^-24) in fp32, rounded to 8 significant bits
  * (to nearest, ties to even) and held in fp16 (infinite where 7 s passes 65504, NaN for a group with a NaN);
- * code = clamp(rint(x / s), -7, 7), value = code * s, which fp16 holds exactly. Byte i of a row holds code + 8 of value
- * 2 i in its low half and that of value 2 i + 1 in its high half: n / 2 bytes a row of n values, n a multiple of 32.
+ * code = clamp(rint(x / s), -7, 7), value = code * s, which fp16 holds exactly.
  *
- * nkv_quantize_q4: x [rows][n] of x_dtype (contiguous, 16-byte aligned) to codes [rows][n / 2] (16-byte aligned) and
- * scales [rows][n / 32]; nkv_dequantize_q4: back to out_dtype, one rounding of code * s.
+ * A weight [rows][n] (n a multiple of 32) is blocks of 16 rows and 128 columns, 1152 bytes each, ceil(n / 128) of them
+ * for a tile of 16 rows, the tiles in order: 64 x 16 bytes of codes, then 64 scales. Piece c + 16 g holds row c, columns
+ * 32 g .. + 31: in 32-bit word k of it, bits 4 p .. + 3 hold code + 8 of
+ * column 8 k + 2 p and bits 4 p + 16 .. + 19 that of column 8 k + 2 p + 1 (p < 4). Rows and columns behind the last have a
+ * scale of 0. nkv_q4_weight_bytes: the size of a weight.
+ * nkv_quantize_q4: x [rows][n] of x_dtype (contiguous) to w4; nkv_dequantize_q4: back to out_dtype, one rounding of
+ * code * s. Buffers 16-byte aligned; at most 2^37 values.
  */
-int nkv_quantize_q4(const void* x, int x_dtype, int64_t rows, int64_t n, uint8_t* codes, uint16_t* scales, void* stream);
-int nkv_dequantize_q4(const uint8_t* codes, const uint16_t* scales, int64_t rows, int64_t n, void* out, int out_dtype,
-                      void* stream);
+int64_t nkv_q4_weight_bytes(int64_t rows, int64_t n);
+int nkv_quantize_q4(const void* x, int x_dtype, int64_t rows, int64_t n, uint8_t* w4, void* stream);
+int nkv_dequantize_q4(const uint8_t* w4, int64_t rows, int64_t n, void* out, int out_dtype, void* stream);
 
 /*
  * Products of a few tokens with 4-bit weights, beside nkv_gemv and nkv_swiglu_gemv: x [tokens][in_features], gamma
- * [in_features], residual and y [tokens][out_features], all of one dtype (NKV_F16 or NKV_BF16), contiguous; codes
- * [out_features][in_features / 2], scales [out_features][in_features / 32]; x, gamma and codes 16-byte aligned.
+ * [in_features], residual and y [tokens][out_features], all of one dtype (NKV_F16 or NKV_BF16), contiguous; w4: a weight
+ * [out_features][in_features] of nkv_quantize_q4; x, gamma and w4 16-byte aligned.
  * y[t][o] = sum_i W[o][i] xn[t][i] (+ residual[t][o]) with xn = x when gamma is NULL, else x * rsqrt(mean(x^2) + eps) *
  * gamma. xn is rounded once to 11 bits (as an operand), everything else is fp32 with one rounding of y. residual may be
  * NULL; y may be residual itself, but must not overlap it otherwise, nor x, gamma or the weight.
  * SwiGLU: act[t][j] = silu(g) * u, g = row j and u = row intermediate + j of the [2 * intermediate][in_features]
  * weight times xn. in_features a multiple of 32, at most 2^20; out_features (intermediate) less than 2^27; at most 2^20 - 16 tokens.
+ * workspace: nkv_gemv_q4_workspace_bytes(dtype, tokens, out_features or intermediate, in_features, gamma != NULL, swiglu) bytes
+ * (0 where one launch makes xn itself, as for few tokens), 16-byte aligned, any contents, one call's at a time.
  */
-int nkv_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
-                const uint16_t* scales, int64_t out_features, int64_t in_features, const void* residual, void* y,
-                void* stream);
-int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
-                       const uint16_t* scales, int64_t intermediate, int64_t in_features, void* act, void* stream);
+int64_t nkv_gemv_q4_workspace_bytes(int dtype, int64_t tokens, int64_t out_features, int64_t in_features, int norm,
+                                    int swiglu);
+int nkv_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4,
+                int64_t out_features, int64_t in_features, const void* residual, void* y,
+                void* workspace, int64_t workspace_bytes, void* stream);
+int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4,
+                       int64_t intermediate, int64_t in_features, void* act, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /*
  * The paged cache in 4 bits: a page is 64 tokens of one KV head, 9216 bytes: K codes [64][64 bytes], V codes, K scales,

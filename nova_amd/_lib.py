@@ -106,11 +106,13 @@ SIGNATURES = {
     "nkv_paged_read_q4": (c_int, _READ),
     "nkv_paged_read_t64": (c_int, _READ[:4] + [P, P] + _READ[4:]),  # (rings and length after num_pages)
     "nkv_paged_quantize_q4": (c_int, _PAGED_QUANTIZE),
-    "nkv_quantize_q4": (c_int, [P, c_int, I64, I64, P, P, P]),
-    "nkv_dequantize_q4": (c_int, [P, P, I64, I64, P, c_int, P]),
-    # x, dtype, tokens, gamma, eps, codes, scales, out_features, in_features, (residual,) y, stream
-    "nkv_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, P, I64, I64, P, P, P]),
-    "nkv_swiglu_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, P, I64, I64, P, P]),
+    "nkv_q4_weight_bytes": (I64, [I64, I64]),
+    "nkv_quantize_q4": (c_int, [P, c_int, I64, I64, P, P]),
+    "nkv_dequantize_q4": (c_int, [P, I64, I64, P, c_int, P]),
+    # x, dtype, tokens, gamma, eps, w4, out_features, in_features, (residual,) y, workspace, workspace_bytes, stream
+    "nkv_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, I64, I64, P, P, P, I64, P]),
+    "nkv_swiglu_gemv_q4": (c_int, [P, c_int, I64, P, c_float, P, I64, I64, P, P, I64, P]),
+    "nkv_gemv_q4_workspace_bytes": (I64, [c_int, I64, I64, I64, c_int, c_int]),
     "nkv_prefill_workspace_bytes": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_default_splits": (I64, [I64, I64, I64, I64]),
     "nkv_prefill_cutting": (c_int, [I64, I64, I64, I64, I64, I64, I64, P]),

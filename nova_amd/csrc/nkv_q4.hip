@@ -16,11 +16,9 @@ namespace {
 
 struct Quant4Args {
   const uint8_t* x;
-  int64_t head_stride;   // pages: elements from head to head
-  int64_t chunks;        // of eight values, all rows'
-  uint8_t* codes;        // a word a chunk
-  uint16_t* scales;      // one for four chunks
-  // pages: row r of head h is token first + r of a sequence, of tensor `which`; tokens whose table entry is outside
+  int64_t head_stride;  // elements from head to head
+  int64_t chunks;       // of eight values, all rows'
+  // row r of head h is token first + r of a sequence, of tensor `which`; tokens whose table entry is outside
   // [0, num_pages) are skipped
   uint8_t* pages;
   const int32_t* table;
@@ -28,46 +26,67 @@ struct Quant4Args {
   int which;
 };
 
-// Eight values a lane, a group to four lanes, both ways bound by memory.
-template <int DT, bool PAGES>
-__global__ __launch_bounds__(256) void quant4_kernel(Quant4Args a) {
+// A prompt's keys or values into their pages: eight values a lane, a group to four lanes; bound by memory.
+template <int DT>
+__global__ __launch_bounds__(256) void quant4_pages_kernel(Quant4Args a) {
   const int64_t step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.chunks; i += step) {  // (four lanes agree: chunks % 4 == 0)
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.chunks; i += step) {  // (16 lanes agree)
     Raw8<DT> r;
     float v[8];
     uint16_t scale;
-    if constexpr (PAGES) {
-      const int64_t row = i >> 4, h = row / a.n, t = row % a.n, tok = a.first + t;
-      const int j = (int)(i & 15), slot = (int)(tok % GT);
-      r.load(a.x + (h * a.head_stride + t * D + 8 * j) * Elem<DT>::SIZE);
-      const int32_t page = a.table[tok / GT];
-      r.get(v);
-      const uint32_t w = q4_quant8(v, scale);
-      if (page < 0 || page >= a.num_pages) continue;
-      uint8_t* p = a.pages + ((int64_t)page * a.hkv + h) * PAGE_Q4_BYTES;
-      *reinterpret_cast<uint32_t*>(p + a.which * Q4_CODES + slot * Q4_ROW + 4 * j) = w;
-      const int to = a.which ? v_scale_at(slot, j / 4) : k_scale_at(slot, j / 4);
-      if (j % 4 == 0) *reinterpret_cast<uint16_t*>(p + 2 * Q4_CODES + a.which * Q4_SCALES + 2 * to) = scale;
-    } else {
-      r.load(a.x + i * (8 * Elem<DT>::SIZE));
-      r.get(v);
-      const uint32_t w = q4_quant8(v, scale);
-      reinterpret_cast<uint32_t*>(a.codes)[i] = w;
-      if (i % 4 == 0) a.scales[i / 4] = scale;
-    }
+    const int64_t row = i >> 4, h = row / a.n, t = row % a.n, tok = a.first + t;
+    const int j = (int)(i & 15), slot = (int)(tok % GT);
+    r.load(a.x + (h * a.head_stride + t * D + 8 * j) * Elem<DT>::SIZE);
+    const int32_t page = a.table[tok / GT];
+    r.get(v);
+    const uint32_t w = q4_quant8(v, scale);
+    if (page < 0 || page >= a.num_pages) continue;
+    uint8_t* p = a.pages + ((int64_t)page * a.hkv + h) * PAGE_Q4_BYTES;
+    *reinterpret_cast<uint32_t*>(p + a.which * Q4_CODES + slot * Q4_ROW + 4 * j) = w;
+    const int to = a.which ? v_scale_at(slot, j / 4) : k_scale_at(slot, j / 4);
+    if (j % 4 == 0) *reinterpret_cast<uint16_t*>(p + 2 * Q4_CODES + a.which * Q4_SCALES + 2 * to) = scale;
+  }
+}
+
+// A weight [rows][n] into blocks: a workgroup takes one, four lanes a row's group of 32, four groups a lane.
+template <int DT>
+__global__ __launch_bounds__(64) void quant4_weight_kernel(const uint8_t* x, int64_t rows, int64_t n, uint8_t* out) {
+  const int64_t nb = (n + W4_COLS - 1) / W4_COLS, kb = blockIdx.x % nb, tile = blockIdx.x / nb;
+  const int lane = threadIdx.x, c = lane >> 2, k = lane & 3;
+  const int64_t row = tile * W4_ROWS + c;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int64_t col = kb * W4_COLS + 32 * g + 8 * k;
+    const bool in = row < rows && col < n;  // (four lanes agree)
+    Raw8<DT> r;
+    float v[8];
+    uint16_t scale;
+    r.zero();
+    if (in) r.load(x + (row * n + col) * Elem<DT>::SIZE);
+    r.get(v);
+    const uint32_t w = q4_quant8<true>(v, scale);
+    uint8_t* to = out + w4_at(row, nb, kb, g);
+    *reinterpret_cast<uint32_t*>(to + 4 * k) = w;
+    if (k == 0) *reinterpret_cast<uint16_t*>(to + w4_scale_from(c + 16 * g)) = in ? scale : (uint16_t)0;
   }
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void dequant4_kernel(const uint32_t* codes, const uint16_t* scales, int64_t chunks, uint8_t* out) {
-  const int64_t step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += step) {
-    const uint32_t w = codes[i];
-    const float s = h2f(scales[i / 4]);
+__global__ __launch_bounds__(64) void dequant4_weight_kernel(const uint8_t* w4, int64_t rows, int64_t n, uint8_t* out) {
+  const int64_t nb = (n + W4_COLS - 1) / W4_COLS, kb = blockIdx.x % nb, tile = blockIdx.x / nb;
+  const int lane = threadIdx.x, c = lane >> 2, k = lane & 3;
+  const int64_t row = tile * W4_ROWS + c;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int64_t col = kb * W4_COLS + 32 * g + 8 * k;
+    if (row >= rows || col >= n) continue;
+    const uint8_t* at = w4 + w4_at(row, nb, kb, g);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(at + 4 * k);
+    const float s = h2f(*reinterpret_cast<const uint16_t*>(at + w4_scale_from(c + 16 * g)));
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = q4_value(w, e, s);
-    store8<DT, false>(out + i * (8 * Elem<DT>::SIZE), v);
+    for (int e = 0; e < 8; ++e) v[e] = q4_value(w, e / 2 + 4 * (e % 2), s);
+    store8<DT, false>(out + (row * n + col) * Elem<DT>::SIZE, v);
   }
 }
 
@@ -596,15 +615,21 @@ int dtype_ok(const char* what, int dtype) {
   return dtype == NKV_F16 || dtype == NKV_BF16 || dtype == NKV_F32 ? NKV_OK : fail(NKV_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
 }
 
-unsigned blocks_of(int64_t chunks) { return (unsigned)std::min<int64_t>(cdiv(chunks, 256), 1 << 20); }
-
-template <bool PAGES>
-int launch_quant4(const char* what, const Quant4Args& a, int dtype, hipStream_t s) {
-  const dim3 grid(blocks_of(a.chunks)), block(256);
-  if (dtype == NKV_F16) hipLaunchKernelGGL((quant4_kernel<NKV_F16, PAGES>), grid, block, 0, s, a);
-  else if (dtype == NKV_BF16) hipLaunchKernelGGL((quant4_kernel<NKV_BF16, PAGES>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((quant4_kernel<NKV_F32, PAGES>), grid, block, 0, s, a);
-  return check_launch(what);
+// The arguments of the weights' quantizers, and the blocks of a launch.
+int weight_args(const char* what, const void* x, int dtype, int64_t rows, int64_t n, const void* w4, int64_t& blocks) {
+  set_error("");
+  blocks = 0;
+  if (int rc = dtype_ok(what, dtype)) return rc;
+  if (rows < 0 || n <= 0 || n % Q4_GROUP || rows >= (int64_t(1) << 40) || n >= (int64_t(1) << 40))
+    return fail(NKV_ERR_INVALID, "%s: sizes rows=%lld n=%lld (n a positive multiple of 32)", what, (long long)rows, (long long)n);
+  const int64_t tiles = cdiv(rows, W4_ROWS), nb = cdiv(n, W4_COLS);
+  if (tiles && nb > ((int64_t(1) << 26) - 1) / tiles)  // (a launch has less than 2^32 threads)
+    return fail(NKV_ERR_INVALID, "%s: rows=%lld n=%lld: more than 2^37 values", what, (long long)rows, (long long)n);
+  if (rows == 0) return NKV_OK;
+  if (!x || !w4) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(x) || !al16(w4)) return fail(NKV_ERR_UNSUPPORTED, "%s: buffers must be 16-byte aligned", what);
+  blocks = tiles * nb;
+  return NKV_OK;
 }
 
 }  // namespace
@@ -613,43 +638,34 @@ int launch_quant4(const char* what, const Quant4Args& a, int dtype, hipStream_t 
 
 using namespace nkv;
 
-extern "C" int nkv_quantize_q4(const void* x, int x_dtype, int64_t rows, int64_t n, uint8_t* codes, uint16_t* scales,
-                               void* stream) {
-  set_error("");
-  const char* what = "quantize_q4";
-  if (int rc = dtype_ok(what, x_dtype)) return rc;
-  if (rows < 0 || n <= 0 || n % Q4_GROUP || (rows && n > (int64_t(1) << 40) / rows))
-    return fail(NKV_ERR_INVALID, "%s: sizes rows=%lld n=%lld (n a positive multiple of 32)", what, (long long)rows, (long long)n);
-  if (rows == 0) return NKV_OK;
-  if (!x || !codes || !scales) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  if (!al16(x) || !al16(codes)) return fail(NKV_ERR_UNSUPPORTED, "%s: x and codes must be 16-byte aligned", what);
-  Quant4Args a{};
-  a.x = static_cast<const uint8_t*>(x);
-  a.chunks = rows * (n / 8);
-  a.codes = codes;
-  a.scales = scales;
-  return launch_quant4<false>(what, a, x_dtype, static_cast<hipStream_t>(stream));
+extern "C" int64_t nkv_q4_weight_bytes(int64_t rows, int64_t n) {
+  return rows > 0 && n > 0 ? cdiv(rows, W4_ROWS) * cdiv(n, W4_COLS) * W4_BLOCK : 0;
 }
 
-extern "C" int nkv_dequantize_q4(const uint8_t* codes, const uint16_t* scales, int64_t rows, int64_t n, void* out,
-                                 int out_dtype, void* stream) {
-  set_error("");
-  const char* what = "dequantize_q4";
-  if (int rc = dtype_ok(what, out_dtype)) return rc;
-  if (rows < 0 || n <= 0 || n % Q4_GROUP || (rows && n > (int64_t(1) << 40) / rows))
-    return fail(NKV_ERR_INVALID, "%s: sizes rows=%lld n=%lld (n a positive multiple of 32)", what, (long long)rows, (long long)n);
-  if (rows == 0) return NKV_OK;
-  if (!codes || !scales || !out) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  if (!al16(codes) || !al16(out)) return fail(NKV_ERR_UNSUPPORTED, "%s: codes and out must be 16-byte aligned", what);
-  const int64_t chunks = rows * (n / 8);
-  const dim3 grid(blocks_of(chunks)), block(256);
+extern "C" int nkv_quantize_q4(const void* x, int x_dtype, int64_t rows, int64_t n, uint8_t* w4, void* stream) {
+  int64_t blocks;
+  if (int rc = weight_args("quantize_q4", x, x_dtype, rows, n, w4, blocks)) return rc;
+  if (!blocks) return NKV_OK;
+  const dim3 grid((unsigned)blocks), block(64);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(codes);
+  const uint8_t* from = static_cast<const uint8_t*>(x);
+  if (x_dtype == NKV_F16) hipLaunchKernelGGL(quant4_weight_kernel<NKV_F16>, grid, block, 0, s, from, rows, n, w4);
+  else if (x_dtype == NKV_BF16) hipLaunchKernelGGL(quant4_weight_kernel<NKV_BF16>, grid, block, 0, s, from, rows, n, w4);
+  else hipLaunchKernelGGL(quant4_weight_kernel<NKV_F32>, grid, block, 0, s, from, rows, n, w4);
+  return check_launch("quantize_q4");
+}
+
+extern "C" int nkv_dequantize_q4(const uint8_t* w4, int64_t rows, int64_t n, void* out, int out_dtype, void* stream) {
+  int64_t blocks;
+  if (int rc = weight_args("dequantize_q4", out, out_dtype, rows, n, w4, blocks)) return rc;
+  if (!blocks) return NKV_OK;
+  const dim3 grid((unsigned)blocks), block(64);
+  hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* to = static_cast<uint8_t*>(out);
-  if (out_dtype == NKV_F16) hipLaunchKernelGGL(dequant4_kernel<NKV_F16>, grid, block, 0, s, words, scales, chunks, to);
-  else if (out_dtype == NKV_BF16) hipLaunchKernelGGL(dequant4_kernel<NKV_BF16>, grid, block, 0, s, words, scales, chunks, to);
-  else hipLaunchKernelGGL(dequant4_kernel<NKV_F32>, grid, block, 0, s, words, scales, chunks, to);
-  return check_launch(what);
+  if (out_dtype == NKV_F16) hipLaunchKernelGGL(dequant4_weight_kernel<NKV_F16>, grid, block, 0, s, w4, rows, n, to);
+  else if (out_dtype == NKV_BF16) hipLaunchKernelGGL(dequant4_weight_kernel<NKV_BF16>, grid, block, 0, s, w4, rows, n, to);
+  else hipLaunchKernelGGL(dequant4_weight_kernel<NKV_F32>, grid, block, 0, s, w4, rows, n, to);
+  return check_launch("dequantize_q4");
 }
 
 extern "C" int nkv_paged_quantize_q4(const void* x, int x_dtype, int64_t x_head_stride, int64_t hkv, int64_t n, int which,
@@ -672,7 +688,12 @@ extern "C" int nkv_paged_quantize_q4(const void* x, int x_dtype, int64_t x_head_
   a.pages = pages;
   a.table = table_row;
   a.n = n; a.hkv = hkv; a.first = first_token; a.num_pages = num_pages; a.which = which;
-  return launch_quant4<true>(what, a, x_dtype, static_cast<hipStream_t>(stream));
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.chunks, 256), 1 << 20)), block(256);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (x_dtype == NKV_F16) hipLaunchKernelGGL(quant4_pages_kernel<NKV_F16>, grid, block, 0, s, a);
+  else if (x_dtype == NKV_BF16) hipLaunchKernelGGL(quant4_pages_kernel<NKV_BF16>, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(quant4_pages_kernel<NKV_F32>, grid, block, 0, s, a);
+  return check_launch(what);
 }
 
 extern "C" int nkv_paged_attn_chunks_q4(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,

@@ -1,10 +1,15 @@
 // The decode step's projections with 4-bit weights (nkv_q4.h) for one token or a few: y = W xn (+ residual), and the
 // first half of a SwiGLU block, xn = x or its RMSNorm.
 //
-// On the matrix cores: 16 rows of W times up to 16 tokens. The weights become exact fp16 operands; lane c + 16 g takes
-// row c's group g of every 128 inputs, 16 bytes, one scale. xn is rounded once to fp16, scaled by a power of two of the
-// token's own, so that bf16's range and large gammas stay within fp16's. The waves of a workgroup cut the inputs among them;
-// everything else in fp32, with one rounding at the end. Bound by the weights' bytes.
+// On the matrix cores: tiles of 16 rows of W times tiles of 16 columns. Lane c + 16 g takes row c's group g of a block's 128
+// inputs, 16 bytes. xn is rounded once to fp16, scaled by a power of two of the token's own, so that bf16's range and large
+// gammas stay within fp16's. The waves of a workgroup cut the inputs among them, a block in turn; everything else in fp32,
+// with one rounding at the end. Bound by the weights' bytes, and by a launch's chain of loads that wait for each other.
+//
+// Three forms, by the tokens and by what is to be done to x:
+// - product4_few_kernel: up to 4 tokens with a norm (or bf16), one launch;
+// - product4_kernel: up to 16 tokens of fp16 as they are, one launch;
+// - product4_many_kernel: the rest, after xn_kernel has laid xn out as the products take it.
 
 #include <algorithm>
 #include <type_traits>
@@ -16,234 +21,554 @@ namespace nkv {
 
 namespace {
 
-constexpr int PW = 4;             // waves of a workgroup
-constexpr int PB = 128;           // inputs of a block: four products deep
-constexpr int PT = 16;            // tokens of a workgroup, at most
-constexpr int PX = 48 * 1024;     // bytes of LDS for xn
-constexpr int P_IN = 1 << 20;     // inputs, at most
+constexpr int PB = 128;       // inputs of a block: four products deep
+constexpr int P_IN = 1 << 20;  // inputs, at most
+constexpr int64_t P_TOKENS = (int64_t(1) << 20) - 16;
 
 struct ProductArgs {
   const uint8_t* x;        // [tokens][in]
   const uint8_t* gamma;    // [in] or NULL
   float eps;
-  const uint8_t* codes;    // [rows][in / 2]
-  const uint16_t* scales;  // [rows][in / 32]
+  const uint8_t* w4;       // blocks of 16 rows and 128 inputs
   int64_t out;             // outputs a token (SwiGLU: half the rows)
   int in;
   const uint8_t* residual;  // [tokens][out] or NULL
   uint8_t* y;
   int64_t tokens;
-  int chunk;               // inputs whose xn is in LDS at a time, a multiple of PW * PB
+  const float* unit;  // [tokens], or NULL: 1
 };
 
-// A few values of element type DT.
 template <int DT>
 __device__ __forceinline__ float load1(const uint8_t* p, int64_t i) {
   const uint16_t b = reinterpret_cast<const uint16_t*>(p)[i];
   return DT == NKV_F16 ? h2f(b) : bf2f(b);
 }
 
-// RT: tiles of 16 rows a workgroup takes; GATED: the second is the up rows of the first's gates.
-template <int DT, int RT, bool GATED>
-__global__ __launch_bounds__(64 * PW, 4) void product4_kernel(ProductArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // [tokens][chunk + 8] fp16; the sums at the end
-  __shared__ float unit[PT], inverse[PT];  // of a token: xn = x * norm * gamma, held times inverse, unit = 1 / inverse
-  __shared__ float norm[PT];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t t0 = (int64_t)blockIdx.y * PT;
-  const int nt = (int)min<int64_t>(PT, a.tokens - t0);
-  const int64_t o0 = (int64_t)blockIdx.x * (GATED ? 16 : 16 * RT);
-  const int blocks = (a.in + PB - 1) / PB, groups = a.in / Q4_GROUP;
+// ---------------------------------------------------------------- xn
 
-  // this lane's rows (rows behind the last: the last, not stored)
-  const uint8_t* wp[RT];
-  const uint16_t* sp[RT];
+// A token's norm factor and the power of two that its xn is held in: the largest comes to 2^14 (not finite: 1).
+struct Factor {
+  float norm, inverse, unit;
+};
+__device__ __forceinline__ Factor factor_of(float ss, float top, bool norm, int in, float eps) {
+  const float r = norm ? rsqrtf(ss / (float)in + eps) : 1.0f;
+  top *= r;
+  const int ex = top > 0.0f && top < 3e38f ? max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
+  return {r, __uint_as_float((uint32_t)(127 - ex) << 23), __uint_as_float((uint32_t)(127 + ex) << 23)};
+}
+// What eight values add to a token's sum of squares and largest product with gamma.
+__device__ __forceinline__ void measure8(const float (&v)[8], const float (&gv)[8], float& ss, float& top) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int64_t row = GATED ? r * a.out + min(o0 + c, a.out - 1) : min(o0 + 16 * r + c, a.out - 1);
-    wp[r] = a.codes + row * (a.in / 2) + 16 * g;
-    sp[r] = a.scales + row * groups + g;
+  for (int e = 0; e < 8; ++e) {
+    ss = __builtin_fmaf(v[e], v[e], ss);
+    top = fmaxf(top, __builtin_fabsf(v[e] * gv[e]));
   }
-  constexpr int AHEAD = 4;
-  uint4 w[AHEAD][RT];
-  uint16_t s[AHEAD][RT];
-  auto load = [&](int e, int kb) {
+}
+__device__ __forceinline__ uint4 xn8(const float (&v)[8], const float (&gv)[8], const Factor& f) {
+  uint32_t h[4];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const bool ok = 4 * kb + g < groups;
-      const u32x4_t* p = reinterpret_cast<const u32x4_t*>(wp[r] + (int64_t)kb * (PB / 2));
-      u32x4_t v = {0, 0, 0, 0};
-      if (ok) v = __builtin_nontemporal_load(p);
-      w[e][r] = uint4{v.x, v.y, v.z, v.w};
-      s[e][r] = ok ? sp[r][4 * kb] : 0;
+  for (int e = 0; e < 4; ++e)
+    h[e] = (uint32_t)f2h(v[2 * e] * f.norm * gv[2 * e] * f.inverse) |
+           ((uint32_t)f2h(v[2 * e + 1] * f.norm * gv[2 * e + 1] * f.inverse) << 16);
+  return uint4{h[0], h[1], h[2], h[3]};
+}
+// xn once for all workgroups of a product, one token a workgroup, as operands: piece (block kb, k, tile n, lane c + 16 g) of 16
+// bytes holds token 16 n + c's inputs 128 kb + 32 g + 8 k .. + 7 (zeros behind the last). Tiles are counted in passes of
+// NT, each of which lies together.
+template <int DT>
+__global__ __launch_bounds__(256) void xn_kernel(ProductArgs a, int nt, uint8_t* xn, float* unit) {
+  __shared__ float part[2][4];
+  const int tid = threadIdx.x;
+  const int64_t t = blockIdx.x;
+  const uint8_t* x = a.x + t * a.in * 2;
+  float ss = 0.0f, top = 0.0f, v[8], gv[8];
+  constexpr int KEEP = 2;  // chunks held from the first pass to the second
+  Raw8<DT> r[KEEP], gr[KEEP];
+  const auto load = [&](int i, Raw8<DT>& xr, Raw8<DT>& g8) {
+    xr.load(x + 2 * i);
+    if (a.gamma) g8.load(a.gamma + 2 * i);
+  };
+  const auto get = [&](const Raw8<DT>& xr, const Raw8<DT>& g8) {
+    xr.get(v);
+    if (a.gamma) {
+      g8.get(gv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gv[e] = 1.0f;
     }
   };
 #pragma unroll
-  for (int e = 0; e < AHEAD; ++e) load(e, wave + PW * e);
-
-  // the tokens' norms and units
-  if (a.gamma || DT != NKV_F16) {
-    for (int t = wave; t < nt; t += PW) {
-      const uint8_t* x = a.x + (t0 + t) * a.in * 2;
-      float ss = 0.0f, top = 0.0f;
-      for (int i = 8 * lane; i < a.in; i += 512) {
-        Raw8<DT> r, gr;
-        r.load(x + 2 * i);
-        float v[8], gv[8];
-        r.get(v);
-        if (a.gamma) {
-          gr.load(a.gamma + 2 * i);
-          gr.get(gv);
-        }
+  for (int k = 0; k < KEEP; ++k)
+    if (const int i = 8 * tid + 2048 * k; i < a.in) load(i, r[k], gr[k]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss = __builtin_fmaf(v[e], v[e], ss);
-          top = fmaxf(top, __builtin_fabsf(a.gamma ? v[e] * gv[e] : v[e]));
-        }
-      }
-      ss = hsum64(ss);
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, shfl_xor(top, o));
-      const float r = a.gamma ? rsqrtf(ss / (float)a.in + a.eps) : 1.0f;
-      top *= r;
-      // the power of two that brings the largest to 2^14
-      const int ex = top > 0.0f && top < 3e38f ? max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
-      if (lane == 0) {
-        norm[t] = r;
-        inverse[t] = __uint_as_float((uint32_t)(127 - ex) << 23);
-        unit[t] = __uint_as_float((uint32_t)(127 + ex) << 23);
-      }
+  for (int k = 0; k < KEEP; ++k)
+    if (8 * tid + 2048 * k < a.in) {
+      get(r[k], gr[k]);
+      measure8(v, gv, ss, top);
     }
-  } else if (tid < PT) {
-    norm[tid] = inverse[tid] = unit[tid] = 1.0f;
+  for (int i = 8 * tid + 2048 * KEEP; i < a.in; i += 2048) {
+    Raw8<DT> x8, g8;
+    load(i, x8, g8);
+    get(x8, g8);
+    measure8(v, gv, ss, top);
   }
-
-  const int stride = 2 * a.chunk + 16;  // bytes of a token's row: 16 tokens' chunks fall on different banks
-  float4_t acc[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) acc[r] = float4_t{0.f, 0.f, 0.f, 0.f};
-  const uint8_t* xp = xs + min(c, nt - 1) * stride + 64 * g;
-  int kb = wave;
-  for (int k0 = 0; k0 < a.in; k0 += a.chunk) {
-    __syncthreads();  // norms are there; the chunk before is read
-    const int n8 = min(a.chunk, (blocks * PB) - k0) / 8;
-    for (int i = tid; i < nt * n8; i += 64 * PW) {
-      const int t = i / n8, k = 8 * (i - t * n8), at = k0 + k;
-      Raw8<DT> r, gr;
-      r.zero();
-      float v[8], gv[8];
-      if (at < a.in) r.load(a.x + ((t0 + t) * a.in + at) * 2);
-      uint4 u;
-      if (!a.gamma && DT == NKV_F16) {
-        u = r.w[0];
-      } else {
-        r.get(v);
-        const float f = inverse[t];
-        if (a.gamma) {
-          gr.zero();
-          if (at < a.in) gr.load(a.gamma + 2 * at);
-          gr.get(gv);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = v[e] * norm[t] * gv[e];
-        }
-        uint32_t h[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = (uint32_t)f2h(v[2 * e] * f) | ((uint32_t)f2h(v[2 * e + 1] * f) << 16);
-        u = uint4{h[0], h[1], h[2], h[3]};
-      }
-      *reinterpret_cast<half8_t*>(xs + t * stride + 2 * k) = paired(u);
-    }
-    __syncthreads();
-    const int end = min(blocks, (k0 + a.chunk) / PB), base = k0 / PB;
-    while (kb < end) {
-#pragma unroll
-      for (int e = 0; e < AHEAD; ++e) {
-        if (kb < end) {  // (the waves differ, their lanes agree)
-          const uint8_t* p = xp + (kb - base) * (2 * PB);
-          half8_t b[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const half8_t*>(p + 16 * k);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const half2_t sc = as_h2((uint32_t)s[0][r] * 0x10001u);
-            acc[r] = mfma32(unpack4(w[0][r].x, sc), b[0], acc[r]);
-            acc[r] = mfma32(unpack4(w[0][r].y, sc), b[1], acc[r]);
-            acc[r] = mfma32(unpack4(w[0][r].z, sc), b[2], acc[r]);
-            acc[r] = mfma32(unpack4(w[0][r].w, sc), b[3], acc[r]);
-          }
-          // the registers move up: chunks may end anywhere
-#pragma unroll
-          for (int f = 0; f + 1 < AHEAD; ++f)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) w[f][r] = w[f + 1][r], s[f][r] = s[f + 1][r];
-          load(AHEAD - 1, kb + PW * AHEAD);
-          kb += PW;
-        }
-      }
-    }
-  }
-
-  // ---- the waves' sums into one
+  ss = sum4rows(row16_sum(ss));
+  top = max4rows(row16_max(top));
+  if ((tid & 63) == 0) part[0][tid >> 6] = ss, part[1][tid >> 6] = top;
   __syncthreads();
-  float* red = reinterpret_cast<float*>(xs);  // [wave][tile][row 16][token 16 + 1]
+  ss = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+  top = fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
+  const Factor f = factor_of(ss, top, a.gamma, a.in, a.eps);
+  const int blocks = (a.in + PB - 1) / PB, tile = (int)(t / 16), n = tile % nt;
+  uint8_t* to = xn + (int64_t)(tile - n) * blocks * 4096 + n * 1024 + (int)(t & 15) * 16;
+  const auto store = [&](int i, uint4 u) {  // input i: block i / 128, g, k
+    *reinterpret_cast<uint4*>(to + ((int64_t)(i >> 7) * 4 + ((i >> 3) & 3)) * (nt * 1024) + ((i >> 5) & 3) * 256) = u;
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (const int i = 8 * tid + 2048 * k; i < a.in) {
+      get(r[k], gr[k]);
+      store(i, xn8(v, gv, f));
+    }
+  for (int i = 8 * tid + 2048 * KEEP; i < a.in; i += 2048) {
+    Raw8<DT> x8, g8;
+    load(i, x8, g8);
+    get(x8, g8);
+    store(i, xn8(v, gv, f));
+  }
+  for (int i = a.in + 8 * tid; i < blocks * PB; i += 2048) store(i, uint4{0, 0, 0, 0});
+  if (tid == 0) unit[t] = f.unit;
+}
+
+// ---------------------------------------------------------------- the weights of a wave
+
+// RT: tiles of 16 rows; GATED: the first half of them are gates, the others their up rows. W: the workgroup's waves.
+template <int RT, bool GATED, int W, int AHEAD>
+struct Weights {
+  static constexpr int TILES = GATED ? RT / 2 : RT;  // of 16 outputs
+  const uint8_t* wp[RT];
+  uint4 w[AHEAD][RT];
+  uint16_t s[AHEAD][RT];
+  int from[RT];
+  __device__ __forceinline__ Weights(const ProductArgs& a, int64_t o0, int lane, int blocks) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {  // (outputs behind the last: the last, not stored)
+      const int64_t row = min(o0 + 16 * (r % TILES) + (lane & 15), a.out - 1) + (r >= TILES ? a.out : 0);
+      wp[r] = a.w4 + w4_at(row, blocks, 0, lane >> 4);
+      from[r] = w4_scale_from((int)(row & 15) + (lane & 48));
+    }
+  }
+  __device__ __forceinline__ void load(int e, int kb) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const uint8_t* p = wp[r] + (int64_t)kb * W4_BLOCK;
+      const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+      w[e][r] = uint4{v.x, v.y, v.z, v.w};
+      s[e][r] = *reinterpret_cast<const uint16_t*>(p + from[r]);
+    }
+  }
+  __device__ __forceinline__ half8_t operand(int e, int r, int k) const {
+    const half2_t sc = as_h2((uint32_t)s[e][r] * 0x10001u);
+    const uint4& x = w[e][r];
+    return unpack4(k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w, sc);
+  }
+};
+
+// The waves' sums into one, and out: tokens t0 .. t0 + nt - 1, outputs o0 ... red: W * RT * NT tiles of 16 x 17 floats. PER:
+// columns of a token.
+template <int DT, int RT, int NT, bool GATED, int W, int PER = 1>
+__device__ __forceinline__ void finish(const ProductArgs& a, const float4_t (&acc)[RT][NT], float* red, int64_t t0, int nt,
+                                       int64_t o0, const float* unit) {
+  constexpr int TILES = GATED ? RT / 2 : RT;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4, wave = tid >> 6;
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[((wave * RT + r) * 16 + 4 * g + i) * 17 + c] = acc[r][i];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[(((wave * RT + r) * NT + n) * 16 + 4 * g + i) * 17 + c] = acc[r][n][i];
   __syncthreads();
-  const int t = tid >> 4, row = tid & 15;
-  if (t >= nt) return;
-  float v[RT];
+  for (int i = tid; i < TILES * NT * 256; i += 64 * W) {
+    const int row = i & 15, t16 = (i >> 4) & 15, n = (i >> 8) % NT, r = (i >> 8) / NT, t = (16 * n + t16) / PER;
+    const int64_t o = o0 + 16 * r + row;
+    if (t >= nt || o >= a.out || t16 % PER) continue;
+    float v[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    v[r] = 0.0f;
-#pragma unroll
-    for (int q = 0; q < PW; ++q) v[r] += red[((q * RT + r) * 16 + row) * 17 + t];
-    v[r] *= unit[t];
-  }
-  auto store = [&](int64_t o, float f) {
+    for (int half = 0; half < (GATED ? 2 : 1); ++half)
+      for (int q = 0; q < W; ++q) v[half] += red[(((q * RT + r + half * TILES) * NT + n) * 16 + row) * 17 + t16];
+    const float f = unit ? unit[t] : 1.0f;
+    v[0] *= f;
+    v[1] *= f;
+    if constexpr (GATED) v[0] = v[0] / (1.0f + expf(-v[0])) * v[1];
     const int64_t at = (t0 + t) * a.out + o;
-    if (a.residual) f += load1<DT>(a.residual, at);
-    reinterpret_cast<uint16_t*>(a.y)[at] = DT == NKV_F16 ? f2h(f) : f2bf(f);
-  };
-  if constexpr (GATED) {
-    if (o0 + row < a.out) store(o0 + row, v[0] / (1.0f + expf(-v[0])) * v[1]);
-  } else {
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-      if (o0 + 16 * r + row < a.out) store(o0 + 16 * r + row, v[r]);
+    if (a.residual) v[0] += load1<DT>(a.residual, at);
+    reinterpret_cast<uint16_t*>(a.y)[at] = DT == NKV_F16 ? f2h(v[0]) : f2bf(v[0]);
   }
 }
 
-template <int DT>
-void launch_product(const ProductArgs& a, bool gated, hipStream_t s) {
-  const int nt = (int)std::min<int64_t>(a.tokens, PT);
-  ProductArgs b = a;
-  const int whole = (int)cdiv(a.in, PW * PB) * (PW * PB);
-  b.chunk = std::min(whole, std::max(PW * PB, PX / (2 * nt) / (PW * PB) * (PW * PB)));
-  const int rt = gated ? 2 : 1;
-  const size_t lds = std::max((size_t)nt * (2 * b.chunk + 16), (size_t)PW * rt * 16 * 17 * 4);
-  const dim3 grid((unsigned)cdiv(a.out, 16), (unsigned)cdiv(a.tokens, PT));
-  if (gated) hipLaunchKernelGGL((product4_kernel<DT, 2, true>), grid, dim3(64 * PW), lds, s, b);
-  else hipLaunchKernelGGL((product4_kernel<DT, 1, false>), grid, dim3(64 * PW), lds, s, b);
+// ---------------------------------------------------------------- a few tokens: one launch
+//
+// Up to 4 tokens, which leave most of a product's 16 columns free: column 4 t + j takes token t's group j of a block alone (its
+// other inputs are 0), so that a group's sum comes out by itself and the scales are applied to it, 4 products' results
+// instead of 32 operands. The codes then need no arithmetic: n = code + 8 is an fp16 denormal, n 2^-24 (a nibble at the
+// mantissa's end) or 16 n 2^-24 (the next one; its inputs are held over 16), which the matrix cores take as they are: 5
+// instructions for 8 codes instead of 13. The offset's share, -8 2^-24 sum(x), starts the sums.
+// Each workgroup makes its tokens' xn itself, in LDS, while its weights are on the way; the waves are shared out to the tokens
+// (a power of two of them, `each` waves a token), a lane takes up to KX chunks of eight inputs.
+
+constexpr int FEW_W = 4, FEW_KX = 5, FEW_AHEAD = 5;
+
+template <int DT, int RT>
+__global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kernel(ProductArgs a, int each) {
+  constexpr int W = FEW_W, KX = FEW_KX, AHEAD = FEW_AHEAD;
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // [tokens][in + 8] fp16, the groups' offsets; sums, at the end
+  __shared__ float2 part[W];
+  __shared__ float unit[4];
+  __shared__ __attribute__((aligned(16))) uint4 zeros[4];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (int)a.tokens, n8 = a.in / 8, blocks = (a.in + PB - 1) / PB;
+  const int token = wave / each, at0 = 64 * (wave % each) + lane;  // this lane's chunks: at0 + 64 each k
+
+  Raw8<DT> xr[KX], gr[KX];
+  const uint8_t* x = a.x + (int64_t)token * a.in * 2;
+#pragma unroll
+  for (int k = 0; k < KX; ++k) {
+    const int i = at0 + 64 * each * k;
+    xr[k].zero();
+    gr[k].zero();
+    if (token < nt && i < n8) {
+      xr[k].load(x + 16 * i);
+      if (a.gamma) gr[k].load(a.gamma + 16 * i);
+    }
+  }
+  // tile r of the workgroup (RT 2: the up rows of the first's gates): codes as the lanes lie, and the scales of rows
+  // 4 g .. + 3, group c % 4, as their sums come out
+  const uint8_t* wp[RT];
+  uint4 w[AHEAD][RT];
+  uint2 s[AHEAD][RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) wp[r] = a.w4 + ((int64_t)blockIdx.x + r * (a.out / 16)) * blocks * W4_BLOCK;
+  auto load = [&](int e, int kb) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const uint8_t* p = wp[r] + (int64_t)kb * W4_BLOCK;
+      const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 16 * lane));
+      w[e][r] = uint4{v.x, v.y, v.z, v.w};
+      s[e][r] = *reinterpret_cast<const uint2*>(p + W4_CODES + 8 * g + 32 * (c & 3));
+    }
+  };
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e)
+    if (wave + W * e < blocks) load(e, wave + W * e);
+
+  const int stride = 2 * (blocks * PB) + 16;  // bytes of a token's row: the tokens' chunks fall on different banks
+  float* offset = reinterpret_cast<float*>(xs + nt * stride);  // [tokens][4 blocks]
+  float v[8], gv[8];
+  auto values = [&](int k) {
+    xr[k].get(v);
+    if (a.gamma) {
+      gr[k].get(gv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gv[e] = 1.0f;
+    }
+  };
+  float ss = 0.0f, top = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KX; ++k)
+    if (64 * (wave % each + each * k) < n8) {  // (the wave agrees)
+      values(k);
+      measure8(v, gv, ss, top);
+    }
+  ss = sum4rows(row16_sum(ss));
+  top = max4rows(row16_max(top));
+  if (lane == 0) part[wave] = float2{ss, top};
+  if (tid < 4) zeros[tid] = uint4{0, 0, 0, 0};
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < KX; ++k)  // (converted again below, for want of registers)
+    asm volatile("" : "+v"(xr[k].w[0].x), "+v"(xr[k].w[0].y), "+v"(xr[k].w[0].z), "+v"(xr[k].w[0].w),
+                 "+v"(gr[k].w[0].x), "+v"(gr[k].w[0].y), "+v"(gr[k].w[0].z), "+v"(gr[k].w[0].w));
+  ss = top = 0.0f;
+  for (int q = token * each; q < (token + 1) * each; ++q) ss += part[q].x, top = fmaxf(top, part[q].y);
+  const Factor f = factor_of(ss, top, a.gamma, a.in, a.eps);
+  if (wave % each == 0 && lane == 0) unit[token] = f.unit * 0x1p24f;
+  if (token < nt) {
+#pragma unroll
+    for (int k = 0; k < KX; ++k) {
+      const int i = at0 + 64 * each * k;
+      if (64 * (wave % each + each * k) >= blocks * (PB / 8)) break;  // (the wave agrees)
+      values(k);  // (behind the inputs: zeros)
+      uint32_t h[4];
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float by = e & 1 ? f.inverse * 0.0625f : f.inverse;
+        const uint16_t lo = f2h(v[2 * e] * f.norm * gv[2 * e] * by), hi = f2h(v[2 * e + 1] * f.norm * gv[2 * e + 1] * by);
+        h[e] = (uint32_t)lo | ((uint32_t)hi << 16);
+        sum = __builtin_fmaf(h2f(lo) + h2f(hi), e & 1 ? 16.0f : 1.0f, sum);
+      }
+      sum += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum), 0xB1, 0xf, 0xf, false));
+      sum += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum), 0x4E, 0xf, 0xf, false));
+      if (i < blocks * (PB / 8)) {
+        *reinterpret_cast<uint4*>(xs + token * stride + 16 * i) = uint4{h[0], h[1], h[2], h[3]};
+        if (i % 4 == 0) offset[token * 4 * blocks + i / 4] = sum * (-8.0f * 0x1p-24f);
+      }
+    }
+  }
+  __syncthreads();
+
+  float4_t acc[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r] = float4_t{0.f, 0.f, 0.f, 0.f};
+  const int mine = min(c >> 2, nt - 1);
+  const bool own = (c & 3) == g;
+  const uint8_t* xp = own ? xs + mine * stride + 64 * g : reinterpret_cast<const uint8_t*>(zeros);
+  const int step = own ? 2 * PB : 0;
+  const float* op = offset + mine * 4 * blocks + (c & 3);
+  for (int kb0 = wave; kb0 < blocks; kb0 += W * AHEAD) {
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      const int kb = kb0 + W * e;
+      if (kb < blocks) {  // (the wave's lanes agree)
+        half8_t b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const half8_t*>(xp + kb * step + 16 * k);
+        const float start = op[4 * kb];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const uint32_t words[4] = {w[e][r].x, w[e][r].y, w[e][r].z, w[e][r].w};
+          float4_t d = {start, start, start, start};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t u = words[k], u8 = u >> 8;
+            d = mfma32(as_h8(uint4{u & 0x000f000fu, u & 0x00f000f0u, u8 & 0x000f000fu, u8 & 0x00f000f0u}), b[k], d);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const half2_t h = as_h2(i < 2 ? s[e][r].x : s[e][r].y);
+            acc[r][i] = __builtin_fmaf((float)(i & 1 ? h.y : h.x), d[i], acc[r][i]);
+          }
+        }
+        if (kb + W * AHEAD < blocks) load(e, kb + W * AHEAD);
+      }
+    }
+  }
+  __syncthreads();  // xn is read
+  // the four groups' columns into the token's
+  float4_t y[RT][1];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float q = acc[r][i];
+      q += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(q), 0xB1, 0xf, 0xf, false));
+      q += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(q), 0x4E, 0xf, 0xf, false));
+      y[r][0][i] = q;
+    }
+  finish<DT, RT, 1, RT == 2, W, 4>(a, y, reinterpret_cast<float*>(xs), 0, nt, 16 * (int64_t)blockIdx.x, unit);
 }
 
-int product(const char* what, const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
-            const uint16_t* scales, int64_t out, int64_t in, const void* residual, void* y, bool gated, void* stream) {
+// ---------------------------------------------------------------- up to 16 tokens of fp16 as they are: one launch
+//
+// Each wave brings its own blocks of x to LDS, 256 bytes a token, in rows that 16 lanes load together, and takes them from
+// there as operands: no workgroup barrier in the loop.
+
+template <int RT, bool GATED, int W>
+__global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_kernel(ProductArgs a) {
+  constexpr int AHEAD = 5, ROW = 2 * PB + 16, SLOT = 16 * ROW, RED = W * RT * 16 * 17 * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[RED > W * SLOT ? RED : W * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = (int)a.tokens, blocks = (a.in + PB - 1) / PB;
+  const int64_t o0 = 16 * (int64_t)blockIdx.x;
+
+  uint4 xr[4];  // the next block: token 4 e + g, inputs 8 c ..
+  const uint8_t* xp = a.x + (int64_t)g * a.in * 2 + 16 * c;
+  auto load_x = [&](int kb) {
+    const bool in = kb * PB + 8 * c < a.in;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      xr[e] = uint4{0, 0, 0, 0};
+      if (in && 4 * e + g < nt) xr[e] = *reinterpret_cast<const uint4*>(xp + ((int64_t)(4 * e) * a.in + (int64_t)kb * PB) * 2);
+    }
+  };
+  load_x(wave);
+  Weights<RT, GATED, W, AHEAD> wt(a, o0, lane, blocks);
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e)
+    if (wave + W * e < blocks) wt.load(e, wave + W * e);
+
+  float4_t acc[RT][1];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r][0] = float4_t{0.f, 0.f, 0.f, 0.f};
+  uint8_t* slot = lds + wave * SLOT;
+  for (int kb0 = wave; kb0 < blocks; kb0 += W * AHEAD) {
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      const int kb = kb0 + W * e;
+      if (kb < blocks) {  // (the wave's lanes agree)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(slot + (4 * i + g) * ROW + 16 * c) = xr[i];
+        if (kb + W < blocks) load_x(kb + W);
+        __builtin_amdgcn_wave_barrier();  // (the wave's own LDS operations stay in order)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const half8_t b = *reinterpret_cast<const half8_t*>(slot + c * ROW + 64 * g + 16 * k);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r][0] = mfma32(wt.operand(e, r, k), b, acc[r][0]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (kb + W * AHEAD < blocks) wt.load(e, kb + W * AHEAD);
+      }
+    }
+  }
+  __syncthreads();
+  finish<NKV_F16, RT, 1, GATED, W>(a, acc, reinterpret_cast<float*>(lds), 0, nt, o0, nullptr);
+}
+
+// ---------------------------------------------------------------- many tokens
+//
+// xn lies as operands (xn_kernel): a wave's loads of it are 1024 bytes in a row, from the XCD's L2 where the workgroups of
+// other rows have it, too.
+
+template <int DT, int RT, int NT, bool GATED, int W, int AHEAD>
+__global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_many_kernel(ProductArgs a) {
+  __shared__ __attribute__((aligned(16))) float red[W * RT * NT * 16 * 17];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t t0 = (int64_t)blockIdx.y * (16 * NT);
+  const int nt = (int)min<int64_t>(16 * NT, a.tokens - t0), blocks = (a.in + PB - 1) / PB;
+  const int64_t o0 = (int64_t)blockIdx.x * (16 * Weights<RT, GATED, W, AHEAD>::TILES);
+
+  half8_t b[4][NT];  // the next block's
+  const uint8_t* xp = a.x + (int64_t)blockIdx.y * NT * blocks * 4096 + 16 * lane;
+  auto load_x = [&](int kb, int k) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) b[k][n] = *reinterpret_cast<const half8_t*>(xp + ((int64_t)(4 * kb + k) * NT + n) * 1024);
+  };
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (wave < blocks) load_x(wave, k);
+  Weights<RT, GATED, W, AHEAD> wt(a, o0, lane, blocks);
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e)
+    if (wave + W * e < blocks) wt.load(e, wave + W * e);
+
+  float4_t acc[RT][NT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[r][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int kb0 = wave; kb0 < blocks; kb0 += W * AHEAD) {
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      const int kb = kb0 + W * e;
+      if (kb < blocks) {  // (the wave's lanes agree)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const half8_t w = wt.operand(e, r, k);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[r][n] = mfma32(w, b[k][n], acc[r][n]);
+          }
+          if (kb + W < blocks) load_x(kb + W, k);
+        }
+        if (kb + W * AHEAD < blocks) wt.load(e, kb + W * AHEAD);
+      }
+    }
+  }
+  finish<DT, RT, NT, GATED, W>(a, acc, red, t0, nt, o0, a.unit + t0);
+}
+
+// ---------------------------------------------------------------- host side
+
+// How many waves share a token in product4_few_kernel; 0: another form is taken. (Gates and ups must be in tiles of their own.)
+int few_each(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
+  if (tokens > 4 || (gated && out % 16) || (!norm && dtype == NKV_F16)) return 0;
+  const int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
+  return cdiv(in, PB) * PB <= each * FEW_KX * 512 ? each : 0;
+}
+// The token tiles of a pass of product4_many_kernel.
+int pass_tiles(int64_t tokens) { return (int)std::min<int64_t>(cdiv(tokens, 16), 4); }
+
+int64_t product_workspace(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
+  if (few_each(dtype, tokens, out, in, norm, gated) || (tokens <= 16 && dtype == NKV_F16 && !norm)) return 0;
+  const int64_t passes = cdiv(tokens, 16 * pass_tiles(tokens));
+  return passes * pass_tiles(tokens) * cdiv(in, PB) * 4096 + 4 * tokens;
+}
+
+template <int DT, bool GATED>
+int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_bytes, hipStream_t s) {
+  constexpr int R1 = GATED ? 2 : 1;
+  const int blocks = (int)cdiv(a.in, PB);
+  const int64_t tiles = cdiv(a.out, 16);
+  const bool norm = a.gamma != nullptr;
+  if (const int each = few_each(DT, a.tokens, a.out, a.in, norm, GATED)) {
+    const size_t lds = std::max((size_t)a.tokens * (2 * blocks * PB + 16 + 16 * blocks), (size_t)FEW_W * R1 * 16 * 17 * 4);
+    hipLaunchKernelGGL((product4_few_kernel<DT, R1>), dim3((unsigned)tiles), dim3(64 * FEW_W), lds, s, a, each);
+    return check_launch(what);
+  }
+  if constexpr (DT == NKV_F16) {
+    if (a.tokens <= 16 && !norm) {
+      if (blocks <= 24) hipLaunchKernelGGL((product4_kernel<R1, GATED, 4>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((product4_kernel<R1, GATED, 16>), dim3((unsigned)tiles), dim3(1024), 0, s, a);
+      return check_launch(what);
+    }
+  }
+  const int64_t need = product_workspace(DT, a.tokens, a.out, a.in, norm, GATED);
+  if (!ws || ws_bytes < need)
+    return fail(NKV_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
+  const int nt = pass_tiles(a.tokens);
+  float* unit = reinterpret_cast<float*>(ws + need - 4 * a.tokens);
+  hipLaunchKernelGGL((xn_kernel<DT>), dim3((unsigned)a.tokens), dim3(256), 0, s, a, nt, ws, unit);
+  if (int rc = check_launch(what)) return rc;
+  a.x = ws;
+  a.unit = unit;
+  const unsigned passes = (unsigned)cdiv(a.tokens, 16 * nt);
+  const auto go = [&](auto kernel, int tiles_wg, int waves) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(tiles, tiles_wg), passes), dim3(64 * waves), 0, s, a);
+  };
+  const bool many = tiles > 2 * CUS;
+  if (nt == 1) {
+    if (blocks <= 24) go(product4_many_kernel<DT, R1, 1, GATED, 4, 5>, 1, 4);
+    else go(product4_many_kernel<DT, R1, 1, GATED, 16, 5>, 1, 16);
+  } else if (nt == 2) {
+    if (many) go(product4_many_kernel<DT, 2 * R1, 2, GATED, 8, 3>, 2, 8);
+    else go(product4_many_kernel<DT, R1, 2, GATED, 8, 3>, 1, 8);
+  } else if (nt == 3) {
+    if (many) go(product4_many_kernel<DT, 2 * R1, 3, GATED, 8, 3>, 2, 8);
+    else go(product4_many_kernel<DT, R1, 3, GATED, 8, 3>, 1, 8);
+  } else {
+    if (many) go(product4_many_kernel<DT, 2 * R1, 4, GATED, 8, 3>, 2, 8);
+    else go(product4_many_kernel<DT, R1, 4, GATED, 8, 3>, 1, 8);
+  }
+  return check_launch(what);
+}
+
+int product(const char* what, const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4, int64_t out, int64_t in, const void* residual, void* y, bool gated, void* workspace,
+            int64_t workspace_bytes, void* stream) {
   set_error("");
   if (dtype != NKV_F16 && dtype != NKV_BF16) return fail(NKV_ERR_INVALID, "%s: dtype %d (fp16 or bf16)", what, dtype);
-  if (out <= 0 || out >= (int64_t(1) << 27) || in <= 0 || in % Q4_GROUP || in > P_IN || tokens < 0 || tokens > 65535 * PT)
+  if (out <= 0 || out >= (int64_t(1) << 27) || in <= 0 || in % Q4_GROUP || in > P_IN || tokens < 0 || tokens > P_TOKENS)
     return fail(NKV_ERR_INVALID, "%s: sizes out=%lld in=%lld tokens=%lld (out in [1, 2^27), in a positive multiple of 32, at most %d, "
-                "tokens at most %d)", what, (long long)out, (long long)in, (long long)tokens, P_IN, 65535 * PT);
+                "tokens at most %lld)", what, (long long)out, (long long)in, (long long)tokens, P_IN, (long long)P_TOKENS);
   if (tokens == 0) return NKV_OK;
-  if (!x || !codes || !scales || !y) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
-  if (!al16(x) || !al16(codes) || !al16(gamma)) return fail(NKV_ERR_UNSUPPORTED, "%s: x, gamma and the codes must be 16-byte aligned", what);
-  ProductArgs a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(gamma), eps, codes, scales, out, (int)in,
-                static_cast<const uint8_t*>(residual), static_cast<uint8_t*>(y), tokens, 0};
-  if (dtype == NKV_F16) launch_product<NKV_F16>(a, gated, static_cast<hipStream_t>(stream));
-  else launch_product<NKV_BF16>(a, gated, static_cast<hipStream_t>(stream));
-  return check_launch(what);
+  if (!x || !w4 || !y) return fail(NKV_ERR_INVALID, "%s: null pointer argument", what);
+  if (!al16(x) || !al16(w4) || !al16(gamma) || !al16(workspace))
+    return fail(NKV_ERR_UNSUPPORTED, "%s: x, gamma, the weight and the workspace must be 16-byte aligned", what);
+  ProductArgs a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(gamma), eps, w4, out, (int)in,
+                static_cast<const uint8_t*>(residual), static_cast<uint8_t*>(y), tokens, nullptr};
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == NKV_F16) {
+    return gated ? launch_product<NKV_F16, true>(what, a, ws, workspace_bytes, s)
+                 : launch_product<NKV_F16, false>(what, a, ws, workspace_bytes, s);
+  }
+  return gated ? launch_product<NKV_BF16, true>(what, a, ws, workspace_bytes, s)
+               : launch_product<NKV_BF16, false>(what, a, ws, workspace_bytes, s);
 }
 
 }  // namespace
@@ -252,14 +577,22 @@ int product(const char* what, const void* x, int dtype, int64_t tokens, const vo
 
 using namespace nkv;
 
-extern "C" int nkv_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
-                           const uint16_t* scales, int64_t out_features, int64_t in_features, const void* residual, void* y,
-                           void* stream) {
-  return product("gemv_q4", x, dtype, tokens, gamma, eps, codes, scales, out_features, in_features, residual, y, false, stream);
+extern "C" int64_t nkv_gemv_q4_workspace_bytes(int dtype, int64_t tokens, int64_t out_features, int64_t in_features, int norm,
+                                                int swiglu) {
+  return tokens > 0 && out_features > 0 && in_features > 0
+             ? product_workspace(dtype, tokens, out_features, in_features, norm != 0, swiglu != 0) : 0;
 }
 
-extern "C" int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* codes,
-                                  const uint16_t* scales, int64_t intermediate, int64_t in_features, void* act, void* stream) {
-  return product("swiglu_gemv_q4", x, dtype, tokens, gamma, eps, codes, scales, intermediate, in_features, nullptr, act, true,
-                 stream);
+extern "C" int nkv_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4,
+                           int64_t out_features, int64_t in_features, const void* residual, void* y,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  return product("gemv_q4", x, dtype, tokens, gamma, eps, w4, out_features, in_features, residual, y, false,
+                 workspace, workspace_bytes, stream);
+}
+
+extern "C" int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4,
+                                  int64_t intermediate, int64_t in_features, void* act, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  return product("swiglu_gemv_q4", x, dtype, tokens, gamma, eps, w4, intermediate, in_features, nullptr, act, true,
+                 workspace, workspace_bytes, stream);
 }

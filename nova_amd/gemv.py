@@ -96,7 +96,7 @@ def _q4_args(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None, n_out: in
     """The checked arguments of a product: the number of tokens and the output."""
     if not isinstance(w, Q4Weight):
         raise ValueError("w must be a Q4Weight (nova_amd.q4.quantize_q4)")
-    n_in, dev = w.shape[1], w.codes.device
+    n_in, dev = w.shape[1], w.data.device
     if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() == 0 or x.shape[-1] != n_in or x.device != dev:
         raise ValueError(f"x must be fp16 / bf16 [.., {n_in}] on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
     if not x.is_contiguous() or x.data_ptr() % 16:
@@ -113,12 +113,19 @@ def _q4_args(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None, n_out: in
     else:
         if out.dtype != x.dtype or out.shape != shape or out.device != dev or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {x.dtype} tensor {list(shape)} on {dev}")
-        for name, t in (("x", x), ("gamma", gamma), ("w's codes", w.codes), ("w's scales", w.scales)):
+        for name, t in (("x", x), ("gamma", gamma), ("w", w.data)):
             if t is not None and overlap(out, t):
                 raise ValueError(f"out must not overlap {name}")
         if residual is not None and residual.data_ptr() != out.data_ptr() and overlap(out, residual):
             raise ValueError("out must be residual itself or not overlap it")
     return x.numel() // n_in, out
+
+
+def _q4_scratch(x: torch.Tensor, tokens: int, n_out: int, n_in: int, gamma: torch.Tensor | None,
+                swiglu: bool) -> tuple[int | None, int]:
+    """Memory of the call's own for the normalized input, where one launch does not make it itself."""
+    n = _lib.load().nkv_gemv_q4_workspace_bytes(_DT[x.dtype], tokens, n_out, n_in, gamma is not None, swiglu)
+    return (_lib.scratch(x.device, n).data_ptr(), n) if n else (None, 0)
 
 
 def rms_gemv_q4(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None = None, eps: float = 1e-6,
@@ -127,11 +134,11 @@ def rms_gemv_q4(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None = None,
     weight; ``gamma=None`` skips the norm. Returns ``[.., out]`` of x's type; ``out`` may be ``residual``.
 
     The normalized input is rounded once, to 11 bits, as the matrix cores' operand; all else is fp32 with one
-    rounding of the result. Made for one token to a few dozen (each 16 tokens read the weight again, from the caches
-    where it fits them)."""
+    rounding of the result. Made for one token to a few dozen (each 64 tokens read the weight again, from the caches
+    where it fits them). The number of tokens chooses the kernel, and so the last bits."""
     tokens, out = _q4_args(x, w, gamma, w.shape[0], out, residual)
-    launch(x.device, "nkv_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps), w.codes.data_ptr(),
-           w.scales.data_ptr(), *w.shape, _lib.ptr(residual), out.data_ptr())
+    launch(x.device, "nkv_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps), w.data.data_ptr(),
+           *w.shape, _lib.ptr(residual), out.data_ptr(), *_q4_scratch(x, tokens, *w.shape, gamma, False))
     return out
 
 
@@ -144,5 +151,6 @@ def swiglu_gemv_q4(x: torch.Tensor, w_gate_up: Q4Weight, gamma: torch.Tensor | N
     inter = w_gate_up.shape[0] // 2
     tokens, out = _q4_args(x, w_gate_up, gamma, inter, out)
     launch(x.device, "nkv_swiglu_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps),
-           w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), inter, w_gate_up.shape[1], out.data_ptr())
+           w_gate_up.data.data_ptr(), inter, w_gate_up.shape[1], out.data_ptr(),
+           *_q4_scratch(x, tokens, inter, w_gate_up.shape[1], gamma, True))
     return out

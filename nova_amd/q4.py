@@ -24,26 +24,22 @@ GROUP = 32
 
 @dataclass(frozen=True)
 class Q4Weight:
-    """A weight ``[out_features, in_features]`` in 4 bits: ``codes`` uint8 ``[out, in / 2]`` (byte i of a row holds
-    code + 8 of inputs 2 i, low half, and 2 i + 1), ``scales`` fp16 ``[out, in / 32]``."""
+    """A weight ``[out_features, in_features]`` in 4 bits, as ``quantize_q4`` lays it out: ``data`` uint8 in blocks of 16 rows
+    and 128 columns, each 1024 bytes of codes and 64 fp16 scales (``nkv_quantize_q4``)."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    data: torch.Tensor
+    shape: tuple[int, int]
 
     def __post_init__(self):
-        c, s = self.codes, self.scales
-        if c.dim() != 2 or c.dtype != torch.uint8 or not c.is_cuda or not c.is_contiguous() or c.data_ptr() % 16 or c.shape[1] % 16:
-            raise ValueError("codes must be a contiguous, 16-byte aligned uint8 CUDA tensor [out, in / 2], in a multiple of 32")
-        if (s.dim() != 2 or s.shape != (c.shape[0], c.shape[1] // 16) or s.dtype != torch.float16 or s.device != c.device
-                or not s.is_contiguous()):
-            raise ValueError(f"scales must be a contiguous fp16 tensor [{c.shape[0]}, {c.shape[1] // 16}] on {c.device}")
-
-    @property
-    def shape(self) -> tuple[int, int]:
-        return self.codes.shape[0], 2 * self.codes.shape[1]
+        d, (rows, n) = self.data, self.shape
+        if rows < 0 or n <= 0 or n % GROUP:
+            raise ValueError(f"shape {self.shape}: in_features must be a positive multiple of {GROUP}")
+        size = -(-rows // 16) * -(-n // 128) * 1152
+        if d.dtype != torch.uint8 or not d.is_cuda or not d.is_contiguous() or d.numel() != size or d.data_ptr() % 16:
+            raise ValueError(f"data must be a contiguous, 16-byte aligned uint8 CUDA tensor of {size} elements")
 
     def nbytes(self) -> int:
-        return self.codes.numel() + 2 * self.scales.numel()
+        return self.data.numel()
 
 
 def quantize_q4(w: torch.Tensor) -> Q4Weight:
@@ -55,16 +51,15 @@ def quantize_q4(w: torch.Tensor) -> Q4Weight:
         raise ValueError(f"in_features {n} must be a positive multiple of {GROUP}")
     w = w.detach()
     w = w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-    codes = torch.empty((rows, n // 2), dtype=torch.uint8, device=w.device)
-    scales = torch.empty((rows, n // GROUP), dtype=torch.float16, device=w.device)
-    launch(w.device, "nkv_quantize_q4", w.data_ptr(), _DT[w.dtype], rows, n, codes.data_ptr(), scales.data_ptr())
-    return Q4Weight(codes, scales)
+    data = torch.empty(_lib.load().nkv_q4_weight_bytes(rows, n), dtype=torch.uint8, device=w.device)
+    launch(w.device, "nkv_quantize_q4", w.data_ptr(), _DT[w.dtype], rows, n, data.data_ptr())
+    return Q4Weight(data, (rows, n))
 
 
 def dequantize_q4(w: Q4Weight, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """The values of ``w`` as ``[out_features, in_features]`` of ``dtype`` (exact in fp16 and fp32)."""
     if dtype not in _DT:
         raise ValueError(f"unsupported dtype {dtype}")
-    out = torch.empty(w.shape, dtype=dtype, device=w.codes.device)
-    launch(out.device, "nkv_dequantize_q4", w.codes.data_ptr(), w.scales.data_ptr(), *w.shape, out.data_ptr(), _DT[dtype])
+    out = torch.empty(w.shape, dtype=dtype, device=w.data.device)
+    launch(out.device, "nkv_dequantize_q4", w.data.data_ptr(), *w.shape, out.data_ptr(), _DT[dtype])
     return out

@@ -20,13 +20,13 @@ def lib():
 
 
 def _quantize(lib, **kw):
-    a = dict(x=PTR, dtype=0, rows=4, n=64, codes=PTR, scales=PTR, stream=None)
+    a = dict(x=PTR, dtype=0, rows=4, n=64, w4=PTR, stream=None)
     a.update(kw)
     return lib.nkv_quantize_q4(*a.values())
 
 
 def _dequantize(lib, **kw):
-    a = dict(codes=PTR, scales=PTR, rows=4, n=64, x=PTR, dtype=0, stream=None)
+    a = dict(w4=PTR, rows=4, n=64, x=PTR, dtype=0, stream=None)
     a.update(kw)
     return lib.nkv_dequantize_q4(*a.values())
 
@@ -34,21 +34,21 @@ def _dequantize(lib, **kw):
 @pytest.mark.parametrize("call", [_quantize, _dequantize])
 @pytest.mark.parametrize("kw,rc", [
     (dict(dtype=3), INVALID), (dict(rows=-1), INVALID), (dict(n=0), INVALID), (dict(n=48), INVALID), (dict(n=-32), INVALID),
-    (dict(rows=1 << 40), INVALID), (dict(x=None), INVALID), (dict(codes=None), INVALID), (dict(scales=None), INVALID),
-    (dict(x=PTR + 8), UNSUPPORTED), (dict(codes=PTR + 4), UNSUPPORTED), (dict(rows=0, x=None), OK)])
+    (dict(rows=1 << 40), INVALID), (dict(rows=1 << 30, n=128), INVALID), (dict(rows=1 << 39, n=1 << 39), INVALID),
+    (dict(x=None), INVALID), (dict(w4=None), INVALID), (dict(x=PTR + 8), UNSUPPORTED), (dict(w4=PTR + 4), UNSUPPORTED), (dict(rows=0, x=None), OK)])
 def test_quantizer_refusals(lib, call, kw, rc):
     assert call(lib, **kw) == rc
     assert rc == OK or lib.nkv_last_error()
 
 
 def _gemv(lib, **kw):
-    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, codes=PTR, scales=PTR, out=64, n_in=64, residual=None, y=PTR, stream=None)
+    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, w4=PTR, out=64, n_in=64, residual=None, y=PTR, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return lib.nkv_gemv_q4(*a.values())
 
 
 def _swiglu(lib, **kw):
-    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, codes=PTR, scales=PTR, out=64, n_in=64, y=PTR, stream=None)
+    a = dict(x=PTR, dtype=0, tokens=2, gamma=None, eps=1e-6, w4=PTR, out=64, n_in=64, y=PTR, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return lib.nkv_swiglu_gemv_q4(*a.values())
 
@@ -57,12 +57,30 @@ def _swiglu(lib, **kw):
 @pytest.mark.parametrize("kw,rc", [
     (dict(dtype=2), INVALID), (dict(dtype=-1), INVALID), (dict(tokens=-1), INVALID), (dict(tokens=1 << 20), INVALID),
     (dict(out=0), INVALID), (dict(out=1 << 27), INVALID), (dict(n_in=0), INVALID), (dict(n_in=40), INVALID),
-    (dict(n_in=(1 << 20) + 32), INVALID), (dict(x=None), INVALID), (dict(codes=None), INVALID), (dict(scales=None), INVALID),
-    (dict(y=None), INVALID), (dict(x=PTR + 2), UNSUPPORTED), (dict(codes=PTR + 8), UNSUPPORTED), (dict(gamma=PTR + 2), UNSUPPORTED),
+    (dict(n_in=(1 << 20) + 32), INVALID), (dict(x=None), INVALID), (dict(w4=None), INVALID),
+    (dict(y=None), INVALID), (dict(x=PTR + 2), UNSUPPORTED), (dict(w4=PTR + 8), UNSUPPORTED), (dict(gamma=PTR + 2), UNSUPPORTED),
+    (dict(ws=PTR + 8), UNSUPPORTED), (dict(tokens=17, gamma=PTR), INVALID), (dict(tokens=17, dtype=1, ws=PTR, ws_bytes=2 * 4096 + 67), INVALID),
     (dict(tokens=0, x=None), OK)])
 def test_product_refusals(lib, call, kw, rc):
     assert call(lib, **kw) == rc
     assert rc == OK or lib.nkv_last_error()
+
+
+def test_product_workspace(lib):
+    """None where one launch makes xn (up to 4 tokens, 10240 inputs in a power of two of tokens, gates and ups in tiles of
+    their own), or where x is taken as it is; else xn in tiles of 16 tokens and blocks of 128 inputs, and a word a token."""
+    need = lib.nkv_gemv_q4_workspace_bytes
+    assert need(0, 4, 100, 2560, 1, 0) == need(1, 2, 100, 5120, 1, 0) == need(0, 1, 160, 10240, 1, 1) == need(1, 3, 16, 32, 0, 1) == 0
+    assert need(0, 16, 100, 9728, 0, 0) == need(0, 1, 100, 40000, 0, 1) == need(0, 0, 100, 64, 1, 0) == 0
+    assert need(0, 1, 100, 64, 1, 1) == 4096 + 4 and need(0, 5, 100, 160, 1, 0) == 2 * 4096 + 20
+    assert need(1, 1, 100, 10272, 0, 0) == 81 * 4096 + 4 and need(0, 17, 100, 64, 0, 0) == 2 * 4096 + 68
+    assert need(0, 65, 100, 128, 1, 0) == 8 * 4096 + 260
+
+
+def test_weight_bytes(lib):
+    need = lib.nkv_q4_weight_bytes
+    assert need(16, 128) == 1152 and need(17, 128) == need(16, 160) == 2304 and need(6144, 2560) == 384 * 20 * 1152
+    assert need(0, 128) == need(16, 0) == 0
 
 
 def _paged_quantize(lib, **kw):
@@ -126,7 +144,7 @@ def test_weights_of_the_host_are_refused():
     with pytest.raises(ValueError):
         q4.quantize_q4(torch.zeros(4, 64))
     with pytest.raises(ValueError):
-        q4.Q4Weight(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.float16))
+        q4.Q4Weight(torch.zeros(1152, dtype=torch.uint8), (4, 64))
     with pytest.raises(ValueError):
         G.rms_gemv_q4(torch.zeros(64, dtype=torch.float16), torch.zeros(4, 64))
     with pytest.raises(ValueError):
