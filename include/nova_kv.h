@@ -835,7 +835,7 @@ int nkv_dequantize_q4(const uint8_t* w4, int64_t rows, int64_t n, void* out, int
  * [in_features], residual and y [tokens][out_features], all of one dtype (NKV_F16 or NKV_BF16), contiguous; w4: a weight
  * [out_features][in_features] of nkv_quantize_q4; x, gamma and w4 16-byte aligned.
  * y[t][o] = sum_i W[o][i] xn[t][i] (+ residual[t][o]) with xn = x when gamma is NULL, else x * rsqrt(mean(x^2) + eps) *
- * gamma. xn is rounded once to 11 bits (as an operand), everything else is fp32 with one rounding of y. residual may be
+ * gamma. xn is rounded once, to 11 bits of bf16 inputs, to 22 of fp16, everything else is fp32 with one rounding of y. residual may be
  * NULL; y may be residual itself, but must not overlap it otherwise, nor x, gamma or the weight.
  * SwiGLU: act[t][j] = silu(g) * u, g = row j and u = row intermediate + j of the [2 * intermediate][in_features]
  * weight times xn. in_features a multiple of 32, at most 2^20; out_features (intermediate) less than 2^27; at most 2^20 - 16 tokens.
@@ -853,10 +853,10 @@ int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gam
 
 /*
  * The paged cache in 4 bits: a page is 64 tokens of one KV head, 9216 bytes: K codes [64][64 bytes], V codes, K scales,
- * V scales (256 fp16 each; token t, channels 32 r .. + 31: K at ((4 (t / 16) + t % 4) * 4 + r) * 4 + t / 4 % 4, V at
- * 64 r + t / 8 * 8 + 2 (t % 4) + t / 4 % 2). pages, tables, batches and plans as for the per-token symmetric pages:
+ * V scales (256 fp16 each; token t, channels 32 r .. + 31: K at 64 r + t, V at 64 r + t / 8 * 8 + 2 (t % 4) + t / 4 % 2).
+ * Bits 4 e .. + 3 of a row's 32-bit word w hold code + 8 of channel 8 w + e, in K's rows of channel 8 (w / 4 + 4 (w % 4)) + e. pages, tables, batches and plans as for the per-token symmetric pages:
  * nkv_paged_quantize_q4 as nkv_paged_quantize_tok, nkv_paged_append_chunks_q4 as nkv_paged_append_chunks_tok,
- * nkv_paged_attn_chunks_q4 as nkv_paged_attn_chunks_tok, nkv_paged_read_q4 as nkv_paged_read_tok. In the attention keys
+ * nkv_paged_attn_chunks_q4 as nkv_paged_attn_chunks_tok (wide: the largest kind of a unit), nkv_paged_read_q4 as nkv_paged_read_tok. In the attention keys
  * and values are exact operands; the softmax's weights and the output are rounded to fp16.
  */
 int nkv_paged_quantize_q4(const void* x, int x_dtype, int64_t x_head_stride, int64_t hkv, int64_t n, int which,

@@ -69,10 +69,12 @@ class ChunkPlan(SpanPlan):
     merges: torch.Tensor = None   # int32 [m, 8]
     ws_bytes: int = 0
     wide: bool = False            # some unit is ROWS256
+    kind: int = ROWS16            # the largest kind of a unit
 
     def __post_init__(self):
         super().__post_init__()
         self.work = self.units.data_ptr(), self.units.shape[0], self.wide, self.merges.data_ptr(), self.merges.shape[0]
+        self.work_q4 = *self.work[:2], self.kind, *self.work[3:]
 
 
 def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
@@ -84,7 +86,7 @@ def check_counts(counts, max_seqs: int, what: str = "counts") -> list[int]:
     return counts
 
 
-def plan_units(starts, counts, gq: int, hkv: int, big_from: int = BIG_FROM) -> tuple[np.ndarray, np.ndarray, int]:
+def plan_units(starts, counts, gq: int, hkv: int, q4: bool = False) -> tuple[np.ndarray, np.ndarray, int]:
     """How the attention of ``counts[b]`` new tokens after ``starts[b]`` is cut.
 
     Returns ``(units, merges, partial_rows)``, int32 ``[n, 8]`` and ``[m, 8]``. The rows of a KV head
@@ -94,6 +96,7 @@ def plan_units(starts, counts, gq: int, hkv: int, big_from: int = BIG_FROM) -> t
     merge entries ``(sequence's first packed token, first row, rows, parts, slot, slots from part to part,
     0, 0)`` join, eight rows each. The longest units come first."""
     rows = np.array(counts, dtype=np.int64) * gq
+    big_from = BIG_FROM_Q4 if q4 else BIG_FROM
     wide = bool((rows > big_from).any())
     size = np.where(rows > big_from, TILE_ROWS[ROWS256], TILE_ROWS[ROWS32])
     n_tiles = -(-rows // size)
@@ -104,13 +107,13 @@ def plan_units(starts, counts, gq: int, hkv: int, big_from: int = BIG_FROM) -> t
     have = np.minimum(size[seq], rows[seq] - row0)
     kind = np.where(size[seq] == TILE_ROWS[ROWS256], ROWS256, np.where(have <= TILE_ROWS[ROWS16], ROWS16, ROWS32))
     steps = (np.array(starts, dtype=np.int64)[seq] + (row0 + have - 1) // gq) // GT + 1
-    parts = _parts(steps, kind, have, hkv, wide)
+    parts = (_parts_q4 if q4 else _parts)(steps, kind, have, hkv, wide)
     # one entry a unit
     tile = np.repeat(np.arange(len(seq)), parts)
     part = np.arange(len(tile)) - np.repeat(np.cumsum(parts) - parts, parts)
     slots = np.where(parts > 1, parts * have, 0)
     slot = np.cumsum(slots) - slots
-    cost = (steps * np.where(kind == ROWS256, STEP_US, GROUP_US) / parts)[tile]
+    cost = (steps * np.where(kind == ROWS256, STEP_US, GROUP_US) / parts)[tile]  # (only its order counts)
     alone = (n_tiles[seq] == 1).astype(np.int64)
     units = np.stack([seq[tile], row0[tile], have[tile], part, parts[tile], slot[tile], kind[tile], alone[tile]], 1)
     units = units[np.argsort(-cost, kind="stable")]
@@ -143,6 +146,42 @@ def _parts(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide
     return parts[time.argmin()]
 
 
+# The 4-bit pages: rows from which tiles are ROWS256 (all as ROWS256 / as ROWS32): 96 rows over 32000 tokens 46 / 41 us, 8 times
+# 128 rows over 4000 47 / 42, 200 rows over 8000 30 / 27; and, in launches of small units (ROWS16, ROWS32), what they take in
+# us: a round of four waves alone on a CU, and beside another workgroup there; a unit's start and end; the second launch, and
+# each part of its longest row. (With wide tiles _parts' prices hold: a step of 1.9 and a unit's start and end of 10.)
+BIG_FROM_Q4 = 200
+ALONE_Q4, SHARED_Q4, START_Q4 = (1.6, 2.35), (1.5, 2.0), (5.0, 7.0)
+MERGE_Q4, MERGE_PART_Q4 = 3.0, 0.1
+
+
+def _parts_q4(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide: bool) -> np.ndarray:
+    """:func:`_parts` for 4-bit pages: the least time among the same cuts, by what their units were measured at. Of 20 batches (1 to 64
+    sequences of 1 to 50 rows over 500 to 131000 tokens, prompts and chunks) 18 get a cut within 7% of the best, all within 12%."""
+    if wide:
+        return _parts(steps, kind, rows, hkv, wide)
+    slow = (kind == ROWS32).astype(np.int64)
+    rounds = -(-steps // 4)
+    most = np.minimum(MAX_PARTS, np.maximum(1, steps // SMALL_PART))
+    round_us = np.array(ALONE_Q4)[slow]
+    us = rounds * round_us
+    best = None
+    for cut in CUTS if len(steps) * hkv < 32 * CUS else CUTS[:1]:  # (far more tiles than slots are not cut)
+        parts = np.clip(np.ceil(us * (cut / us.max())).astype(np.int64), 1, most)
+        alone = -(-rounds // parts)
+        # all of it over the CUs, as far as the units fill them evenly
+        k = int(parts.sum()) * hkv / CUS
+        uneven = 1.1 * max(1.0, int(np.ceil(k - 0.1)) / k) if k <= 2.1 else 1.2 + 0.03 * k
+        total = float((alone * np.array(SHARED_Q4)[slow] * parts).sum()) * hkv / CUS
+        time = START_Q4[int(slow.max())] + max(float((alone * round_us).max()), total * uneven)
+        cut_rows = int(np.where(parts > 1, parts, 0) @ rows) * hkv
+        if cut_rows:
+            time += MERGE_Q4 + MERGE_PART_Q4 * int(parts.max()) + cut_rows * PARTIAL_US
+        if best is None or time < best[0]:
+            best = time, parts
+    return best[1]
+
+
 def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:
     n = np.array(counts, dtype=np.int64)
     if sum(counts) >= 1 << 24:
@@ -158,16 +197,17 @@ def span_plan(counts: list[int], starts: list[int], pos: torch.Tensor) -> SpanPl
     return SpanPlan(counts, int(cu[-1]), pos, first, ints[:len(cu)], ints[len(cu):])
 
 
-def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int, big_from: int = BIG_FROM) -> ChunkPlan:
+def chunk_plan(counts: list[int], lengths: list[int], pos: torch.Tensor, gq: int, hkv: int, q4: bool = False) -> ChunkPlan:
     cu, seq_of = _packed(counts)
-    units, merges, rows = plan_units(lengths, counts, gq, hkv, big_from)
+    units, merges, rows = plan_units(lengths, counts, gq, hkv, q4)
     # one copy to the device; the entries are 32 bytes, so that each of them stays aligned
     ints = torch.from_numpy(np.concatenate((units.ravel(), merges.ravel(), cu, seq_of))).to(pos.device)
     new = torch.tensor(counts, dtype=torch.int64).to(pos.device)
     u, m = units.size, units.size + merges.size
     return ChunkPlan(counts, int(cu[-1]), pos, pos[:len(counts)], ints[m:m + len(cu)], ints[m + len(cu):], new,
                      ints[:u].view(-1, UNIT_INTS), ints[u:m].view(-1, UNIT_INTS),
-                     int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)), bool((units[:, 6] == ROWS256).any()))
+                     int(_lib.load().nkv_paged_chunks_workspace_bytes(hkv, rows)), bool((units[:, 6] == ROWS256).any()),
+                     int(units[:, 6].max(initial=ROWS16)))
 
 
 def launch(device: torch.device, name: str, *args) -> None:

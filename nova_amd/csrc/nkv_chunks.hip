@@ -18,6 +18,23 @@ namespace {
 
 // ---------------------------------------------------------------- append
 
+// The sum of a 16-lane row's squares in pairs of neighbours: four of a lane's values one after another, then their
+// sums, the lanes', .. ; each product and sum rounded.
+__device__ __forceinline__ float squares_in_pairs(const float (&v)[8]) {
+  float s[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s[h] = __fmul_rn(v[4 * h], v[4 * h]);
+#pragma unroll
+    for (int e = 1; e < 4; ++e) s[h] = __fadd_rn(s[h], __fmul_rn(v[4 * h + e], v[4 * h + e]));
+  }
+  float x = __fadd_rn(s[0], s[1]);
+  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, false)));
+  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, false)));
+  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, false)));  // half mirror
+  return __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, false)));  // mirror
+}
+
 // The value of lane l ^ 8 of the same 16-lane row (a rotation by 8).
 __device__ __forceinline__ float row16_other_half(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
@@ -80,10 +97,22 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
       slot_of = (int)(at.pos & (GT - 1));
     }
     if (rotate) {
-      const double turns = (double)at.pos * (double)a.inv_freq[tid] * 0.15915494309189533577;  // 1 / 2 pi
-      const float part = (float)(turns - __builtin_rint(turns));
-      turn[0][tid] = cospif(2.0f * part);
-      turn[1][tid] = sinpif(2.0f * part);
+      if constexpr (F == Q4) {
+        // (rounded from 64 bits: an error of fp32's last place turns codes of 4 bits, which are 2^20 times as far apart, in
+        // one value of a million; the angle less its whole turns, 2 pi in two parts)
+        const double angle = (double)at.pos * (double)a.inv_freq[tid];
+        const double n = __builtin_rint(angle * 0.15915494309189533577);  // 1 / 2 pi
+        const double r = __builtin_fma(-n, 2.4492935982947064e-16, __builtin_fma(-n, 6.283185307179586477, angle));
+        double s, c;
+        sincospi(r * 0.31830988618379067154, &s, &c);
+        turn[0][tid] = (float)c;
+        turn[1][tid] = (float)s;
+      } else {
+        const double turns = (double)at.pos * (double)a.inv_freq[tid] * 0.15915494309189533577;  // 1 / 2 pi
+        const float part = (float)(turns - __builtin_rint(turns));
+        turn[0][tid] = cospif(2.0f * part);
+        turn[1][tid] = sinpif(2.0f * part);
+      }
     }
   }
   __syncthreads();
@@ -111,15 +140,25 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
     if (!is_v) {
       if (norm) {
         float ss = 0.0f;
+        if constexpr (F == Q4) {
+          ss = squares_in_pairs(v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
-        const float r = rsqrtf(row16_sum(ss) * (1.0f / D) + a.eps);
+          for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
+          ss = row16_sum(ss);
+        }
+        const float r = rsqrtf(ss * (1.0f / D) + a.eps);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (is_q ? gq[e] : gk[e]);
       }
       if (rotate) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], cs[e], row16_other_half(v[e]) * sn[e]);
+        for (int e = 0; e < 8; ++e) {
+          const float other = __fmul_rn(row16_other_half(v[e]), sn[e]);
+          // (Q4: each product rounded, as the elementary operations are)
+          if constexpr (F == Q4) v[e] = __fadd_rn(__fmul_rn(v[e], cs[e]), other);
+          else v[e] = __builtin_fmaf(v[e], cs[e], other);
+        }
       }
     }
     if (is_q) {
@@ -130,7 +169,7 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
       if constexpr (F == Q4) {
         uint16_t scale;
         const uint32_t codes = q4_quant8(v, scale);
-        *reinterpret_cast<uint32_t*>(page + which * Q4_CODES + slot_of * Q4_ROW + 4 * j) = codes;
+        *reinterpret_cast<uint32_t*>(page + which * Q4_CODES + slot_of * Q4_ROW + 4 * word_at(which, j)) = codes;
         if (j % 4 == 0) {
           const int to = which ? v_scale_at(slot_of, j / 4) : k_scale_at(slot_of, j / 4);
           *reinterpret_cast<uint16_t*>(page + 2 * Q4_CODES + which * Q4_SCALES + 2 * to) = scale;
@@ -199,7 +238,7 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
       } else if (page >= 0) {
         const uint8_t* p = a.pages + (page * a.b.hkv + h) * PAGE;
         if constexpr (F == Q4) {
-          codes[f].x = *reinterpret_cast<const uint32_t*>(p + which * Q4_CODES + slot * Q4_ROW + 4 * j);
+          codes[f].x = *reinterpret_cast<const uint32_t*>(p + which * Q4_CODES + slot * Q4_ROW + 4 * word_at(which, j));
           const int from = which ? v_scale_at(slot, j / 4) : k_scale_at(slot, j / 4);
           scale[f] = *reinterpret_cast<const uint16_t*>(p + 2 * Q4_CODES + which * Q4_SCALES + 2 * from);
           continue;

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void quant4_pages_kernel(Quant4Args a) {
     const uint32_t w = q4_quant8(v, scale);
     if (page < 0 || page >= a.num_pages) continue;
     uint8_t* p = a.pages + ((int64_t)page * a.hkv + h) * PAGE_Q4_BYTES;
-    *reinterpret_cast<uint32_t*>(p + a.which * Q4_CODES + slot * Q4_ROW + 4 * j) = w;
+    *reinterpret_cast<uint32_t*>(p + a.which * Q4_CODES + slot * Q4_ROW + 4 * word_at(a.which, j)) = w;
     const int to = a.which ? v_scale_at(slot, j / 4) : k_scale_at(slot, j / 4);
     if (j % 4 == 0) *reinterpret_cast<uint16_t*>(p + 2 * Q4_CODES + a.which * Q4_SCALES + 2 * to) = scale;
   }
@@ -95,7 +95,9 @@ __global__ __launch_bounds__(64) void dequant4_weight_kernel(const uint8_t* w4, 
 // softmax(q K^T / sqrt(128)) V. K and V are exact fp16 operands (nkv_q4.h); what is rounded to fp16 is the softmax's weights
 // and the output. The units of up to 32 rows ("small"): a workgroup's waves take the part's pages in turn, each its own
 // page against all the rows, and their states are merged in LDS at the end. K's codes go from memory to registers: lane
-// c + 16 g of tile b takes the 16 bytes of channels 32 g .. + 31 of token 16 (c / 4) + 4 b + c % 4, one scale's codes.
+// c + 16 g of tile b takes 16 bytes of token 16 (c / 4) + 4 b + c % 4, channels 32 j + 8 g .. + 7 of each group j. A product
+// is of one group's 32 channels, so that the scale multiplies its results and the codes need no arithmetic (tiny4; the
+// offset's share, -8 2^-24 sum(q), starts the sum): 5 instructions for 8 codes instead of 17 and a scale.
 // V's codes and the scales go to LDS, where the transposing read gives lane c + 16 g channel 16 cb + c of tokens 16 g ..
 // + 15: those that its scores are of.
 
@@ -175,6 +177,13 @@ __device__ __forceinline__ void weigh(Sum4& x, const float4_t (&S)[4], float sl2
 
 __device__ __forceinline__ half2_t twice(uint32_t bits) { return as_h2(bits | (bits << 16)); }
 
+// 16 bytes of global memory, named as such: a flat load shares LDS's counter, and every wait for LDS would be one for it.
+__device__ __forceinline__ uint4 load_global16(const uint8_t* p, bool once) {
+  const auto* from = reinterpret_cast<const __attribute__((address_space(1))) u32x4_t*>(reinterpret_cast<uintptr_t>(p));
+  const u32x4_t v = once ? __builtin_nontemporal_load(from) : *from;
+  return uint4{v.x, v.y, v.z, v.w};
+}
+
 // W: waves of the workgroup.
 template <int RB, int W>
 __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
@@ -189,80 +198,130 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_Q4_BYTES;
 
   uint4 kn[4];  // the next page's K codes
+  // (a group without a page: any page's bytes, all of them masked)
   auto issue = [&](int page, int sb) {
+    page = max(page, 0);
+    const int lane = tail_tid() & 63;  // (opaque: the offsets are made again at each use, for want of registers)
     const uint8_t* p = reinterpret_cast<const uint8_t*>(uniform_ptr(pages + page * page_stride));
-    const uint8_t* k = p + (16 * (c >> 2) + (c & 3)) * Q4_ROW + 16 * g;
+    const uint32_t k = (uint32_t)((16 * ((lane >> 2) & 3) + (lane & 3)) * Q4_ROW + 16 * (lane >> 4));
 #pragma unroll
-    for (int b = 0; b < 4; ++b) kn[b] = *reinterpret_cast<const uint4*>(k + 4 * b * Q4_ROW);
+    for (int b = 0; b < 4; ++b) kn[b] = load_global16(p + (k + 4 * b * Q4_ROW), u.alone);
     const uint32_t slot = __builtin_amdgcn_readfirstlane(lds_addr(lds)) + (2 * wave + sb) * Q4_SLOT;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // earlier reads of this slot are done
+    const uint32_t v = (uint32_t)(Q4_CODES + (lane >> 2) * Q4_ROW + (((lane & 3) ^ swz4(lane >> 2)) << 4));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = 16 * e + (lane >> 2);
-      dma16(p, (uint32_t)(Q4_CODES + row * Q4_ROW + (((lane & 3) ^ swz4(row)) << 4)), slot + 1024 * e);
+    for (int e = 0; e < 4; ++e) {  // (rows 16 e + lane / 4: the key is theirs)
+      if (u.alone) dma16_stream(p, v + 1024 * e, slot + 1024 * e);
+      else dma16(p, v + 1024 * e, slot + 1024 * e);
     }
-    dma16(p, (uint32_t)(2 * Q4_CODES + 16 * lane), slot + Q4_CODES);
+    if (u.alone) dma16_stream(p, (uint32_t)(2 * Q4_CODES + 16 * lane), slot + Q4_CODES);
+    else dma16(p, (uint32_t)(2 * Q4_CODES + 16 * lane), slot + Q4_CODES);
   };
 
   int64_t s = s0 + wave;
   const int mine = s < s1 ? (int)((s1 - s + W - 1) / W) : 0;  // pages of this wave
   Pages pg(a.b, u.seq, s, W, mine);
-  half8_t qb[RB][4];  // channels 32 g + 8 k ..
-  int tq[RB];         // the token of row c: the last one that it attends
+  half8_t qb[RB][4];  // channels 32 k + 8 g ..; the pairs that meet 16 n are held over 16, all times a power of two
+  float4_t start[RB][4];  // the offset's share of group k
+  float sl2[RB];       // what turns row c's sums into scores (log2 domain)
+  int tq[RB];          // the token of row c: the last one that it attends
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int r = 16 * rb + c, row = u.row0 + r;
     const bool ok = r < at.rows;
     const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
     tq[rb] = tk;
-    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs + 32 * g;
+    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs + 8 * g;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint4 w = {0, 0, 0, 0};
-      if (ok) w = *reinterpret_cast<const uint4*>(qr + 8 * k);
+      if (ok) w = *reinterpret_cast<const uint4*>(qr + 32 * k);
       qb[rb][k] = paired(w);
     }
   }
   int page = pg.at(0);
-  if (page >= 0) issue(page, 0);
+  if (mine > 0) issue(page, 0);
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    // (the row's largest comes to 2^14, so that over 16 what is lost is 2^-35 of it, at most; not finite: as it is)
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf((float)qb[rb][k][e]));
+    top = max4rows(top);
+    const int up = top > 0.0f && top < 65536.0f ? 127 + 14 - (int)(__float_as_uint(top) >> 23) : 0;
+    const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+    sl2[rb] = a.sl2 * 0x1p24f * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = e & 2 ? 0.0625f : 1.0f;  // (pairs of two)
+        qb[rb][k][e] = (_Float16)((float)qb[rb][k][e] * (by * f));
+        sum = __builtin_fmaf((float)qb[rb][k][e], 1.0f / f, sum);
+      }
+      sum = sum4rows(sum) * (-8.0f * 0x1p-24f);
+      start[rb][k] = float4_t{sum, sum, sum, sum};
+    }
+  }
 
   const int64_t whole = (at.start + u.row0 / a.gq + 1) / GT;  // steps that every row of the tile sees whole
   Sum4 st[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) init(st[rb]);
+  const uint32_t bias = bias1024();
 
   for (int t = 0; t < mine; ++t, s += W) {
     const int sb = t & 1;
-    const bool here = page >= 0;
-    uint4 kc[4];
+    const bool here = page >= 0;  // a group without a page takes no part
     wait_groups_all();
+    uint4 kc[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) kc[b] = kn[b];
     page = pg.at(t + 1);
-    if (page >= 0) issue(page, sb ^ 1);
-    if (!here) continue;  // a group without a page takes no part
+    if (t + 1 < mine) issue(page, sb ^ 1);  // (a whole step ahead: issued after K's products, 45 us instead of NN)
 
     uint8_t* slot = lds + (2 * wave + sb) * Q4_SLOT;
-    const uint2 ks = *reinterpret_cast<const uint2*>(slot + Q4_CODES + 8 * (4 * c + g));
+    const uint8_t* ksc = slot + Q4_CODES + 32 * (tail_tid() >> 4 & 3);
     float4_t S[RB][4];
+    uint2 ks[2][4];  // of tokens 16 g + 4 b .. + 3, group k; the next tile's on the way
+    auto load_ks = [&](int b) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ks[b & 1][k] = *reinterpret_cast<const uint2*>(ksc + 2 * GT * k + 8 * b);
+    };
+    load_ks(0);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const half2_t sc = twice(b < 2 ? (b & 1 ? ks.x >> 16 : ks.x & 0xffffu) : (b & 1 ? ks.y >> 16 : ks.y & 0xffffu));
-      const half8_t kop[4] = {unpack4(kc[b].x, sc), unpack4(kc[b].y, sc), unpack4(kc[b].z, sc), unpack4(kc[b].w, sc)};
+      // (a tile after the other, for want of registers: what is opaque stays in order)
+      asm volatile("" : "+v"(kc[b].x), "+v"(kc[b].y), "+v"(kc[b].z), "+v"(kc[b].w));
+      if (b < 3) load_ks(b + 1);
+      const uint32_t words[4] = {kc[b].x, kc[b].y, kc[b].z, kc[b].w};
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float4_t x = {0.f, 0.f, 0.f, 0.f};
+      for (int rb = 0; rb < RB; ++rb) S[rb][b] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x = mfma32(kop[k], qb[rb][k], x);
-        S[rb][b] = x;
+      for (int k = 0; k < 4; ++k) {
+        const half8_t kop = tiny4(words[k]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const float4_t d = mfma32(kop, qb[rb][k], start[rb][k]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const half2_t h = as_h2(i < 2 ? ks[b & 1][k].x : ks[b & 1][k].y);
+            S[rb][b][i] = __builtin_fmaf((float)(i & 1 ? h.y : h.x), d[i], S[rb][b][i]);
+          }
+        }
       }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) asm volatile("" : "+v"(S[rb][b]));
     }
     uint16_t* vsc = reinterpret_cast<uint16_t*>(slot + Q4_CODES + Q4_SCALES);
-    if (s >= whole) {
+    if (s >= whole || !here) {
       // Masked places: tokens behind a row's own, and the page's rows behind the sequence's last token, which hold
       // anything. Their weight is 0, but 0 times a V that is not finite is NaN, so such scales become 0; where a row does
       // attend such a token, its score becomes NaN instead. (Positions count from the sequence's first new token: they fit.)
-      const int l = tail_tid() & 63, first = (int)(s * GT - at.start);
+      const int l = tail_tid() & 63, first = here ? (int)(s * GT - at.start) : 1 << 30;
       bool bad = false;
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp) bad |= (vsc[v_scale_at(l, grp)] & 0x7fffu) > Q4_LARGEST;
@@ -285,12 +344,13 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
     }
     half8_t ph[RB][2];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) weigh(st[rb], S[rb], a.sl2, ph[rb], g);
-    const int vrow = 16 * g + c;
-    const uint8_t* vp = slot + vrow * Q4_ROW;
+    for (int rb = 0; rb < RB; ++rb) weigh(st[rb], S[rb], sl2[rb], ph[rb], g);
+    const int vl = tail_tid() & 63;
+    const uint8_t* vp = slot + vl * Q4_ROW;  // (row 16 g + c)
 #pragma unroll
     for (int grp = 0; grp < 4; ++grp) {
-      const uint4* sp = reinterpret_cast<const uint4*>(slot + Q4_CODES + Q4_SCALES + 2 * (grp * GT + 16 * g));
+      asm volatile("" : "+v"(vp));  // (as above)
+      const uint4* sp = reinterpret_cast<const uint4*>(slot + Q4_CODES + Q4_SCALES + 2 * (grp * GT + 16 * (vl >> 4)));
       const uint4 s0w = sp[0], s1w = sp[1];
       const half2_t sv[2][4] = {{as_h2(s0w.x), as_h2(s0w.y), as_h2(s0w.z), as_h2(s0w.w)},
                                 {as_h2(s1w.x), as_h2(s1w.y), as_h2(s1w.z), as_h2(s1w.w)}};
@@ -298,14 +358,16 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
       for (int e = 0; e < 2; ++e) {
         const int cb = 2 * grp + e;
         const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (lds_v2i_t*)(const lds_void_t*)(vp + 8 * e + ((grp ^ swz4(vrow)) << 4))));
+            (lds_v2i_t*)(const lds_void_t*)(vp + 8 * e + ((grp ^ swz4(vl)) << 4))));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const half8_t vop = unpack4(w ? vw.y : vw.x, sv[w]);
+          const half8_t vop = unpack4(w ? vw.y : vw.x, sv[w], bias);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) st[rb].acc[cb] = mfma32(ph[rb][w], vop, st[rb].acc[cb]);
         }
       }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) asm volatile("" : "+v"(st[rb].acc[2 * grp]), "+v"(st[rb].acc[2 * grp + 1]));
     }
   }
 
@@ -327,9 +389,9 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
     __syncthreads();
     const int l32 = tid & 31;
 #pragma unroll
-    for (int p = 0; p < 8 / W; ++p) {
+    for (int p = 0; p < (8 + W - 1) / W; ++p) {
       const int r16 = 2 * W * p + (tid >> 5), r = 16 * rb + r16;
-      if (r >= at.rows) continue;
+      if (r16 >= 16 || r >= at.rows) continue;
       const float* base = reinterpret_cast<const float*>(lds) + r16 * CH_PART;
       RowSum sum = {NEG_INF, 0.0f, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -394,7 +456,8 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
   // steps that some row of the tile does not see whole: masked places may hold anything there (attend4_small)
   const int tile_whole = (int)((at.start + u.row0 / a.gq + 1) / GT) - s0;
   // Page t from its stage into its tiles; with the rules for masked places where `check` (a token whose V is not finite
-  // gets a K that is not). Wave w: K's tile b = w / 2, channels 32 g + 16 (w % 2) .. + 15; V's channels 16 w .. + 15.
+  // gets a K that is not). Wave w: K's tile b = w / 2, groups 2 (w % 2) and the next; V's channels 16 w .. + 15.
+  const uint32_t bias = bias1024();
   auto convert = [&](int t, int slot, auto check) {
     const uint8_t* sg = lds + WD_ST + slot * PAGE_Q4_BYTES;
     const int lane = tail_tid() & 63, c = lane & 15, g = lane >> 4, b = wave >> 1;
@@ -403,14 +466,14 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
     const u32x2 vw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
         (lds_v2i_t*)(const lds_void_t*)(sg + Q4_CODES + vrow * Q4_ROW + 8 * (wave & 1) + (((wave >> 1) ^ (c >> 2)) << 4))));
     const uint16_t* sc = reinterpret_cast<const uint16_t*>(sg + 2 * Q4_CODES);
-    uint32_t ks = sc[(4 * c + g) * 4 + b];
+    uint32_t k0 = sc[2 * (wave & 1) * GT + krow], k1 = sc[(2 * (wave & 1) + 1) * GT + krow];
     const uint4* vp = reinterpret_cast<const uint4*>(sc + Q4_SCALES / 2 + (wave >> 1) * GT + 16 * g);
     const uint4 v0 = vp[0], v1 = vp[1];
     uint32_t vs[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     if constexpr (decltype(check)::value) {
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp)
-        if ((sc[Q4_SCALES / 2 + v_scale_at(krow, grp)] & 0x7fffu) > Q4_LARGEST) ks = 0x7e00u;
+        if ((sc[Q4_SCALES / 2 + v_scale_at(krow, grp)] & 0x7fffu) > Q4_LARGEST) k0 = k1 = 0x7e00u;
       const int left = (int)min<int64_t>(GT, len - (int64_t)(s0 + t) * GT);  // tokens that the page has
 #pragma unroll
       for (int e = 0; e < 8; ++e) {  // the pair of tokens 16 g + 8 (e / 4) + e % 4 and 4 further
@@ -419,15 +482,14 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
         if (((vs[e] >> 16) & 0x7fffu) > Q4_LARGEST || tok + 4 >= left) vs[e] &= 0xffffu;
       }
     }
-    const half2_t k2 = twice(ks);
     const half2_t va[4] = {as_h2(vs[0]), as_h2(vs[1]), as_h2(vs[2]), as_h2(vs[3])};
     const half2_t vb[4] = {as_h2(vs[4]), as_h2(vs[5]), as_h2(vs[6]), as_h2(vs[7])};
     uint8_t* kt = lds + (t & 1) * WD_TILE + 16 * lane + 2048 * wave;  // (operand 4 b + k of wave 2 b + k / 2)
     uint8_t* vt = lds + WD_VT + (t & 1) * WD_TILE + 16 * lane + 1024 * wave;
-    *reinterpret_cast<half8_t*>(kt) = unpack4(kw.x, k2);
-    *reinterpret_cast<half8_t*>(kt + 1024) = unpack4(kw.y, k2);
-    *reinterpret_cast<half8_t*>(vt) = unpack4(vw.x, va);
-    *reinterpret_cast<half8_t*>(vt + 8192) = unpack4(vw.y, vb);
+    *reinterpret_cast<half8_t*>(kt) = unpack4(kw.x, twice(k0), bias);
+    *reinterpret_cast<half8_t*>(kt + 1024) = unpack4(kw.y, twice(k1), bias);
+    *reinterpret_cast<half8_t*>(vt) = unpack4(vw.x, va, bias);
+    *reinterpret_cast<half8_t*>(vt + 8192) = unpack4(vw.y, vb, bias);
   };
 
   const int row0 = u.row0 + wave * (WD_RB * 16);  // first row of this wave
@@ -438,11 +500,11 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
     const int row = row0 + 16 * rb + c;
     const bool ok = row < rows;
     const int tk = ok ? row / a.gq : 0, hd = h * a.gq + (ok ? row % a.gq : 0);
-    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs + 32 * g;
+    const uint16_t* qr = a.q + (at.first_token + tk) * a.q_ts + hd * a.q_hs + 8 * g;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint4 w = {0, 0, 0, 0};
-      if (ok) w = *reinterpret_cast<const uint4*>(qr + 8 * k);
+      if (ok) w = *reinterpret_cast<const uint4*>(qr + 32 * k);
       qb[rb][k] = paired(w);
     }
   }
@@ -600,13 +662,14 @@ __global__ __launch_bounds__(Q4_THREADS, 1) void attn_q4_kernel(ChunkArgs a) {
 }
 
 constexpr int Q4_SMALL = 4;  // waves of a workgroup in a launch of small units alone
-__global__ __launch_bounds__(64 * Q4_SMALL, 2) void attn_q4_small_kernel(ChunkArgs a) {
+template <int RB>
+__global__ __launch_bounds__(64 * Q4_SMALL, RB == 1 ? 3 : 2) void attn_q4_small_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * Q4_SMALL * Q4_SLOT];
   const int h = blockIdx.x % a.b.hkv;
   const Unit u = a.units[blockIdx.x / a.b.hkv];
-  if (!unit_ok(a, u, 32)) return;
-  if (u.rows <= 16) attend4_small<1, Q4_SMALL>(a, u, h, lds);
-  else attend4_small<2, Q4_SMALL>(a, u, h, lds);
+  if (!unit_ok(a, u, 16 * RB)) return;
+  if (RB == 1 || u.rows <= 16) attend4_small<1, Q4_SMALL>(a, u, h, lds);
+  else attend4_small<RB, Q4_SMALL>(a, u, h, lds);
 }
 
 // ---------------------------------------------------------------- host side
@@ -713,8 +776,9 @@ extern "C" int nkv_paged_attn_chunks_q4(const uint16_t* q, int64_t q_token_strid
   if (!any) return NKV_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(n_units * hkv));
-  if (wide) hipLaunchKernelGGL(attn_q4_kernel, grid, dim3(Q4_THREADS), 0, s, a);
-  else hipLaunchKernelGGL(attn_q4_small_kernel, grid, dim3(64 * Q4_SMALL), 0, s, a);
+  if (wide == ROWS256) hipLaunchKernelGGL(attn_q4_kernel, grid, dim3(Q4_THREADS), 0, s, a);
+  else if (wide == ROWS16) hipLaunchKernelGGL(attn_q4_small_kernel<1>, grid, dim3(64 * Q4_SMALL), 0, s, a);
+  else hipLaunchKernelGGL(attn_q4_small_kernel<2>, grid, dim3(64 * Q4_SMALL), 0, s, a);
   if (int rc = check_launch(what)) return rc;
   return launch_merges(what, a, reinterpret_cast<const Merge*>(merges), n_merges, s);
 }

@@ -2,8 +2,8 @@
 // first half of a SwiGLU block, xn = x or its RMSNorm.
 //
 // On the matrix cores: tiles of 16 rows of W times tiles of 16 columns. Lane c + 16 g takes row c's group g of a block's 128
-// inputs, 16 bytes. xn is rounded once to fp16, scaled by a power of two of the token's own, so that bf16's range and large
-// gammas stay within fp16's. The waves of a workgroup cut the inputs among them, a block in turn; everything else in fp32,
+// inputs, 16 bytes. xn is held in fp16 (parts_of it), scaled by a power of two of the token's own, so that bf16's range
+// and large gammas stay within fp16's. The waves of a workgroup cut the inputs among them, a block in turn; everything else in fp32,
 // with one rounding at the end. Bound by the weights' bytes, and by a launch's chain of loads that wait for each other.
 //
 // Three forms, by the tokens and by what is to be done to x:
@@ -64,18 +64,27 @@ __device__ __forceinline__ void measure8(const float (&v)[8], const float (&gv)[
     top = fmaxf(top, __builtin_fabsf(v[e] * gv[e]));
   }
 }
-__device__ __forceinline__ uint4 xn8(const float (&v)[8], const float (&gv)[8], const Factor& f) {
-  uint32_t h[4];
+// xn of eight inputs as fp16, and what that leaves off (lo).
+__device__ __forceinline__ uint4 xn8(const float (&v)[8], const float (&gv)[8], const Factor& f, uint4& lo) {
+  uint32_t h[4], l[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    h[e] = (uint32_t)f2h(v[2 * e] * f.norm * gv[2 * e] * f.inverse) |
-           ((uint32_t)f2h(v[2 * e + 1] * f.norm * gv[2 * e + 1] * f.inverse) << 16);
+  for (int e = 0; e < 4; ++e) {
+    const float a = v[2 * e] * f.norm * gv[2 * e] * f.inverse, b = v[2 * e + 1] * f.norm * gv[2 * e + 1] * f.inverse;
+    const uint16_t ha = f2h(a), hb = f2h(b);
+    h[e] = (uint32_t)ha | ((uint32_t)hb << 16);
+    l[e] = (uint32_t)f2h(a - h2f(ha)) | ((uint32_t)f2h(b - h2f(hb)) << 16);
+  }
+  lo = uint4{l[0], l[1], l[2], l[3]};
   return uint4{h[0], h[1], h[2], h[3]};
 }
+
+// The fp16 parts that xn is held in: two where a norm made it of fp16 inputs, whose product would else have 1.4 to 1.6 times
+// the error of a result that is rounded once, a SwiGLU's 1.8 times; in bf16's error nothing of it shows.
+constexpr int parts_of(int dt, bool norm) { return dt == NKV_F16 && norm ? 2 : 1; }
 // xn once for all workgroups of a product, one token a workgroup, as operands: piece (block kb, k, tile n, lane c + 16 g) of 16
 // bytes holds token 16 n + c's inputs 128 kb + 32 g + 8 k .. + 7 (zeros behind the last). Tiles are counted in passes of
-// NT, each of which lies together.
-template <int DT>
+// NT, each of which lies together. P: parts of xn (parts_of), the second of tile n as tile NT + n.
+template <int DT, int P>
 __global__ __launch_bounds__(256) void xn_kernel(ProductArgs a, int nt, uint8_t* xn, float* unit) {
   __shared__ float part[2][4];
   const int tid = threadIdx.x;
@@ -120,23 +129,28 @@ __global__ __launch_bounds__(256) void xn_kernel(ProductArgs a, int nt, uint8_t*
   top = fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
   const Factor f = factor_of(ss, top, a.gamma, a.in, a.eps);
   const int blocks = (a.in + PB - 1) / PB, tile = (int)(t / 16), n = tile % nt;
-  uint8_t* to = xn + (int64_t)(tile - n) * blocks * 4096 + n * 1024 + (int)(t & 15) * 16;
-  const auto store = [&](int i, uint4 u) {  // input i: block i / 128, g, k
-    *reinterpret_cast<uint4*>(to + ((int64_t)(i >> 7) * 4 + ((i >> 3) & 3)) * (nt * 1024) + ((i >> 5) & 3) * 256) = u;
+  uint8_t* to = xn + (int64_t)(tile - n) * (P * blocks) * 4096 + n * 1024 + (int)(t & 15) * 16;
+  const auto store = [&](int i, uint4 u, uint4 lo) {  // input i: block i / 128, g, k
+    uint8_t* at = to + ((int64_t)(i >> 7) * 4 + ((i >> 3) & 3)) * (P * nt * 1024) + ((i >> 5) & 3) * 256;
+    *reinterpret_cast<uint4*>(at) = u;
+    if constexpr (P == 2) *reinterpret_cast<uint4*>(at + nt * 1024) = lo;
   };
+  uint4 lo = {0, 0, 0, 0};
 #pragma unroll
   for (int k = 0; k < KEEP; ++k)
     if (const int i = 8 * tid + 2048 * k; i < a.in) {
       get(r[k], gr[k]);
-      store(i, xn8(v, gv, f));
+      const uint4 hi = xn8(v, gv, f, lo);
+      store(i, hi, lo);
     }
   for (int i = 8 * tid + 2048 * KEEP; i < a.in; i += 2048) {
     Raw8<DT> x8, g8;
     load(i, x8, g8);
     get(x8, g8);
-    store(i, xn8(v, gv, f));
+    const uint4 hi = xn8(v, gv, f, lo);
+    store(i, hi, lo);
   }
-  for (int i = a.in + 8 * tid; i < blocks * PB; i += 2048) store(i, uint4{0, 0, 0, 0});
+  for (int i = a.in + 8 * tid; i < blocks * PB; i += 2048) store(i, uint4{0, 0, 0, 0}, uint4{0, 0, 0, 0});
   if (tid == 0) unit[t] = f.unit;
 }
 
@@ -150,6 +164,7 @@ struct Weights {
   uint4 w[AHEAD][RT];
   uint16_t s[AHEAD][RT];
   int from[RT];
+  uint32_t bias = bias1024();
   __device__ __forceinline__ Weights(const ProductArgs& a, int64_t o0, int lane, int blocks) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {  // (outputs behind the last: the last, not stored)
@@ -170,45 +185,51 @@ struct Weights {
   __device__ __forceinline__ half8_t operand(int e, int r, int k) const {
     const half2_t sc = as_h2((uint32_t)s[e][r] * 0x10001u);
     const uint4& x = w[e][r];
-    return unpack4(k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w, sc);
+    return unpack4(k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w, sc, bias);
   }
 };
 
-// The waves' sums into one, and out: tokens t0 .. t0 + nt - 1, outputs o0 ... red: W * RT * NT tiles of 16 x 17 floats. PER:
-// columns of a token.
+// The waves' sums into one, and out, a tile of outputs at a time: tokens t0 .. t0 + nt - 1, outputs o0 ... red: room for
+// red_floats. PER: columns of a token.
+constexpr int red_floats(int nt, bool gated, int w) { return w * (gated ? 2 : 1) * nt * 16 * 17; }
 template <int DT, int RT, int NT, bool GATED, int W, int PER = 1>
 __device__ __forceinline__ void finish(const ProductArgs& a, const float4_t (&acc)[RT][NT], float* red, int64_t t0, int nt,
                                        int64_t o0, const float* unit) {
-  constexpr int TILES = GATED ? RT / 2 : RT;
+  constexpr int HALVES = GATED ? 2 : 1, TILES = RT / HALVES;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4, wave = tid >> 6;
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int r = 0; r < TILES; ++r) {
+    if (r) __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[(((wave * RT + r) * NT + n) * 16 + 4 * g + i) * 17 + c] = acc[r][n][i];
-  __syncthreads();
-  for (int i = tid; i < TILES * NT * 256; i += 64 * W) {
-    const int row = i & 15, t16 = (i >> 4) & 15, n = (i >> 8) % NT, r = (i >> 8) / NT, t = (16 * n + t16) / PER;
-    const int64_t o = o0 + 16 * r + row;
-    if (t >= nt || o >= a.out || t16 % PER) continue;
-    float v[2] = {0.0f, 0.0f};
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int half = 0; half < (GATED ? 2 : 1); ++half)
-      for (int q = 0; q < W; ++q) v[half] += red[(((q * RT + r + half * TILES) * NT + n) * 16 + row) * 17 + t16];
-    const float f = unit ? unit[t] : 1.0f;
-    v[0] *= f;
-    v[1] *= f;
-    if constexpr (GATED) v[0] = v[0] / (1.0f + expf(-v[0])) * v[1];
-    const int64_t at = (t0 + t) * a.out + o;
-    if (a.residual) v[0] += load1<DT>(a.residual, at);
-    reinterpret_cast<uint16_t*>(a.y)[at] = DT == NKV_F16 ? f2h(v[0]) : f2bf(v[0]);
+        for (int i = 0; i < 4; ++i) red[(((wave * HALVES + h) * NT + n) * 16 + 4 * g + i) * 17 + c] = acc[r + h * TILES][n][i];
+    __syncthreads();
+    for (int i = tid; i < NT * 256; i += 64 * W) {
+      const int row = i & 15, t16 = (i >> 4) & 15, n = i >> 8, t = (16 * n + t16) / PER;
+      const int64_t o = o0 + 16 * r + row;
+      if (t >= nt || o >= a.out || t16 % PER) continue;
+      float v[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int q = 0; q < W; ++q) v[h] += red[(((q * HALVES + h) * NT + n) * 16 + row) * 17 + t16];
+      const float f = unit ? unit[t] : 1.0f;
+      v[0] *= f;
+      v[1] *= f;
+      if constexpr (GATED) v[0] = v[0] / (1.0f + expf(-v[0])) * v[1];
+      const int64_t at = (t0 + t) * a.out + o;
+      if (a.residual) v[0] += load1<DT>(a.residual, at);
+      reinterpret_cast<uint16_t*>(a.y)[at] = DT == NKV_F16 ? f2h(v[0]) : f2bf(v[0]);
+    }
   }
 }
 
 // ---------------------------------------------------------------- a few tokens: one launch
 //
-// Up to 4 tokens, which leave most of a product's 16 columns free: column 4 t + j takes token t's group j of a block alone (its
+// Passes of 4 tokens, which leave most of a product's 16 columns free: column 4 t + j takes token t's group j of a block alone (its
 // other inputs are 0), so that a group's sum comes out by itself and the scales are applied to it, 4 products' results
 // instead of 32 operands. The codes then need no arithmetic: n = code + 8 is an fp16 denormal, n 2^-24 (a nibble at the
 // mantissa's end) or 16 n 2^-24 (the next one; its inputs are held over 16), which the matrix cores take as they are: 5
@@ -218,20 +239,23 @@ __device__ __forceinline__ void finish(const ProductArgs& a, const float4_t (&ac
 
 constexpr int FEW_W = 4, FEW_KX = 5, FEW_AHEAD = 5;
 
-template <int DT, int RT>
+// M: the products that xn's parts take. One is enough for two tokens' two parts: a part is a token to the columns.
+
+template <int DT, int RT, int M>
 __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kernel(ProductArgs a, int each) {
-  constexpr int W = FEW_W, KX = FEW_KX, AHEAD = FEW_AHEAD;
-  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // [tokens][in + 8] fp16, the groups' offsets; sums, at the end
+  constexpr int W = FEW_W, KX = FEW_KX, AHEAD = FEW_AHEAD, P = parts_of(DT, true);
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // [tokens][P][in + 8] fp16, the groups' offsets; sums, at the end
   __shared__ float2 part[W];
   __shared__ float unit[4];
   __shared__ __attribute__((aligned(16))) uint4 zeros[4];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nt = (int)a.tokens, n8 = a.in / 8, blocks = (a.in + PB - 1) / PB;
+  const int64_t t0 = 4 * (int64_t)blockIdx.y;
+  const int nt = (int)min<int64_t>(4, a.tokens - t0), n8 = a.in / 8, blocks = (a.in + PB - 1) / PB;
   const int token = wave / each, at0 = 64 * (wave % each) + lane;  // this lane's chunks: at0 + 64 each k
 
   Raw8<DT> xr[KX], gr[KX];
-  const uint8_t* x = a.x + (int64_t)token * a.in * 2;
+  const uint8_t* x = a.x + (t0 + token) * a.in * 2;
 #pragma unroll
   for (int k = 0; k < KX; ++k) {
     const int i = at0 + 64 * each * k;
@@ -262,8 +286,9 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
   for (int e = 0; e < AHEAD; ++e)
     if (wave + W * e < blocks) load(e, wave + W * e);
 
-  const int stride = 2 * (blocks * PB) + 16;  // bytes of a token's row: the tokens' chunks fall on different banks
-  float* offset = reinterpret_cast<float*>(xs + nt * stride);  // [tokens][4 blocks]
+  const int part_size = 2 * (blocks * PB) + 16;  // (the rows' chunks fall on different banks)
+  const int stride = P * part_size;              // bytes of a token
+  float* offset = reinterpret_cast<float*>(xs + nt * stride);  // [tokens][P][4 blocks]
   float v[8], gv[8];
   auto values = [&](int k) {
     xr[k].get(v);
@@ -300,20 +325,29 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
       const int i = at0 + 64 * each * k;
       if (64 * (wave % each + each * k) >= blocks * (PB / 8)) break;  // (the wave agrees)
       values(k);  // (behind the inputs: zeros)
-      uint32_t h[4];
-      float sum = 0.0f;
+      uint32_t h[P][4];
+      float sum[P] = {};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float by = e & 1 ? f.inverse * 0.0625f : f.inverse;
-        const uint16_t lo = f2h(v[2 * e] * f.norm * gv[2 * e] * by), hi = f2h(v[2 * e + 1] * f.norm * gv[2 * e + 1] * by);
-        h[e] = (uint32_t)lo | ((uint32_t)hi << 16);
-        sum = __builtin_fmaf(h2f(lo) + h2f(hi), e & 1 ? 16.0f : 1.0f, sum);
+        float a0 = v[2 * e] * f.norm * gv[2 * e] * by, a1 = v[2 * e + 1] * f.norm * gv[2 * e + 1] * by;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const uint16_t h0 = f2h(a0), h1 = f2h(a1);
+          h[p][e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
+          sum[p] = __builtin_fmaf(h2f(h0) + h2f(h1), e & 1 ? 16.0f : 1.0f, sum[p]);
+          a0 -= h2f(h0);
+          a1 -= h2f(h1);
+        }
       }
-      sum += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum), 0xB1, 0xf, 0xf, false));
-      sum += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum), 0x4E, 0xf, 0xf, false));
-      if (i < blocks * (PB / 8)) {
-        *reinterpret_cast<uint4*>(xs + token * stride + 16 * i) = uint4{h[0], h[1], h[2], h[3]};
-        if (i % 4 == 0) offset[token * 4 * blocks + i / 4] = sum * (-8.0f * 0x1p-24f);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        sum[p] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum[p]), 0xB1, 0xf, 0xf, false));
+        sum[p] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(sum[p]), 0x4E, 0xf, 0xf, false));
+        if (i < blocks * (PB / 8)) {
+          *reinterpret_cast<uint4*>(xs + token * stride + p * part_size + 16 * i) = uint4{h[p][0], h[p][1], h[p][2], h[p][3]};
+          if (i % 4 == 0) offset[(token * P + p) * 4 * blocks + i / 4] = sum[p] * (-8.0f * 0x1p-24f);
+        }
       }
     }
   }
@@ -322,28 +356,33 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
   float4_t acc[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) acc[r] = float4_t{0.f, 0.f, 0.f, 0.f};
-  const int mine = min(c >> 2, nt - 1);
+  // column 4 v + j: group j of row v of xs (token v, or, where a part is a token, v / P of its part v % P)
+  constexpr int ROWS = P / M;  // of xs, a token
+  const int mine = min(c >> 2, ROWS * nt - 1);
   const bool own = (c & 3) == g;
-  const uint8_t* xp = own ? xs + mine * stride + 64 * g : reinterpret_cast<const uint8_t*>(zeros);
-  const int step = own ? 2 * PB : 0;
-  const float* op = offset + mine * 4 * blocks + (c & 3);
+  const uint8_t* xp = own ? xs + mine * (M * part_size) + 64 * g : reinterpret_cast<const uint8_t*>(zeros);
+  const int step = own ? 2 * PB : 0, part_step = own ? part_size : 0;
+  const float* op = offset + mine * (M * 4 * blocks) + (c & 3);
   for (int kb0 = wave; kb0 < blocks; kb0 += W * AHEAD) {
 #pragma unroll
     for (int e = 0; e < AHEAD; ++e) {
       const int kb = kb0 + W * e;
       if (kb < blocks) {  // (the wave's lanes agree)
-        half8_t b[4];
+        half8_t b[4 * M];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const half8_t*>(xp + kb * step + 16 * k);
-        const float start = op[4 * kb];
+        for (int k = 0; k < 4 * M; ++k)
+          b[k] = *reinterpret_cast<const half8_t*>(xp + kb * step + (k / 4) * part_step + 16 * (k % 4));
+        float start = op[4 * kb];
+        if constexpr (M == 2) start += op[4 * (blocks + kb)];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const uint32_t words[4] = {w[e][r].x, w[e][r].y, w[e][r].z, w[e][r].w};
           float4_t d = {start, start, start, start};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t u = words[k], u8 = u >> 8;
-            d = mfma32(as_h8(uint4{u & 0x000f000fu, u & 0x00f000f0u, u8 & 0x000f000fu, u8 & 0x00f000f0u}), b[k], d);
+            const half8_t n = tiny4(words[k]);
+#pragma unroll
+            for (int p = 0; p < M; ++p) d = mfma32(n, b[4 * p + k], d);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -365,9 +404,10 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
       float q = acc[r][i];
       q += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(q), 0xB1, 0xf, 0xf, false));
       q += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(q), 0x4E, 0xf, 0xf, false));
+      if constexpr (ROWS == 2) q += shfl_xor(q, 4);  // and the token's two parts
       y[r][0][i] = q;
     }
-  finish<DT, RT, 1, RT == 2, W, 4>(a, y, reinterpret_cast<float*>(xs), 0, nt, 16 * (int64_t)blockIdx.x, unit);
+  finish<DT, RT, 1, RT == 2, W, 4 * ROWS>(a, y, reinterpret_cast<float*>(xs), t0, nt, 16 * (int64_t)blockIdx.x, unit);
 }
 
 // ---------------------------------------------------------------- up to 16 tokens of fp16 as they are: one launch
@@ -377,7 +417,7 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
 
 template <int RT, bool GATED, int W>
 __global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_kernel(ProductArgs a) {
-  constexpr int AHEAD = 5, ROW = 2 * PB + 16, SLOT = 16 * ROW, RED = W * RT * 16 * 17 * 4;
+  constexpr int AHEAD = 5, ROW = 2 * PB + 16, SLOT = 16 * ROW, RED = 4 * red_floats(1, GATED, W);
   __shared__ __attribute__((aligned(16))) uint8_t lds[RED > W * SLOT ? RED : W * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -433,20 +473,21 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_kernel(P
 // xn lies as operands (xn_kernel): a wave's loads of it are 1024 bytes in a row, from the XCD's L2 where the workgroups of
 // other rows have it, too.
 
-template <int DT, int RT, int NT, bool GATED, int W, int AHEAD>
-__global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_many_kernel(ProductArgs a) {
-  __shared__ __attribute__((aligned(16))) float red[W * RT * NT * 16 * 17];
+template <int DT, int P, int RT, int NT, bool GATED, int W, int AHEAD>
+__global__ __launch_bounds__(64 * W, 8 / W) void product4_many_kernel(ProductArgs a) {
+  constexpr int XT = P * NT;
+  __shared__ __attribute__((aligned(16))) float red[red_floats(NT, GATED, W)];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t t0 = (int64_t)blockIdx.y * (16 * NT);
   const int nt = (int)min<int64_t>(16 * NT, a.tokens - t0), blocks = (a.in + PB - 1) / PB;
   const int64_t o0 = (int64_t)blockIdx.x * (16 * Weights<RT, GATED, W, AHEAD>::TILES);
 
-  half8_t b[4][NT];  // the next block's
-  const uint8_t* xp = a.x + (int64_t)blockIdx.y * NT * blocks * 4096 + 16 * lane;
+  half8_t b[4][XT];  // the next block's
+  const uint8_t* xp = a.x + (int64_t)blockIdx.y * XT * blocks * 4096 + 16 * lane;
   auto load_x = [&](int kb, int k) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) b[k][n] = *reinterpret_cast<const half8_t*>(xp + ((int64_t)(4 * kb + k) * NT + n) * 1024);
+    for (int n = 0; n < XT; ++n) b[k][n] = *reinterpret_cast<const half8_t*>(xp + ((int64_t)(4 * kb + k) * XT + n) * 1024);
   };
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -472,7 +513,7 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_many_ker
           for (int r = 0; r < RT; ++r) {
             const half8_t w = wt.operand(e, r, k);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[r][n] = mfma32(w, b[k][n], acc[r][n]);
+            for (int n = 0; n < XT; ++n) acc[r][n % NT] = mfma32(w, b[k][n], acc[r][n % NT]);
           }
           if (kb + W < blocks) load_x(kb + W, k);
         }
@@ -486,8 +527,11 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_many_ker
 // ---------------------------------------------------------------- host side
 
 // How many waves share a token in product4_few_kernel; 0: another form is taken. (Gates and ups must be in tiles of their own.)
+// More than 4 tokens take several passes over the weight, in the same launch: where their workgroups do not fill the card twice
+// that is less than the launch of xn (NN).
 int few_each(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
-  if (tokens > 4 || (gated && out % 16) || (!norm && dtype == NKV_F16)) return 0;
+  if ((gated && out % 16) || (!norm && dtype == NKV_F16)) return 0;
+  if (tokens > 4 && cdiv(tokens, 4) * cdiv(out, 16) > 2 * CUS) return 0;
   const int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
   return cdiv(in, PB) * PB <= each * FEW_KX * 512 ? each : 0;
 }
@@ -497,7 +541,7 @@ int pass_tiles(int64_t tokens) { return (int)std::min<int64_t>(cdiv(tokens, 16),
 int64_t product_workspace(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
   if (few_each(dtype, tokens, out, in, norm, gated) || (tokens <= 16 && dtype == NKV_F16 && !norm)) return 0;
   const int64_t passes = cdiv(tokens, 16 * pass_tiles(tokens));
-  return passes * pass_tiles(tokens) * cdiv(in, PB) * 4096 + 4 * tokens;
+  return passes * pass_tiles(tokens) * cdiv(in, PB) * 4096 * parts_of(dtype, norm) + 4 * tokens;
 }
 
 template <int DT, bool GATED>
@@ -507,8 +551,12 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   const int64_t tiles = cdiv(a.out, 16);
   const bool norm = a.gamma != nullptr;
   if (const int each = few_each(DT, a.tokens, a.out, a.in, norm, GATED)) {
-    const size_t lds = std::max((size_t)a.tokens * (2 * blocks * PB + 16 + 16 * blocks), (size_t)FEW_W * R1 * 16 * 17 * 4);
-    hipLaunchKernelGGL((product4_few_kernel<DT, R1>), dim3((unsigned)tiles), dim3(64 * FEW_W), lds, s, a, each);
+    const size_t xn = std::min<int64_t>(a.tokens, 4) * (parts_of(DT, true) * (2 * blocks * PB + 16 + 16 * blocks));
+    const size_t lds = std::max(xn, (size_t)4 * red_floats(1, GATED, FEW_W));
+    const dim3 grid((unsigned)tiles, (unsigned)cdiv(a.tokens, 4)), block(64 * FEW_W);
+    constexpr int P = parts_of(DT, true);
+    if (a.tokens <= 2) hipLaunchKernelGGL((product4_few_kernel<DT, R1, 1>), grid, block, lds, s, a, each);
+    else hipLaunchKernelGGL((product4_few_kernel<DT, R1, P>), grid, block, lds, s, a, each);
     return check_launch(what);
   }
   if constexpr (DT == NKV_F16) {
@@ -523,7 +571,9 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
     return fail(NKV_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
   const int nt = pass_tiles(a.tokens);
   float* unit = reinterpret_cast<float*>(ws + need - 4 * a.tokens);
-  hipLaunchKernelGGL((xn_kernel<DT>), dim3((unsigned)a.tokens), dim3(256), 0, s, a, nt, ws, unit);
+  const dim3 each_token((unsigned)a.tokens);
+  if (parts_of(DT, norm) == 2) hipLaunchKernelGGL((xn_kernel<DT, 2>), each_token, dim3(256), 0, s, a, nt, ws, unit);
+  else hipLaunchKernelGGL((xn_kernel<DT, 1>), each_token, dim3(256), 0, s, a, nt, ws, unit);
   if (int rc = check_launch(what)) return rc;
   a.x = ws;
   a.unit = unit;
@@ -531,19 +581,32 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   const auto go = [&](auto kernel, int tiles_wg, int waves) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(tiles, tiles_wg), passes), dim3(64 * waves), 0, s, a);
   };
-  const bool many = tiles > 2 * CUS;
-  if (nt == 1) {
-    if (blocks <= 24) go(product4_many_kernel<DT, R1, 1, GATED, 4, 5>, 1, 4);
-    else go(product4_many_kernel<DT, R1, 1, GATED, 16, 5>, 1, 16);
-  } else if (nt == 2) {
-    if (many) go(product4_many_kernel<DT, 2 * R1, 2, GATED, 8, 3>, 2, 8);
-    else go(product4_many_kernel<DT, R1, 2, GATED, 8, 3>, 1, 8);
-  } else if (nt == 3) {
-    if (many) go(product4_many_kernel<DT, 2 * R1, 3, GATED, 8, 3>, 2, 8);
-    else go(product4_many_kernel<DT, R1, 3, GATED, 8, 3>, 1, 8);
+  // Rows a wave takes, and waves of a workgroup (us, with xn's launch; 17 / 32 / 48 / 64 tokens): 6144 x 2560 as two tiles of
+  // 16 rows and 8 waves 9.1 / 9.5 / 10.9 / 11.8, as one tile 10.5 / 10.8 / 12.6 / 13.6; 2560 x 4096 10.7 / 11.3 / 13.7 /
+  // 15.2 and 8.9 / 9.2 / 11.1 / 12.4: two where the workgroups still fill the card. Gates and ups (2 x 9728 x 2560, one tile of
+  // each) as 8 waves 15.1 / 15.5 / 21.0 / 24.0, as 4 waves 16.3 / 16.7 / 19.3 / 21.3: the sums of more tokens take registers.
+  const auto pass = [&](auto n, auto p) {
+    constexpr int NT = decltype(n)::value, P = decltype(p)::value;
+    if constexpr (GATED) {
+      if constexpr (NT <= 2) go(product4_many_kernel<DT, P, 2, NT, true, 8, 3>, 1, 8);
+      else go(product4_many_kernel<DT, P, 2, NT, true, 4, 5>, 1, 4);
+    } else if (tiles >= CUS) {
+      go(product4_many_kernel<DT, P, 2, NT, false, 8, 3>, 2, 8);
+    } else {
+      go(product4_many_kernel<DT, P, 1, NT, false, 8, 5>, 1, 8);
+    }
+  };
+  const auto with_tiles = [&](auto p) {
+    if (nt == 1) pass(std::integral_constant<int, 1>{}, p);
+    else if (nt == 2) pass(std::integral_constant<int, 2>{}, p);
+    else if (nt == 3) pass(std::integral_constant<int, 3>{}, p);
+    else pass(std::integral_constant<int, 4>{}, p);
+  };
+  if constexpr (DT == NKV_F16) {
+    if (norm) with_tiles(std::integral_constant<int, 2>{});
+    else with_tiles(std::integral_constant<int, 1>{});
   } else {
-    if (many) go(product4_many_kernel<DT, 2 * R1, 4, GATED, 8, 3>, 2, 8);
-    else go(product4_many_kernel<DT, R1, 4, GATED, 8, 3>, 1, 8);
+    with_tiles(std::integral_constant<int, 1>{});
   }
   return check_launch(what);
 }

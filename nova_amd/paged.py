@@ -362,7 +362,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
     page_bytes = PAGE_BYTES_TOK
     has_rings = False
     _calls = {name: f"nkv_paged_{name}_tok" for name in ("quantize", "append_chunks", "attn_chunks", "read")}
-    _big_from = C.BIG_FROM
+    _q4 = False
 
     def prefill(self, b: int, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store a prompt of n tokens (``[1, H_kv, n, 128]``) for sequence ``b``: every token
@@ -415,7 +415,7 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
             if n:
                 self.reserve(b, self._len[b] + n)
         return C.chunk_plan(counts, self._len[:len(counts)], self.pos, self.num_q_heads // self.num_kv_heads,
-                            self.num_kv_heads, self._big_from)
+                            self.num_kv_heads, self._q4)
 
     def append_chunks(self, plan: ChunkPlan, qkv: torch.Tensor, layer: int, q_gamma: torch.Tensor | None = None,
                       k_gamma: torch.Tensor | None = None, eps: float = 1e-6, inv_freq: torch.Tensor | None = None,
@@ -494,9 +494,13 @@ class PagedKVInt8TokCache(PagedKVInt8Cache):
         ws = _lib.scratch(dev, plan.ws_bytes) if plan.ws_bytes else None
         C.launch(dev, self._calls["attn_chunks"], query.data_ptr(), query.stride(0), query.stride(1), total,
                  self.pages[layer].data_ptr(), self.page_table.data_ptr(), self.page_table.stride(0), self.num_pages,
-                 *plan.where, plan.nseq, hq, hkv, D, *plan.work, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), _lib.ptr(ws),
+                 *plan.where, plan.nseq, hq, hkv, D, *self._work(plan), out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), _lib.ptr(ws),
                  plan.ws_bytes)
         return out
+
+    @staticmethod
+    def _work(plan: ChunkPlan) -> tuple:
+        return plan.work
 
     def advance_chunks(self, plan: ChunkPlan, accepted: list[int] | None = None) -> None:
         """``pos`` moves past the step's tokens, or past the first ``accepted[b]`` of each sequence's (drafted
@@ -539,6 +543,11 @@ class PagedKVQ4Cache(PagedKVInt8TokCache):
 
     page_bytes = PAGE_BYTES_Q4
     _calls = {name: f"nkv_paged_{name}_q4" for name in PagedKVInt8TokCache._calls}
+    _q4 = True
+
+    @staticmethod
+    def _work(plan: ChunkPlan) -> tuple:
+        return plan.work_q4
 
     def plan(self, lengths: list[int] | None = None) -> None:
         raise NotImplementedError("the 4-bit cache steps by plan_chunks")

@@ -59,7 +59,7 @@ def _swiglu(lib, **kw):
     (dict(out=0), INVALID), (dict(out=1 << 27), INVALID), (dict(n_in=0), INVALID), (dict(n_in=40), INVALID),
     (dict(n_in=(1 << 20) + 32), INVALID), (dict(x=None), INVALID), (dict(w4=None), INVALID),
     (dict(y=None), INVALID), (dict(x=PTR + 2), UNSUPPORTED), (dict(w4=PTR + 8), UNSUPPORTED), (dict(gamma=PTR + 2), UNSUPPORTED),
-    (dict(ws=PTR + 8), UNSUPPORTED), (dict(tokens=17, gamma=PTR), INVALID), (dict(tokens=17, dtype=1, ws=PTR, ws_bytes=2 * 4096 + 67), INVALID),
+    (dict(ws=PTR + 8), UNSUPPORTED), (dict(tokens=17, n_in=2592, gamma=PTR), INVALID), (dict(tokens=17, dtype=1, n_in=2592, ws=PTR, ws_bytes=42 * 4096 + 67), INVALID),
     (dict(tokens=0, x=None), OK)])
 def test_product_refusals(lib, call, kw, rc):
     assert call(lib, **kw) == rc
@@ -67,14 +67,16 @@ def test_product_refusals(lib, call, kw, rc):
 
 
 def test_product_workspace(lib):
-    """None where one launch makes xn (up to 4 tokens, 10240 inputs in a power of two of tokens, gates and ups in tiles of
-    their own), or where x is taken as it is; else xn in tiles of 16 tokens and blocks of 128 inputs, and a word a token."""
+    """None where one launch makes xn (passes of 4 tokens, 10240 inputs in a power of two of tokens, gates and ups in tiles of
+    their own, few workgroups if passes), or where x is taken as it is; else xn in tiles of 16 tokens and blocks of 128 inputs
+    (in two parts for a norm of fp16), and a word a token."""
     need = lib.nkv_gemv_q4_workspace_bytes
-    assert need(0, 4, 100, 2560, 1, 0) == need(1, 2, 100, 5120, 1, 0) == need(0, 1, 160, 10240, 1, 1) == need(1, 3, 16, 32, 0, 1) == 0
+    assert need(0, 4, 100000, 2560, 1, 0) == need(1, 2, 100, 5120, 1, 0) == need(0, 1, 160, 10240, 1, 1) == need(1, 3, 16, 32, 0, 1) == 0
     assert need(0, 16, 100, 9728, 0, 0) == need(0, 1, 100, 40000, 0, 1) == need(0, 0, 100, 64, 1, 0) == 0
-    assert need(0, 1, 100, 64, 1, 1) == 4096 + 4 and need(0, 5, 100, 160, 1, 0) == 2 * 4096 + 20
+    assert need(0, 8, 4096, 2560, 1, 0) == need(1, 16, 2048, 2560, 0, 0) == need(1, 64, 512, 64, 1, 1) == 0
+    assert need(0, 1, 100, 64, 1, 1) == 8192 + 4 and need(1, 1, 100, 64, 1, 1) == 4096 + 4 and need(0, 5, 4100, 160, 1, 0) == 4 * 4096 + 20
     assert need(1, 1, 100, 10272, 0, 0) == 81 * 4096 + 4 and need(0, 17, 100, 64, 0, 0) == 2 * 4096 + 68
-    assert need(0, 65, 100, 128, 1, 0) == 8 * 4096 + 260
+    assert need(0, 65, 5000, 128, 1, 0) == 16 * 4096 + 260
 
 
 def test_weight_bytes(lib):
@@ -153,7 +155,7 @@ def test_weights_of_the_host_are_refused():
 
 def test_scale_places_are_one_each():
     """The header's places of a page's 256 scales, each taken once."""
-    k = [((4 * (t // 16) + t % 4) * 4 + r) * 4 + t // 4 % 4 for t in range(64) for r in range(4)]
+    k = [64 * r + t for t in range(64) for r in range(4)]
     v = [64 * r + t // 8 * 8 + 2 * (t % 4) + t // 4 % 2 for t in range(64) for r in range(4)]
     assert sorted(k) == sorted(v) == list(range(256))
     assert PAGE_BYTES_Q4 == 2 * (64 * 64 + 512) == 9216

@@ -4,7 +4,7 @@ and read, against plain computations in 64 bits.
 Tolerances, from the roundings of the operators (u = 2^-11, half a step of fp16; U the output type's half step):
 
 - codes and scales: the format's arithmetic is fp32 division and rounding, which numpy repeats bit for bit.
-- products: xn is rounded to 11 bits (u; x itself where it is fp16 without a norm), its fp32 norm is 2^-20 off, the sums
+- products: xn is rounded to 11 bits at least (u; x itself where it is fp16 without a norm), its fp32 norm is 2^-20 off, the sums
   of in / 4 products a wave (each addition 2^-24) and the waves' are fp32, the output is rounded once:
   ``|err| <= U |y| + (e + (in / 4 + 40) 2^-24) sum|W xn| + 540 2^-24 sum(s |xn|) + 2^-35 max|xn| sum|W|``, e = u + 2^-19
   with a norm, u for bf16 (whose small values fall to denormals: half a step is 2^-25, of inputs held over 16 2^-21, the
@@ -16,7 +16,8 @@ Tolerances, from the roundings of the operators (u = 2^-11, half a step of fp16;
   2^-8 + 2^-17 of amax / 7; a code is within half of the value over the stored scale, moved by
   8 * 2^-19 (the value) + 2^-20 (the quotient); beyond 7.5 it is clamped (a scale is at most 2^-8 too small: 7.03).
 - attention: keys and values are exact operands, each weight is rounded to fp16 (u), a score is off by
-  d = 130 * 2^-24 * sum|q k| / sqrt(128) (fp32 sums; it moves a weight and the sum of weights), an exponential by
+  d = 2^-24 (130 sum|q k| + 540 sum(s |q|)) / sqrt(128) (fp32 sums; the second term: codes held with an offset of 8, 15 at
+  most, give a group's sum of 32 channels and its offset 36 additions; it moves a weight and the sum of weights), an exponential by
   2^-22, a sum over up to 10000 tokens (at most 640 additions one after another in a lane or an accumulator, the joins)
   by 700 * 2^-24 < u / 8, weights below 2^-36 of the largest fall to 0 (10000 of them: 2^-22), and the output is rounded
   once: ``|err| <= u |out| + (u + u / 4 + 2 d) max|v| + 2^-24``.
@@ -174,6 +175,7 @@ PRODUCTS = [
     (1, 48, 40000, torch.float16, True, True), (16, 33, 20000, torch.float16, False, False), (7, 4096, 128, torch.float16, True, False),
     (15, 129, 608, torch.float16, False, True), (31, 2100, 416, torch.bfloat16, True, False), (48, 640, 2560, torch.float16, False, True),
     # the largest calls of one launch, and the next ones
+    (8, 4096, 160, torch.float16, True, False), (8, 4100, 160, torch.bfloat16, True, True), (30, 1040, 96, torch.float16, True, True),
     (4, 48, 2560, torch.bfloat16, True, False), (4, 48, 2592, torch.float16, True, False), (2, 32, 5120, torch.float16, True, True),
     (1, 32, 10240, torch.float16, True, True), (1, 32, 10272, torch.bfloat16, True, True), (16, 528, 288, torch.float16, False, True),
     (17, 8224, 256, torch.float16, False, True), (40, 8300, 256, torch.bfloat16, True, False), (64, 8200, 224, torch.float16, True, False),
@@ -304,7 +306,7 @@ def _held_with_step(lens, counts, hq, hkv, seed):
 
 
 _T, _R = np.arange(64)[:, None], np.arange(4)[None]
-PLACE = (((4 * (_T // 16) + _T % 4) * 4 + _R) * 4 + _T // 4 % 4, 64 * _R + _T // 8 * 8 + 2 * (_T % 4) + _T // 4 % 2)
+PLACE = (64 * _R + _T, 64 * _R + _T // 8 * 8 + 2 * (_T % 4) + _T // 4 % 2)
 
 
 def _bytes(which, slot):
@@ -322,6 +324,8 @@ def _codes(cache, layer, b, n):
     h, out = cache.num_kv_heads, []
     for which in (0, 1):
         c = _unpacked(rows[:, :, 4096 * which:4096 * (which + 1)].reshape(groups, h, GT, 64))
+        if which == 0:  # (K's words 4 j + g and 4 g + j in each other's place)
+            c = c.reshape(groups, h, GT, 4, 4, 8).swapaxes(3, 4).reshape(groups, h, GT, D)
         s = np.ascontiguousarray(rows[:, :, 8192 + 512 * which:8704 + 512 * which]).view(np.float16)[:, :, PLACE[which]]
         out += [c.transpose(0, 2, 1, 3).reshape(groups * GT, h, D)[:n], s.astype(np.float64).transpose(0, 2, 1, 3).reshape(groups * GT, h, 4)[:n]]
     return out
@@ -333,9 +337,9 @@ def _values(cache, layer, b, n):
         return kc * np.repeat(ks, 32, -1), vc * np.repeat(vs, 32, -1)
 
 
-def _attend64(q, k, v, start, gq, u=1.25 * U16):
+def _attend64(q, k, v, ks, start, gq, u=1.25 * U16):
     """Softmax attention of tokens at positions start .. over k, v ``[n, H_kv, 128]`` in 64 bits: output,
-    log-sum-exp and the bound of the module's docstring."""
+    log-sum-exp and the bound of the module's docstring. ks: K's scales ``[n, H_kv, 4]``."""
     m, hq, _ = q.shape
     out, lse, tol = np.zeros((m, hq, D)), np.full((m, hq), -np.inf), np.zeros((m, hq, D))
     for i in range(m):
@@ -347,7 +351,8 @@ def _attend64(q, k, v, start, gq, u=1.25 * U16):
             p = np.exp(s - top)
             out[i, h] = p @ vv / p.sum()
             lse[i, h] = top + np.log(p.sum())
-            d = 130 * 2.0 ** -24 * (np.abs(kk) @ np.abs(q[i, h])).max() / np.sqrt(D)
+            d = 2.0 ** -24 / np.sqrt(D) * (130 * np.abs(kk) @ np.abs(q[i, h])
+                                           + 540 * ks[:n, h // gq] @ np.abs(q[i, h]).reshape(4, 32).sum(1)).max()
             tol[i, h] = U16 * np.abs(out[i, h]) + (u + 2 * d) * np.abs(vv).max() + 2.0 ** -24
     return out, lse, tol
 
@@ -359,7 +364,7 @@ def _check_attention(cache, layer, plan, q, out, lse, starts):
     for b, n in enumerate(plan.counts):
         if n:
             k, v = _values(cache, layer, b, starts[b] + n)
-            want, wl, tol = _attend64(q64[at:at + n], k, v, starts[b], gq)
+            want, wl, tol = _attend64(q64[at:at + n], k, v, _codes(cache, layer, b, starts[b] + n)[1], starts[b], gq)
             err = np.abs(out[at:at + n] - want)
             assert (err <= tol).all(), f"sequence {b}: off by {(err / tol).max():.2f} of the bound"
             if lse is not None:
@@ -603,9 +608,10 @@ def test_groups_without_a_page_take_no_part(counts):
     table = cache.page_table[0].clone()
     cache.page_table[0, 2:4] = cache.page_table[0, 0]  # (any page: its tokens are left out below)
     k, v = _values(cache, 0, 0, lens[0] + counts[0])
+    ks = _codes(cache, 0, 0, lens[0] + counts[0])[1]
     cache.page_table[0] = table
     keep = np.r_[0:128, 256:lens[0] + counts[0]]
-    want, _, tol = _attend64(_f(q)[:counts[0]], k[keep], v[keep], lens[0] - 128, hq // hkv)
+    want, _, tol = _attend64(_f(q)[:counts[0]], k[keep], v[keep], ks[keep], lens[0] - 128, hq // hkv)
     assert (np.abs(_f(out)[:counts[0]] - want) <= tol).all()
 
 
