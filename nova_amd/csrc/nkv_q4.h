@@ -10,7 +10,7 @@
 // 16 g holds row c, columns 32 g .. + 31: word k columns 8 k .. + 7 of those, nibble p code + 8 of column 2 p, nibble
 // p + 4 of column 2 p + 1, so that unpack4 gives them in order. The blocks of a tile of 16 rows follow each other; rows
 // and columns behind the last hold zeros. A wave's load is a block's 1024 bytes in a row: with rows of in / 2 bytes, 16
-// pieces of 64 bytes, the q/k/v product of one token took 6.7 us instead of 4.6 (without its norm).
+// pieces of 64 bytes, the q/k/v product of one token took 6.7 us instead of 5.5.
 //
 // In the cache a row is a token's 128 channels of one KV head, 64 bytes: nibble e of word w holds code + 8 of channel 8 w + e,
 // K's words 4 j + g and 4 g + j in each other's place (j, g < 4), so that 16 bytes hold eight channels of each group.

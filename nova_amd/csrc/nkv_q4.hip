@@ -281,7 +281,7 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
 #pragma unroll
     for (int b = 0; b < 4; ++b) kc[b] = kn[b];
     page = pg.at(t + 1);
-    if (t + 1 < mine) issue(page, sb ^ 1);  // (a whole step ahead: issued after K's products, 45 us instead of NN)
+    if (t + 1 < mine) issue(page, sb ^ 1);  // (a whole step ahead: 64 x 2000 tokens 36 us; issued after K's products 45)
 
     uint8_t* slot = lds + (2 * wave + sb) * Q4_SLOT;
     const uint8_t* ksc = slot + Q4_CODES + 32 * (tail_tid() >> 4 & 3);

@@ -19,6 +19,12 @@ Two ways to run a layer:
   fused into the lm_head GEMV. ``use_decode_kernels(fused_qkv=False)`` splits the attention
   block into the qkv GEMV, the head norms + RoPE, ``update_attend`` and the o_proj GEMV (the
   same bits). The same fp16 roundings as the torch path, up to fp32 summation order.
+  ``use_decode_kernels(weights="q4")`` takes the projections and the lm_head in 4 bits
+  (``nova_amd.q4``): a one-token step is then the q/k/v product behind its norm, the head norms + RoPE,
+  ``update_attend``, o_proj with the residual add, gate/up with SwiGLU behind its norm, down with the residual add.
+
+``forward_chunks`` runs a packed batch's new tokens over a paged cache (``nova_amd.paged``: per-token int8 or
+4-bit pages) in kernel mode, with 4-bit or fp16 weights: prompts' chunks, drafted tokens and decode tokens in one step.
 """
 
 from __future__ import annotations
@@ -141,6 +147,7 @@ class SkeletonLayer(nn.Module):
         self.post_norm = nn.Parameter(torch.ones(cfg.hidden_size, **factory)) if self.mlp is not None else None
         self.w_qkv: torch.Tensor | None = None
         self.w_gate_up: torch.Tensor | None = None
+        self.q4: dict | None = None  # qkv, o, gate_up, down in 4 bits
 
     def forward(self, h, cos, sin, mask, cache):
         h = h + self.attn(_rms(h, self.norm, self.eps), cos, sin, mask, cache)
@@ -156,6 +163,38 @@ class SkeletonLayer(nn.Module):
             if self.mlp is not None:
                 self.w_gate_up = _stack_linears(self.mlp.gate_proj, self.mlp.up_proj)
 
+    def quantize_weights(self) -> None:
+        """The stacked weights in 4 bits, beside the fp16 ones (which prefills still run on)."""
+        from .q4 import quantize_q4
+
+        if self.q4 is None:
+            self.stack_weights()
+            self.q4 = {"qkv": quantize_q4(self.w_qkv), "o": quantize_q4(self.attn.o_proj.weight)}
+            if self.mlp is not None:
+                self.q4 |= {"gate_up": quantize_q4(self.w_gate_up), "down": quantize_q4(self.mlp.down_proj.weight)}
+
+    def _mlp_chunks(self, h: torch.Tensor) -> torch.Tensor:
+        from . import gemv as G
+
+        if self.mlp is None:
+            return h
+        if self.q4 is None:
+            return h + self.mlp(_rms(h, self.post_norm, self.eps))
+        act = G.swiglu_gemv_q4(h, self.q4["gate_up"], self.post_norm, self.eps)
+        return G.rms_gemv_q4(act, self.q4["down"], residual=h, out=h)
+
+    def forward_chunks(self, h: torch.Tensor, cache, plan, inv_freq: torch.Tensor) -> torch.Tensor:
+        """New tokens of a packed batch (``h`` ``[tokens, hidden]``) over a paged cache; returns the new residual stream."""
+        from . import gemv as G
+
+        a, q4 = self.attn, self.q4
+        qkv = (F.linear(_rms(h, self.norm, self.eps), self.w_qkv) if q4 is None
+               else G.rms_gemv_q4(h, q4["qkv"], self.norm, self.eps))
+        q = cache.append_chunks(plan, qkv, a.layer_idx, a.q_norm, a.k_norm, a.cfg.rms_eps, inv_freq)
+        o = cache.attend_chunks(plan, q, a.layer_idx).view(h.shape[0], -1)
+        h = h + a.o_proj(o) if q4 is None else G.rms_gemv_q4(o, q4["o"], residual=h)
+        return self._mlp_chunks(h)
+
     def decode_kernels(self, h: torch.Tensor, cache, pos: torch.Tensor, inv_freq: torch.Tensor,
                        fused_qkv: bool = True) -> torch.Tensor:
         """One decode token (``h`` of ``hidden_size`` elements) through the layer on the HIP
@@ -167,6 +206,12 @@ class SkeletonLayer(nn.Module):
         cfg, a = self.attn.cfg, self.attn
         hq, hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         x = h.reshape(-1)
+        if self.q4 is not None:
+            qkv = G.rms_gemv_q4(x, self.q4["qkv"], self.norm, self.eps)
+            G.qk_norm_rope_(qkv, hq, hkv, a.q_norm, a.k_norm, cfg.rms_eps, inv_freq, pos)
+            q, k, v = qkv.view(1, hq + 2 * hkv, 1, d).split((hq, hkv, hkv), 1)
+            o = cache.update_attend(k, v, q, a.layer_idx)
+            return self._mlp_chunks(G.rms_gemv_q4(o.reshape(-1), self.q4["o"], residual=x)).view(h.shape)
         if fused_qkv and hasattr(cache, "update_attend_block") and hq // hkv <= 4 and x.numel() % 8 == 0 \
                 and x.numel() <= 3072 and hq * d <= 4096:
             # the projection, the head norms + RoPE, the attention step, o_proj and the residual
@@ -261,6 +306,7 @@ class SkeletonForCausalLM(nn.Module):
         factory = {} if device is None else {"device": torch.device(device), "dtype": dtype or torch.float16}
         self.model = SkeletonText(cfg, **factory)
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False, **factory)
+        self.lm_head_q4 = None
         g = torch.Generator(device=factory.get("device", "cpu")).manual_seed(seed)
         with torch.no_grad():
             for p in self.parameters():
@@ -269,9 +315,12 @@ class SkeletonForCausalLM(nn.Module):
                     p.copy_(r.mul_(p.shape[-1] ** -0.5))
                     del r
 
-    def use_decode_kernels(self, on: bool = True, fused_qkv: bool = True) -> "SkeletonForCausalLM":
+    def use_decode_kernels(self, on: bool = True, fused_qkv: bool = True, weights: str = "fp16") -> "SkeletonForCausalLM":
         """Run one-token decode steps on the HIP kernels (fp16 CUDA model, int8 cache); with
-        ``fused_qkv`` each layer's projection, head norms, RoPE and attention step are one launch."""
+        ``fused_qkv`` each layer's projection, head norms, RoPE and attention step are one launch. ``weights``
+        ``"q4"``: the projections and the lm_head of those steps, and of :meth:`forward_chunks`, in 4 bits."""
+        if weights not in ("fp16", "q4"):
+            raise ValueError(f"weights {weights!r}: 'fp16' or 'q4'")
         self.model.fused_qkv = bool(fused_qkv)
         if on:
             w = self.lm_head.weight
@@ -279,6 +328,13 @@ class SkeletonForCausalLM(nn.Module):
                 raise ValueError("use_decode_kernels() needs the model in fp16 on the GPU")
             for layer in self.model.layers:
                 layer.stack_weights()
+                if weights == "q4":
+                    layer.quantize_weights()
+                else:
+                    layer.q4 = None
+            from .q4 import quantize_q4
+
+            self.lm_head_q4 = quantize_q4(w) if weights == "q4" else None
             # the RoPE frequencies as the torch path promotes them (fp16 after ``.half()``)
             self.model.inv_freq32 = self.model.inv_freq.float().contiguous()
         self.model.decode_kernels = bool(on)
@@ -291,9 +347,28 @@ class SkeletonForCausalLM(nn.Module):
         if hidden.shape[:-1].numel() == 1:
             from . import gemv as G
 
+            if self.lm_head_q4 is not None:
+                return G.rms_gemv_q4(hidden.contiguous(), self.lm_head_q4, self.model.norm, self.config.rms_eps)
             logits = G.rms_gemv(hidden.reshape(-1), self.lm_head.weight, self.model.norm, self.config.rms_eps)
             return logits.view(*hidden.shape[:-1], -1)
         return self.lm_head(_rms(hidden, self.model.norm, self.config.rms_eps))
+
+    def forward_chunks(self, input_ids: torch.Tensor, cache, plan) -> torch.Tensor:
+        """The logits ``[tokens, vocab]`` of a packed batch's new tokens ``input_ids`` ``[tokens]`` over a paged cache
+        (``PagedKVInt8TokCache`` or ``PagedKVQ4Cache``; ``plan`` of its ``plan_chunks``), in kernel mode. The caller
+        moves the sequences on (``cache.advance_chunks``)."""
+        if not self.model.decode_kernels:
+            raise RuntimeError("forward_chunks() runs in kernel mode: call use_decode_kernels() first")
+        if input_ids.dim() != 1 or input_ids.shape[0] != plan.total:
+            raise ValueError(f"input_ids must be [{plan.total}], got {tuple(input_ids.shape)}")
+        h = self.model.embed_tokens(input_ids)
+        for layer in self.model.layers:
+            h = layer.forward_chunks(h, cache, plan, self.model.inv_freq32)
+        if self.lm_head_q4 is not None:
+            from . import gemv as G
+
+            return G.rms_gemv_q4(h, self.lm_head_q4, self.model.norm, self.config.rms_eps)
+        return self.lm_head(_rms(h, self.model.norm, self.config.rms_eps))
 
     def forward(self, input_ids, past_key_values=None, attention_mask=None, window_mask=None,
                 cross_mode: str = "off", logits_to_keep: int = 0, position_ids=None):

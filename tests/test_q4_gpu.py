@@ -821,3 +821,102 @@ def test_streams_other_than_the_tensors_own():
     for outs in got:
         for a, b in outs:
             assert torch.equal(a, want) and torch.equal(b, product)
+
+
+# ---------------------------------------------------------------- a decoder
+
+
+def _decoder(cfg):
+    """A decoder whose weights are values of the 4-bit format: the same weights in fp16 and in 4 bits."""
+    from nova_amd.skeleton import SkeletonForCausalLM
+
+    model = SkeletonForCausalLM(cfg, seed=3).half().cuda().eval()
+    with torch.no_grad():
+        for layer in model.model.layers:
+            a, mlp = layer.attn, layer.mlp
+            for lin in (a.q_proj, a.k_proj, a.v_proj, a.o_proj) + (() if mlp is None else (mlp.gate_proj, mlp.up_proj, mlp.down_proj)):
+                lin.weight.copy_(dequantize_q4(quantize_q4(lin.weight.detach())))
+        model.lm_head.weight.copy_(dequantize_q4(quantize_q4(model.lm_head.weight.detach())))
+    return model
+
+
+def _apart(a, b):
+    return float((a.float() - b.float()).norm() / b.float().norm())
+
+
+def _config(**more):
+    from nova_amd.skeleton import SkeletonConfig
+
+    return SkeletonConfig(**(dict(num_hidden_layers=3, num_attention_heads=8, num_key_value_heads=2, hidden_size=512, intermediate_size=992,
+                                  vocab_size=300) | more))
+
+
+@pytest.mark.parametrize("paged, bound", [(PagedKVInt8TokCache, 1e-2), (PagedKVQ4Cache, 0.125)])
+def test_a_decoder_over_packed_batches(paged, bound):
+    """Prompts, drafts and single tokens through forward_chunks with the weights in fp16 and in 4 bits, the same values. Some
+    ten roundings a layer differ, by 2^-11 / sqrt(3) of the value each: over three layers 2e-3 of the logits' norm, five
+    times that allowed. Behind them an 8-bit code turns for 2% of the channels, by 1 / 127 of the largest one: nothing.
+    A 4-bit code's step is a seventh of the largest channel, 2.5 / 7 = 0.36 of the rms. Inputs off by d of their rms turn
+    0.8 d / 0.36 of the codes by 0.36: keys and values off by sqrt(0.29 d). The first layer's inputs are the same and its
+    products off by 2^-11 / sqrt(3): d = 3e-4, 0.01 behind it. The second layer's are off by 0.01 then: 0.054 behind it; the third's
+    by 0.054 at most: 0.125. (That the first bound stood at 0.03 was a mistake: it took the first layer's d for all three.)"""
+    cfg = _config()
+    model = _decoder(cfg)
+    with pytest.raises(ValueError):
+        model.use_decode_kernels(weights="q3")
+    counts, prompts = [5, 1, 70], [40, 3, 0]
+    g = torch.Generator().manual_seed(5)
+    ids = [torch.randint(0, cfg.vocab_size, (p + 3 * n,), generator=g).cuda() for p, n in zip(prompts, counts)]
+    logits = {}
+    for weights in ("fp16", "q4"):
+        model.use_decode_kernels(weights=weights)
+        cache = paged(3, 2, D, 8, 3, 40, 12)
+        at, logits[weights] = [0, 0, 0], []
+        with torch.inference_mode():
+            for step in range(4):
+                now = prompts if step == 0 else counts
+                tokens = torch.cat([x[a:a + n] for x, a, n in zip(ids, at, now)])
+                plan = cache.plan_chunks(now)
+                logits[weights].append(model.forward_chunks(tokens, cache, plan))
+                cache.advance_chunks(plan)
+                at = [a + n for a, n in zip(at, now)]
+    with pytest.raises(ValueError):
+        model.forward_chunks(tokens[:-1], cache, plan)
+    model.use_decode_kernels(False)
+    with pytest.raises(RuntimeError):
+        model.forward_chunks(tokens, cache, plan)
+    for a, b in zip(logits["q4"], logits["fp16"]):
+        assert a.shape == b.shape and a.shape[1] == cfg.vocab_size
+        assert _apart(a, b) < bound
+
+
+@pytest.mark.parametrize("intermediate", [992, 0])
+def test_a_decoder_of_single_tokens(intermediate):
+    """One-token steps over the int8 cache, captured, eager and with fp16 weights of the same values (the bound: above)."""
+    from nova_amd.decode import GraphDecoder
+
+    cfg = _config(intermediate_size=intermediate)
+    model = _decoder(cfg)
+    ids = torch.randint(0, cfg.vocab_size, (1, 100), generator=torch.Generator().manual_seed(9)).cuda()
+    fed = torch.randint(0, cfg.vocab_size, (6, 1, 1), generator=torch.Generator().manual_seed(10)).cuda()
+    logits = {}
+    for weights, captured in (("fp16", True), ("q4", True), ("q4", False)):
+        model.use_decode_kernels(weights=weights)
+        dec = GraphDecoder(model, max_len=256, quant="int8")
+        dec.prefill(ids)
+        if captured:
+            dec.capture(warmup=2)
+        logits[weights, captured] = []
+        for token in fed:
+            dec.input_ids.copy_(token)
+            if captured:
+                dec.step()
+                out = dec.logits
+            else:
+                with torch.inference_mode():
+                    out = dec._body()
+            logits[weights, captured].append(out.clone())
+    model.use_decode_kernels(False)
+    for plain, replayed, eager in zip(*logits.values()):
+        assert torch.equal(replayed, eager)
+        assert replayed.shape == plain.shape and _apart(replayed, plain) < 1e-2
