@@ -854,10 +854,12 @@ int nkv_swiglu_gemv_q4(const void* x, int dtype, int64_t tokens, const void* gam
 /*
  * The paged cache in 4 bits: a page is 64 tokens of one KV head, 9216 bytes: K codes [64][64 bytes], V codes, K scales,
  * V scales (256 fp16 each; token t, channels 32 r .. + 31: K at 64 r + t, V at 64 r + t / 8 * 8 + 2 (t % 4) + t / 4 % 2).
- * Bits 4 e .. + 3 of a row's 32-bit word w hold code + 8 of channel 8 w + e, in K's rows of channel 8 (w / 4 + 4 (w % 4)) + e. pages, tables, batches and plans as for the per-token symmetric pages:
+ * Bits 4 e .. + 3 of a row's 32-bit word w hold code + 8 of channel 8 w + e, in K's rows of channel 8 (w / 4 + 4 (w % 4)) + e.
+ * pages, tables, batches and plans as for the per-token symmetric pages:
  * nkv_paged_quantize_q4 as nkv_paged_quantize_tok, nkv_paged_append_chunks_q4 as nkv_paged_append_chunks_tok,
- * nkv_paged_attn_chunks_q4 as nkv_paged_attn_chunks_tok (wide: the largest kind of a unit), nkv_paged_read_q4 as nkv_paged_read_tok. In the attention keys
- * and values are exact operands; the softmax's weights and the output are rounded to fp16.
+ * nkv_paged_attn_chunks_q4 as nkv_paged_attn_chunks_tok (wide: the largest kind of a unit; parts at most
+ * 2^15), nkv_paged_read_q4 as nkv_paged_read_tok. In the attention keys and values are exact operands; the softmax's weights
+ * and the output are rounded to fp16.
  */
 int nkv_paged_quantize_q4(const void* x, int x_dtype, int64_t x_head_stride, int64_t hkv, int64_t n, int which,
                           uint8_t* pages, const int32_t* table_row, int64_t first_token, int64_t num_pages, void* stream);

@@ -165,21 +165,18 @@ def _parts_q4(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, w
     most = np.minimum(MAX_PARTS, np.maximum(1, steps // SMALL_PART))
     round_us = np.array(ALONE_Q4)[slow]
     us = rounds * round_us
-    best = None
-    for cut in CUTS if len(steps) * hkv < 32 * CUS else CUTS[:1]:  # (far more tiles than slots are not cut)
-        parts = np.clip(np.ceil(us * (cut / us.max())).astype(np.int64), 1, most)
-        alone = -(-rounds // parts)
-        # all of it over the CUs, as far as the units fill them evenly
-        k = int(parts.sum()) * hkv / CUS
-        uneven = 1.1 * max(1.0, int(np.ceil(k - 0.1)) / k) if k <= 2.1 else 1.2 + 0.03 * k
-        total = float((alone * np.array(SHARED_Q4)[slow] * parts).sum()) * hkv / CUS
-        time = START_Q4[int(slow.max())] + max(float((alone * round_us).max()), total * uneven)
-        cut_rows = int(np.where(parts > 1, parts, 0) @ rows) * hkv
-        if cut_rows:
-            time += MERGE_Q4 + MERGE_PART_Q4 * int(parts.max()) + cut_rows * PARTIAL_US
-        if best is None or time < best[0]:
-            best = time, parts
-    return best[1]
+    # (far more tiles than slots are not cut)
+    cuts = np.array(CUTS if len(steps) * hkv < 32 * CUS else CUTS[:1])[:, None]
+    parts = np.clip(np.ceil(us * (cuts / us.max())).astype(np.int64), 1, most)
+    alone = -(-rounds // parts)
+    # all of it over the CUs, as far as the units fill them evenly
+    k = parts.sum(1) * (hkv / CUS)
+    uneven = np.where(k <= 2.1, 1.1 * np.maximum(1.0, np.ceil(k - 0.1) / k), 1.2 + 0.03 * k)
+    total = (alone * np.array(SHARED_Q4)[slow] * parts).sum(1) * (hkv / CUS)
+    cut_rows = (np.where(parts > 1, parts, 0) @ rows) * hkv
+    merges = np.where(cut_rows > 0, MERGE_Q4 + MERGE_PART_Q4 * parts.max(1) + cut_rows * PARTIAL_US, 0.0)
+    time = START_Q4[int(slow.max())] + np.maximum((alone * round_us).max(1), total * uneven) + merges
+    return parts[time.argmin()]
 
 
 def _packed(counts: list[int]) -> tuple[np.ndarray, np.ndarray]:

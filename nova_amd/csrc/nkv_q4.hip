@@ -184,6 +184,11 @@ __device__ __forceinline__ uint4 load_global16(const uint8_t* p, bool once) {
   return uint4{v.x, v.y, v.z, v.w};
 }
 
+// n part / parts, without the 64-bit division that it looks like (parts: 2^15 at most).
+__device__ __forceinline__ int cut_at(int n, int part, int parts) {
+  return n / parts * part + n % parts * part / parts;
+}
+
 // W: waves of the workgroup.
 template <int RB, int W>
 __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u, int h, uint8_t* lds) {
@@ -192,8 +197,8 @@ __device__ __forceinline__ void attend4_small(const ChunkArgs& a, const Unit& u,
   const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
   const int fresh = a.b.cu[u.seq + 1] - a.b.cu[u.seq];  // the sequence's new tokens
   // (whole rounds of the waves, so that no wave idles in a part's last one)
-  const int64_t rounds = (at.steps + W - 1) / W;
-  const int64_t s0 = rounds * u.part / u.parts * W, s1 = min(rounds * (u.part + 1) / u.parts * W, at.steps);
+  const int rounds = (int)((at.steps + W - 1) / W);
+  const int64_t s0 = (int64_t)cut_at(rounds, u.part, u.parts) * W, s1 = min((int64_t)cut_at(rounds, u.part + 1, u.parts) * W, at.steps);
   const uint8_t* pages = a.pages + (int64_t)h * PAGE_Q4_BYTES;
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_Q4_BYTES;
 
@@ -434,7 +439,7 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const TileAt at = tile_at(a, u.seq, u.row0, u.rows);
-  const int s0 = (int)(at.steps * u.part / u.parts), n = (int)(at.steps * (u.part + 1) / u.parts) - s0;
+  const int s0 = cut_at((int)at.steps, u.part, u.parts), n = cut_at((int)at.steps, u.part + 1, u.parts) - s0;
   const int64_t len = at.start + (a.b.cu[u.seq + 1] - a.b.cu[u.seq]);
   const uint8_t* pages = a.pages + (int64_t)h * PAGE_Q4_BYTES;
   const int64_t page_stride = (int64_t)a.b.hkv * PAGE_Q4_BYTES;
@@ -492,6 +497,9 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
     *reinterpret_cast<half8_t*>(vt + 8192) = unpack4(vw.y, vb, bias);
   };
 
+  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
+  issue(p0, 0);
+  issue(p1, 1);
   const int row0 = u.row0 + wave * (WD_RB * 16);  // first row of this wave
   const int rows = u.row0 + at.rows;
   half8_t qb[WD_RB][4];
@@ -508,9 +516,6 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
       qb[rb][k] = paired(w);
     }
   }
-  int p0 = pg.at(0), p1 = pg.at(1), p2 = pg.at(2), p3 = pg.at(3);  // the pages of steps t .. t + 3
-  issue(p0, 0);
-  issue(p1, 1);
   Sum4 st[WD_RB];
 #pragma unroll
   for (int rb = 0; rb < WD_RB; ++rb) init(st[rb]);
@@ -648,7 +653,8 @@ __device__ __forceinline__ void attend4_wide(const ChunkArgs& a, const Unit& u, 
 }
 
 __device__ __forceinline__ bool unit_ok(const ChunkArgs& a, const Unit& u, int most) {
-  return u.seq >= 0 && u.seq < a.b.nseq && u.row0 >= 0 && u.rows > 0 && u.rows <= most && u.part >= 0 && u.part < u.parts && u.slot >= 0;
+  return u.seq >= 0 && u.seq < a.b.nseq && u.row0 >= 0 && u.rows > 0 && u.rows <= most && u.part >= 0 && u.part < u.parts &&
+         u.parts <= (1 << 15) && u.slot >= 0;
 }
 
 __global__ __launch_bounds__(Q4_THREADS, 1) void attn_q4_kernel(ChunkArgs a) {

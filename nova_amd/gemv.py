@@ -11,6 +11,8 @@ the library is missing: there is no torch fallback here.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -121,10 +123,15 @@ def _q4_args(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None, n_out: in
     return x.numel() // n_in, out
 
 
+@functools.lru_cache(maxsize=4096)  # (the sizes decide; 1 of a call's 7.5 us on the host)
+def _q4_bytes(*sizes: int) -> int:
+    return _lib.load().nkv_gemv_q4_workspace_bytes(*sizes)
+
+
 def _q4_scratch(x: torch.Tensor, tokens: int, n_out: int, n_in: int, gamma: torch.Tensor | None,
                 swiglu: bool) -> tuple[int | None, int]:
     """Memory of the call's own for the normalized input, where one launch does not make it itself."""
-    n = _lib.load().nkv_gemv_q4_workspace_bytes(_DT[x.dtype], tokens, n_out, n_in, gamma is not None, swiglu)
+    n = _q4_bytes(_DT[x.dtype], tokens, n_out, n_in, gamma is not None, swiglu)
     return (_lib.scratch(x.device, n).data_ptr(), n) if n else (None, 0)
 
 
