@@ -7,7 +7,7 @@
 // with one rounding at the end. Bound by the weights' bytes, and by a launch's chain of loads that wait for each other.
 //
 // Three forms, by the tokens and by what is to be done to x:
-// - product4_few_kernel: up to 4 tokens with a norm (or bf16), one launch;
+// - product4_few_kernel: up to 4 tokens with a norm (or bf16), more for small weights (few_each), one launch;
 // - product4_kernel: up to 16 tokens of fp16 as they are, one launch;
 // - product4_many_kernel: the rest, after xn_kernel has laid xn out as the products take it.
 
@@ -527,11 +527,13 @@ __global__ __launch_bounds__(64 * W, 8 / W) void product4_many_kernel(ProductArg
 // ---------------------------------------------------------------- host side
 
 // How many waves share a token in product4_few_kernel; 0: another form is taken. (Gates and ups must be in tiles of their own.)
-// More than 4 tokens take several passes over the weight, in the same launch: where their workgroups do not fill the card twice
-// that is less than the launch of xn (NN).
+// Passes of 4 tokens, all in one launch, are less than the launch of xn as long as their workgroups do not fill the card
+// (us, passes / xn and product: 5 to 16 tokens over 1024 x 2560 7.2 / 7.4 fp16, 6.1 / 6.9 bf16; over 512 x 1024 4.7 / 5.9 and
+// 4.2 / 5.5; over 2560 x 2560, 320 workgroups and more, 9.2 / 7.5 and 7.5 / 6.9). One product's worth, 2 tokens in two parts or 4
+// in one, always is: 4 bf16 tokens over 6144 x 2560 7.5 / 8.1; with two products (fp16) 9.3 / 8.8.
 int few_each(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
   if ((gated && out % 16) || (!norm && dtype == NKV_F16)) return 0;
-  if (tokens > 4 && cdiv(tokens, 4) * cdiv(out, 16) > 2 * CUS) return 0;
+  if (tokens * parts_of(dtype, true) > 4 && cdiv(tokens, 4) * cdiv(out, 16) > CUS) return 0;
   const int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
   return cdiv(in, PB) * PB <= each * FEW_KX * 512 ? each : 0;
 }

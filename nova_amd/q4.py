@@ -22,7 +22,7 @@ from .kvquant import _DT
 GROUP = 32
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Q4Weight:
     """A weight ``[out_features, in_features]`` in 4 bits, as ``quantize_q4`` lays it out: ``data`` uint8 in blocks of 16 rows
     and 128 columns, each 1024 bytes of codes and 64 fp16 scales (``nkv_quantize_q4``)."""

@@ -167,11 +167,11 @@ class SkeletonLayer(nn.Module):
         """The stacked weights in 4 bits, beside the fp16 ones (which prefills still run on)."""
         from .q4 import quantize_q4
 
-        if self.q4 is None:
-            self.stack_weights()
-            self.q4 = {"qkv": quantize_q4(self.w_qkv), "o": quantize_q4(self.attn.o_proj.weight)}
-            if self.mlp is not None:
-                self.q4 |= {"gate_up": quantize_q4(self.w_gate_up), "down": quantize_q4(self.mlp.down_proj.weight)}
+        self.stack_weights()
+        q4 = {"qkv": quantize_q4(self.w_qkv), "o": quantize_q4(self.attn.o_proj.weight)}
+        if self.mlp is not None:
+            q4 |= {"gate_up": quantize_q4(self.w_gate_up), "down": quantize_q4(self.mlp.down_proj.weight)}
+        self.q4 = q4
 
     def _mlp_chunks(self, h: torch.Tensor) -> torch.Tensor:
         from . import gemv as G
@@ -318,9 +318,13 @@ class SkeletonForCausalLM(nn.Module):
     def use_decode_kernels(self, on: bool = True, fused_qkv: bool = True, weights: str = "fp16") -> "SkeletonForCausalLM":
         """Run one-token decode steps on the HIP kernels (fp16 CUDA model, int8 cache); with
         ``fused_qkv`` each layer's projection, head norms, RoPE and attention step are one launch. ``weights``
-        ``"q4"``: the projections and the lm_head of those steps, and of :meth:`forward_chunks`, in 4 bits."""
+        ``"q4"``: the projections and the lm_head of those steps, and of :meth:`forward_chunks`, in 4 bits, made of the
+        fp16 weights as they are now."""
         if weights not in ("fp16", "q4"):
             raise ValueError(f"weights {weights!r}: 'fp16' or 'q4'")
+        cfg = self.config
+        if on and weights == "q4" and (cfg.hidden_size % 32 or cfg.intermediate_size % 32):
+            raise ValueError(f"hidden size {cfg.hidden_size}, intermediate size {cfg.intermediate_size}: 4-bit weights need multiples of 32")
         self.model.fused_qkv = bool(fused_qkv)
         if on:
             w = self.lm_head.weight
@@ -353,6 +357,7 @@ class SkeletonForCausalLM(nn.Module):
             return logits.view(*hidden.shape[:-1], -1)
         return self.lm_head(_rms(hidden, self.model.norm, self.config.rms_eps))
 
+    @torch.no_grad()
     def forward_chunks(self, input_ids: torch.Tensor, cache, plan) -> torch.Tensor:
         """The logits ``[tokens, vocab]`` of a packed batch's new tokens ``input_ids`` ``[tokens]`` over a paged cache
         (``PagedKVInt8TokCache`` or ``PagedKVQ4Cache``; ``plan`` of its ``plan_chunks``), in kernel mode. The caller

@@ -2,10 +2,14 @@
 
 from __future__ import annotations
 
+import random
+
+import numpy as np
 import pytest
 import torch
 
 from nova_amd import _lib
+from nova_amd import chunks as C
 from nova_amd import gemv as G
 from nova_amd import q4
 from nova_amd.paged import PAGE_BYTES_Q4
@@ -71,9 +75,10 @@ def test_product_workspace(lib):
     their own, few workgroups if passes), or where x is taken as it is; else xn in tiles of 16 tokens and blocks of 128 inputs
     (in two parts for a norm of fp16), and a word a token."""
     need = lib.nkv_gemv_q4_workspace_bytes
-    assert need(0, 4, 100000, 2560, 1, 0) == need(1, 2, 100, 5120, 1, 0) == need(0, 1, 160, 10240, 1, 1) == need(1, 3, 16, 32, 0, 1) == 0
+    assert need(1, 4, 100000, 2560, 1, 0) == need(0, 2, 100000, 2560, 1, 0) == need(1, 2, 100, 5120, 1, 0) == need(0, 1, 160, 10240, 1, 1) == need(1, 3, 16, 32, 0, 1) == 0
     assert need(0, 16, 100, 9728, 0, 0) == need(0, 1, 100, 40000, 0, 1) == need(0, 0, 100, 64, 1, 0) == 0
-    assert need(0, 8, 4096, 2560, 1, 0) == need(1, 16, 2048, 2560, 0, 0) == need(1, 64, 512, 64, 1, 1) == 0
+    assert need(0, 8, 2048, 2560, 1, 0) == need(1, 16, 1024, 2560, 0, 0) == need(1, 64, 256, 64, 1, 1) == 0
+    assert need(0, 3, 4112, 128, 1, 0) == 2 * 4096 + 12 and need(0, 8, 2049, 128, 1, 0) == need(1, 9, 1376, 256, 1, 0) - 4 == 2 * 4096 + 32
     assert need(0, 1, 100, 64, 1, 1) == 8192 + 4 and need(1, 1, 100, 64, 1, 1) == 4096 + 4 and need(0, 5, 4100, 160, 1, 0) == 4 * 4096 + 20
     assert need(1, 1, 100, 10272, 0, 0) == 81 * 4096 + 4 and need(0, 17, 100, 64, 0, 0) == 2 * 4096 + 68
     assert need(0, 65, 5000, 128, 1, 0) == 16 * 4096 + 260
@@ -168,3 +173,45 @@ def test_values_are_fp16_numbers():
     s = s[7 * s.double() <= 65504].double()
     for c in range(8):
         assert torch.equal((c * s).to(torch.float16).double(), c * s)
+
+
+def _batches():
+    rng = random.Random(11)
+    yield [0], [1], 1, 1
+    yield [63, 64, 65], [1, 1, 1], 4, 8
+    yield [131000] * 4, [1] * 4, 4, 2
+    yield [8192], [51], 4, 8  # 204 rows: one tile of 256
+    yield [8192], [50], 4, 8  # 200: seven of 32
+    yield [1500, 4097, 700, 0, 6000, 3333], [384, 1, 129, 257, 5, 1], 4, 8
+    yield [0, 0], [0, 0], 4, 8
+    for _ in range(60):
+        n = rng.randint(1, 40)
+        yield ([rng.choice([0, rng.randint(0, 9000), rng.randint(0, 200000)]) for _ in range(n)],
+               [rng.choice([0, 1, 4, rng.randint(1, 60), rng.randint(1, 700)]) for _ in range(n)], rng.choice([1, 2, 3, 4, 5, 7, 8, 16]),
+               rng.choice([1, 2, 4, 8]))
+
+
+@pytest.mark.parametrize("starts,counts,gq,hkv", list(_batches()))
+def test_units_of_the_4_bit_cache(starts, counts, gq, hkv):
+    """Each row and part once, the parts' slots apart, their rows merged once; tiles of 256 rows only beyond 200."""
+    units, merges, slots = C.plan_units(starts, counts, gq, hkv, q4=True)
+    rows_of, used, cut = {}, [], {}
+    for seq, row0, rows, part, parts, slot, kind, alone in units.tolist():
+        assert 0 <= part < parts <= C.MAX_PARTS and 0 < rows <= C.TILE_ROWS[kind] and alone == (rows == counts[seq] * gq)
+        assert (kind == C.ROWS256) == (counts[seq] * gq > C.BIG_FROM_Q4)
+        rows_of.setdefault(seq, []).extend((row, part, parts) for row in range(row0, row0 + rows))
+        if parts > 1:
+            used.extend(range(slot + part * rows, slot + (part + 1) * rows))
+            cut[seq, row0] = rows, parts, slot
+    for b, n in enumerate(counts):
+        got = rows_of.get(b, [])
+        assert len(got) == len(set(got)) and {r for r, _, _ in got} == set(range(n * gq))
+        of_row = {}
+        for row, part, parts in got:
+            of_row.setdefault((row, parts), []).append(part)
+        assert len(of_row) == n * gq and all(sorted(p) == list(range(parts)) for (_, parts), p in of_row.items())
+    assert sorted(used) == list(range(slots))
+    first = np.concatenate(([0], np.cumsum(counts)))
+    want = {(first[seq], row0 + r, parts, slot + r, rows) for (seq, row0), (rows, parts, slot) in cut.items() for r in range(rows)}
+    got = [(f, row0 + r, parts, slot + r, stride) for f, row0, rows, parts, slot, stride, _, _ in merges.tolist() for r in range(rows)]
+    assert len(got) == len(set(got)) and set(got) == want

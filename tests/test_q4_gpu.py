@@ -872,14 +872,13 @@ def test_a_decoder_over_packed_batches(paged, bound):
         model.use_decode_kernels(weights=weights)
         cache = paged(3, 2, D, 8, 3, 40, 12)
         at, logits[weights] = [0, 0, 0], []
-        with torch.inference_mode():
-            for step in range(4):
-                now = prompts if step == 0 else counts
-                tokens = torch.cat([x[a:a + n] for x, a, n in zip(ids, at, now)])
-                plan = cache.plan_chunks(now)
-                logits[weights].append(model.forward_chunks(tokens, cache, plan))
-                cache.advance_chunks(plan)
-                at = [a + n for a, n in zip(at, now)]
+        for step in range(4):
+            now = prompts if step == 0 else counts
+            tokens = torch.cat([x[a:a + n] for x, a, n in zip(ids, at, now)])
+            plan = cache.plan_chunks(now)
+            logits[weights].append(model.forward_chunks(tokens, cache, plan))
+            cache.advance_chunks(plan)
+            at = [a + n for a, n in zip(at, now)]
     with pytest.raises(ValueError):
         model.forward_chunks(tokens[:-1], cache, plan)
     model.use_decode_kernels(False)
@@ -920,3 +919,81 @@ def test_a_decoder_of_single_tokens(intermediate):
     for plain, replayed, eager in zip(*logits.values()):
         assert torch.equal(replayed, eager)
         assert replayed.shape == plain.shape and _apart(replayed, plain) < 1e-2
+
+
+class _NoCache:
+    """The caller's cache of a prompt that is all there is."""
+
+    pos = torch.zeros(1, dtype=torch.int64)
+
+    def update(self, k, v, layer):
+        return k, v
+
+
+def test_packed_steps_are_the_torch_layers():
+    """forward_chunks over the int8 cache against the torch layers over whole prompts. A cached value is off by 2.5 to 3 rms / 127 /
+    sqrt(12) = 0.0066 of its rms: so are a score (by that much, the query's rms being 1) and what the weights gather, 0.0093 a
+    layer together, 0.016 over three; twice that, and the roundings (above), are allowed."""
+    cfg = _config()
+    model = _decoder(cfg)
+    lens = [40, 3, 131, 1]
+    ids = [torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(20 + n)).cuda() for n in lens]
+    _NoCache.pos = _NoCache.pos.cuda()
+    with torch.no_grad():
+        want = [model(x[None], past_key_values=_NoCache())[0] for x in ids]
+    model.use_decode_kernels()
+    cache = PagedKVInt8TokCache(3, 2, D, 8, 4, 40, 12)
+    got = [[] for _ in ids]
+    for at, now in (([0, 0, 0, 0], [30, 2, 64, 0]), ([30, 2, 64, 0], [10, 1, 67, 1])):
+        plan = cache.plan_chunks(now)
+        out = model.forward_chunks(torch.cat([x[a:a + n] for x, a, n in zip(ids, at, now)]), cache, plan)
+        cache.advance_chunks(plan)
+        for b, part in enumerate(out.split(now)):
+            got[b].append(part)
+    for w, g in zip(want, got):
+        assert _apart(torch.cat(g), w) < 0.034
+
+
+def test_weights_are_quantized_as_they_are_now():
+    cfg = _config(num_hidden_layers=1)
+    model = _decoder(cfg).use_decode_kernels(weights="q4")
+    with torch.no_grad():
+        model.model.layers[0].attn.v_proj.weight.neg_()
+        model.lm_head.weight.mul_(2)
+    model.use_decode_kernels(weights="q4")
+    layer = model.model.layers[0]
+    assert torch.equal(dequantize_q4(layer.q4["qkv"]), layer.w_qkv) and torch.equal(dequantize_q4(model.lm_head_q4), model.lm_head.weight)
+    with pytest.raises(ValueError):
+        _decoder_of(hidden_size=500)
+
+
+def _decoder_of(**more):
+    from nova_amd.skeleton import SkeletonForCausalLM
+
+    return SkeletonForCausalLM(_config(**more), seed=3).half().cuda().use_decode_kernels(weights="q4")
+
+
+# where one form of the product ends and the next begins (256 workgroups of passes; two tokens' parts in one product)
+EDGES = [(3, 4096, 96, torch.float16), (3, 4112, 96, torch.float16), (4, 4112, 96, torch.bfloat16), (8, 2048, 160, torch.float16),
+         (8, 2064, 160, torch.bfloat16), (9, 1360, 224, torch.float16), (9, 1376, 224, torch.float16), (2, 4112, 96, torch.float16)]
+
+
+@pytest.mark.parametrize("tokens,n_out,n_in,dtype", EDGES)
+def test_products_at_the_edges_of_their_forms(tokens, n_out, n_in, dtype):
+    x, gamma = _randn((tokens, n_in), 150 + tokens, dtype=dtype).cuda(), (1 + _randn((n_in,), 151, 0.2, torch.float32)).to(dtype).cuda()
+    w = quantize_q4(_randn((n_out, n_in), 152, 0.05, dtype).cuda())
+    _check_product(x, w, gamma, 1e-6, None, G.rms_gemv_q4(x, w, gamma))
+    if n_out % 32 == 0:
+        _check_product(x, w, gamma, 1e-6, None, G.swiglu_gemv_q4(x, w, gamma), gated=True)
+
+
+def test_a_step_without_tokens():
+    cache = _held_with_step([70, 0], [0, 0], 8, 2, 160)
+    before = cache.pages[0].clone()
+    plan = cache.plan_chunks([0, 0])
+    q = cache.append_chunks(plan, torch.zeros(0, 12 * D, dtype=torch.float16, device="cuda"), 0)
+    assert q.shape == (0, 8, D) and cache.attend_chunks(plan, q, 0).shape == (0, 8, D)
+    assert torch.equal(cache.pages[0], before)
+    w = quantize_q4(_randn((48, 64), 161).cuda())
+    x = torch.zeros(0, 64, dtype=torch.float16, device="cuda")
+    assert G.rms_gemv_q4(x, w).shape == (0, 48) and G.swiglu_gemv_q4(x, w).shape == (0, 24)
