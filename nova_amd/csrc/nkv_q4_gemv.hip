@@ -583,19 +583,30 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   const auto go = [&](auto kernel, int tiles_wg, int waves) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(tiles, tiles_wg), passes), dim3(64 * waves), 0, s, a);
   };
-  // Rows a wave takes, and waves of a workgroup (us, with xn's launch; 17 / 32 / 48 / 64 tokens): 6144 x 2560 as two tiles of
-  // 16 rows and 8 waves 9.1 / 9.5 / 10.9 / 11.8, as one tile 10.5 / 10.8 / 12.6 / 13.6; 2560 x 4096 10.7 / 11.3 / 13.7 /
-  // 15.2 and 8.9 / 9.2 / 11.1 / 12.4: two where the workgroups still fill the card. Gates and ups (2 x 9728 x 2560, one tile of
-  // each) as 8 waves 15.1 / 15.5 / 21.0 / 24.0, as 4 waves 16.3 / 16.7 / 19.3 / 21.3: the sums of more tokens take registers.
+  // Tiles of 16 rows that a workgroup takes, and its waves: each tile more reads xn that much less often (from the L2: what
+  // bounds these calls), as long as the workgroups fill the card. us, with xn's launch, 17 / 32 / 48 / 64 tokens:
+  // 2560 x 4096 as one tile 8.9 / 9.2 / 11.1 / 12.4, as two 10.7 / 11.3 / 13.7 / 15.2; 6144 x 2560 as one 10.5 / 10.8 / 12.6 /
+  // 13.6, as two 9.1 / 9.5 / 10.9 / 11.8; 10240 x 2560 fp16 as two 16.7 / 17.4 / 21.8 / 24.7, as three 12.9 / 13.7 / 16.4 /
+  // 18.3; 16384 x 2560 as two 17.7 / 18.4 / 22.8, as four 15.2 / 16.3 / 19.8; 32000 x 2560 29.1 / 30.1 / 38.3 and 24.2 /
+  // 25.6 / 32.5 (bf16 19.4 / 20.2 / 29.2 / 32.7 and 20.8 / 21.3 / 26.2 / 28.4). 64 tokens in two parts have no
+  // registers for four.
+  // Gates and ups, up to 32 tokens: three tiles of each where that is one round of workgroups (17 tokens, as one / as three:
+  // 9728 of 2560 fp16 22.0 / 17.5, bf16 14.9 / 14.5; 11008 of 4096 31.6 / 24.5 and 22.3 / 20.6) or where xn is as much as four
+  // operands (18944 of 2560 fp16 33.9 / 29.7; bf16 22.4 / 25.0). More tokens' sums take the registers: one tile of each, 4
+  // waves (48 and 64 tokens over 9728 of 2560, bf16 19.3 / 21.3; as 8 waves 21.0 / 24.0).
   const auto pass = [&](auto n, auto p) {
     constexpr int NT = decltype(n)::value, P = decltype(p)::value;
-    if constexpr (GATED) {
-      if constexpr (NT <= 2) go(product4_many_kernel<DT, P, 2, NT, true, 8, 3>, 1, 8);
-      else go(product4_many_kernel<DT, P, 2, NT, true, 4, 5>, 1, 4);
-    } else if (tiles >= CUS) {
-      go(product4_many_kernel<DT, P, 2, NT, false, 8, 3>, 2, 8);
+    if constexpr (GATED && NT > 2) {
+      go(product4_many_kernel<DT, P, 2, NT, true, 4, 5>, 1, 4);
+    } else if constexpr (GATED) {
+      if (tiles > 2 * CUS && (tiles <= 3 * CUS || P * NT == 4)) go(product4_many_kernel<DT, P, 6, NT, true, 8, 2>, 3, 8);
+      else go(product4_many_kernel<DT, P, 2, NT, true, 8, 3>, 1, 8);
     } else {
-      go(product4_many_kernel<DT, P, 1, NT, false, 8, 5>, 1, 8);
+      if constexpr (P * NT < 8)
+        if (tiles > 3 * CUS) return go(product4_many_kernel<DT, P, 4, NT, false, 8, 2>, 4, 8);
+      if (tiles > 2 * CUS && tiles <= 3 * CUS) go(product4_many_kernel<DT, P, 3, NT, false, 8, 2>, 3, 8);
+      else if (tiles >= CUS) go(product4_many_kernel<DT, P, 2, NT, false, 8, 3>, 2, 8);
+      else go(product4_many_kernel<DT, P, 1, NT, false, 8, 5>, 1, 8);
     }
   };
   const auto with_tiles = [&](auto p) {

@@ -975,7 +975,13 @@ def _decoder_of(**more):
 
 # where one form of the product ends and the next begins (256 workgroups of passes; two tokens' parts in one product)
 EDGES = [(3, 4096, 96, torch.float16), (3, 4112, 96, torch.float16), (4, 4112, 96, torch.bfloat16), (8, 2048, 160, torch.float16),
-         (8, 2064, 160, torch.bfloat16), (9, 1360, 224, torch.float16), (9, 1376, 224, torch.float16), (2, 4112, 96, torch.float16)]
+         (8, 2064, 160, torch.bfloat16), (9, 1360, 224, torch.float16), (9, 1376, 224, torch.float16), (2, 4112, 96, torch.float16),
+         # tiles of a workgroup: 513 to 768 tiles of 16 rows three, more four (two of 64 tokens in two parts)
+         (17, 8192, 96, torch.float16), (17, 8208, 160, torch.float16), (33, 12288, 96, torch.bfloat16), (50, 8230, 64, torch.float16),
+         (64, 12304, 96, torch.float16), (40, 12304, 96, torch.float16), (64, 12310, 160, torch.bfloat16), (10, 12320, 64, torch.float16),
+         # .. and of gates and ups, of half as many outputs
+         (5, 16416, 96, torch.bfloat16), (20, 24576, 64, torch.float16), (20, 24608, 64, torch.bfloat16), (32, 24608, 96, torch.float16),
+         (16, 24608, 64, torch.float16), (20, 16394, 64, torch.float16)]
 
 
 @pytest.mark.parametrize("tokens,n_out,n_in,dtype", EDGES)
@@ -983,7 +989,7 @@ def test_products_at_the_edges_of_their_forms(tokens, n_out, n_in, dtype):
     x, gamma = _randn((tokens, n_in), 150 + tokens, dtype=dtype).cuda(), (1 + _randn((n_in,), 151, 0.2, torch.float32)).to(dtype).cuda()
     w = quantize_q4(_randn((n_out, n_in), 152, 0.05, dtype).cuda())
     _check_product(x, w, gamma, 1e-6, None, G.rms_gemv_q4(x, w, gamma))
-    if n_out % 32 == 0:
+    if n_out % 2 == 0:
         _check_product(x, w, gamma, 1e-6, None, G.swiglu_gemv_q4(x, w, gamma), gated=True)
 
 
