@@ -24,6 +24,7 @@ namespace {
 constexpr int PB = 128;       // inputs of a block: four products deep
 constexpr int P_IN = 1 << 20;  // inputs, at most
 constexpr int64_t P_TOKENS = (int64_t(1) << 20) - 16;
+constexpr int XCDS = 8;       // workgroups are dealt to them in turn
 
 struct ProductArgs {
   const uint8_t* x;        // [tokens][in]
@@ -471,7 +472,8 @@ __global__ __launch_bounds__(64 * W, W == 16 ? 1 : 8 / W) void product4_kernel(P
 // ---------------------------------------------------------------- many tokens
 //
 // xn lies as operands (xn_kernel): a wave's loads of it are 1024 bytes in a row, from the XCD's L2 where the workgroups of
-// other rows have it, too.
+// other rows have it, too. A pass is 16 NT tokens; the passes of the same rows are dealt to one XCD, next to each other, so
+// that all but the first find the weights in its L2 (64 tokens over 2560 x 9728 in passes of 16: 25.2 us, so 20.9).
 
 template <int DT, int P, int RT, int NT, bool GATED, int W, int AHEAD>
 __global__ __launch_bounds__(64 * W, 8 / W) void product4_many_kernel(ProductArgs a) {
@@ -479,12 +481,15 @@ __global__ __launch_bounds__(64 * W, 8 / W) void product4_many_kernel(ProductArg
   __shared__ __attribute__((aligned(16))) float red[red_floats(NT, GATED, W)];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t t0 = (int64_t)blockIdx.y * (16 * NT);
+  const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x;  // (gridDim.x: a multiple of the XCDs)
+  const uint32_t pass = (id / XCDS) % gridDim.y, rows = id / (XCDS * gridDim.y) * XCDS + id % XCDS;
+  const int64_t t0 = (int64_t)pass * (16 * NT);
   const int nt = (int)min<int64_t>(16 * NT, a.tokens - t0), blocks = (a.in + PB - 1) / PB;
-  const int64_t o0 = (int64_t)blockIdx.x * (16 * Weights<RT, GATED, W, AHEAD>::TILES);
+  const int64_t o0 = (int64_t)rows * (16 * Weights<RT, GATED, W, AHEAD>::TILES);
+  if (o0 >= a.out) return;
 
   half8_t b[4][XT];  // the next block's
-  const uint8_t* xp = a.x + (int64_t)blockIdx.y * XT * blocks * 4096 + 16 * lane;
+  const uint8_t* xp = a.x + (int64_t)pass * XT * blocks * 4096 + 16 * lane;
   auto load_x = [&](int kb, int k) {
 #pragma unroll
     for (int n = 0; n < XT; ++n) b[k][n] = *reinterpret_cast<const half8_t*>(xp + ((int64_t)(4 * kb + k) * XT + n) * 1024);
@@ -537,13 +542,39 @@ int few_each(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool
   const int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
   return cdiv(in, PB) * PB <= each * FEW_KX * 512 ? each : 0;
 }
-// The token tiles of a pass of product4_many_kernel.
-int pass_tiles(int64_t tokens) { return (int)std::min<int64_t>(cdiv(tokens, 16), 4); }
+// A cut of product4_many_kernel's work: the token tiles of a pass, and the tiles of 16 outputs of a workgroup.
+struct Cut {
+  int nt, rt;
+};
+// A workgroup's time goes with the operands that it makes of the codes and those of xn that it loads (from the L2, which is
+// what it waits for), rt + parts nt a step; the launch's with that and the rounds of workgroups. us, xn's launch among it, 17 /
+// 32 / 48 / 64 tokens, (nt, rt): 2560 x 9728 (2, 1) 16.3 / 16.8, (3, 1) 20.8, (1, 2) 16.3 / 16.9 / 17.4 / 24, (2, 2) 19.3 / 20.0 /
+// 20.0 / 20.6, (4, 1) 23.4, (1, 4) 22.4 / 23.0 / 23.4 / 23.7; 6144 x 2560 fp16 (2, 2) 11.0 / 11.4, (1, 3) 10.4 / 10.7, (3, 2) 13.8,
+// (2, 3) 12.4 / 12.7 / 13.1 / 13.9, (4, 2) 15.7; 10240 x 2560 fp16 with rt 2 16.7 / 17.4 / 21.8 / 24.7, with 3 12.9 / 13.7 /
+// 16.4 / 18.3; 16384 x 2560 with 2 17.7 / 18.4 / 22.8, with 4 15.2 / 16.3 / 19.8. (32000 x 2560 bf16 with 2 19.4 / 20.2 / 29.2
+// / 32.7, with 4 20.8 / 21.3 / 26.2 / 28.4: there the weights' bytes count, too.) Of the same the one with fewer passes.
+// Gates and ups: three tiles of each, up to 32 tokens, where that is one round of workgroups (17 tokens, as one / as three:
+// 9728 of 2560 fp16 22.0 / 17.5, bf16 14.9 / 14.5; 11008 of 4096 31.6 / 24.5 and 22.3 / 20.6) or where xn is as much as four
+// operands (18944 of 2560 fp16 33.9 / 29.7; bf16 22.4 / 25.0). More tokens' sums take the registers: one tile of each.
+Cut many_cut(int parts, int64_t tokens, int64_t out, bool gated) {
+  const int64_t tiles = cdiv(out, 16), t16 = cdiv(tokens, 16);
+  const int most = (int)std::min<int64_t>(t16, 4);
+  if (gated) return {most, most <= 2 && tiles > 2 * CUS && (tiles <= 3 * CUS || parts * most == 4) ? 3 : 1};
+  Cut best = {0, 0};
+  int64_t least = 0;
+  for (int nt = most; nt >= 1; --nt)
+    for (int rt = 1; rt <= 4; ++rt) {
+      if (parts * nt == 8 && rt == 4) continue;  // (no registers for it)
+      const int64_t time = cdiv(cdiv(tiles, rt) * cdiv(t16, nt), CUS) * (rt + parts * nt);
+      if (best.nt == 0 || time < least) best = {nt, rt}, least = time;
+    }
+  return best;
+}
 
 int64_t product_workspace(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
   if (few_each(dtype, tokens, out, in, norm, gated) || (tokens <= 16 && dtype == NKV_F16 && !norm)) return 0;
-  const int64_t passes = cdiv(tokens, 16 * pass_tiles(tokens));
-  return passes * pass_tiles(tokens) * cdiv(in, PB) * 4096 * parts_of(dtype, norm) + 4 * tokens;
+  const int parts = parts_of(dtype, norm), nt = many_cut(parts, tokens, out, gated).nt;
+  return cdiv(tokens, 16 * nt) * nt * cdiv(in, PB) * 4096 * parts + 4 * tokens;
 }
 
 template <int DT, bool GATED>
@@ -571,7 +602,8 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   const int64_t need = product_workspace(DT, a.tokens, a.out, a.in, norm, GATED);
   if (!ws || ws_bytes < need)
     return fail(NKV_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
-  const int nt = pass_tiles(a.tokens);
+  const Cut cut = many_cut(parts_of(DT, norm), a.tokens, a.out, GATED);
+  const int nt = cut.nt;
   float* unit = reinterpret_cast<float*>(ws + need - 4 * a.tokens);
   const dim3 each_token((unsigned)a.tokens);
   if (parts_of(DT, norm) == 2) hipLaunchKernelGGL((xn_kernel<DT, 2>), each_token, dim3(256), 0, s, a, nt, ws, unit);
@@ -579,34 +611,24 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   if (int rc = check_launch(what)) return rc;
   a.x = ws;
   a.unit = unit;
-  const unsigned passes = (unsigned)cdiv(a.tokens, 16 * nt);
-  const auto go = [&](auto kernel, int tiles_wg, int waves) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(tiles, tiles_wg), passes), dim3(64 * waves), 0, s, a);
+  const int64_t passes = cdiv(a.tokens, 16 * nt), groups = cdiv(cdiv(tiles, cut.rt), XCDS) * XCDS;
+  if (groups * passes >= (int64_t(1) << 31))
+    return fail(NKV_ERR_INVALID, "%s: sizes out=%lld tokens=%lld (less than 2^31 workgroups)", what, (long long)a.out, (long long)a.tokens);
+  const auto go = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)passes), dim3(64 * waves), 0, s, a);
   };
-  // Tiles of 16 rows that a workgroup takes, and its waves: each tile more reads xn that much less often (from the L2: what
-  // bounds these calls), as long as the workgroups fill the card. us, with xn's launch, 17 / 32 / 48 / 64 tokens:
-  // 2560 x 4096 as one tile 8.9 / 9.2 / 11.1 / 12.4, as two 10.7 / 11.3 / 13.7 / 15.2; 6144 x 2560 as one 10.5 / 10.8 / 12.6 /
-  // 13.6, as two 9.1 / 9.5 / 10.9 / 11.8; 10240 x 2560 fp16 as two 16.7 / 17.4 / 21.8 / 24.7, as three 12.9 / 13.7 / 16.4 /
-  // 18.3; 16384 x 2560 as two 17.7 / 18.4 / 22.8, as four 15.2 / 16.3 / 19.8; 32000 x 2560 29.1 / 30.1 / 38.3 and 24.2 /
-  // 25.6 / 32.5 (bf16 19.4 / 20.2 / 29.2 / 32.7 and 20.8 / 21.3 / 26.2 / 28.4). 64 tokens in two parts have no
-  // registers for four.
-  // Gates and ups, up to 32 tokens: three tiles of each where that is one round of workgroups (17 tokens, as one / as three:
-  // 9728 of 2560 fp16 22.0 / 17.5, bf16 14.9 / 14.5; 11008 of 4096 31.6 / 24.5 and 22.3 / 20.6) or where xn is as much as four
-  // operands (18944 of 2560 fp16 33.9 / 29.7; bf16 22.4 / 25.0). More tokens' sums take the registers: one tile of each, 4
-  // waves (48 and 64 tokens over 9728 of 2560, bf16 19.3 / 21.3; as 8 waves 21.0 / 24.0).
   const auto pass = [&](auto n, auto p) {
     constexpr int NT = decltype(n)::value, P = decltype(p)::value;
-    if constexpr (GATED && NT > 2) {
-      go(product4_many_kernel<DT, P, 2, NT, true, 4, 5>, 1, 4);
+    if constexpr (GATED && NT > 2) {  // (as 4 waves 19.3 and 21.3 us of 48 and 64 tokens, as 8 21.0 and 24.0)
+      go(product4_many_kernel<DT, P, 2, NT, true, 4, 5>, 4);
     } else if constexpr (GATED) {
-      if (tiles > 2 * CUS && (tiles <= 3 * CUS || P * NT == 4)) go(product4_many_kernel<DT, P, 6, NT, true, 8, 2>, 3, 8);
-      else go(product4_many_kernel<DT, P, 2, NT, true, 8, 3>, 1, 8);
+      if (cut.rt == 3) go(product4_many_kernel<DT, P, 6, NT, true, 8, 2>, 8);
+      else go(product4_many_kernel<DT, P, 2, NT, true, 8, 3>, 8);
     } else {
-      if constexpr (P * NT < 8)
-        if (tiles > 3 * CUS) return go(product4_many_kernel<DT, P, 4, NT, false, 8, 2>, 4, 8);
-      if (tiles > 2 * CUS && tiles <= 3 * CUS) go(product4_many_kernel<DT, P, 3, NT, false, 8, 2>, 3, 8);
-      else if (tiles >= CUS) go(product4_many_kernel<DT, P, 2, NT, false, 8, 3>, 2, 8);
-      else go(product4_many_kernel<DT, P, 1, NT, false, 8, 5>, 1, 8);
+      if (cut.rt == 1) return go(product4_many_kernel<DT, P, 1, NT, false, 8, 5>, 8);
+      if (cut.rt == 2) return go(product4_many_kernel<DT, P, 2, NT, false, 8, 3>, 8);
+      if (cut.rt == 3) return go(product4_many_kernel<DT, P, 3, NT, false, 8, 2>, 8);
+      if constexpr (P * NT < 8) go(product4_many_kernel<DT, P, 4, NT, false, 8, 2>, 8);
     }
   };
   const auto with_tiles = [&](auto p) {

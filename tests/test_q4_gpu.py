@@ -981,7 +981,11 @@ EDGES = [(3, 4096, 96, torch.float16), (3, 4112, 96, torch.float16), (4, 4112, 9
          (64, 12304, 96, torch.float16), (40, 12304, 96, torch.float16), (64, 12310, 160, torch.bfloat16), (10, 12320, 64, torch.float16),
          # .. and of gates and ups, of half as many outputs
          (5, 16416, 96, torch.bfloat16), (20, 24576, 64, torch.float16), (20, 24608, 64, torch.bfloat16), (32, 24608, 96, torch.float16),
-         (16, 24608, 64, torch.float16), (20, 16394, 64, torch.float16)]
+         (16, 24608, 64, torch.float16), (20, 16394, 64, torch.float16),
+         # passes of 16 to 64 tokens of one, two, three and four tiles of outputs, with and without rest
+         (48, 2560, 320, torch.bfloat16), (49, 2500, 320, torch.bfloat16), (64, 2560, 256, torch.float16), (100, 1030, 96, torch.float16),
+         (40, 6144, 96, torch.float16), (128, 2100, 160, torch.bfloat16), (200, 400, 96, torch.float16), (150, 16640, 64, torch.bfloat16),
+         (130, 8200, 64, torch.float16), (257, 20, 64, torch.bfloat16)]
 
 
 @pytest.mark.parametrize("tokens,n_out,n_in,dtype", EDGES)
