@@ -113,7 +113,11 @@ def plan_units(starts, counts, gq: int, hkv: int, q4: bool = False) -> tuple[np.
     part = np.arange(len(tile)) - np.repeat(np.cumsum(parts) - parts, parts)
     slots = np.where(parts > 1, parts * have, 0)
     slot = np.cumsum(slots) - slots
-    cost = (steps * np.where(kind == ROWS256, STEP_US, GROUP_US) / parts)[tile]  # (only its order counts)
+    if q4 and wide:
+        rounds, round_us, start = _wide_q4(steps, kind)
+        cost = (rounds * round_us / parts + start)[tile]
+    else:
+        cost = (steps * np.where(kind == ROWS256, STEP_US, GROUP_US) / parts)[tile]  # (only its order counts)
     alone = (n_tiles[seq] == 1).astype(np.int64)
     units = np.stack([seq[tile], row0[tile], have[tile], part, parts[tile], slot[tile], kind[tile], alone[tile]], 1)
     units = units[np.argsort(-cost, kind="stable")]
@@ -149,17 +153,20 @@ def _parts(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide
 # The 4-bit pages: rows from which tiles are ROWS256 (all as ROWS256 / as ROWS32): 96 rows over 32000 tokens 46 / 41 us, 8 times
 # 128 rows over 4000 47 / 42, 200 rows over 8000 30 / 27; and, in launches of small units (ROWS16, ROWS32), what they take in
 # us: a round of four waves alone on a CU, and beside another workgroup there; a unit's start and end; the second launch, and
-# each part of its longest row. (With wide tiles _parts' prices hold: a step of 1.9 and a unit's start and end of 10.)
+# each part of its longest row.
 BIG_FROM_Q4 = 200
 ALONE_Q4, SHARED_Q4, START_Q4 = (1.6, 2.35), (1.5, 2.0), (5.0, 7.0)
 MERGE_Q4, MERGE_PART_Q4 = 3.0, 0.1
+# Launches with wide tiles, by kind: a round of eight waves or a wide tile's step, and a unit's start and end.
+WIDE_STEP_Q4, WIDE_START_Q4 = (2.5, 3.2, 1.9), (7.0, 8.0, 10.0)
+WIDE_CUTS_Q4 = (1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 8, 12, 16, 24, 32, 64, 128, 256)
 
 
 def _parts_q4(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, wide: bool) -> np.ndarray:
     """:func:`_parts` for 4-bit pages: the least time among the same cuts, by what their units were measured at. Of 20 batches (1 to 64
     sequences of 1 to 50 rows over 500 to 131000 tokens, prompts and chunks) 18 get a cut within 7% of the best, all within 12%."""
     if wide:
-        return _parts(steps, kind, rows, hkv, wide)
+        return _parts_q4_wide(steps, kind, rows, hkv)
     slow = (kind == ROWS32).astype(np.int64)
     rounds = -(-steps // 4)
     most = np.minimum(MAX_PARTS, np.maximum(1, steps // SMALL_PART))
@@ -176,6 +183,35 @@ def _parts_q4(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int, w
     cut_rows = (np.where(parts > 1, parts, 0) @ rows) * hkv
     merges = np.where(cut_rows > 0, MERGE_Q4 + MERGE_PART_Q4 * parts.max(1) + cut_rows * PARTIAL_US, 0.0)
     time = START_Q4[int(slow.max())] + np.maximum((alone * round_us).max(1), total * uneven) + merges
+    return parts[time.argmin()]
+
+
+def _wide_q4(steps: np.ndarray, kind: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """In a launch with wide tiles: each tile's rounds (of eight waves; a wide tile's steps), a round's price, the start's."""
+    return np.where(kind == ROWS256, steps, -(-steps // 8)), np.array(WIDE_STEP_Q4)[kind], np.array(WIDE_START_Q4)[kind]
+
+
+def _parts_q4_wide(steps: np.ndarray, kind: np.ndarray, rows: np.ndarray, hkv: int) -> np.ndarray:
+    """The same for launches with wide tiles, one workgroup a CU, the longest units first: where they are up to twice the CUs, the
+    shortest follow the units that end first. Of 17 batches (prompts and chunks, alone and beside up to 40 sequences of 1 to
+    4 rows) 15 get a cut within 4% of the best, all within 14%; by _parts' prices 12 sequences of 8000 tokens beside a prompt
+    take 49 us instead of 33, one of 30000 33 instead of 21."""
+    small = kind != ROWS256
+    rounds, round_us, start = _wide_q4(steps, kind)
+    us = rounds * round_us
+    most = np.minimum(MAX_PARTS, np.where(small, np.maximum(1, steps // SMALL_PART), steps))
+    longest = int((us + start).argmax())
+    cuts = np.array(WIDE_CUTS_Q4 if len(steps) * hkv < 16 * CUS else WIDE_CUTS_Q4[:1])[:, None]
+    target = np.maximum(us[longest] / cuts + start[longest] - start, 1.0)
+    parts = np.clip(np.ceil(us / target - 1e-9).astype(np.int64), 1, most)
+    unit = np.where(small, -(-rounds // parts), rounds / parts) * round_us + start
+    n, last = parts.sum(1) * hkv, unit.max(1)
+    cut_rows = (np.where(parts > 1, parts, 0) @ rows) * hkv
+    merges = np.where(cut_rows > 0, MERGE_US + cut_rows * PARTIAL_US, 0.0)
+    time = np.maximum(last, (unit * parts).sum(1) * (hkv / CUS)) + np.where(n > 2 * CUS, unit.min(1), 0.0) + merges
+    for c in np.nonzero((n > CUS) & (n <= 2 * CUS))[0]:
+        each = np.sort(np.repeat(unit[c], parts[c] * hkv))[::-1]
+        time[c] = max(time[c], (each[CUS:] + each[2 * CUS - n[c]:CUS][::-1]).max() + merges[c])
     return parts[time.argmin()]
 
 
