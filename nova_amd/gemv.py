@@ -7,6 +7,9 @@ the projection that produces it, SwiGLU (``LeanMLP``, src/nova/layers.py:173-174
 gate/up projection, and the q/k head norms plus RoPE into one launch. Each function takes
 fp16 CUDA tensors and the caller's preallocated ``out`` (graph capture), and raises when
 the library is missing: there is no torch fallback here.
+
+``rms_gemv_q4`` and ``swiglu_gemv_q4`` are the same projections with 4-bit weights (``nova_amd.q4``), for any number of
+tokens in fp16 or bf16.
 """
 
 from __future__ import annotations
