@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from .chunks import launch, overlap
+from .chunks import launch
 from .kvquant import _DT
 from .q4 import Q4Weight
 
@@ -101,28 +101,28 @@ def _q4_args(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None, n_out: in
     """The checked arguments of a product: the number of tokens and the output."""
     if not isinstance(w, Q4Weight):
         raise ValueError("w must be a Q4Weight (nova_amd.q4.quantize_q4)")
-    n_in, dev = w.shape[1], w.data.device
-    if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() == 0 or x.shape[-1] != n_in or x.device != dev:
-        raise ValueError(f"x must be fp16 / bf16 [.., {n_in}] on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    n_in, dev, dtype, shape = w.shape[1], w.data.device, x.dtype, x.shape
+    if dtype not in (torch.float16, torch.bfloat16) or not shape or shape[-1] != n_in or x.device != dev:
+        raise ValueError(f"x must be fp16 / bf16 [.., {n_in}] on {dev}, got {tuple(shape)} {dtype} on {x.device}")
     if not x.is_contiguous() or x.data_ptr() % 16:
         raise ValueError("x must be contiguous and 16-byte aligned")
-    if gamma is not None and (gamma.dtype != x.dtype or gamma.shape != (n_in,) or gamma.device != dev
+    if gamma is not None and (gamma.dtype != dtype or gamma.shape != (n_in,) or gamma.device != dev
                               or not gamma.is_contiguous() or gamma.data_ptr() % 16):
-        raise ValueError(f"gamma must be a contiguous, 16-byte aligned {x.dtype} tensor of {n_in} elements on {dev}")
-    shape = (*x.shape[:-1], n_out)
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != shape or residual.device != dev
+        raise ValueError(f"gamma must be a contiguous, 16-byte aligned {dtype} tensor of {n_in} elements on {dev}")
+    shape = (*shape[:-1], n_out)
+    if residual is not None and (residual.dtype != dtype or residual.shape != shape or residual.device != dev
                                  or not residual.is_contiguous()):
-        raise ValueError(f"residual must be a contiguous {x.dtype} tensor {list(shape)} on {dev}")
+        raise ValueError(f"residual must be a contiguous {dtype} tensor {list(shape)} on {dev}")
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(shape)
     else:
-        if out.dtype != x.dtype or out.shape != shape or out.device != dev or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {x.dtype} tensor {list(shape)} on {dev}")
-        for name, t in (("x", x), ("gamma", gamma), ("w", w.data)):
-            if t is not None and overlap(out, t):
+        if out.dtype != dtype or out.shape != shape or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {dtype} tensor {list(shape)} on {dev}")
+        first = out.data_ptr()
+        end = first + out.nbytes
+        for name, t in (("x", x), ("gamma", gamma), ("w", w.data), ("residual, unless it is the same", residual)):
+            if t is not None and first < (at := t.data_ptr()) + t.nbytes and at < end and not (t is residual and at == first):
                 raise ValueError(f"out must not overlap {name}")
-        if residual is not None and residual.data_ptr() != out.data_ptr() and overlap(out, residual):
-            raise ValueError("out must be residual itself or not overlap it")
     return x.numel() // n_in, out
 
 
