@@ -19,20 +19,27 @@ namespace {
 // ---------------------------------------------------------------- append
 
 // The sum of a 16-lane row's squares in pairs of neighbours: four of a lane's values one after another, then their
-// sums, the lanes', .. ; each product and sum rounded.
+// sums, the lanes', .. ; each product and sum rounded (not contracted).
 __device__ __forceinline__ float squares_in_pairs(const float (&v)[8]) {
+#pragma clang fp contract(off)
   float s[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    s[h] = __fmul_rn(v[4 * h], v[4 * h]);
+    s[h] = v[4 * h] * v[4 * h];
 #pragma unroll
-    for (int e = 1; e < 4; ++e) s[h] = __fadd_rn(s[h], __fmul_rn(v[4 * h + e], v[4 * h + e]));
+    for (int e = 1; e < 4; ++e) s[h] = s[h] + v[4 * h + e] * v[4 * h + e];
   }
-  float x = __fadd_rn(s[0], s[1]);
-  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, false)));
-  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, false)));
-  x = __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, false)));  // half mirror
-  return __fadd_rn(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, false)));  // mirror
+  float x = s[0] + s[1];
+  x = x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, false));
+  x = x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, false));
+  x = x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, false));  // half mirror
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, false));  // mirror
+}
+// v c + o s, each product and the sum rounded.
+__device__ __forceinline__ float turned(float v, float c, float o, float s) {
+#pragma clang fp contract(off)
+  const float a = v * c, b = o * s;
+  return a + b;
 }
 
 // The value of lane l ^ 8 of the same 16-lane row (a rotation by 8).
@@ -154,10 +161,9 @@ __global__ __launch_bounds__(256) void append_chunks_kernel(AppendArgs a) {
       if (rotate) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float other = __fmul_rn(row16_other_half(v[e]), sn[e]);
-          // (Q4: each product rounded, as the elementary operations are)
-          if constexpr (F == Q4) v[e] = __fadd_rn(__fmul_rn(v[e], cs[e]), other);
-          else v[e] = __builtin_fmaf(v[e], cs[e], other);
+          const float other = row16_other_half(v[e]);
+          if constexpr (F == Q4) v[e] = turned(v[e], cs[e], other, sn[e]);  // (as the elementary operations are)
+          else v[e] = __builtin_fmaf(v[e], cs[e], other * sn[e]);
         }
       }
     }
