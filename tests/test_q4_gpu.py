@@ -1007,3 +1007,57 @@ def test_a_step_without_tokens():
     w = quantize_q4(_randn((48, 64), 161).cuda())
     x = torch.zeros(0, 64, dtype=torch.float16, device="cuda")
     assert G.rms_gemv_q4(x, w).shape == (0, 48) and G.swiglu_gemv_q4(x, w).shape == (0, 24)
+
+
+def test_a_captured_decoder_step_follows_the_sequences():
+    """forward_chunks with 4-bit weights over 4-bit pages, captured once and replayed as the sequences grow, with eager steps
+    of a second cache between."""
+    cfg = _config(num_hidden_layers=2)
+    model = _decoder(cfg).use_decode_kernels(weights="q4")
+    prompts, counts = [100, 7, 0], [1, 3, 1]
+    gen = torch.Generator().manual_seed(31)
+    caches = [PagedKVQ4Cache(2, 2, D, 8, 3, 20, 6) for _ in range(2)]
+    first = torch.randint(0, cfg.vocab_size, (sum(prompts),), generator=gen).cuda()
+    for cache in caches:
+        plan = cache.plan_chunks(prompts)
+        model.forward_chunks(first, cache, plan)
+        cache.advance_chunks(plan)
+        for b in range(3):
+            cache.reserve(b, prompts[b] + 40)
+    plans = [cache.plan_chunks(counts) for cache in caches]
+    tokens = torch.zeros(sum(counts), dtype=torch.int64, device="cuda")
+    before = [p.clone() for p in caches[0].pages]
+
+    def step():
+        logits = model.forward_chunks(tokens, caches[0], plans[0])
+        caches[0].pos[:3].add_(plans[0].new)
+        return logits
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()  # (loads what a capture may not)
+    torch.cuda.current_stream().wait_stream(side)
+    caches[0].pos[:3] = torch.tensor(prompts, device="cuda")
+    for page, held in zip(caches[0].pages, before):
+        page.copy_(held)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for r in range(5):
+        tokens.copy_(torch.randint(0, cfg.vocab_size, tokens.shape, generator=gen).cuda())
+        graph.replay()
+        caches[0].note_chunks(plans[0])
+        want = model.forward_chunks(tokens, caches[1], plans[1])
+        caches[1].advance_chunks(plans[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), r
+        assert all(torch.equal(a, b) for a, b in zip(caches[0].pages, caches[1].pages)) and torch.equal(caches[0].pos, caches[1].pos)
+
+
+@pytest.mark.parametrize("tokens", [1000, 2500])
+def test_products_of_many_tokens(tokens):
+    x, gamma = _randn((tokens, 160), 170, dtype=torch.float16).cuda(), (1 + _randn((160,), 171, 0.2, torch.float32)).half().cuda()
+    w = quantize_q4(_randn((80, 160), 172, 0.05).cuda())
+    _check_product(x, w, gamma, 1e-6, None, G.rms_gemv_q4(x, w, gamma))
+    _check_product(x, w, gamma, 1e-6, None, G.swiglu_gemv_q4(x, w, gamma), gated=True)
