@@ -230,7 +230,7 @@ __device__ __forceinline__ void finish(const ProductArgs& a, const float4_t (&ac
 
 // ---------------------------------------------------------------- a few tokens: one launch
 //
-// Passes of 4 tokens, which leave most of a product's 16 columns free: column 4 t + j takes token t's group j of a block alone (its
+// Passes of up to 4 tokens, which leave most of a product's 16 columns free: column 4 t + j takes token t's group j of a block alone (its
 // other inputs are 0), so that a group's sum comes out by itself and the scales are applied to it, 4 products' results
 // instead of 32 operands. The codes then need no arithmetic: n = code + 8 is an fp16 denormal, n 2^-24 (a nibble at the
 // mantissa's end) or 16 n 2^-24 (the next one; its inputs are held over 16), which the matrix cores take as they are: 5
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(64 * FEW_W, RT == 1 ? 4 : 3) void product4_few_kern
   __shared__ __attribute__((aligned(16))) uint4 zeros[4];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t t0 = 4 * (int64_t)blockIdx.y;
-  const int nt = (int)min<int64_t>(4, a.tokens - t0), n8 = a.in / 8, blocks = (a.in + PB - 1) / PB;
+  const int64_t t0 = W / each * (int64_t)blockIdx.y;
+  const int nt = (int)min<int64_t>(W / each, a.tokens - t0), n8 = a.in / 8, blocks = (a.in + PB - 1) / PB;
   const int token = wave / each, at0 = 64 * (wave % each) + lane;  // this lane's chunks: at0 + 64 each k
 
   Raw8<DT> xr[KX], gr[KX];
@@ -531,17 +531,26 @@ __global__ __launch_bounds__(64 * W, 8 / W) void product4_many_kernel(ProductArg
 
 // ---------------------------------------------------------------- host side
 
-// How many waves share a token in product4_few_kernel; 0: another form is taken. (Gates and ups must be in tiles of their own.)
-// Passes of 4 tokens, all in one launch, are less than the launch of xn as long as their workgroups do not fill the card
+// How many waves share a token in product4_few_kernel, whose pass is 4 / each tokens; 0: another form is taken. (Gates and ups
+// must be in tiles of their own.)
+// Passes, all in one launch, are less than the launch of xn as long as their workgroups do not fill the card
 // (us, passes / xn and product: 5 to 16 tokens over 1024 x 2560 7.2 / 7.4 fp16, 6.1 / 6.9 bf16; over 512 x 1024 4.7 / 5.9 and
 // 4.2 / 5.5; over 2560 x 2560, 320 workgroups and more, 9.2 / 7.5 and 7.5 / 6.9). One product's worth, 2 tokens in two parts or 4
-// in one, always is: 4 bf16 tokens over 6144 x 2560 7.5 / 8.1; with two products (fp16) 9.3 / 8.8.
+// in one, always is: 4 bf16 tokens over 6144 x 2560 7.5 / 8.1; with two products (fp16) 9.3 / 8.8. More inputs than a token's
+// waves hold take more waves a token, and passes of fewer: of two 7.9 / 8.6 (fp16, 4 tokens over 1000 x 4096; bf16 7.4 / 7.9),
+// of one 14.0 / 15.9 and 12.1 / 13.7 (fp16, 512 x 9728 and 1024 x 8192; bf16 13.2 / 13.1, 11.4 / 11.7, and 333 x 9728 14.4 / 13.2:
+// not for bf16).
 int few_each(int dtype, int64_t tokens, int64_t out, int64_t in, bool norm, bool gated) {
   if ((gated && out % 16) || (!norm && dtype == NKV_F16)) return 0;
-  if (tokens * parts_of(dtype, true) > 4 && cdiv(tokens, 4) * cdiv(out, 16) > CUS) return 0;
-  const int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
-  return cdiv(in, PB) * PB <= each * FEW_KX * 512 ? each : 0;
+  int each = tokens == 1 ? 4 : tokens == 2 ? 2 : 1;
+  while (each < 4 && cdiv(in, PB) * PB > each * FEW_KX * 512) each *= 2;
+  if (cdiv(in, PB) * PB > each * FEW_KX * 512) return 0;
+  const int64_t pass = 4 / each, passes = cdiv(tokens, pass);
+  const int parts = parts_of(dtype, true);
+  if (parts == 1 && pass == 1 && tokens > 1) return 0;
+  return (passes == 1 && tokens * parts <= 4) || passes * cdiv(out, 16) <= CUS ? each : 0;
 }
+
 // A cut of product4_many_kernel's work: the token tiles of a pass, and the tiles of 16 outputs of a workgroup.
 struct Cut {
   int nt, rt;
@@ -584,11 +593,12 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   const int64_t tiles = cdiv(a.out, 16);
   const bool norm = a.gamma != nullptr;
   if (const int each = few_each(DT, a.tokens, a.out, a.in, norm, GATED)) {
-    const size_t xn = std::min<int64_t>(a.tokens, 4) * (parts_of(DT, true) * (2 * blocks * PB + 16 + 16 * blocks));
+    const int64_t pass = std::min<int64_t>(a.tokens, FEW_W / each);
+    const size_t xn = pass * (parts_of(DT, true) * (2 * blocks * PB + 16 + 16 * blocks));
     const size_t lds = std::max(xn, (size_t)4 * red_floats(1, GATED, FEW_W));
-    const dim3 grid((unsigned)tiles, (unsigned)cdiv(a.tokens, 4)), block(64 * FEW_W);
+    const dim3 grid((unsigned)tiles, (unsigned)cdiv(a.tokens, FEW_W / each)), block(64 * FEW_W);
     constexpr int P = parts_of(DT, true);
-    if (a.tokens <= 2) hipLaunchKernelGGL((product4_few_kernel<DT, R1, 1>), grid, block, lds, s, a, each);
+    if (pass <= 2) hipLaunchKernelGGL((product4_few_kernel<DT, R1, 1>), grid, block, lds, s, a, each);
     else hipLaunchKernelGGL((product4_few_kernel<DT, R1, P>), grid, block, lds, s, a, each);
     return check_launch(what);
   }

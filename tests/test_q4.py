@@ -63,7 +63,7 @@ def _swiglu(lib, **kw):
     (dict(out=0), INVALID), (dict(out=1 << 27), INVALID), (dict(n_in=0), INVALID), (dict(n_in=40), INVALID),
     (dict(n_in=(1 << 20) + 32), INVALID), (dict(x=None), INVALID), (dict(w4=None), INVALID),
     (dict(y=None), INVALID), (dict(x=PTR + 2), UNSUPPORTED), (dict(w4=PTR + 8), UNSUPPORTED), (dict(gamma=PTR + 2), UNSUPPORTED),
-    (dict(ws=PTR + 8), UNSUPPORTED), (dict(tokens=17, n_in=2592, gamma=PTR), INVALID), (dict(tokens=17, dtype=1, n_in=2592, ws=PTR, ws_bytes=42 * 4096 + 67), INVALID),
+    (dict(ws=PTR + 8), UNSUPPORTED), (dict(tokens=17, n_in=2592, out=40000, gamma=PTR), INVALID), (dict(tokens=17, dtype=1, n_in=2592, out=40000, ws=PTR, ws_bytes=42 * 4096 + 67), INVALID),
     (dict(tokens=0, x=None), OK)])
 def test_product_refusals(lib, call, kw, rc):
     assert call(lib, **kw) == rc

@@ -985,7 +985,10 @@ EDGES = [(3, 4096, 96, torch.float16), (3, 4112, 96, torch.float16), (4, 4112, 9
          # passes of 16 to 64 tokens of one, two, three and four tiles of outputs, with and without rest
          (48, 2560, 320, torch.bfloat16), (49, 2500, 320, torch.bfloat16), (64, 2560, 256, torch.float16), (100, 1030, 96, torch.float16),
          (40, 6144, 96, torch.float16), (128, 2100, 160, torch.bfloat16), (200, 400, 96, torch.float16), (150, 16640, 64, torch.bfloat16),
-         (130, 8200, 64, torch.float16), (257, 20, 64, torch.bfloat16)]
+         (130, 8200, 64, torch.float16), (257, 20, 64, torch.bfloat16),
+         # more inputs than a token's waves hold: passes of two, of one
+         (3, 100, 2592, torch.float16), (4, 100, 5120, torch.bfloat16), (7, 530, 4096, torch.float16), (5, 40, 5152, torch.float16),
+         (12, 333, 9728, torch.float16), (13, 333, 9728, torch.float16), (2, 40, 10240, torch.bfloat16), (3, 40, 10272, torch.float16)]
 
 
 @pytest.mark.parametrize("tokens,n_out,n_in,dtype", EDGES)
