@@ -656,8 +656,8 @@ int launch_product(const char* what, ProductArgs a, uint8_t* ws, int64_t ws_byte
   return check_launch(what);
 }
 
-int product(const char* what, const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4, int64_t out, int64_t in, const void* residual, void* y, bool gated, void* workspace,
-            int64_t workspace_bytes, void* stream) {
+int product(const char* what, const void* x, int dtype, int64_t tokens, const void* gamma, float eps, const uint8_t* w4, int64_t out,
+            int64_t in, const void* residual, void* y, bool gated, void* workspace, int64_t workspace_bytes, void* stream) {
   set_error("");
   if (dtype != NKV_F16 && dtype != NKV_BF16) return fail(NKV_ERR_INVALID, "%s: dtype %d (fp16 or bf16)", what, dtype);
   if (out <= 0 || out >= (int64_t(1) << 27) || in <= 0 || in % Q4_GROUP || in > P_IN || tokens < 0 || tokens > P_TOKENS)
