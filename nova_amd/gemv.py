@@ -143,9 +143,9 @@ def rms_gemv_q4(x: torch.Tensor, w: Q4Weight, gamma: torch.Tensor | None = None,
     """``W @ rms_norm(x) (+ residual)`` for each token of ``x`` ``[.., in]`` (fp16 or bf16, contiguous) with a 4-bit
     weight; ``gamma=None`` skips the norm. Returns ``[.., out]`` of x's type; ``out`` may be ``residual``.
 
-    The normalized input is rounded once, to 11 bits of bf16 inputs and 22 of fp16, as the matrix cores' operands; all else is fp32 with one
-    rounding of the result. Made for one token to a few dozen (each 64 tokens read the weight again, from the caches
-    where it fits them). The number of tokens chooses the kernel, and so the last bits."""
+    The normalized input is rounded once, to 11 bits of bf16 inputs and 22 of fp16, as the matrix cores' operands; all
+    else is fp32 with one rounding of the result. Made for one token to a few dozen (each 16 to 64 tokens read the weight again, from the
+    caches where it fits them). The number of tokens chooses the kernel, and so the last bits."""
     tokens, out = _q4_args(x, w, gamma, w.shape[0], out, residual)
     launch(x.device, "nkv_gemv_q4", x.data_ptr(), _DT[x.dtype], tokens, _lib.ptr(gamma), float(eps), w.data.data_ptr(),
            *w.shape, _lib.ptr(residual), out.data_ptr(), *_q4_scratch(x, tokens, *w.shape, gamma, False))
