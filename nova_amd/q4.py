@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .chunks import launch
+from .chunks import launch, overlap
 from .kvquant import _DT
 
 GROUP = 32
@@ -42,8 +42,9 @@ class Q4Weight:
         return self.data.numel()
 
 
-def quantize_q4(w: torch.Tensor) -> Q4Weight:
-    """``w`` ``[out_features, in_features]`` (fp16 / bf16 / fp32, on the GPU; ``in_features`` a multiple of 32) in 4 bits."""
+def quantize_q4(w: torch.Tensor, out: Q4Weight | None = None) -> Q4Weight:
+    """``w`` ``[out_features, in_features]`` (fp16 / bf16 / fp32, on the GPU; ``in_features`` a multiple of 32) in 4 bits.
+    ``out``: a weight of the same shape to overwrite (captured graphs that read it go on)."""
     if w.dim() != 2 or w.dtype not in _DT or not w.is_cuda:
         raise ValueError(f"w must be a 2-d fp16 / bf16 / fp32 CUDA tensor, got {tuple(w.shape)} {w.dtype} on {w.device}")
     rows, n = w.shape
@@ -51,9 +52,12 @@ def quantize_q4(w: torch.Tensor) -> Q4Weight:
         raise ValueError(f"in_features {n} must be a positive multiple of {GROUP}")
     w = w.detach()
     w = w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-    data = torch.empty(_lib.load().nkv_q4_weight_bytes(rows, n), dtype=torch.uint8, device=w.device)
-    launch(w.device, "nkv_quantize_q4", w.data_ptr(), _DT[w.dtype], rows, n, data.data_ptr())
-    return Q4Weight(data, (rows, n))
+    if out is None:
+        out = Q4Weight(torch.empty(_lib.load().nkv_q4_weight_bytes(rows, n), dtype=torch.uint8, device=w.device), (rows, n))
+    elif out.shape != (rows, n) or out.data.device != w.device or overlap(out.data, w):
+        raise ValueError(f"out must be a Q4Weight of {(rows, n)} on {w.device} apart from w")
+    launch(w.device, "nkv_quantize_q4", w.data_ptr(), _DT[w.dtype], rows, n, out.data.data_ptr())
+    return out
 
 
 def dequantize_q4(w: Q4Weight, dtype: torch.dtype = torch.float16) -> torch.Tensor:

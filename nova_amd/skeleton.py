@@ -126,6 +126,13 @@ class SkeletonMLP(nn.Module):
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
+def _quantized(w: torch.Tensor, held):
+    """``w`` in 4 bits, in the memory of ``held`` if it is the same weight's of before."""
+    from .q4 import quantize_q4
+
+    return quantize_q4(w, held if held is not None and held.shape == tuple(w.shape) and held.data.device == w.device else None)
+
+
 def _stack_linears(*lins: nn.Linear) -> torch.Tensor:
     """One ``[sum(out), in]`` weight holding the given layers' weights, which become views of it."""
     w = torch.cat([lin.weight.detach() for lin in lins]).contiguous()
@@ -147,7 +154,8 @@ class SkeletonLayer(nn.Module):
         self.post_norm = nn.Parameter(torch.ones(cfg.hidden_size, **factory)) if self.mlp is not None else None
         self.w_qkv: torch.Tensor | None = None
         self.w_gate_up: torch.Tensor | None = None
-        self.q4: dict | None = None  # qkv, o, gate_up, down in 4 bits
+        self.q4: dict | None = None  # qkv, o, gate_up, down in 4 bits, where they are used
+        self.q4_held: dict = {}      # the same, kept for graphs that were captured with them
 
     def forward(self, h, cos, sin, mask, cache):
         h = h + self.attn(_rms(h, self.norm, self.eps), cos, sin, mask, cache)
@@ -165,13 +173,11 @@ class SkeletonLayer(nn.Module):
 
     def quantize_weights(self) -> None:
         """The stacked weights in 4 bits, beside the fp16 ones (which prefills still run on)."""
-        from .q4 import quantize_q4
-
         self.stack_weights()
-        q4 = {"qkv": quantize_q4(self.w_qkv), "o": quantize_q4(self.attn.o_proj.weight)}
+        weights = {"qkv": self.w_qkv, "o": self.attn.o_proj.weight}
         if self.mlp is not None:
-            q4 |= {"gate_up": quantize_q4(self.w_gate_up), "down": quantize_q4(self.mlp.down_proj.weight)}
-        self.q4 = q4
+            weights |= {"gate_up": self.w_gate_up, "down": self.mlp.down_proj.weight}
+        self.q4 = self.q4_held = {name: _quantized(w, self.q4_held.get(name)) for name, w in weights.items()}
 
     def _mlp_chunks(self, h: torch.Tensor) -> torch.Tensor:
         from . import gemv as G
@@ -306,7 +312,7 @@ class SkeletonForCausalLM(nn.Module):
         factory = {} if device is None else {"device": torch.device(device), "dtype": dtype or torch.float16}
         self.model = SkeletonText(cfg, **factory)
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False, **factory)
-        self.lm_head_q4 = None
+        self.lm_head_q4 = self.lm_head_q4_held = None
         g = torch.Generator(device=factory.get("device", "cpu")).manual_seed(seed)
         with torch.no_grad():
             for p in self.parameters():
@@ -319,7 +325,7 @@ class SkeletonForCausalLM(nn.Module):
         """Run one-token decode steps on the HIP kernels (fp16 CUDA model, int8 cache); with
         ``fused_qkv`` each layer's projection, head norms, RoPE and attention step are one launch. ``weights``
         ``"q4"``: the projections and the lm_head of those steps, and of :meth:`forward_chunks`, in 4 bits, made of the
-        fp16 weights as they are now."""
+        fp16 weights as they are now (in the memory of the last time, which captured steps go on reading)."""
         if weights not in ("fp16", "q4"):
             raise ValueError(f"weights {weights!r}: 'fp16' or 'q4'")
         cfg = self.config
@@ -336,9 +342,10 @@ class SkeletonForCausalLM(nn.Module):
                     layer.quantize_weights()
                 else:
                     layer.q4 = None
-            from .q4 import quantize_q4
-
-            self.lm_head_q4 = quantize_q4(w) if weights == "q4" else None
+            if weights == "q4":
+                self.lm_head_q4 = self.lm_head_q4_held = _quantized(w, self.lm_head_q4_held)
+            else:
+                self.lm_head_q4 = None
             # the RoPE frequencies as the torch path promotes them (fp16 after ``.half()``)
             self.model.inv_freq32 = self.model.inv_freq.float().contiguous()
         self.model.decode_kernels = bool(on)

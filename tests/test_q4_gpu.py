@@ -1064,3 +1064,40 @@ def test_products_of_many_tokens(tokens):
     w = quantize_q4(_randn((80, 160), 172, 0.05).cuda())
     _check_product(x, w, gamma, 1e-6, None, G.rms_gemv_q4(x, w, gamma))
     _check_product(x, w, gamma, 1e-6, None, G.swiglu_gemv_q4(x, w, gamma), gated=True)
+
+
+def test_captured_steps_outlive_a_change_of_the_weights_mode():
+    """A captured step goes on with its 4-bit weights while the decoder runs on fp16 ones, and with new values once they are
+    quantized again."""
+    from nova_amd.decode import GraphDecoder
+
+    model = _decoder(_config(num_hidden_layers=2)).use_decode_kernels(weights="q4")
+    ids = torch.randint(0, 300, (1, 70), generator=torch.Generator().manual_seed(9)).cuda()
+    dec = GraphDecoder(model, max_len=256, quant="int8")
+    dec.prefill(ids)
+    dec.capture(warmup=2)
+    start = [(t, t.clone()) for t in (dec.input_ids, dec.cache.pos, dec.cache._written, dec.cache._qlen)]
+
+    def replay():
+        for t, held in start:
+            t.copy_(held)
+        dec.step()
+        torch.cuda.synchronize()
+        return dec.logits.clone()
+
+    want = replay()
+    model.use_decode_kernels(weights="fp16")
+    junk = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(16)]  # (what was freed would be taken)
+    assert torch.equal(replay(), want)
+    model.use_decode_kernels(weights="q4")
+    assert torch.equal(replay(), want)
+    with torch.no_grad():
+        model.lm_head.weight.mul_(2)
+    model.use_decode_kernels(weights="q4")
+    assert torch.equal(replay(), want * 2) and len(junk) == 16
+    w = _randn((32, 64), 180).cuda()
+    held = quantize_q4(w)
+    assert quantize_q4(-w, out=held) is held and torch.equal(dequantize_q4(held), -dequantize_q4(quantize_q4(w)))
+    for bad in (_randn((32, 96), 181).cuda(), _randn((16, 64), 181).cuda()):
+        with pytest.raises(ValueError):
+            quantize_q4(bad, out=held)
